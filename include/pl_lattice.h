@@ -293,6 +293,72 @@ int pl_export_lattice(const void* workspace, const float* positions, const float
                       int32_t* vertex_item, int32_t* pixel_vertex, float* pixel_weight,
                       void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------------
+ * Training beside the filter: products of channels with an epilogue, their gradients, and activations kept in 8 bits.
+ * Rows are points (batch and spatial dimensions together), channels last.  The reference ships none of it: its users
+ * (README.md:15-16, CRF-as-RNN) train the unaries, the kernels' weights and the labels' compatibility around the filter. */
+
+typedef enum pl_dtype { PL_F32 = 0, PL_F16 = 1, PL_BF16 = 2 } pl_dtype;
+typedef enum pl_activation { PL_ACT_NONE = 0, PL_ACT_RELU = 1, PL_ACT_SOFTMAX = 2 } pl_activation;
+
+/* n values in 8 bits (device): codes[n] and a header for every 32 consecutive values, scales[(n + 31) / 32].  A block's
+ * header is (e + 127) | signed << 8, e the least exponent from -126 to 120 (signed: 121) at which its largest magnitude is at
+ * most 255 (no value negative) or 127 (signed) steps of 2^e; its codes are round-half-even(x 2^-e), unsigned or in two's
+ * complement, at most 255 (127 either way): half a step off at most, exact for whole steps; magnitudes beyond 255 2^120
+ * (127 2^121) come back as that.  A block that holds an infinity or a NaN has the header 255 and comes back as
+ * NaN throughout. */
+typedef struct pl_packed {
+    uint8_t* codes;
+    int16_t* scales;
+} pl_packed;
+
+/* An activation that a backward pass reads: in 8 bits if packed.codes is set, else as it was. */
+typedef struct pl_kept {
+    const void* full;
+    pl_packed packed;
+} pl_kept;
+
+/* z[rows, n] = x[rows, k] @ weight[k, n] (+ x2[rows, k2] @ weight2[k2, n] if k2 > 0) (+ bias[n]) (+ residual_scale * residual[rows, n])
+ * out = z, max(z, 0) or softmax of z over the n channels.  Up to 128 channels each.
+ * dtype: of x, x2, residual, out and their gradients; weight_dtype: of weights, bias and their gradients, PL_F32 or dtype.
+ * Products and sums are float or better whatever the types; every result is rounded once.  A row of a softmax whose z
+ * are all -infinity (a residual that forbids every channel: a padded point) comes out as zeros, with zero gradients.  x and
+ * the weights have to be finite: a row of x that is not makes its row of out NaN. */
+typedef struct pl_mix {
+    int64_t rows;
+    int k, k2, n;
+    int activation;   /* pl_activation */
+    int dtype, weight_dtype;   /* pl_dtype */
+    float residual_scale;
+} pl_mix;
+
+/* The gradients to compute, NULL for those that are not wanted. */
+typedef struct pl_mix_gradients {
+    void *x, *x2, *weight, *weight2, *bias, *residual;
+} pl_mix_gradients;
+
+/* Host structures by value or pointer, device pointers inside; x2, weight2, bias, residual may be NULL where the formula
+ * leaves them out.  keep_*: where to put x, x2 and out in 8 bits besides (codes NULL: not wanted); with relu no positive value
+ * of out gets code 0, so that its gradient's mask is exact.  out must not overlap the inputs.
+ * No counterpart in the reference. */
+int pl_channel_mix(const pl_mix* m, void* out, const void* x, const void* x2, const void* weight, const void* weight2,
+                   const void* bias, const void* residual, pl_packed keep_x, pl_packed keep_x2, pl_packed keep_out, void* stream);
+
+/* Bytes of workspace that pl_channel_mix_backward takes for these sizes.  No counterpart in the reference. */
+int pl_channel_mix_workspace_bytes(const pl_mix* m, size_t* bytes);
+
+/* The gradients of pl_channel_mix, from that of its output and what the forward pass kept: out (with an activation), x for
+ * d.weight, x2 for d.weight2; weight for d.x, weight2 for d.x2.  Sums over rows in a fixed order: the same inputs give
+ * the same bits.  The outputs must overlap neither each other nor the inputs.  No counterpart in the reference. */
+int pl_channel_mix_backward(const pl_mix* m, const void* grad_out, pl_kept out, pl_kept x, pl_kept x2, const void* weight,
+                            const void* weight2, pl_mix_gradients d, void* workspace, size_t workspace_bytes, void* stream);
+
+/* n values to 8 bits and back (pl_dtype of x).  keep_nonzero: a value that is not zero gets code 1 or -1 where 0 would be
+ * nearer.  No counterpart in the reference. */
+int pl_pack_activations(pl_packed packed, const void* x, int64_t n, int dtype, int keep_nonzero, void* stream);
+/* No counterpart in the reference. */
+int pl_unpack_activations(void* x, pl_packed packed, int64_t n, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

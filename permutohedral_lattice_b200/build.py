@@ -2,8 +2,9 @@
 
     python -m permutohedral_lattice_b200.build [--force] [--verbose]
 
--fmad=false: no multiply-add contraction anywhere in the translation unit; the lattice geometry must
-round every operation separately to select the same simplices as the reference CPU code.
+-fmad=false for pl_lattice.cu: no multiply-add contraction anywhere in the translation unit; the lattice geometry must
+round every operation separately to select the same simplices as the reference CPU code.  The sources are compiled side
+by side, each when it or a header is newer than its object.
 """
 import os
 import subprocess
@@ -13,10 +14,10 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libpl_lattice.so")
-SOURCES = [os.path.join(CSRC, "pl_lattice.cu")]
+SOURCES = [os.path.join(CSRC, "pl_lattice.cu"), os.path.join(CSRC, "channel_mix.cu")]
 HEADERS = [os.path.join(CSRC, h) for h in ("simplex.cuh", "common.cuh", "lattice_build.cuh", "splat.cuh",
                                              "blur_slice.cuh", "small.cuh", "export.cuh", "fp64.cuh", "direct_index.cuh", "direct_bounds.h", "crf.cuh",
-                                             "smem_limit.h")] + [
+                                             "smem_limit.h", "host_calls.h")] + [
     os.path.join(ROOT, "include", "pl_lattice.h")]
 
 
@@ -31,12 +32,24 @@ def build(force=False, verbose=False):
     deps = SOURCES + HEADERS
     if not force and os.path.exists(LIB) and all(os.path.getmtime(LIB) >= os.path.getmtime(d) for d in deps):
         return LIB
-    cmd = [nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-           "-fmad=false", "-Xcompiler", "-fPIC", "-shared", "-o", LIB] + SOURCES
+    flags = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
     if verbose:
-        cmd.insert(1, "-Xptxas")
-        cmd.insert(2, "-v")
-    subprocess.check_call(cmd)
+        flags += ["-Xptxas", "-v"]
+    objects, running = [], []
+    for src in SOURCES:
+        obj = src[:-3] + ".o"
+        objects.append(obj)
+        if not force and os.path.exists(obj) and all(os.path.getmtime(obj) >= os.path.getmtime(d) for d in [src] + HEADERS):
+            continue
+        own = ["-fmad=false"] if os.path.basename(src) == "pl_lattice.cu" else []
+        running.append((obj, subprocess.Popen([nvcc_path()] + flags + own + ["-c", "-o", obj, src])))
+    failed = [obj for obj, process in running if process.wait() != 0]
+    for obj in failed:      # whatever is left of it is not newer than its source
+        if os.path.exists(obj):
+            os.remove(obj)
+    if failed:
+        raise RuntimeError("nvcc failed for " + ", ".join(failed))
+    subprocess.check_call([nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", LIB] + objects)
     return LIB
 
 

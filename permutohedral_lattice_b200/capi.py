@@ -28,7 +28,8 @@ EXPORTED_SYMBOLS = [
     "pl_workspace_bytes_f64", "pl_compute_positions_f64", "pl_filter_f64", "pl_lattice_filter_f64",
     "pl_export_lattice_f64", "pl_debug_direct_index", "pl_crf_update_f32", "pl_crf_step_f32", "pl_crf_start_f32", "pl_launch_count",
     "pl_direct_index_min_entries", "pl_watch_next_call", "pl_cancel_watch", "pl_await_watched_call",
-    "pl_watched_calls_status",
+    "pl_watched_calls_status", "pl_channel_mix", "pl_channel_mix_workspace_bytes", "pl_channel_mix_backward",
+    "pl_pack_activations", "pl_unpack_activations",
 ]
 STATIC_SCRATCH_BYTES = 64 << 20
 NUM_STAGE_EVENTS = 6
@@ -39,6 +40,28 @@ class PlStats(ctypes.Structure):
     _fields_ = [("num_vertices", ctypes.c_int64), ("num_entries", ctypes.c_int64),
                 ("table_slots", ctypes.c_int64), ("device_status", ctypes.c_int32),
                 ("direct_index", ctypes.c_int32), ("max_entries", ctypes.c_int64)]
+
+
+PL_F32, PL_F16, PL_BF16 = 0, 1, 2
+PL_ACT_NONE, PL_ACT_RELU, PL_ACT_SOFTMAX = 0, 1, 2
+
+
+class PlPacked(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p)]
+
+
+class PlKept(ctypes.Structure):
+    _fields_ = [("full", ctypes.c_void_p), ("packed", PlPacked)]
+
+
+class PlMix(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("k", ctypes.c_int), ("k2", ctypes.c_int), ("n", ctypes.c_int),
+                ("activation", ctypes.c_int), ("dtype", ctypes.c_int), ("weight_dtype", ctypes.c_int),
+                ("residual_scale", ctypes.c_float)]
+
+
+class PlMixGradients(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("x", "x2", "weight", "weight2", "bias", "residual")]
 
 
 class PlError(RuntimeError):
@@ -99,6 +122,12 @@ def lib():
         L.pl_await_watched_call.argtypes = [ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(i), vp]
         L.pl_launch_count.argtypes = []
         L.pl_launch_count.restype = ctypes.c_ulonglong
+        mix = ctypes.POINTER(PlMix)
+        L.pl_channel_mix.argtypes = [mix, vp, vp, vp, vp, vp, vp, vp, PlPacked, PlPacked, PlPacked, vp]
+        L.pl_channel_mix_workspace_bytes.argtypes = [mix, ctypes.POINTER(ctypes.c_size_t)]
+        L.pl_channel_mix_backward.argtypes = [mix, vp, PlKept, PlKept, PlKept, vp, vp, PlMixGradients, vp, ctypes.c_size_t, vp]
+        L.pl_pack_activations.argtypes = [PlPacked, vp, i64, i, i, vp]
+        L.pl_unpack_activations.argtypes = [vp, PlPacked, i64, i, vp]
         _lib = L
     return _lib
 

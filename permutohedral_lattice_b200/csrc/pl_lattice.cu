@@ -54,7 +54,7 @@
 #include "export.cuh"
 #include "fp64.cuh"
 #include "crf.cuh"
-#include "smem_limit.h"
+#include "host_calls.h"
 
 namespace pl {
 
@@ -68,18 +68,12 @@ static thread_local cudaEvent_t* g_stage_events = nullptr;
 // Kernel launches issued by the library since it was loaded (pl_launch_count): memsets and event
 // records are not counted.
 static std::atomic<unsigned long long> g_launches{0};
-#define PL_COUNT_LAUNCHES(n) g_launches.fetch_add((n), std::memory_order_relaxed)
+void count_launches(int n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
 
-static int cuda_fail(cudaError_t e, const char* where) {
+int cuda_fail(cudaError_t e, const char* where) {
     snprintf(g_cuda_error, sizeof(g_cuda_error), "%s: %s", where, cudaGetErrorString(e));
     return PL_CUDA_ERROR;
 }
-
-#define PL_CUDA(call)                                   \
-    do {                                                \
-        cudaError_t e_ = (call);                        \
-        if (e_ != cudaSuccess) return cuda_fail(e_, #call); \
-    } while (0)
 
 // Pinned words in which watched calls (pl_watch_next_call) report their counters: a 64-byte line each, handed
 // to a thread when it first watches a call and taken back when the thread ends (the pool is as large as the
@@ -395,7 +389,7 @@ static dim3 tile_grid(const Geom& g) {
 }
 
 static int g_num_sms = 0;
-static int num_sms() {
+int num_sms() {
     if (g_num_sms == 0) {
         int dev = 0, sms = 0;
         if (cudaGetDevice(&dev) != cudaSuccess ||
@@ -405,27 +399,6 @@ static int num_sms() {
     }
     return g_num_sms;
 }
-
-// Raises a kernel's dynamic shared-memory limit (and sets its carve-out preference) when this call needs more than any
-// call before it on the current device.
-template <auto Kernel>
-static int ensure_dynamic_smem(size_t bytes, bool max_carveout = false) {
-    static SmemLimit limit;
-    int dev = -1;
-    PL_CUDA(cudaGetDevice(&dev));
-    return limit.raise(dev, bytes, [&](size_t n) -> int {
-        PL_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)n));
-        if (max_carveout)
-            PL_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                         cudaSharedmemCarveoutMaxShared));
-        return PL_OK;
-    });
-}
-#define PL_TRY(call)                     \
-    do {                                 \
-        const int rc_ = (call);          \
-        if (rc_ != PL_OK) return rc_;    \
-    } while (0)
 
 // Rows of the per-tile shared-memory vertex-row cache of slice_tiles (48 KB of rows at most).
 static int rows_cap_for(int pd, int vd) {
