@@ -17,7 +17,8 @@ LIB = os.path.join(PKG, "libpl_lattice.so")
 SOURCES = [os.path.join(CSRC, "pl_lattice.cu"), os.path.join(CSRC, "channel_mix.cu")]
 HEADERS = [os.path.join(CSRC, h) for h in ("simplex.cuh", "common.cuh", "lattice_build.cuh", "splat.cuh",
                                              "blur_slice.cuh", "small.cuh", "export.cuh", "fp64.cuh", "direct_index.cuh", "direct_bounds.h", "crf.cuh",
-                                             "smem_limit.h", "host_calls.h")] + [
+                                             "smem_limit.h", "host_calls.h", "mix_common.cuh",
+                                             "mix_forward.cuh", "mix_backward.cuh")] + [
     os.path.join(ROOT, "include", "pl_lattice.h")]
 
 
