@@ -8,6 +8,11 @@
 // A translation unit of its own: nothing here has to round like the reference's geometry.
 #include <cuda_runtime.h>
 #include <algorithm>
+#include <stdlib.h>
+#include <stdio.h>
+#ifndef MIXF_MT
+#define MIXF_MT 2
+#endif
 #include <stdint.h>
 
 #include "host_calls.h"
@@ -17,29 +22,42 @@
 
 namespace pl {
 
-// Values to codes and back: eight lanes a block of 32, 16 bytes of floats a lane.  wide: every address is a multiple of what its
-// accesses take (16 bytes of float, 8 of 16-bit values, 4 of codes).
+// Values to codes and back.  wide: every address is a multiple of what its accesses take (16 bytes of float, 8 of 16-bit values,
+// 4 of codes).
 template <typename T>
 __global__ void __launch_bounds__(256) pack_blocks(uint8_t* __restrict__ codes, int16_t* __restrict__ scales,
                                                    const T* __restrict__ x, long long n, int keep_nonzero, int wide) {
     const int lane = threadIdx.x & 31;
-    const long long step = (long long)gridDim.x * 1024;
-    for (long long i0 = (long long)blockIdx.x * 1024 + (threadIdx.x & ~31) * 4; i0 < n; i0 += step) {   // (the same for a warp)
-        const long long i = i0 + 4 * lane;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (wide && i + 3 < n) load4(v, x + i);
-        else
+    int at[2];
+    runs_of_lane(at[0], at[1]);
+    const long long step = (long long)gridDim.x * 2048;
+    for (long long i0 = (long long)blockIdx.x * 2048 + (threadIdx.x >> 5) * 256; i0 < n; i0 += step) {   // (the same for a warp)
+        float v[8];
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (i + j < n) v[j] = to_float(x[i + j]);
+        for (int u = 0; u < 2; u++) {
+            const long long i = i0 + at[u];
+            float q[4];
+            if (wide && i + 3 < n) load4(q, x + i);
+            else
+#pragma unroll
+                for (int j = 0; j < 4; j++) q[j] = i + j < n ? to_float(x[i + j]) : 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[4 * u + j] = q[j];
+        }
         u32 header;
-        const u32 c = encode4(v, header, keep_nonzero != 0);
-        if (wide && i + 3 < n) *reinterpret_cast<u32*>(codes + i) = c;
-        else
+        const uint2 c = encode8(v, header, keep_nonzero != 0);
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (i + j < n) codes[i + j] = (uint8_t)(c >> (8 * j));
-        if ((lane & 7) == 0 && i < n) scales[i / PACK_BLOCK] = (int16_t)header;
+        for (int u = 0; u < 2; u++) {
+            const long long i = i0 + at[u];
+            const u32 w = u ? c.y : c.x;
+            if (wide && i + 3 < n) *reinterpret_cast<u32*>(codes + i) = w;
+            else
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (i + j < n) codes[i + j] = (uint8_t)(w >> (8 * j));
+        }
+        const long long b = i0 / PACK_BLOCK + (lane >> 2);
+        if ((lane & 3) == 0 && b * PACK_BLOCK < n) scales[b] = (int16_t)header;
     }
 }
 
@@ -84,7 +102,7 @@ static bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_
 template <typename T>
 static int launch_pack(pl_packed to, const void* x, int64_t n, bool keep_nonzero, cudaStream_t st) {
     const bool wide = aligned(x, 4 * sizeof(T)) && aligned(to.codes, 4);
-    pack_blocks<T><<<grid_for(n, 1024, 8), 256, 0, st>>>(to.codes, to.scales, static_cast<const T*>(x), n, keep_nonzero, wide);
+    pack_blocks<T><<<grid_for(n, 2048, 8), 256, 0, st>>>(to.codes, to.scales, static_cast<const T*>(x), n, keep_nonzero, wide);
     PL_COUNT_LAUNCHES(1);
     PL_CUDA(cudaGetLastError());
     return PL_OK;
@@ -104,35 +122,46 @@ static int launch_unpack(void* x, const pl_packed& from, int64_t n, cudaStream_t
 }
 
 constexpr size_t SMEM_SM = 228 * 1024, SMEM_CTA = 227 * 1024;   // shared memory of an SM, and the most that a CTA may have
-// How many warps, stages and CTAs a kernel of `rows_per_warp` rows a warp runs with: smem(warps, stages) bytes a CTA.
-// Four warps a CTA where that still gives every SM a tile, two stages where they fit.
+// How a kernel runs whose warps have tiles of their own, smem(warps, stages, blocks) bytes a CTA: blocks of rows in a tile, stages of
+// a warp, warps of a CTA, CTAs.
 struct MixLaunch {
-    int warps, stages, ctas;
+    int warps, stages, blocks, ctas;
     size_t smem;
 };
 template <typename Smem>
-static MixLaunch mix_launch(long long rows, int rows_per_warp, int most_ctas, Smem smem) {
+static MixLaunch mix_launch(long long rows, int block_rows, size_t block_bytes, int most_ctas, int most_stages, int most_blocks, Smem smem) {
+    static const char* e = getenv("PLX");   // warps stages blocks ctas
+    int ew = 0, es = 0, eb = 0, ec = 0;
+    if (e) sscanf(e, "%d %d %d %d", &ew, &es, &eb, &ec);
     MixLaunch l;
-    l.warps = 4;
-    while (l.warps > 1 && rows <= (long long)rows_per_warp * l.warps / 2 * num_sms()) l.warps /= 2;
-    l.stages = rows > (long long)rows_per_warp * l.warps * num_sms() ? 2 : 1;
-    while (l.stages > 1 && smem(l.warps, l.stages) > SMEM_CTA) l.stages--;
-    while (l.warps > 1 && smem(l.warps, l.stages) > SMEM_CTA) l.warps--;
-    l.smem = smem(l.warps, l.stages);
+    const long long all = (rows + block_rows - 1) / block_rows;
+    // A tile of some 4 KB, as long as there are tiles for four warps of every SM; a CTA of four warps, as long as there are tiles for
+    // every SM.
+    l.blocks = (int)std::max<size_t>(1, std::min<size_t>(most_blocks, 4096 / block_bytes));
+    if (eb) l.blocks = std::min(eb, most_blocks);
+    while (l.blocks > 1 && all < (long long)l.blocks * 4 * num_sms()) l.blocks--;
+    const long long tiles = (all + l.blocks - 1) / l.blocks;
+    l.warps = (int)std::max(1ll, std::min((long long)(ew ? ew : 4), tiles / num_sms()));
+    l.stages = tiles > (long long)l.warps * num_sms() ? std::min(es ? es : 2, most_stages) : 1;
+    while (l.stages > 1 && smem(l.warps, l.stages, l.blocks) > SMEM_CTA) l.stages--;
+    while (l.blocks > 1 && smem(l.warps, l.stages, l.blocks) > SMEM_CTA) l.blocks--;
+    while (l.warps > 1 && smem(l.warps, l.stages, l.blocks) > SMEM_CTA) l.warps--;
+    l.smem = smem(l.warps, l.stages, l.blocks);
     const int fit = (int)std::max<size_t>(1, SMEM_SM / (l.smem + 1024));
-    const long long per_tile = (long long)rows_per_warp * l.warps;
-    l.ctas = (int)std::min<long long>((rows + per_tile - 1) / per_tile, (long long)num_sms() * std::min(most_ctas, fit));
+    const long long per_cta = (long long)block_rows * l.blocks * l.warps;
+    l.ctas = (int)std::min<long long>((rows + per_cta - 1) / per_cta, (long long)num_sms() * std::min(ec ? ec : most_ctas, fit));
     return l;
 }
 
-template <typename TI, typename TO, int NT, int MT>
+template <typename TI, typename TO, int NT, int MT, bool PARTS>
 static int launch_forward(MixArgs a, cudaStream_t st) {
-    const MixLaunch l = mix_launch(a.rows, 16 * MT, 4, [&](int warps, int stages) {
-        return MixSmem<TI, TO>(16 * MT * warps, a.k, a.k2, a.n, NT).bytes(stages);
-    });
-    a.stages = l.stages;
-    PL_TRY((ensure_dynamic_smem<mix_forward<TI, TO, NT, MT>>(l.smem)));
-    mix_forward<TI, TO, NT, MT><<<l.ctas, 32 * (l.warps + 1), l.smem, st>>>(a);
+    const MixLaunch l = mix_launch(a.rows, 16 * MT, 16 * MT * (sizeof(TI) * (a.k + a.k2 + (a.residual ? a.n : 0)) + sizeof(TO) * a.n), 6, MIX_STAGES, 8,
+                                   [&](int warps, int stages, int blocks) {
+                                       return MixSmem<TI, TO>(16 * MT * blocks, a.k, a.k2, a.n, NT).bytes(warps, stages);
+                                   });
+    a.stages = l.stages, a.blocks = l.blocks;
+    PL_TRY((ensure_dynamic_smem<mix_forward<TI, TO, NT, MT, PARTS>>(l.smem)));
+    mix_forward<TI, TO, NT, MT, PARTS><<<l.ctas, 32 * l.warps, l.smem, st>>>(a);
     PL_COUNT_LAUNCHES(1);
     PL_CUDA(cudaGetLastError());
     return PL_OK;
@@ -142,16 +171,25 @@ static int launch_forward(MixArgs a, cudaStream_t st) {
 static bool keeps_in_forward(int n) { return n <= 64; }
 template <typename TI, typename TO>
 static int forward_any(const MixArgs& a, cudaStream_t st) {
-    return a.n <= 8    ? launch_forward<TI, TO, 1, 2>(a, st)
-           : a.n <= 16 ? launch_forward<TI, TO, 2, 2>(a, st)
-           : a.n <= 24 ? launch_forward<TI, TO, 3, 2>(a, st)
-           : a.n <= 32 ? launch_forward<TI, TO, 4, 2>(a, st)
-           : a.n <= 64 ? launch_forward<TI, TO, 8, 2>(a, st)
-                       : launch_forward<TI, TO, 16, 1>(a, st);
+    if (a.k + a.k2 <= 96) {
+        if (a.n <= 8) return launch_forward<TI, TO, 1, MIXF_MT, false>(a, st);
+        if (a.n <= 16) return launch_forward<TI, TO, 2, MIXF_MT, false>(a, st);
+        if (a.n <= 24) return launch_forward<TI, TO, 3, MIXF_MT, false>(a, st);
+        if (a.n <= 32) return launch_forward<TI, TO, 4, MIXF_MT, false>(a, st);
+    }
+    return a.n <= 8    ? launch_forward<TI, TO, 1, MIXF_MT, true>(a, st)
+           : a.n <= 16 ? launch_forward<TI, TO, 2, MIXF_MT, true>(a, st)
+           : a.n <= 24 ? launch_forward<TI, TO, 3, MIXF_MT, true>(a, st)
+           : a.n <= 32 ? launch_forward<TI, TO, 4, MIXF_MT, true>(a, st)
+           : a.n <= 40 ? launch_forward<TI, TO, 5, 2, true>(a, st)
+           : a.n <= 48 ? launch_forward<TI, TO, 6, 2, true>(a, st)
+           : a.n <= 56 ? launch_forward<TI, TO, 7, 2, true>(a, st)
+           : a.n <= 64 ? launch_forward<TI, TO, 8, 2, true>(a, st)
+                       : launch_forward<TI, TO, 16, 1, true>(a, st);
 }
 
 constexpr int BACK_CTAS = 4;   // of an SM, at most: as many shares of dW there may be
-static bool narrow(const pl_mix* m) { return m->k + m->k2 <= 80 && m->n <= 32; }
+static bool narrow(const pl_mix* m) { return up8(m->k) + up8(m->k2) <= 80 && m->n <= 32; }
 static size_t shares_bytes(const pl_mix* m) {
     return up16(sizeof(float) * (size_t)(m->k + m->k2 + 1) * m->n * num_sms() * BACK_CTAS);
 }
@@ -169,24 +207,31 @@ static int add_shares(const MixBackArgs& a, const pl_mix_gradients& d, int ctas,
     return PL_OK;
 }
 
-template <typename T, bool WORK, int MB, int NB>
+template <typename T, bool PACKED, int MB, int NB>
 static int launch_narrow(MixBackArgs a, const pl_mix_gradients& d, cudaStream_t st) {
-    const MixLaunch l = mix_launch(a.rows, 32, BACK_CTAS, [&](int warps, int stages) {
-        return std::max(mix_back_smem(a, warps, NB, sizeof(T), WORK).bytes(stages), mix_share_bytes(warps, MB, NB));
-    });
-    a.stages = l.stages;
-    PL_TRY((ensure_dynamic_smem<mix_backward<T, WORK, MB, NB>>(l.smem)));
-    mix_backward<T, WORK, MB, NB><<<l.ctas, 32 * (l.warps + 1), l.smem, st>>>(a);
+    // in 8 bits: one stage, and as many blocks of rows as give 32 headers of each array (see mix_backward)
+    const int widest = std::max(a.n, std::max(a.k, a.k2));
+    const MixLaunch l = mix_launch(a.rows, 32, 32 * sizeof(T) * (2 * a.n + 2 * (a.k + a.k2)), BACK_CTAS, PACKED ? 1 : MIX_STAGES,
+                                   PACKED ? std::max(1, 32 / widest) : 8, [&](int warps, int stages, int blocks) {
+                                       MixBackArgs b = a;
+                                       b.blocks = blocks, b.stages = stages;
+                                       return std::max(MixBackSmem(b, warps, NB, sizeof(T), PACKED).bytes(warps), mix_share_bytes(warps, MB, NB));
+                                   });
+    a.stages = l.stages, a.blocks = l.blocks;
+    PL_TRY((ensure_dynamic_smem<mix_backward<T, PACKED, MB, NB>>(l.smem)));
+    mix_backward<T, PACKED, MB, NB><<<l.ctas, 32 * l.warps, l.smem, st>>>(a);
     PL_COUNT_LAUNCHES(1);
     PL_CUDA(cudaGetLastError());
     return a.shares ? add_shares(a, d, l.ctas, st) : PL_OK;
 }
-template <typename T, bool WORK>
+// dW in blocks of eight channels, a multiple of 16 in all: what narrow() allows is at most 80.
+template <typename T, bool PACKED>
 static int narrow_any(const MixBackArgs& a, const pl_mix_gradients& d, cudaStream_t st) {
-    return a.k + a.k2 <= 16 && a.n <= 8    ? launch_narrow<T, WORK, 1, 1>(a, d, st)
-           : a.k + a.k2 <= 48 && a.n <= 24 ? launch_narrow<T, WORK, 3, 3>(a, d, st)
-           : a.n <= 16                     ? launch_narrow<T, WORK, 5, 2>(a, d, st)
-                                           : launch_narrow<T, WORK, 5, 4>(a, d, st);
+    const int rows = up8(a.k) + up8(a.k2);
+    return rows <= 16 && a.n <= 8    ? launch_narrow<T, PACKED, 1, 1>(a, d, st)
+           : rows <= 48 && a.n <= 24 ? launch_narrow<T, PACKED, 3, 3>(a, d, st)
+           : a.n <= 16               ? launch_narrow<T, PACKED, 5, 2>(a, d, st)
+                                     : launch_narrow<T, PACKED, 5, 4>(a, d, st);
 }
 
 template <typename T>
@@ -217,7 +262,7 @@ static int launch_wide(const MixBackArgs& a, const pl_mix_gradients& d, cudaStre
 template <typename T>
 static int launch_back(const pl_mix* m, const MixBackArgs& a, const pl_mix_gradients& d, cudaStream_t st) {
     if (!narrow(m)) return launch_wide<T>(a, d, st);
-    return (a.want_x && a.x.codes) || (a.want_x2 && a.x2.codes) ? narrow_any<T, true>(a, d, st) : narrow_any<T, false>(a, d, st);
+    return a.out.codes || a.x.codes || a.x2.codes ? narrow_any<T, true>(a, d, st) : narrow_any<T, false>(a, d, st);
 }
 
 static bool whole(const pl_packed& p) { return p.codes && p.scales; }
@@ -311,6 +356,7 @@ int pl_channel_mix_backward(const pl_mix* m, const void* grad_out, pl_kept out, 
     if (a.want_x2) a.x2 = kept(x2);
     a.weight = weight, a.weight2 = weight2, a.weight_dtype = m->weight_dtype;
     a.dx = d.x, a.dx2 = d.x2, a.dresidual = d.residual;
+    a.bias = d.bias != nullptr;
     if (d.weight || d.weight2 || d.bias) a.shares = static_cast<float*>(workspace);
     a.dz = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + shares_bytes(m));
     const cudaStream_t st = (cudaStream_t)stream;

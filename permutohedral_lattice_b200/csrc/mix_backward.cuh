@@ -1,18 +1,22 @@
 // The gradients of act(x W [+ x2 W2] + ...): dz from the upstream gradient and the output, dx = dz W^T, dW = x^T dz.
 //
-// mix_backward (up to 80 input and 32 output channels): everything in one pass over memory.  A consumer warp takes 32 rows:
-// dz in registers and to shared memory, its share of dW into registers that last for the whole kernel, dx into the place
-// where x came in, and bulk copies out.  At the end a CTA's warps add their shares of dW up, mix_add_shares those of the
-// CTAs, in double and in a fixed order.
+// mix_backward (up to 80 input and 32 output channels): everything in one pass over memory, by tiles of a warp's own (see
+// mix_common.cuh).  A warp takes 32 rows at a time: dz to the place where the output came in, their share of dW into registers
+// that last for the whole kernel, dx into the place where x came in.  At the end a CTA's warps add their shares of dW up,
+// mix_add_shares those of the CTAs, in double and in a fixed order.
 //
 // Beyond that dW does not fit a warp's registers: mix_dz writes dz to the workspace, mix_forward multiplies it by the
 // transposed weights, mix_backward_weights gives a CTA's warps blocks of dW to sum over all its rows.
 #pragma once
+#include <type_traits>
 #include "mix_common.cuh"
 #include "mix_forward.cuh"
 
 namespace pl {
 
+#ifndef MIXB_C
+#define MIXB_C (MB * NB > 12 ? 2 : 3)
+#endif
 struct Kept {   // an activation as it was, or in 8 bits
     const void* full;
     const uint8_t* codes;
@@ -28,146 +32,135 @@ struct MixBackArgs {
     int weight_dtype;
     void *dx, *dx2, *dresidual;        // NULL: not wanted
     float* shares;                     // [CTAs][(k + k2 + 1) n]: dW, dW2 and dbias; NULL: none of them wanted
+    int bias;                          // dbias is wanted
     float* dz;                         // the wide way: [rows][n]
-    int want_x, want_x2, stages;       // want: its product with dz
+    int want_x, want_x2;               // its product with dz is wanted
+    int stages, blocks;                // blocks of 32 rows in a tile
 };
 
-// Rows of dz and of W^T in shared memory: 8 rows by 4 columns in 32 banks.
-__host__ __device__ constexpr int mix_dz_stride(int nt) { return 8 * nt + 4; }
+// W^T and dz in shared memory: blocks of 8 x 8 as the lanes take them, both terms (see mix_common.cuh); nb of them for eight rows.
+constexpr int MIX_BLOCK = 512;
 
-// What a consumer warp's 32 rows take of a stage and of its own memory, in bytes.
+// Shared memory, in bytes.  A stage holds a tile's rows of the gradient (dresidual leaves from there), the output, x and x2 (dx and
+// dx2 leave from there); a warp's own memory dz of the 32 rows that it works on and, where some of them come in 8 bits, the output,
+// then x and x2 as floats (dx and dx2 leave from there then).
 struct MixBackSmem {
-    size_t weights, own, stage0;
-    size_t dz, work, own_bytes;                          // of a warp: dz, then x and x2 as floats
-    size_t y_at, ys_at, x_at, xs_at, x2_at, x2s_at, stage_bytes;   // of a stage: the gradient first
-    __host__ __device__ MixBackSmem(int warps, int k, int k2, int n, int nb, int size /* of a value */, bool work_rows, bool y, bool y_packed,
-                                    bool x, bool x_packed, bool x2, bool x2_packed) {
-        const size_t tp = 32 * warps;
-        weights = 128;
-        own = up16(weights + sizeof(float) * (size_t)(up8(k) + up8(k2)) * mix_dz_stride(nb));
-        dz = 0;
-        work = up16(sizeof(float) * 32 * mix_dz_stride(nb));
-        own_bytes = work + (work_rows ? sizeof(float) * 32 * (size_t)(k + k2) : 0);
-        stage0 = own + own_bytes * warps;
-        auto room = [&](bool there, bool packed, size_t c) { return !there ? (size_t)0 : up16(packed ? tp * c : tp * c * size); };
-        auto heads = [&](bool there, bool packed, size_t c) { return there && packed ? up16(2 * tp * c / PACK_BLOCK) : (size_t)0; };
-        y_at = up16(tp * n * size);
-        ys_at = y_at + room(y, y_packed, n);
-        x_at = ys_at + heads(y, y_packed, n);
-        // without work rows dx leaves from where x came in, or would have
-        xs_at = x_at + room(x || !work_rows, x_packed && work_rows, k);
-        x2_at = xs_at + heads(x, x_packed, k);
-        x2s_at = x2_at + room((x2 || !work_rows) && k2, x2_packed && work_rows, k2);
-        stage_bytes = up16(x2s_at + heads(x2, x2_packed, k2));
+    size_t weights, stage0, stage_bytes, own0, own_bytes;
+    size_t y_at, x_at, x2_at;   // of a stage
+    size_t work_at, work2_at;   // of a warp's own memory, dz before
+    __host__ __device__ MixBackSmem(const MixBackArgs& a, int warps, int nb, int size /* of a value */, bool packed) {
+        const size_t rows = 32 * (size_t)a.blocks;
+        const int k = a.k, k2 = a.k2, n = a.n;
+        weights = up16(sizeof(u64) * MIX_WARPS * MIX_STAGES);   // barriers before
+        stage0 = weights + (size_t)(up8(k) + up8(k2)) / 8 * nb * MIX_BLOCK;
+        y_at = up16(rows * n * size);
+        x_at = y_at + (a.activation == PL_ACT_NONE ? 0 : up16(rows * n * (a.out.codes ? 1 : size)));
+        x2_at = x_at + (packed && !a.want_x ? 0 : up16(rows * k * (a.x.codes ? 1 : size)));
+        stage_bytes = x2_at + (packed && !a.want_x2 ? 0 : up16(rows * k2 * (a.x2.codes ? 1 : size)));
+        work_at = 4 * nb * MIX_BLOCK;
+        work2_at = work_at + (packed ? up16(sizeof(float) * 32 * (size_t)k) : 0);
+        own_bytes = work2_at + (packed ? up16(sizeof(float) * 32 * (size_t)(k + k2 > n ? k2 : n - k)) : 0);
+        own0 = stage0 + stage_bytes * a.stages * warps;
     }
-    __host__ __device__ size_t bytes(int stages) const { return stage0 + stage_bytes * stages; }
+    __host__ __device__ size_t bytes(int warps) const { return own0 + own_bytes * warps + 128; }   // (reads of eight channels pass the last one)
 };
-__host__ __device__ inline MixBackSmem mix_back_smem(const MixBackArgs& a, int warps, int nb, int size, bool work) {
-    return MixBackSmem(warps, a.k, a.k2, a.n, nb, size, work, a.activation != PL_ACT_NONE, a.out.codes != nullptr, a.want_x != 0,
-                       a.x.codes != nullptr, a.want_x2 != 0, a.x2.codes != nullptr);
-}
 
-// WORK: x or x2 comes in 8 bits; both are then multiplied from floats of the warp's own memory.
-template <typename T, bool WORK, int MB, int NB>
-__global__ void __launch_bounds__(160, MB * NB > 12 ? 2 : 3) mix_backward(MixBackArgs a) {
+// PACKED: some of the output, x and x2 come in 8 bits; all are then read from floats of the warp's own memory.  One stage, and the
+// headers of its blocks in registers: there are at most 32 of the output and 96 of x or x2 in a tile (see narrow_any).
+template <typename T, bool PACKED, int MB, int NB>
+__global__ void __launch_bounds__(128, MIXB_C) mix_backward(MixBackArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
-    const int warps = (int)blockDim.x / 32 - 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tp = 32 * warps, k = a.k, k2 = a.k2, n = a.n, stages = a.stages;
-    const MixBackSmem at = mix_back_smem(a, warps, NB, sizeof(T), WORK);
-    const bool reads_y = a.activation != PL_ACT_NONE, y_packed = a.out.codes != nullptr;
-    u64* full = reinterpret_cast<u64*>(smem);
-    u64* empty = full + MIX_STAGES;
-    float* w_s = reinterpret_cast<float*>(smem + at.weights);
-    if (threadIdx.x == 0)
-        for (int s = 0; s < stages; s++) {
-            mbar_init(&full[s], 32);
-            mbar_init(&empty[s], warps);
-        }
-    __syncthreads();
-    const long long tiles = (a.rows + tp - 1) / tp;
+    typedef typename std::conditional<PACKED, float, T>::type TX;   // of the rows that are worked on
+    const int warps = (int)blockDim.x / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tile_rows = 32 * a.blocks, k = a.k, k2 = a.k2, n = a.n, stages = PACKED ? 1 : a.stages;
+    const MixBackSmem at(a, warps, NB, sizeof(T), PACKED);
+    const bool reads_y = a.activation != PL_ACT_NONE;
+    u64* bars = reinterpret_cast<u64*>(smem) + MIX_STAGES * warp;
+    unsigned char* stage0 = smem + at.stage0 + at.stage_bytes * stages * warp;
     const T* grad = static_cast<const T*>(a.grad);
-
-    if (warp == warps) {   // the producer
-        int s = 0, round = 0;
-        for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-            if (round && !mbar_wait(&empty[s], (round - 1) & 1)) break;
-            unsigned char* stage = smem + at.stage0 + at.stage_bytes * s;
-            const long long row0 = tile * tp;
-            const int here = (int)min((long long)tp, a.rows - row0);
-            const bool whole = here == tp;
-            unsigned bytes = 0;
-            const void* from[4];
-            unsigned char* to[4];
-            unsigned size[4];
-            int copies = 0;
-            auto values_in = [&](size_t place, const T* p, int c) {
-                p += row0 * c;
-                if (whole && aligned16(p)) {
-                    from[copies] = p, to[copies] = stage + place, size[copies] = (unsigned)(tp * c * sizeof(T));
-                    bytes += size[copies++];
-                } else {
-                    copy_in<sizeof(T)>(stage + place, p, here * c);
-                }
+    const long long tiles = (a.rows + tile_rows - 1) / tile_rows, step = (long long)gridDim.x * warps;
+    const long long first = (long long)blockIdx.x * warps + warp;
+    if (lane == 0)
+        for (int s = 0; s < stages; s++) mbar_init(&bars[s], 1);
+    __syncwarp();
+    auto kept_aligned = [](const Kept& p) { return p.codes ? aligned16(p.codes) : aligned16(p.full); };
+    auto kept_bytes = [&](const Kept& p, int c) { return (u32)(tile_rows * c * (p.codes ? 1 : sizeof(T))); };
+    // (codes of an odd number of 32-row blocks of an odd number of channels: 32 c bytes, a multiple of 16 all the same)
+    const bool bulk_in = aligned16(grad) && (!reads_y || kept_aligned(a.out)) && (!a.want_x || kept_aligned(a.x)) && (!a.want_x2 || kept_aligned(a.x2));
+    const u32 tile_bytes = (u32)(tile_rows * n * sizeof(T)) + (reads_y ? kept_bytes(a.out, n) : 0) + (a.want_x ? kept_bytes(a.x, k) : 0) +
+                           (a.want_x2 ? kept_bytes(a.x2, k2) : 0);
+    u32 heads_y = 0, heads_x[3] = {0, 0, 0}, heads_x2[3] = {0, 0, 0};
+    auto fetch = [&](long long tile, int s) {
+        unsigned char* stage = stage0 + at.stage_bytes * s;
+        const long long row0 = tile * tile_rows;
+        if (row0 >= a.rows) return;
+        const int here = (int)min((long long)tile_rows, a.rows - row0);
+        if constexpr (PACKED) {
+            auto heads_in = [&](u32* heads, int most, const Kept& p, int c) {
+                if (!p.codes) return;
+                const int count = (here * c + PACK_BLOCK - 1) / PACK_BLOCK;
+                const int16_t* from = p.scales + row0 * c / PACK_BLOCK;
+#pragma unroll
+                for (int i = 0; i < most; i++)
+                    if (32 * i + lane < count) heads[i] = (u32)(u16)from[32 * i + lane];
             };
-            auto codes_in = [&](size_t place, size_t heads_place, const Kept& p, int c) {
-                const uint8_t* q = p.codes + row0 * c;
-                if (whole && aligned16(q)) {
-                    from[copies] = q, to[copies] = stage + place, size[copies] = (unsigned)(tp * c);
-                    bytes += size[copies++];
-                } else {
-                    copy_in<1>(stage + place, q, here * c);
-                }
-                copy_in<2>(stage + heads_place, p.scales + row0 * c / PACK_BLOCK, (here * c + PACK_BLOCK - 1) / PACK_BLOCK);
-            };
-            auto kept_in = [&](size_t place, size_t heads_place, const Kept& p, int c) {
-                if (p.codes) codes_in(place, heads_place, p, c);
-                else values_in(place, static_cast<const T*>(p.full), c);
-            };
-            values_in(0, grad, n);
-            if (reads_y) kept_in(at.y_at, at.ys_at, a.out, n);
-            if (a.want_x) kept_in(at.x_at, at.xs_at, a.x, k);
-            if (a.want_x2) kept_in(at.x2_at, at.x2s_at, a.x2, k2);
-            if (!whole) {   // rows that are not there: their dz is zero, their x must not be NaN
-                auto zero = [&](size_t place, bool packed, int c) {
-                    if (packed) return;   // (the decoding writes zeros)
-                    T* p = reinterpret_cast<T*>(stage + place);
-                    for (int i = here * c + lane; i < tp * c; i += 32) p[i] = from_float<T>(0.f);
-                };
-                if (a.want_x) zero(at.x_at, a.x.codes != nullptr, k);
-                if (a.want_x2) zero(at.x2_at, a.x2.codes != nullptr, k2);
-            }
-            cp_async_wait_all();
-            if (lane == 0 && bytes) {
-                mbar_expect_tx(&full[s], bytes);   // (lane 0's arrival)
-                for (int i = 0; i < copies; i++) bulk_load(to[i], from[i], size[i], &full[s]);
-            } else {
-                mbar_arrive(&full[s]);
-            }
-            if (++s == stages) s = 0, round++;
+            if (reads_y) heads_in(&heads_y, 1, a.out, n);
+            if (a.want_x) heads_in(heads_x, 3, a.x, k);
+            if (a.want_x2) heads_in(heads_x2, 3, a.x2, k2);
         }
-        return;
-    }
+        auto from = [&](const Kept& p, int c) -> const void* {
+            return p.codes ? static_cast<const void*>(p.codes + row0 * c) : static_cast<const void*>(static_cast<const T*>(p.full) + row0 * c);
+        };
+        if (bulk_in && here == tile_rows) {
+            if (lane == 0) {
+                mbar_expect_tx(&bars[s], tile_bytes);
+                bulk_load(stage, grad + row0 * n, (u32)(tile_rows * n * sizeof(T)), &bars[s]);
+                if (reads_y) bulk_load(stage + at.y_at, from(a.out, n), kept_bytes(a.out, n), &bars[s]);
+                if (a.want_x) bulk_load(stage + at.x_at, from(a.x, k), kept_bytes(a.x, k), &bars[s]);
+                if (a.want_x2) bulk_load(stage + at.x2_at, from(a.x2, k2), kept_bytes(a.x2, k2), &bars[s]);
+            }
+        } else {
+            auto rows_in = [&](size_t place, const Kept& p, int c) {
+                if (p.codes) {
+                    copy_in(stage + place, p.codes + row0 * c, here * c);
+                    return;
+                }
+                copy_in(stage + place, static_cast<const T*>(p.full) + row0 * c, here * c);
+                // rows of a block that are not there: their dz is zero, their x must not be NaN
+                T* to = reinterpret_cast<T*>(stage + place);
+                for (int i = here * c + lane; i < (here + 31) / 32 * 32 * c; i += 32) to[i] = from_float<T>(0.f);
+            };
+            copy_in(stage, grad + row0 * n, here * n);
+            if (reads_y) rows_in(at.y_at, a.out, n);
+            if (a.want_x) rows_in(at.x_at, a.x, k);
+            if (a.want_x2) rows_in(at.x2_at, a.x2, k2);
+            if (lane == 0) mbar_expect_tx(&bars[s], 0);
+        }
+    };
+    for (int s = 0; s < stages; s++) fetch(first + s * step, s);
 
     // W^T: a row an input channel, zeros behind the last channel of either side
-    constexpr int DS = mix_dz_stride(NB);
-    const int kp = up8(k), threads = 32 * warps;
-    for (int i = threadIdx.x; i < (kp + up8(k2)) * DS; i += threads) {
-        const int r = i / DS, c = i - r * DS;
+    const int kp = up8(k), all_p = kp + up8(k2);
+    for (int i = threadIdx.x; i < all_p * 8 * NB; i += blockDim.x) {
+        const int r = i / (8 * NB), c = i - r * (8 * NB);
         const bool second = r >= kp;
         const int j = second ? r - kp : r;
         const void* w = second ? a.weight2 : a.weight;
-        w_s[i] = c < n && j < (second ? k2 : k) && w ? load_weight(w, j * n + c, a.weight_dtype) : 0.f;
+        u32 hi, lo;
+        split(c < n && j < (second ? k2 : k) && w ? load_weight(w, j * n + c, a.weight_dtype) : 0.f, hi, lo);
+        // the product's rows are the output channels c, its columns the input channels r
+        u32* to = reinterpret_cast<u32*>(smem + at.weights + ((r >> 3) * NB + (c >> 3)) * MIX_BLOCK + (4 * (r & 7) + (c & 3)) * 16 + 4 * (c >> 2 & 1));
+        to[0] = hi, to[2] = lo;
     }
-    asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
+    __syncthreads();
 
-    const int g = lane >> 2, t = lane & 3, r0 = 32 * warp;
+    const int g = lane >> 2, t = lane & 3;
     const bool split_w = a.weight_dtype == PL_F32;
     // 8-bit codes times a power of two need no second term, nor do 16 bits
-    const bool split_x = sizeof(T) == 4 && !(WORK && (!a.want_x || a.x.codes) && (!a.want_x2 || a.x2.codes));
-    const bool bulk_x = a.dx && aligned16(a.dx), bulk_x2 = a.dx2 && aligned16(a.dx2), bulk_r = a.dresidual && aligned16(a.dresidual);
-    unsigned char* own = smem + at.own + at.own_bytes * warp;
-    float* dz_s = reinterpret_cast<float*>(own + at.dz);      // [32][DS]
-    float* work = reinterpret_cast<float*>(own + at.work);    // [32][k], [32][k2]
+    const bool split_x = sizeof(T) == 4 && !(PACKED && (!a.want_x || a.x.codes) && (!a.want_x2 || a.x2.codes));
+    const bool bulk_out = aligned16(a.dx) && aligned16(a.dx2) && aligned16(a.dresidual);   // (NULL counts as aligned)
+    unsigned char* own = smem + at.own0 + at.own_bytes * warp;
+    const u32 dz_at = shared_address(own), w_at = shared_address(smem + at.weights);
     float acc[MB][NB][4], sums[NB];
 #pragma unroll
     for (int i = 0; i < MB; i++)
@@ -178,143 +171,218 @@ __global__ void __launch_bounds__(160, MB * NB > 12 ? 2 : 3) mix_backward(MixBac
 #pragma unroll
     for (int j = 0; j < NB; j++) sums[j] = 0.f;
 
+    constexpr int J = 2 * NB;   // channels of a row that a lane looks at: every fourth
+    bool alive = true;
     int s = 0, parity = 0;
-    for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        unsigned char* stage = smem + at.stage0 + at.stage_bytes * s;
-        const bool arrived = mbar_wait(&full[s], parity);
-        const long long row0 = tile * tp + r0;
-        const int here = (int)max(0ll, min(32ll, a.rows - row0));
-        if (here > 0) {
-            T* g_s = reinterpret_cast<T*>(stage) + r0 * n;
-            // dz: four lanes a row, each every fourth channel, from another one on in every row so that banks differ
-            constexpr int J = 2 * NB;
-            const T* y_s = reinterpret_cast<const T*>(stage + at.y_at) + r0 * n;
-            const uint8_t* yc_s = stage + at.y_at + r0 * n;
-            const int16_t* ys_s = reinterpret_cast<const int16_t*>(stage + at.ys_at) + warp * n;   // 32 rows: n blocks
-#pragma unroll
-            for (int p = 0; p < 4; p++) {
-                const int row = 8 * p + g;
-                float y[J], d[J], sum = 0.f;
-#pragma unroll
-                for (int j = 0; j < J; j++) {
-                    const int c = 4 * ((j + g) % J) + t, i = row * n + c;
-                    const bool there = c < n && row < here;
-                    d[j] = there ? to_float(g_s[i]) : 0.f;
-                    y[j] = 0.f;
-                    if (there && reads_y) y[j] = y_packed ? decode_value(yc_s[i], (u32)(u16)ys_s[i >> 5]) : to_float(y_s[i]);
-                    sum = fmaf(y[j], d[j], sum);
-                }
-                if (a.activation == PL_ACT_SOFTMAX) {
-                    sum += __shfl_xor_sync(~0u, sum, 1);
-                    sum += __shfl_xor_sync(~0u, sum, 2);
-                }
-#pragma unroll
-                for (int j = 0; j < J; j++) {
-                    const int c = 4 * ((j + g) % J) + t;
-                    float z = a.activation == PL_ACT_SOFTMAX ? y[j] * (d[j] - sum) : a.activation == PL_ACT_RELU ? (y[j] > 0.f ? d[j] : 0.f) : d[j];
-                    if (!arrived) z = NAN;   // gave up: nothing that could pass for a result
-                    if (c >= n || row >= here) z = 0.f;
-                    dz_s[row * DS + c] = z;
-                    if (a.dresidual && c < n) g_s[row * n + c] = from_float<T>(a.scale * z);
-                }
-            }
-            const T* x_s = reinterpret_cast<const T*>(stage + at.x_at) + r0 * k;
-            const T* x2_s = reinterpret_cast<const T*>(stage + at.x2_at) + r0 * k2;
-            if constexpr (WORK) {
-                auto decode = [&](float* to, const Kept& from, size_t place, size_t heads_place, int c) {
-                    const int count = here * c;
-                    const uint8_t* codes = stage + place + r0 * c;
-                    const int16_t* heads = reinterpret_cast<const int16_t*>(stage + heads_place) + warp * c;
-                    const T* values = reinterpret_cast<const T*>(stage + place) + r0 * c;
-                    for (int i = 4 * lane; i < 32 * c; i += 128) {
+    for (long long tile = first; tile < tiles; tile += step) {
+        unsigned char* stage = stage0 + at.stage_bytes * s;
+        cp_async_wait_all();
+        alive = alive && mbar_wait(&bars[s], parity);
+        alive = __all_sync(~0u, alive);
+        __syncwarp();   // what the lanes copied is there for all
+        const long long tile0 = tile * tile_rows;
+        const int rows_here = (int)min((long long)tile_rows, a.rows - tile0);
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows_here; r0 += 32) {
+            const int here = min(32, rows_here - r0);
+            // 32 rows from 8 bits to floats; rows that are not there to zeros
+            auto decode = [&](float* to, const Kept& p, const unsigned char* place, const u32* heads, int most, int c) {
+                const int count = here * c;
+                const T* values = reinterpret_cast<const T*>(place) + r0 * c;
+                for (int i0 = 0; i0 < 32 * c; i0 += 128) {
+                    const int i = i0 + 4 * lane;
+                    if (p.codes) {
+                        const int b = r0 / 32 * c + i / 32;
+                        u32 head = __shfl_sync(~0u, heads[0], b);
+                        if (most > 1 && a.blocks * c > 32) {
+                            const u32 second = __shfl_sync(~0u, heads[most > 1 ? 1 : 0], b), third = __shfl_sync(~0u, heads[most > 2 ? 2 : 0], b);
+                            head = b < 32 ? head : b < 64 ? second : third;
+                        }
+                        if (i >= 32 * c) continue;
                         float v[4];
-                        if (from.codes) {
-                            decode4(v, *reinterpret_cast<const u32*>(codes + i), (u32)(u16)heads[min(i, count - 1) >> 5]);
+                        decode4(v, *reinterpret_cast<const u32*>(place + r0 * c + i), head);
+                        if (here < 32) {
 #pragma unroll
                             for (int e = 0; e < 4; e++)
                                 if (i + e >= count) v[e] = 0.f;
-                        } else {
-                            load4(v, values + i);
                         }
                         store4(to + i, v);
+                    } else if (i < 32 * c) {
+                        float v[4];
+                        load4(v, values + i);
+                        store4(to + i, v);
                     }
-                };
-                if (a.want_x) decode(work, a.x, at.x_at, at.xs_at, k);
-                if (a.want_x2) decode(work + 32 * k, a.x2, at.x2_at, at.x2s_at, k2);
+                }
+            };
+            float* work = reinterpret_cast<float*>(own + at.work_at);
+            float* work2 = reinterpret_cast<float*>(own + at.work2_at);
+            if constexpr (PACKED) {
+                if (reads_y) decode(work, a.out, stage + at.y_at, &heads_y, 1, n);
+                __syncwarp();
+            }
+            // dz: four lanes a row, rows 8 p + g.  A lane's values are just what it takes of dz as the left side of dz W^T; for x^T dz, where
+            // others take them, they go to shared memory.
+            const u32 g_at = shared_address(stage) + r0 * n * sizeof(T);
+            const u32 y_at = PACKED ? shared_address(work) : shared_address(stage + at.y_at) + r0 * n * sizeof(T);
+            float d[4][J];
+#pragma unroll
+            for (int p = 0; p < 4; p++) {
+                const int row = 8 * p + g;
+                const u32 g_row = g_at + (row * n + t) * sizeof(T), y_row = y_at + (row * n + t) * sizeof(TX);
+                float y[J];
+#pragma unroll
+                for (int j = 0; j < J; j++) {
+                    d[p][j] = y[j] = 0.f;
+                    if (4 * j + t < n) {
+                        d[p][j] = lds_value<T>(g_row + 4 * j * sizeof(T));
+                        if (reads_y) y[j] = lds_value<TX>(y_row + 4 * j * sizeof(TX));
+                    }
+                }
+                if (a.activation == PL_ACT_SOFTMAX) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int j = 0; j < J; j++) sum = fmaf(y[j], d[p][j], sum);
+                    sum += __shfl_xor_sync(~0u, sum, 1);
+                    sum += __shfl_xor_sync(~0u, sum, 2);
+#pragma unroll
+                    for (int j = 0; j < J; j++) d[p][j] = y[j] * (d[p][j] - sum);   // (zeros behind the last channel)
+                } else if (a.activation == PL_ACT_RELU) {
+#pragma unroll
+                    for (int j = 0; j < J; j++) d[p][j] = y[j] > 0.f ? d[p][j] : 0.f;
+                }
+                if (!alive || here < 32) {
+#pragma unroll
+                    for (int j = 0; j < J; j++)
+                        if (row >= here || 4 * j + t >= n) d[p][j] = 0.f;   // rows that are not there may hold anything
+                        else if (!alive) d[p][j] = NAN;                     // gave up: nothing that could pass for a result
+                }
+                if (a.dresidual) {
+#pragma unroll
+                    for (int j = 0; j < J; j++)
+                        if (4 * j + t < n) sts_value<T>(g_row + 4 * j * sizeof(T), a.scale * d[p][j]);   // (where this lane has read)
+                }
+                if (a.shares) {
+#pragma unroll
+                    for (int j = 0; j < J; j++) {
+                        const u32 to = dz_at + (p * NB + j / 2) * MIX_BLOCK + (4 * (4 * (j & 1) + t) + (g & 3)) * 16 + 4 * (g >> 2);
+                        u32 hi, lo;
+                        split(d[p][j], hi, lo);
+                        sts_value<float>(to, __uint_as_float(hi));
+                        sts_value<float>(to + 8, __uint_as_float(lo));
+                    }
+                }
+            }
+            if constexpr (PACKED) {
+                __syncwarp();
+                if (a.want_x) decode(work, a.x, stage + at.x_at, heads_x, 3, k);
+                if (a.want_x2) decode(work2, a.x2, stage + at.x2_at, heads_x2, 3, k2);
             }
             __syncwarp();
+            const u32 x_at = PACKED ? shared_address(work) : shared_address(stage + at.x_at) + r0 * k * sizeof(T);
+            const u32 x2_at = PACKED ? shared_address(work2) : shared_address(stage + at.x2_at) + r0 * k2 * sizeof(T);
             if (a.shares) {
-                for (int r = 0; r < 32; r += 8) {
+                // dW in blocks of eight channels of x, then of x2: channels behind the last give rows of dW that nobody reads.  32 rows'
+                // products by themselves, then added to the sums as floats are: the tensor cores cut what they add to, and a sum over
+                // many rows would drift.  (Eight rows' where there are too few registers.)
+                constexpr bool LONG = MB * NB <= 9;
+                float part[LONG ? MB : 1][NB][4];
+                if constexpr (LONG) {
+#pragma unroll
+                    for (int i = 0; i < MB; i++)
+#pragma unroll
+                        for (int j = 0; j < NB; j++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) part[i][j][e] = 0.f;
+                }
+                u32 from[2 * MB];
+#pragma unroll
+                for (int i = 0; i < 2 * MB; i++) {
+                    const bool second = 8 * i >= kp && 8 * i < all_p;
+                    from[i] = second ? x2_at + (t * k2 + g + 8 * i - kp) * sizeof(TX) : x_at + (t * k + g + (8 * i < kp ? 8 * i : 0)) * sizeof(TX);
+                }
+                u32 dz_from = dz_at + lane * 16;
+#pragma unroll 1
+                for (int r = 0; r < 32; r += 8, dz_from += NB * MIX_BLOCK) {
                     u32 b_hi[NB][2], b_lo[NB][2];
 #pragma unroll
                     for (int j = 0; j < NB; j++) {
-                        const float v0 = dz_s[(r + t) * DS + 8 * j + g], v1 = dz_s[(r + t + 4) * DS + 8 * j + g];
-                        sums[j] += v0 + v1;
-                        split(v0, b_hi[j][0], b_lo[j][0]);
-                        split(v1, b_hi[j][1], b_lo[j][1]);
+                        const uint4 b = lds4(dz_from + MIX_BLOCK * j);
+                        b_hi[j][0] = b.x, b_hi[j][1] = b.y, b_lo[j][0] = b.z, b_lo[j][1] = b.w;
+                        if (a.bias) sums[j] += (__uint_as_float(b.x) + __uint_as_float(b.z)) + (__uint_as_float(b.y) + __uint_as_float(b.w));
                     }
 #pragma unroll
                     for (int i = 0; i < MB; i++) {
                         u32 a_hi[4], a_lo[4];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int c = 16 * i + g + (e & 1 ? 8 : 0), row = r + t + (e & 2 ? 4 : 0);
-                            float v = 0.f;
-                            if (c < k) {
-                                if (a.want_x) v = WORK ? work[row * k + c] : to_float(x_s[row * k + c]);
-                            } else if (c < k + k2) {
-                                if (a.want_x2) v = WORK ? work[32 * k + row * k2 + c - k] : to_float(x2_s[row * k2 + c - k]);
+                        for (int h = 0; h < 2; h++) {
+                            const bool second = 8 * (2 * i + h) >= kp && 8 * (2 * i + h) < all_p;
+                            const u32 four = (second ? k2 : k) * 4 * (u32)sizeof(TX);
+                            u32& p = from[2 * i + h];
+                            const float v0 = lds_value<TX>(p), v1 = lds_value<TX>(p + four);
+                            p += 2 * four;
+                            if (split_x) {
+                                split(v0, a_hi[h], a_lo[h]);
+                                split(v1, a_hi[2 + h], a_lo[2 + h]);
+                            } else {
+                                a_hi[h] = __float_as_uint(v0), a_hi[2 + h] = __float_as_uint(v1);
                             }
-                            split(v, a_hi[e], a_lo[e]);
                         }
-                        // Eight rows' products by themselves, then added to the sums as floats are: the tensor cores cut what they
-                        // add to, and a sum over many rows would drift.
-                        float part[NB][4];
+                        float (&to)[NB][4] = part[LONG ? i : 0];
 #pragma unroll
-                        for (int j = 0; j < NB; j++)
+                        for (int j = 0; j < NB; j++) {
+                            if constexpr (LONG) mma8(to[j], a_hi, b_hi[j]);
+                            else mma8_first(to[j], a_hi, b_hi[j]);
+                        }
 #pragma unroll
-                            for (int e = 0; e < 4; e++) part[j][e] = 0.f;
+                        for (int j = 0; j < NB; j++) mma8(to[j], a_hi, b_lo[j]);
                         if (split_x) {
 #pragma unroll
-                            for (int j = 0; j < NB; j++) mma8(part[j], a_lo, b_hi[j]);
+                            for (int j = 0; j < NB; j++) mma8(to[j], a_lo, b_hi[j]);
                         }
+                        if constexpr (!LONG) {
 #pragma unroll
-                        for (int j = 0; j < NB; j++) mma8(part[j], a_hi, b_lo[j]);
+                            for (int j = 0; j < NB; j++)
 #pragma unroll
-                        for (int j = 0; j < NB; j++) mma8(part[j], a_hi, b_hi[j]);
+                                for (int e = 0; e < 4; e++) acc[i][j][e] += to[j][e];
+                        }
+                    }
+                }
+                if constexpr (LONG) {
+#pragma unroll
+                    for (int i = 0; i < MB; i++)
 #pragma unroll
                         for (int j = 0; j < NB; j++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++) acc[i][j][e] += part[j][e];
-                    }
+                            for (int e = 0; e < 4; e++) acc[i][j][e] += part[i][j][e];
                 }
+                __syncwarp();   // x has been read: dx may take its place
             }
-            __syncwarp();   // x has been read: dx may take its place
-            auto product = [&](T* to, const float* w, int c_count) {
-                for (int c0 = 0; c0 < c_count; c0 += 24) {
+            // dx and dx2, three blocks of eight channels at a time, to where x and x2 were
+            if (a.dx || a.dx2) {
+                const int blocks = all_p / 8;
+#pragma unroll 1
+                for (int c0 = a.dx ? 0 : kp / 8; c0 < (a.dx2 ? blocks : kp / 8); c0 += 3) {
+                    const u32 w_block = w_at + c0 * NB * MIX_BLOCK + lane * 16;
                     float part[2][3][4];
 #pragma unroll
-                    for (int m = 0; m < 2; m++)
-#pragma unroll
-                        for (int j = 0; j < 3; j++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) part[m][j][e] = 0.f;
-#pragma unroll
                     for (int q = 0; q < NB; q++) {
-                        u32 a_hi[2][4], a_lo[2][4];
+                        u32 a_hi[2][4], a_lo[2][4], b_hi[3][2], b_lo[3][2];
 #pragma unroll
                         for (int m = 0; m < 2; m++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                split(dz_s[(16 * m + g + (e & 1 ? 8 : 0)) * DS + 8 * q + t + (e & 2 ? 4 : 0)], a_hi[m][e], a_lo[m][e]);
-                        u32 b_hi[3][2], b_lo[3][2];
+                            for (int e = 0; e < 4; e++) split(d[2 * m + (e & 1)][2 * q + (e >> 1)], a_hi[m][e], a_lo[m][e]);
 #pragma unroll
-                        for (int j = 0; j < 3; j++) {
-                            const bool there = c0 + 8 * j < c_count;   // rows behind belong to the second input, or to nobody
-                            const float* wc = w + (size_t)(c0 + 8 * j + g) * DS + 8 * q + t;
-                            split(there ? wc[0] : 0.f, b_hi[j][0], b_lo[j][0]);
-                            split(there ? wc[4] : 0.f, b_hi[j][1], b_lo[j][1]);
+                        for (int j = 0; j < 3; j++) {   // (behind the last block lie a stage's values: results that nobody keeps)
+                            const uint4 b = lds4(w_block + (j * NB + q) * MIX_BLOCK);
+                            b_hi[j][0] = b.x, b_hi[j][1] = b.y, b_lo[j][0] = b.z, b_lo[j][1] = b.w;
                         }
+#pragma unroll
+                        for (int j = 0; j < 3; j++)
+#pragma unroll
+                            for (int m = 0; m < 2; m++) {
+                                if (q == 0) mma8_first(part[m][j], a_hi[m], b_hi[j]);
+                                else mma8(part[m][j], a_hi[m], b_hi[j]);
+                            }
 #pragma unroll
                         for (int j = 0; j < 3; j++)
 #pragma unroll
@@ -325,47 +393,47 @@ __global__ void __launch_bounds__(160, MB * NB > 12 ? 2 : 3) mix_backward(MixBac
 #pragma unroll
                                 for (int m = 0; m < 2; m++) mma8(part[m][j], a_hi[m], b_lo[j]);
                         }
-#pragma unroll
-                        for (int j = 0; j < 3; j++)
-#pragma unroll
-                            for (int m = 0; m < 2; m++) mma8(part[m][j], a_hi[m], b_hi[j]);
                     }
 #pragma unroll
-                    for (int m = 0; m < 2; m++)
+                    for (int j = 0; j < 3; j++) {
+                        const bool second = c0 + j >= kp / 8;
+                        const int width = second ? k2 : k, c = 8 * (c0 + j) - (second ? kp : 0) + 2 * t;
+                        if (c0 + j >= blocks || !(second ? a.dx2 : a.dx)) continue;
+                        const u32 to = (second ? x2_at : x_at) + (g * width + c) * sizeof(T);
 #pragma unroll
-                        for (int j = 0; j < 3; j++)
+                        for (int e = 0; e < 2; e++)
+                            if (c + e < width) {
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const int c = c0 + 8 * j + 2 * t + (e & 1), row = 16 * m + g + (e & 2 ? 8 : 0);
-                                if (c < c_count) to[row * c_count + c] = from_float<T>(part[m][j][e]);
+                                for (int m = 0; m < 4; m++)
+                                    sts_value<T>(to + (8 * m * width + e) * sizeof(T), part[m / 2][j][2 * (m & 1) + e]);
                             }
+                    }
                 }
-            };
-            T* dx_s = WORK ? reinterpret_cast<T*>(work) : const_cast<T*>(x_s);
-            T* dx2_s = WORK ? reinterpret_cast<T*>(work + 32 * k) : const_cast<T*>(x2_s);
-            if (a.dx) product(dx_s, w_s, k);
-            if (a.dx2) product(dx2_s, w_s + (size_t)kp * DS, k2);
+            }
             fence_async_proxy();
             __syncwarp();
-            const bool all = here == 32;
-            if (a.dresidual) copy_out(static_cast<T*>(a.dresidual) + row0 * n, g_s, here * n, bulk_r && all);
-            if (a.dx) copy_out(static_cast<T*>(a.dx) + row0 * k, dx_s, here * k, bulk_x && all);
-            if (a.dx2) copy_out(static_cast<T*>(a.dx2) + row0 * k2, dx2_s, here * k2, bulk_x2 && all);
-            if (lane == 0) {
-                bulk_commit();
-                bulk_wait_read();
-            }
+            const bool bulk = bulk_out && here == 32;
+            const long long row0 = tile0 + r0;
+            const T* dx_s = PACKED ? reinterpret_cast<T*>(work) : reinterpret_cast<T*>(stage + at.x_at) + r0 * k;
+            const T* dx2_s = PACKED ? reinterpret_cast<T*>(work2) : reinterpret_cast<T*>(stage + at.x2_at) + r0 * k2;
+            if (a.dresidual) copy_out(static_cast<T*>(a.dresidual) + row0 * n, reinterpret_cast<T*>(stage) + r0 * n, here * n, bulk);
+            if (a.dx) copy_out(static_cast<T*>(a.dx) + row0 * k, dx_s, here * k, bulk);
+            if (a.dx2) copy_out(static_cast<T*>(a.dx2) + row0 * k2, dx2_s, here * k2, bulk);
+            if (lane == 0) bulk_commit();
+            if (lane == 0 && (PACKED || r0 + 32 >= rows_here)) bulk_wait_read();   // (work rows are written again by the next block)
+            __syncwarp();
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[s]);
+        if (alive) fetch(tile + stages * step, s);
         if (++s == stages) s = 0, parity ^= 1;
     }
+    if (!alive)   // gave up once: no copy may be in flight when the CTA goes on
+        for (int i = 0; i < stages; i++) mbar_wait(&bars[i], 0), mbar_wait(&bars[i], 1);
 
-    // the CTA's share of dW and dbias: the warps' sums through shared memory (dz's place and behind; every copy out has read its own)
+    // the CTA's share of dW and dbias: the warps' sums through shared memory, in place of all that was there
     if (!a.shares) return;
     constexpr int PER = MB * 16 * NB * 8 + NB * 8;
-    float* mine = reinterpret_cast<float*>(smem + at.weights);   // the weights are not needed any more, nor is what lies behind them
-    asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
+    float* mine = reinterpret_cast<float*>(smem + at.weights);
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < MB; i++)
 #pragma unroll
@@ -380,11 +448,11 @@ __global__ void __launch_bounds__(160, MB * NB > 12 ? 2 : 3) mix_backward(MixBac
         v += __shfl_xor_sync(~0u, v, 2);
         if (t == 0) mine[warp * PER + MB * 16 * 8 * NB + 8 * j + g] = v;
     }
-    asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
+    __syncthreads();
     const int count = (k + k2 + 1) * n;
     float* share = a.shares + (size_t)blockIdx.x * count;
-    for (int i = threadIdx.x; i < count; i += threads) {
-        const int r = i / n, c = i - r * n, from = (r < k + k2 ? r : MB * 16) * 8 * NB + c;
+    for (int i = threadIdx.x; i < count; i += blockDim.x) {
+        const int r = i / n, c = i - r * n, from = (r < k ? r : r < k + k2 ? r - k + kp : MB * 16) * 8 * NB + c;
         float v = 0.f;
         for (int w = 0; w < warps; w++) v += mine[w * PER + from];
         share[i] = v;
@@ -392,7 +460,7 @@ __global__ void __launch_bounds__(160, MB * NB > 12 ? 2 : 3) mix_backward(MixBac
 }
 // Shared memory that the sum of the shares takes, from the weights on.
 __host__ __device__ constexpr size_t mix_share_bytes(int warps, int mb, int nb) {
-    return 128 + sizeof(float) * (size_t)warps * (mb * 16 * nb * 8 + nb * 8);
+    return up16(sizeof(u64) * MIX_WARPS * MIX_STAGES) + sizeof(float) * (size_t)warps * (mb * 16 * nb * 8 + nb * 8);
 }
 
 // Sums of the CTAs' shares, in double, in the order of the CTAs: eight threads an element.

@@ -31,11 +31,19 @@ __device__ __forceinline__ float load_weight(const void* w, int i, int dtype) {
 // 2^-23 of it: v = hi + lo, hi the nearest one, lo what is left cut to 11 bits; a product of two floats is then hi hi + hi lo +
 // lo hi up to 2^-22.  Numbers of 16 bits and 8-bit codes are their own hi, which saves a term.  Lane 4 g + t of a warp holds
 //   a: (g, t), (g + 8, t), (g, t + 4), (g + 8, t + 4)    b: (t, g), (t + 4, g)    c: (g, 2t), (g, 2t + 1), (g + 8, 2t), (g + 8, 2t + 1)
+// and wants each of them in registers that follow one another.  So b's that are read more than once lie in shared memory as the
+// lanes take them, 16 bytes a lane: the high terms of both, then the low ones.  (Lying row by row as pairs of terms they took two accesses
+// and four moves: a third of all instructions of the gradients at 21 labels.)
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ void mma8(float (&c)[4], const u32 (&a)[4], const u32 (&b)[2]) {
     asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ void mma8_first(float (&c)[4], const u32 (&a)[4], const u32 (&b)[2]) {   // to nothing
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
 }
 __device__ __forceinline__ void split(float v, u32& hi, u32& lo) {
     hi = (__float_as_uint(v) + 0x1000u) & 0xFFFFE000u;
@@ -101,81 +109,159 @@ __device__ __forceinline__ void store4(T* p, const float (&v)[4]) {
     *reinterpret_cast<uint2*>(p) = q;
 }
 
-// Four values of a block to codes, eight lanes a block (all lanes of the warp take part).  Returns the four codes.
-__device__ __forceinline__ u32 encode4(const float (&v)[4], u32& header, bool keep_nonzero) {
-    u32 most = 0, negative = 0;
+// Eight values of a block to codes, four lanes a block (all lanes of the warp take part): v[0..3] and v[4..7] are two runs of four
+// consecutive values, their codes the two words.  A product with a power of two, rounded to a whole number by adding 1.5 2^23 to
+// it: the sum's low byte is the code.
+__device__ __forceinline__ uint2 encode8(const float (&v)[8], u32& header, bool keep_nonzero) {
+    const int lane = threadIdx.x & 31;
+    u32 bits[8], any = 0, most = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const u32 bits = __float_as_uint(v[i]);
-        most = max(most, bits & 0x7FFFFFFFu);
-        negative |= v[i] < 0.f ? 1u : 0u;
+    for (int i = 0; i < 8; i++) {
+        bits[i] = __float_as_uint(v[i]);
+        any |= bits[i];
+    }
+    bool is_signed = false;
+    if (__any_sync(~0u, any >> 31)) {   // (signs of zeros do not count)
+        float least = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            bits[i] &= 0x7FFFFFFFu;
+            least = fminf(least, v[i]);
+        }
+        is_signed = (__ballot_sync(~0u, least < 0.f) >> (lane & 28) & 15u) != 0;
     }
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-        most = max(most, __shfl_xor_sync(~0u, most, o));
-        negative |= __shfl_xor_sync(~0u, negative, o);
-    }
-    header = block_header(most, negative != 0);
-    u32 codes = 0;
+    for (int i = 0; i < 8; i++) most = max(most, bits[i]);
+    most = max(most, __shfl_xor_sync(~0u, most, 1));
+    most = max(most, __shfl_xor_sync(~0u, most, 2));
+    // block_header, but for its upper limit and for NaN: adding what the fraction may lack carries into the exponent where it has more
+    const u32 low = (u32)max((int)((most + (is_signed ? 0x1FFFFu : 0xFFFFu)) >> 23) - (is_signed ? 6 : 7), 1);
+    header = low | (is_signed ? 256u : 0u);
+    if (low >= 247 || keep_nonzero) {
+        header = block_header(most, is_signed);
+        u32 c[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; i++) codes |= encode_value(v[i], header, keep_nonzero) << (8 * i);
-    return codes;
+        for (int i = 0; i < 8; i++) c[i / 4] |= encode_value(v[i], header, keep_nonzero) << (8 * (i & 3));
+        return make_uint2(c[0], c[1]);
+    }
+    const float per_step = __uint_as_float((254u - low) << 23), whole = 12582912.f;
+    u32 c[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) c[i] = __float_as_uint(fmaf(v[i], per_step, whole));
+    return make_uint2(__byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410));
 }
+// Where a lane's two runs of four lie in the 256 values of its warp: blocks take their halves in another order each, so that the
+// lanes that access memory together lie in different banks.
+__device__ __forceinline__ void runs_of_lane(int& first, int& second) {
+    const int lane = threadIdx.x & 31, block = lane >> 2, at = block * PACK_BLOCK + 4 * (lane & 3), swap = 16 * (block & 1);
+    first = at + swap, second = at + 16 - swap;
+}
+// Four codes to values: a byte in the last place of 2^23 is 2^23 more than it stands for, and so is a signed one with its sign
+// turned round, but for another 128.
 __device__ __forceinline__ void decode4(float (&v)[4], u32 codes, u32 header) {
     const float step = block_step(header);
     const bool is_signed = (header & 256u) != 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const u32 c = (codes >> (8 * i)) & 255u;
-        v[i] = (float)(is_signed ? (int)(signed char)c : (int)c) * step;
-    }
+    const float less = is_signed ? 8388608.f + 128.f : 8388608.f;
+    if (is_signed) codes ^= 0x80808080u;
+    v[0] = (__uint_as_float(__byte_perm(codes, 0x4B000000u, 0x7440)) - less) * step;
+    v[1] = (__uint_as_float(__byte_perm(codes, 0x4B000000u, 0x7441)) - less) * step;
+    v[2] = (__uint_as_float(__byte_perm(codes, 0x4B000000u, 0x7442)) - less) * step;
+    v[3] = (__uint_as_float(__byte_perm(codes, 0x4B000000u, 0x7443)) - less) * step;
 }
 
 // `count` values in shared memory, whole blocks from the first one on, to 8 bits by one warp.  wide: codes is 4-byte aligned.
 template <typename T>
 __device__ __forceinline__ void pack_by_warp(const T* values, int count, uint8_t* __restrict__ codes, int16_t* __restrict__ scales,
                                              bool keep_nonzero, bool wide) {
-    const int lane = threadIdx.x & 31, blocks = (count + PACK_BLOCK - 1) / PACK_BLOCK;
-    for (int b0 = 0; b0 < blocks; b0 += 4) {
-        const int b = b0 + (lane >> 3), i = b * PACK_BLOCK + 4 * (lane & 7);
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (i + 3 < count) load4(v, values + i);
-        else
+    int at[2];
+    runs_of_lane(at[0], at[1]);
+    for (int i0 = 0; i0 < count; i0 += 256) {
+        float v[8];
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (i + j < count) v[j] = to_float(values[i + j]);
+        for (int u = 0; u < 2; u++) {
+            const int i = i0 + at[u];
+            float q[4] = {0.f, 0.f, 0.f, 0.f};
+            if (i + 3 < count) load4(q, values + i);
+            else if (i < count) {
+#pragma unroll
+                for (int j = 0; j < 3; j++)
+                    if (i + j < count) q[j] = to_float(values[i + j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[4 * u + j] = q[j];
+        }
         u32 header;
-        const u32 c = encode4(v, header, keep_nonzero);
-        if (wide && i + 3 < count) *reinterpret_cast<u32*>(codes + i) = c;
-        else
+        const uint2 c = encode8(v, header, keep_nonzero);
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (i + j < count) codes[i + j] = (uint8_t)(c >> (8 * j));
-        if ((lane & 7) == 0 && b < blocks) scales[b] = (int16_t)header;
+        for (int u = 0; u < 2; u++) {
+            const int i = i0 + at[u];
+            const u32 w = u ? c.y : c.x;
+            if (wide && i + 3 < count) *reinterpret_cast<u32*>(codes + i) = w;
+            else
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (i + j < count) codes[i + j] = (uint8_t)(w >> (8 * j));
+        }
+        const int lane = threadIdx.x & 31, b = i0 / PACK_BLOCK + (lane >> 2);
+        if ((lane & 3) == 0 && b * PACK_BLOCK < count) scales[b] = (int16_t)header;
     }
 }
 
 // ---------------------------------------------------------------------------------------------
-// Rows of a tile between global and shared memory.  A producer warp fills stages; a stage's `full` barrier counts its 32
-// lanes and the bytes of the bulk copies, its `empty` barrier the consumer warps.
+// Tiles.  Every warp has its own: some rows of every operand, contiguous in memory whatever the number of channels, in a stage
+// of shared memory of its own, fetched and sent out by bulk copies (one lane asks for them), the results in the place of what
+// has been read.  Warps share the weights of their CTA and nothing else, and meet nobody at a tile.  What does not start on a
+// 16-byte boundary, and the last rows, are copied by the lanes.
 // ---------------------------------------------------------------------------------------------
-__device__ __forceinline__ void mbar_arrive(u64* bar) {
-    const unsigned a = (unsigned)__cvta_generic_to_shared(bar);
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(a) : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+constexpr int MIX_WARPS = 4, MIX_STAGES = 2;   // of a CTA and of a warp, at most
 
-// The lanes of a warp copy `bytes` from global to shared memory, any alignment of the source that its type has.
-template <int SIZE>
-__device__ __forceinline__ void copy_in(void* to, const void* from, int count) {
+__device__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// A warp copies `count` elements to shared memory; they are there after cp_async_wait_all and __syncwarp.
+template <typename E>
+__device__ __forceinline__ void copy_in(void* to, const E* from, int count) {
     const int lane = threadIdx.x & 31;
-    if constexpr (SIZE == 4) {
-        for (int i = lane; i < count; i += 32) cp_async4(static_cast<u32*>(to) + i, static_cast<const u32*>(from) + i);
-    } else if constexpr (SIZE == 2) {
-        for (int i = lane; i < count; i += 32) static_cast<u16*>(to)[i] = static_cast<const u16*>(from)[i];
+    if constexpr (sizeof(E) == 4) {
+        for (int i = lane; i < count; i += 32) cp_async4(static_cast<E*>(to) + i, from + i);
     } else {
-        for (int i = lane; i < count; i += 32) static_cast<uint8_t*>(to)[i] = static_cast<const uint8_t*>(from)[i];
+        for (int i = lane; i < count; i += 32) static_cast<E*>(to)[i] = from[i];
+    }
+}
+// Shared memory by its own 32-bit addresses.
+__device__ __forceinline__ u32 shared_address(const void* p) { return (u32)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ float lds(u32 at) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ float lds_value(u32 at) {
+    if constexpr (sizeof(T) == 4) {
+        return lds(at);
+    } else {
+        u16 bits;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(at));
+        return to_float(*reinterpret_cast<T*>(&bits));
+    }
+}
+__device__ __forceinline__ uint4 lds4(u32 at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint2 lds2(u32 at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ void sts_value(u32 at, float v) {
+    if constexpr (sizeof(T) == 4) {
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+    } else {
+        T h = from_float<T>(v);
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(*reinterpret_cast<u16*>(&h)) : "memory");
     }
 }
 // A warp's finished rows from shared to global memory: one bulk copy, or plain stores.  Lane 0 waits later (bulk_wait_read).
@@ -188,6 +274,13 @@ __device__ __forceinline__ void copy_out(T* to, const T* from, int count, bool b
         for (int i = lane; i < count; i += 32) to[i] = from[i];
     }
 }
-__device__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2_approx(float v) {   // 2^v, within 2^-22 of it
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
 
 }  // namespace pl
