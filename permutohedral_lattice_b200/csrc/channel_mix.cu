@@ -142,7 +142,10 @@ static MixLaunch mix_launch(long long rows, int block_rows, size_t block_bytes, 
     while (l.blocks > 1 && all < (long long)l.blocks * 4 * num_sms()) l.blocks--;
     const long long tiles = (all + l.blocks - 1) / l.blocks;
     l.warps = (int)std::max(1ll, std::min((long long)(ew ? ew : 4), tiles / num_sms()));
+    // Two stages where three CTAs of an SM have room for them: what a warp waits for a tile is otherwise better hidden by other warps
+    // (the gradients of 21 labels: 700 us with two stages and eight warps an SM, 602 with one and twelve).
     l.stages = tiles > (long long)l.warps * num_sms() ? std::min(es ? es : 2, most_stages) : 1;
+    if (!es && l.stages == 2 && 3 * (smem(l.warps, 2, l.blocks) + 1024) > SMEM_SM) l.stages = 1;
     while (l.stages > 1 && smem(l.warps, l.stages, l.blocks) > SMEM_CTA) l.stages--;
     while (l.blocks > 1 && smem(l.warps, l.stages, l.blocks) > SMEM_CTA) l.blocks--;
     while (l.warps > 1 && smem(l.warps, l.stages, l.blocks) > SMEM_CTA) l.warps--;
@@ -153,15 +156,15 @@ static MixLaunch mix_launch(long long rows, int block_rows, size_t block_bytes, 
     return l;
 }
 
-template <typename TI, typename TO, int NT, int MT, bool PARTS>
+template <typename TI, typename TO, int NT, int MT, int WAY>
 static int launch_forward(MixArgs a, cudaStream_t st) {
     const MixLaunch l = mix_launch(a.rows, 16 * MT, 16 * MT * (sizeof(TI) * (a.k + a.k2 + (a.residual ? a.n : 0)) + sizeof(TO) * a.n), 6, MIX_STAGES, 8,
                                    [&](int warps, int stages, int blocks) {
-                                       return MixSmem<TI, TO>(16 * MT * blocks, a.k, a.k2, a.n, NT).bytes(warps, stages);
+                                       return MixSmem<TI, TO>(16 * MT * blocks, a.k, a.k2, a.n, NT, WAY).bytes(warps, stages);
                                    });
     a.stages = l.stages, a.blocks = l.blocks;
-    PL_TRY((ensure_dynamic_smem<mix_forward<TI, TO, NT, MT, PARTS>>(l.smem)));
-    mix_forward<TI, TO, NT, MT, PARTS><<<l.ctas, 32 * l.warps, l.smem, st>>>(a);
+    PL_TRY((ensure_dynamic_smem<mix_forward<TI, TO, NT, MT, WAY>>(l.smem)));
+    mix_forward<TI, TO, NT, MT, WAY><<<l.ctas, 32 * l.warps, l.smem, st>>>(a);
     PL_COUNT_LAUNCHES(1);
     PL_CUDA(cudaGetLastError());
     return PL_OK;
@@ -169,23 +172,43 @@ static int launch_forward(MixArgs a, cudaStream_t st) {
 // Output channels in steps of 8: the accumulators of a warp's rows are in registers.  From 65 channels on a warp takes
 // 16 rows in place of 32.
 static bool keeps_in_forward(int n) { return n <= 64; }
+template <typename TI, typename TO, int WAY>
+static int forward_of(const MixArgs& a, cudaStream_t st) {
+    if (a.n <= 8) return launch_forward<TI, TO, 1, 2, WAY>(a, st);
+    if (a.n <= 16) return launch_forward<TI, TO, 2, 2, WAY>(a, st);
+    if (a.n <= 24) return launch_forward<TI, TO, 3, 2, WAY>(a, st);
+    if (a.n <= 32) return launch_forward<TI, TO, 4, 2, WAY>(a, st);
+    if constexpr (WAY != MIX_PLAIN) {
+        return a.n <= 40   ? launch_forward<TI, TO, 5, 2, WAY>(a, st)
+               : a.n <= 48 ? launch_forward<TI, TO, 6, 2, WAY>(a, st)
+               : a.n <= 56 ? launch_forward<TI, TO, 7, 2, WAY>(a, st)
+               : a.n <= 64 ? launch_forward<TI, TO, 8, 2, WAY>(a, st)
+                           : launch_forward<TI, TO, 16, 1, WAY>(a, st);
+    }
+    return PL_INTERNAL_ERROR;
+}
+template <typename TO>
+static int launch_forward_wide(const MixArgs& a, cudaStream_t st) {
+    const size_t smem = wide_smem(a.k, a.k2);
+    PL_TRY((ensure_dynamic_smem<mix_forward_wide<TO>>(smem)));
+    const long long tiles = (a.rows + 15) / 16;
+    const unsigned ctas = (unsigned)std::min<long long>((tiles + WIDE_WARPS - 1) / WIDE_WARPS, num_sms());
+    mix_forward_wide<TO><<<ctas, 32 * WIDE_WARPS, smem, st>>>(a);
+    PL_COUNT_LAUNCHES(1);
+    PL_CUDA(cudaGetLastError());
+    return PL_OK;
+}
 template <typename TI, typename TO>
 static int forward_any(const MixArgs& a, cudaStream_t st) {
-    if (a.k + a.k2 <= 96) {
-        if (a.n <= 8) return launch_forward<TI, TO, 1, MIXF_MT, false>(a, st);
-        if (a.n <= 16) return launch_forward<TI, TO, 2, MIXF_MT, false>(a, st);
-        if (a.n <= 24) return launch_forward<TI, TO, 3, MIXF_MT, false>(a, st);
-        if (a.n <= 32) return launch_forward<TI, TO, 4, MIXF_MT, false>(a, st);
+    if constexpr (sizeof(TI) == 4) {
+        if (a.n > 64) return launch_forward_wide<TO>(a, st);
     }
-    return a.n <= 8    ? launch_forward<TI, TO, 1, MIXF_MT, true>(a, st)
-           : a.n <= 16 ? launch_forward<TI, TO, 2, MIXF_MT, true>(a, st)
-           : a.n <= 24 ? launch_forward<TI, TO, 3, MIXF_MT, true>(a, st)
-           : a.n <= 32 ? launch_forward<TI, TO, 4, MIXF_MT, true>(a, st)
-           : a.n <= 40 ? launch_forward<TI, TO, 5, 2, true>(a, st)
-           : a.n <= 48 ? launch_forward<TI, TO, 6, 2, true>(a, st)
-           : a.n <= 56 ? launch_forward<TI, TO, 7, 2, true>(a, st)
-           : a.n <= 64 ? launch_forward<TI, TO, 8, 2, true>(a, st)
-                       : launch_forward<TI, TO, 16, 1, true>(a, st);
+    if constexpr (sizeof(TI) == 2) {
+        if (a.weight_dtype != PL_F32) return forward_of<TI, TO, MIX_PAIRS>(a, st);
+    }
+    // few products to a sum: what the tensor cores cut stays below 2^-21 of it
+    if (a.k + a.k2 <= 96 && a.n <= 32) return forward_of<TI, TO, MIX_PLAIN>(a, st);
+    return forward_of<TI, TO, MIX_PARTED>(a, st);
 }
 
 constexpr int BACK_CTAS = 4;   // of an SM, at most: as many shares of dW there may be
@@ -253,7 +276,7 @@ static int launch_wide(const MixBackArgs& a, const pl_mix_gradients& d, cudaStre
     }
     if (!a.shares) return PL_OK;
     PL_TRY((ensure_dynamic_smem<mix_backward_weights<T>>(WIDE_SMEM)));
-    const unsigned ctas = grid_for(a.rows, WIDE_ROWS, 2);
+    const unsigned ctas = grid_for(a.rows, WIDE_ROWS, 1);
     mix_backward_weights<T><<<dim3(ctas, a.want_x2 ? 2 : 1), 256, WIDE_SMEM, st>>>(a);
     PL_COUNT_LAUNCHES(1);
     PL_CUDA(cudaGetLastError());

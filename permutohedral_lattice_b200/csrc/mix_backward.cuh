@@ -38,8 +38,9 @@ struct MixBackArgs {
     int stages, blocks;                // blocks of 32 rows in a tile
 };
 
-// W^T and dz in shared memory: blocks of 8 x 8 as the lanes take them, both terms (see mix_common.cuh); nb of them for eight rows.
-constexpr int MIX_BLOCK = 512;
+// W^T and dz in shared memory: blocks of 8 x 8 as the lanes take them, both terms of W^T (see mix_common.cuh), dz as it is; nb of them
+// for eight rows.
+constexpr int MIX_BLOCK = 512, MIX_DZ_BLOCK = 256;
 
 // Shared memory, in bytes.  A stage holds a tile's rows of the gradient (dresidual leaves from there), the output, x and x2 (dx and
 // dx2 leave from there); a warp's own memory dz of the 32 rows that it works on and, where some of them come in 8 bits, the output,
@@ -57,7 +58,7 @@ struct MixBackSmem {
         x_at = y_at + (a.activation == PL_ACT_NONE ? 0 : up16(rows * n * (a.out.codes ? 1 : size)));
         x2_at = x_at + (packed && !a.want_x ? 0 : up16(rows * k * (a.x.codes ? 1 : size)));
         stage_bytes = x2_at + (packed && !a.want_x2 ? 0 : up16(rows * k2 * (a.x2.codes ? 1 : size)));
-        work_at = 4 * nb * MIX_BLOCK;
+        work_at = 4 * nb * MIX_DZ_BLOCK;
         work2_at = work_at + (packed ? up16(sizeof(float) * 32 * (size_t)k) : 0);
         own_bytes = work2_at + (packed ? up16(sizeof(float) * 32 * (size_t)(k + k2 > n ? k2 : n - k)) : 0);
         own0 = stage0 + stage_bytes * a.stages * warps;
@@ -224,53 +225,61 @@ __global__ void __launch_bounds__(128, MIXB_C) mix_backward(MixBackArgs a) {
             // others take them, they go to shared memory.
             const u32 g_at = shared_address(stage) + r0 * n * sizeof(T);
             const u32 y_at = PACKED ? shared_address(work) : shared_address(stage + at.y_at) + r0 * n * sizeof(T);
-            float d[4][J];
+            float d[4][J], y[4][J];
+            const u32 g_row = g_at + (g * n + t) * sizeof(T), y_row = y_at + (g * n + t) * sizeof(TX);
 #pragma unroll
-            for (int p = 0; p < 4; p++) {
-                const int row = 8 * p + g;
-                const u32 g_row = g_at + (row * n + t) * sizeof(T), y_row = y_at + (row * n + t) * sizeof(TX);
-                float y[J];
+            for (int p = 0; p < 4; p++)
 #pragma unroll
                 for (int j = 0; j < J; j++) {
-                    d[p][j] = y[j] = 0.f;
+                    d[p][j] = y[p][j] = 0.f;
                     if (4 * j + t < n) {
-                        d[p][j] = lds_value<T>(g_row + 4 * j * sizeof(T));
-                        if (reads_y) y[j] = lds_value<TX>(y_row + 4 * j * sizeof(TX));
+                        d[p][j] = lds_value<T>(g_row + (8 * p * n + 4 * j) * sizeof(T));
+                        if (reads_y) y[p][j] = lds_value<TX>(y_row + (8 * p * n + 4 * j) * sizeof(TX));
                     }
                 }
-                if (a.activation == PL_ACT_SOFTMAX) {
-                    float sum = 0.f;
+            if (a.activation == PL_ACT_SOFTMAX) {
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int j = 0; j < J; j++) sum = fmaf(y[j], d[p][j], sum);
-                    sum += __shfl_xor_sync(~0u, sum, 1);
-                    sum += __shfl_xor_sync(~0u, sum, 2);
+                for (int j = 0; j < J; j++)
 #pragma unroll
-                    for (int j = 0; j < J; j++) d[p][j] = y[j] * (d[p][j] - sum);   // (zeros behind the last channel)
-                } else if (a.activation == PL_ACT_RELU) {
+                    for (int p = 0; p < 4; p++) sum[p] = fmaf(y[p][j], d[p][j], sum[p]);
 #pragma unroll
-                    for (int j = 0; j < J; j++) d[p][j] = y[j] > 0.f ? d[p][j] : 0.f;
-                }
-                if (!alive || here < 32) {
+                for (int o = 1; o < 4; o <<= 1)
+#pragma unroll
+                    for (int p = 0; p < 4; p++) sum[p] += __shfl_xor_sync(~0u, sum[p], o);
+#pragma unroll
+                for (int p = 0; p < 4; p++)
+#pragma unroll
+                    for (int j = 0; j < J; j++) d[p][j] = y[p][j] * (d[p][j] - sum[p]);   // (behind the last channel: see below)
+            } else if (a.activation == PL_ACT_RELU) {
+#pragma unroll
+                for (int p = 0; p < 4; p++)
+#pragma unroll
+                    for (int j = 0; j < J; j++) d[p][j] = y[p][j] > 0.f ? d[p][j] : 0.f;
+            }
+            if (!alive || here < 32) {
+#pragma unroll
+                for (int p = 0; p < 4; p++)
 #pragma unroll
                     for (int j = 0; j < J; j++)
-                        if (row >= here || 4 * j + t >= n) d[p][j] = 0.f;   // rows that are not there may hold anything
-                        else if (!alive) d[p][j] = NAN;                     // gave up: nothing that could pass for a result
-                }
-                if (a.dresidual) {
+                        if (8 * p + g >= here || 4 * j + t >= n) d[p][j] = 0.f;   // rows that are not there may hold anything
+                        else if (!alive) d[p][j] = NAN;                           // gave up: nothing that could pass for a result
+            }
+            // Behind the last channel dz is zero, or NaN in a row that is NaN throughout: as good for dx, and in columns of dW that nobody reads.
+            if (a.shares) {
+#pragma unroll
+                for (int p = 0; p < 4; p++)
 #pragma unroll
                     for (int j = 0; j < J; j++)
-                        if (4 * j + t < n) sts_value<T>(g_row + 4 * j * sizeof(T), a.scale * d[p][j]);   // (where this lane has read)
-                }
-                if (a.shares) {
+                        sts_value<float>(dz_at + (p * NB + j / 2) * MIX_DZ_BLOCK + (4 * (4 * (j & 1) + t) + (g & 3)) * 8 + 4 * (g >> 2), d[p][j]);
+            }
+            if (a.dresidual) {
 #pragma unroll
-                    for (int j = 0; j < J; j++) {
-                        const u32 to = dz_at + (p * NB + j / 2) * MIX_BLOCK + (4 * (4 * (j & 1) + t) + (g & 3)) * 16 + 4 * (g >> 2);
-                        u32 hi, lo;
-                        split(d[p][j], hi, lo);
-                        sts_value<float>(to, __uint_as_float(hi));
-                        sts_value<float>(to + 8, __uint_as_float(lo));
+                for (int j = 0; j < J; j++)
+                    if (4 * j + t < n) {
+#pragma unroll
+                        for (int p = 0; p < 4; p++) sts_value<T>(g_row + (8 * p * n + 4 * j) * sizeof(T), a.scale * d[p][j]);   // (where this lane has read)
                     }
-                }
             }
             if constexpr (PACKED) {
                 __syncwarp();
@@ -300,15 +309,16 @@ __global__ void __launch_bounds__(128, MIXB_C) mix_backward(MixBackArgs a) {
                     const bool second = 8 * i >= kp && 8 * i < all_p;
                     from[i] = second ? x2_at + (t * k2 + g + 8 * i - kp) * sizeof(TX) : x_at + (t * k + g + (8 * i < kp ? 8 * i : 0)) * sizeof(TX);
                 }
-                u32 dz_from = dz_at + lane * 16;
+                u32 dz_from = dz_at + lane * 8;
 #pragma unroll 1
-                for (int r = 0; r < 32; r += 8, dz_from += NB * MIX_BLOCK) {
+                for (int r = 0; r < 32; r += 8, dz_from += NB * MIX_DZ_BLOCK) {
                     u32 b_hi[NB][2], b_lo[NB][2];
 #pragma unroll
                     for (int j = 0; j < NB; j++) {
-                        const uint4 b = lds4(dz_from + MIX_BLOCK * j);
-                        b_hi[j][0] = b.x, b_hi[j][1] = b.y, b_lo[j][0] = b.z, b_lo[j][1] = b.w;
-                        if (a.bias) sums[j] += (__uint_as_float(b.x) + __uint_as_float(b.z)) + (__uint_as_float(b.y) + __uint_as_float(b.w));
+                        const uint2 b = lds2(dz_from + MIX_DZ_BLOCK * j);
+                        split(__uint_as_float(b.x), b_hi[j][0], b_lo[j][0]);
+                        split(__uint_as_float(b.y), b_hi[j][1], b_lo[j][1]);
+                        if (a.bias) sums[j] += __uint_as_float(b.x) + __uint_as_float(b.y);
                     }
 #pragma unroll
                     for (int i = 0; i < MB; i++) {
@@ -357,45 +367,45 @@ __global__ void __launch_bounds__(128, MIXB_C) mix_backward(MixBackArgs a) {
                 }
                 __syncwarp();   // x has been read: dx may take its place
             }
-            // dx and dx2, three blocks of eight channels at a time, to where x and x2 were
+            // dx and dx2, CH blocks of eight channels at a time, to where x and x2 were
             if (a.dx || a.dx2) {
+                constexpr int CH = MB == 3 ? 6 : MB == 1 ? 2 : 5;
                 const int blocks = all_p / 8;
 #pragma unroll 1
-                for (int c0 = a.dx ? 0 : kp / 8; c0 < (a.dx2 ? blocks : kp / 8); c0 += 3) {
-                    const u32 w_block = w_at + c0 * NB * MIX_BLOCK + lane * 16;
-                    float part[2][3][4];
+                for (int c0 = a.dx ? 0 : kp / 8; c0 < (a.dx2 ? blocks : kp / 8); c0 += CH) {
+                    float part[2][CH][4];
 #pragma unroll
                     for (int q = 0; q < NB; q++) {
-                        u32 a_hi[2][4], a_lo[2][4], b_hi[3][2], b_lo[3][2];
+                        u32 a_hi[2][4], a_lo[2][4], b_hi[CH][2], b_lo[CH][2];
 #pragma unroll
                         for (int m = 0; m < 2; m++)
 #pragma unroll
                             for (int e = 0; e < 4; e++) split(d[2 * m + (e & 1)][2 * q + (e >> 1)], a_hi[m][e], a_lo[m][e]);
 #pragma unroll
-                        for (int j = 0; j < 3; j++) {   // (behind the last block lie a stage's values: results that nobody keeps)
-                            const uint4 b = lds4(w_block + (j * NB + q) * MIX_BLOCK);
+                        for (int j = 0; j < CH; j++) {   // (behind the last block: that block again, and results that nobody keeps)
+                            const uint4 b = lds4(w_at + (min(c0 + j, blocks - 1) * NB + q) * MIX_BLOCK + lane * 16);
                             b_hi[j][0] = b.x, b_hi[j][1] = b.y, b_lo[j][0] = b.z, b_lo[j][1] = b.w;
                         }
 #pragma unroll
-                        for (int j = 0; j < 3; j++)
+                        for (int j = 0; j < CH; j++)
 #pragma unroll
                             for (int m = 0; m < 2; m++) {
                                 if (q == 0) mma8_first(part[m][j], a_hi[m], b_hi[j]);
                                 else mma8(part[m][j], a_hi[m], b_hi[j]);
                             }
 #pragma unroll
-                        for (int j = 0; j < 3; j++)
+                        for (int j = 0; j < CH; j++)
 #pragma unroll
                             for (int m = 0; m < 2; m++) mma8(part[m][j], a_lo[m], b_hi[j]);
                         if (split_w) {
 #pragma unroll
-                            for (int j = 0; j < 3; j++)
+                            for (int j = 0; j < CH; j++)
 #pragma unroll
                                 for (int m = 0; m < 2; m++) mma8(part[m][j], a_hi[m], b_lo[j]);
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < 3; j++) {
+                    for (int j = 0; j < CH; j++) {
                         const bool second = c0 + j >= kp / 8;
                         const int width = second ? k2 : k, c = 8 * (c0 + j) - (second ? kp : 0) + 2 * t;
                         if (c0 + j >= blocks || !(second ? a.dx2 : a.dx)) continue;
@@ -515,20 +525,19 @@ __global__ void __launch_bounds__(256) mix_dz(MixBackArgs a) {
 }
 
 // dW of one input (blockIdx.y: x or x2) and, with the first, dbias: a CTA's eight warps each sum blocks of 64 x 32 of it over all the
-// CTA's rows, 32 rows at a time through shared memory.
-constexpr int WIDE_ROWS = 32, WIDE_DS = MIX_MOST + 8, WIDE_XS = MIX_MOST + 8;
-constexpr size_t WIDE_SMEM = sizeof(float) * WIDE_ROWS * (WIDE_DS + WIDE_XS);
+// CTA's rows, 32 rows at a time through shared memory; the next 32 are on their way in registers meanwhile.
+constexpr int WIDE_ROWS = 32, WIDE_DS = MIX_MOST + 8;   // (rows of 136 floats: 4 rows by 8 channels in 32 banks)
+constexpr size_t WIDE_SMEM = sizeof(float) * 2 * 2 * WIDE_ROWS * WIDE_DS;
 template <typename T>
-__global__ void __launch_bounds__(256) mix_backward_weights(MixBackArgs a) {
-    extern __shared__ __align__(16) float wide_smem[];
-    float* dz_s = wide_smem;                          // [32][WIDE_DS]
-    float* x_s = dz_s + WIDE_ROWS * WIDE_DS;          // [32][WIDE_XS]
+__global__ void __launch_bounds__(256, 1) mix_backward_weights(MixBackArgs a) {
+    extern __shared__ __align__(16) float wide_s[];   // [2][dz, x][32][WIDE_DS]
     const bool second = blockIdx.y != 0;
     const int n = a.n, k = second ? a.k2 : a.k, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int m0 = 64 * (warp & 1), c0 = 32 * (warp >> 1);
     const bool want = second ? a.want_x2 != 0 : a.want_x != 0;
     const Kept& from = second ? a.x2 : a.x;
     const bool split_x = sizeof(T) == 4 && !from.codes;
+    const bool works = c0 < n && (m0 == 0 || m0 < k);   // (the first half of the rows of dW sums dbias, too)
     float acc[4][4][4], sums[4];
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -539,27 +548,42 @@ __global__ void __launch_bounds__(256) mix_backward_weights(MixBackArgs a) {
             for (int e = 0; e < 4; e++) acc[i][j][e] = 0.f;
         }
     const long long tiles = (a.rows + WIDE_ROWS - 1) / WIDE_ROWS;
-    for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        __syncthreads();
-        const long long row0 = tile * WIDE_ROWS;
-        for (int r = warp; r < WIDE_ROWS; r += 8) {
-            const bool there = row0 + r < a.rows;
-            for (int c = lane; c < MIX_MOST; c += 32) {
-                const long long i = (row0 + r) * n + c, ix = (row0 + r) * k + c;
-                dz_s[r * WIDE_DS + c] = there && c < n ? a.dz[i] : 0.f;
-                float v = 0.f;
-                if (there && want && c < k)
-                    v = from.codes ? decode_value(from.codes[ix], (u32)(u16)from.scales[ix / PACK_BLOCK]) : to_float(static_cast<const T*>(from.full)[ix]);
-                x_s[r * WIDE_XS + c] = v;
+    const int c = threadIdx.x & 127, r_first = threadIdx.x >> 7;   // this thread's channel, and the first of its rows: every second
+    float next_d[16], next_x[16];
+    auto fetch = [&](long long tile) {
+        const long long row0 = tile * WIDE_ROWS + r_first;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const long long row = row0 + 2 * i;
+            const bool there = row < a.rows;
+            next_d[i] = there && c < n ? a.dz[row * n + c] : 0.f;
+            next_x[i] = 0.f;
+            if (there && want && c < k) {
+                const long long at = row * k + c;
+                next_x[i] = from.codes ? decode_value(from.codes[at], (u32)(u16)from.scales[at / PACK_BLOCK]) : to_float(static_cast<const T*>(from.full)[at]);
             }
         }
-        __syncthreads();
-        if (c0 >= n || (m0 >= k && m0)) continue;   // (the first half of the rows of dW sums dbias, too)
-        for (int r = 0; r < WIDE_ROWS; r += 8) {
+    };
+    fetch(blockIdx.x);
+    int buffer = 0;
+    for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x, buffer ^= 1) {
+        float* dz_s = wide_s + buffer * 2 * WIDE_ROWS * WIDE_DS;
+        float* x_s = dz_s + WIDE_ROWS * WIDE_DS;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            dz_s[(r_first + 2 * i) * WIDE_DS + c] = next_d[i];
+            x_s[(r_first + 2 * i) * WIDE_DS + c] = next_x[i];
+        }
+        __syncthreads();   // (nobody writes this buffer again before everybody has passed the next barrier)
+        fetch(tile + gridDim.x);
+        if (!works) continue;
+        u32 d_at = shared_address(dz_s) + (t * WIDE_DS + c0 + g) * 4, x_at = shared_address(x_s) + (t * WIDE_DS + m0 + g) * 4;
+#pragma unroll 1
+        for (int r = 0; r < WIDE_ROWS; r += 8, d_at += 8 * WIDE_DS * 4, x_at += 8 * WIDE_DS * 4) {
             u32 b_hi[4][2], b_lo[4][2];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const float v0 = dz_s[(r + t) * WIDE_DS + c0 + 8 * j + g], v1 = dz_s[(r + t + 4) * WIDE_DS + c0 + 8 * j + g];
+                const float v0 = lds(d_at + 32 * j), v1 = lds(d_at + 4 * WIDE_DS * 4 + 32 * j);
                 sums[j] += v0 + v1;
                 split(v0, b_hi[j][0], b_lo[j][0]);
                 split(v1, b_hi[j][1], b_lo[j][1]);
@@ -570,21 +594,20 @@ __global__ void __launch_bounds__(256) mix_backward_weights(MixBackArgs a) {
                 if (m0 + 16 * i >= k) break;
                 u32 a_hi[4], a_lo[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    split(x_s[(r + t + (e & 2 ? 4 : 0)) * WIDE_XS + m0 + 16 * i + g + (e & 1 ? 8 : 0)], a_hi[e], a_lo[e]);
+                for (int e = 0; e < 4; e++) {
+                    const float v = lds(x_at + (e & 2 ? 4 : 0) * WIDE_DS * 4 + 64 * i + (e & 1 ? 32 : 0));
+                    if (split_x) split(v, a_hi[e], a_lo[e]);
+                    else a_hi[e] = __float_as_uint(v);
+                }
                 float part[4][4];
 #pragma unroll
-                for (int j = 0; j < 4; j++)
+                for (int j = 0; j < 4; j++) mma8_first(part[j], a_hi, b_hi[j]);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) part[j][e] = 0.f;
+                for (int j = 0; j < 4; j++) mma8(part[j], a_hi, b_lo[j]);
                 if (split_x) {
 #pragma unroll
                     for (int j = 0; j < 4; j++) mma8(part[j], a_lo, b_hi[j]);
                 }
-#pragma unroll
-                for (int j = 0; j < 4; j++) mma8(part[j], a_hi, b_lo[j]);
-#pragma unroll
-                for (int j = 0; j < 4; j++) mma8(part[j], a_hi, b_hi[j]);
 #pragma unroll
                 for (int j = 0; j < 4; j++)
 #pragma unroll
@@ -601,8 +624,8 @@ __global__ void __launch_bounds__(256) mix_backward_weights(MixBackArgs a) {
         for (int j = 0; j < 4; j++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const int r = m0 + 16 * i + g + (e & 2 ? 8 : 0), c = c0 + 8 * j + 2 * t + (e & 1);
-                if (r < k && c < n) rows[r * n + c] = acc[i][j][e];
+                const int row = m0 + 16 * i + g + (e & 2 ? 8 : 0), col = c0 + 8 * j + 2 * t + (e & 1);
+                if (row < k && col < n) rows[row * n + col] = acc[i][j][e];
             }
     if (second || m0) return;
 #pragma unroll
@@ -610,8 +633,8 @@ __global__ void __launch_bounds__(256) mix_backward_weights(MixBackArgs a) {
         float v = sums[j];
         v += __shfl_xor_sync(~0u, v, 1);
         v += __shfl_xor_sync(~0u, v, 2);
-        const int c = c0 + 8 * j + g;
-        if (t == 0 && c < n) share[(size_t)(a.k + a.k2) * n + c] = v;
+        const int col = c0 + 8 * j + g;
+        if (t == 0 && col < n) share[(size_t)(a.k + a.k2) * n + col] = v;
     }
 }
 

@@ -3,6 +3,7 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 #include "common.cuh"
 
 namespace pl {
@@ -44,6 +45,19 @@ __device__ __forceinline__ void mma8_first(float (&c)[4], const u32 (&a)[4], con
     asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
+}
+// Two 16-bit values a register, m16n8k16, products exact and sums in float: a: channels 2t, 2t + 1 of rows g and g + 8, then 2t + 8, 2t + 9;
+// b: rows 2t, 2t + 1 of column g, then 2t + 8, 2t + 9.
+template <typename T>
+__device__ __forceinline__ void mma16(float (&c)[4], const u32 (&a)[4], const u32 (&b)[2]) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 __device__ __forceinline__ void split(float v, u32& hi, u32& lo) {
     hi = (__float_as_uint(v) + 0x1000u) & 0xFFFFE000u;
@@ -233,6 +247,16 @@ __device__ __forceinline__ u32 shared_address(const void* p) { return (u32)__cvt
 __device__ __forceinline__ float lds(u32 at) {
     float v;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ u32 lds_u32(u32 at) {
+    u32 v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ u32 lds_u16(u32 at) {
+    u16 v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
     return v;
 }
 template <typename T>

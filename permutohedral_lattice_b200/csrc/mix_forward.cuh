@@ -10,7 +10,7 @@
 namespace pl {
 
 #ifndef MIXF_C
-#define MIXF_C (NT <= 4 ? 4 : 2)
+#define MIXF_C (NT <= 4 ? 4 : WAY == MIX_PAIRS ? 3 : 2)
 #endif
 struct MixArgs {
     long long rows;
@@ -26,13 +26,21 @@ struct MixArgs {
 
 __host__ __device__ constexpr int up8(int v) { return (v + 7) & ~7; }
 __host__ __device__ constexpr size_t up16(size_t v) { return (v + 15) & ~(size_t)15; }
-// Weights in shared memory: blocks of 8 x 8 as the lanes take them, with up to 32 output channels both terms of each (see mix_common.cuh).
-__host__ __device__ constexpr bool mix_both_terms(int nt) { return nt <= 4; }
-__host__ __device__ constexpr int mix_block_bytes(int nt) { return mix_both_terms(nt) ? 512 : 256; }
-__host__ __device__ constexpr size_t mix_weight_bytes(int nt, int rows) { return (size_t)rows / 8 * nt * mix_block_bytes(nt); }
+// How the products are made.  Plain and parted: m16n8k8 on terms of floats, parted adds up eight channels' products before they
+// join the sums (see mix_product8).  Pairs: m16n8k16, for 16-bit values times weights of the same type.
+enum MixWay { MIX_PLAIN, MIX_PARTED, MIX_PAIRS };
+
+// Weights in shared memory: blocks of 8 (16 in pairs) x 8 as the lanes take them, both terms of each with up to 32 output channels
+// (see mix_common.cuh).
+__host__ __device__ constexpr bool mix_both_terms(int nt, int way) { return nt <= 4 && way != MIX_PAIRS; }
+__host__ __device__ constexpr int mix_block_bytes(int nt, int way) { return mix_both_terms(nt, way) ? 512 : 256; }
+__host__ __device__ constexpr int mix_step(int way) { return way == MIX_PAIRS ? 16 : 8; }   // channels of one product
+__host__ __device__ constexpr int up_to(int v, int m) { return (v + m - 1) / m * m; }
+__host__ __device__ constexpr size_t mix_weight_bytes(int nt, int way, int rows) { return (size_t)rows / mix_step(way) * nt * mix_block_bytes(nt, way); }
 // The first of the bytes of row r, column c.
-__host__ __device__ constexpr int mix_weight_at(int nt, int r, int c) {
-    return ((r >> 3) * nt + (c >> 3)) * mix_block_bytes(nt) + (4 * (c & 7) + (r & 3)) * (mix_block_bytes(nt) / 32) + 4 * (r >> 2 & 1);
+__host__ __device__ constexpr int mix_weight_at(int nt, int way, int r, int c) {
+    return way == MIX_PAIRS ? ((r >> 4) * nt + (c >> 3)) * 256 + (4 * (c & 7) + (r >> 1 & 3)) * 8 + 4 * (r >> 3 & 1) + 2 * (r & 1)
+                            : ((r >> 3) * nt + (c >> 3)) * mix_block_bytes(nt, way) + (4 * (c & 7) + (r & 3)) * (mix_block_bytes(nt, way) / 32) + 4 * (r >> 2 & 1);
 }
 // Column blocks all of whose channels are there, whatever n: those of up to 64 channels are compiled one by one.
 __host__ __device__ constexpr int mix_full_blocks(int nt) { return nt <= 8 ? nt - 1 : nt / 2; }
@@ -40,9 +48,9 @@ __host__ __device__ constexpr int mix_full_blocks(int nt) { return nt <= 8 ? nt 
 template <typename TI, typename TO>
 struct MixSmem {   // byte offsets; a stage holds `rows` rows of x, x2 and of the residual, in whose place the output leaves
     size_t weights, bias, stage0, x2_at, r_at, stage_bytes;
-    __host__ __device__ MixSmem(int rows, int k, int k2, int n, int nt) {
+    __host__ __device__ MixSmem(int rows, int k, int k2, int n, int nt, int way) {
         weights = up16(sizeof(u64) * MIX_WARPS * MIX_STAGES);   // barriers before
-        bias = up16(weights + mix_weight_bytes(nt, up8(k) + up8(k2)));
+        bias = up16(weights + mix_weight_bytes(nt, way, up_to(k, mix_step(way)) + up_to(k2, mix_step(way))));
         stage0 = up16(bias + sizeof(float) * 8 * nt);
         x2_at = up16(sizeof(TI) * (size_t)rows * k);
         r_at = x2_at + up16(sizeof(TI) * (size_t)rows * k2);
@@ -51,29 +59,38 @@ struct MixSmem {   // byte offsets; a stage holds `rows` rows of x, x2 and of th
     __host__ __device__ size_t bytes(int warps, int stages) const { return stage0 + stage_bytes * stages * warps; }
 };
 
-// acc += eight channels of a block's rows times eight weight rows, which begin at w.  rows: where the lane's rows begin at its channel.
-// PARTS: their products by themselves, then added to the sums as floats are.  The tensor cores cut what they add to: of
-// sums of more than a hundred terms that cancel (128 labels: dz W^T) it cost 1.6 bits.
-template <typename TI, int NT, int MT, bool PARTS, bool EDGE>
-__device__ __forceinline__ void mix_product8(float (&acc)[MT][NT][4], const u32 (&rows)[2 * MT], int left, u32 w, bool split_w) {
-    constexpr int JG = NT % 4 == 0 ? 4 : NT % 3 == 0 ? 3 : NT % 2 == 0 ? 2 : NT == 1 ? 1 : NT;
+// The left side of a product of eight channels, as it is: those of the lane's 2 MT rows, which begin (at its channel) at rows[].
+template <typename TI, int MT>
+__device__ __forceinline__ void mix_load_left(float (&v)[MT][4], const u32 (&rows)[2 * MT], int left) {
     const int t = threadIdx.x & 3;
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[m][i] = 0.f;   // behind the last channel lies another row, which may hold NaN
+            if (t + (i & 2 ? 4 : 0) < left) v[m][i] = lds_value<TI>(rows[2 * m + (i & 1)] + (i & 2 ? 4 : 0) * sizeof(TI));
+        }
+}
+// acc += the left side times eight weight rows, which begin at w.
+// PARTS: the products by themselves, then added to the sums as floats are.  The tensor cores cut what they add to: of
+// sums of more than a hundred terms that cancel (128 labels: dz W^T) it cost 1.6 bits.
+template <typename TI, int NT, int MT, bool PARTS>
+__device__ __forceinline__ void mix_product8(float (&acc)[MT][NT][4], const float (&v)[MT][4], u32 w, bool split_w) {
+    constexpr int JG = NT % 4 == 0 ? 4 : NT % 3 == 0 ? 3 : NT % 2 == 0 ? 2 : NT == 1 ? 1 : NT;
     u32 a_hi[MT][4], a_lo[MT][4];
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            float v = 0.f;
-            if (!EDGE || t + (i & 2 ? 4 : 0) < left) v = lds_value<TI>(rows[2 * m + (i & 1)] + (i & 2 ? 4 : 0) * sizeof(TI));   // behind lies another row, which may hold NaN
-            if constexpr (sizeof(TI) == 4) split(v, a_hi[m][i], a_lo[m][i]);
-            else a_hi[m][i] = __float_as_uint(v);
+            if constexpr (sizeof(TI) == 4) split(v[m][i], a_hi[m][i], a_lo[m][i]);
+            else a_hi[m][i] = __float_as_uint(v[m][i]);
         }
 #pragma unroll
     for (int j0 = 0; j0 < NT; j0 += JG) {
         u32 b_hi[JG][2], b_lo[JG][2];
 #pragma unroll
         for (int j = 0; j < JG; j++) {
-            if constexpr (mix_both_terms(NT)) {
+            if constexpr (mix_both_terms(NT, MIX_PLAIN)) {
                 const uint4 b = lds4(w + 512 * (j0 + j));
                 b_hi[j][0] = b.x, b_hi[j][1] = b.y, b_lo[j][0] = b.z, b_lo[j][1] = b.w;
             } else {
@@ -106,30 +123,137 @@ __device__ __forceinline__ void mix_product8(float (&acc)[MT][NT][4], const u32 
         }
     }
 }
-// All k channels of the rows that begin at x_at.
+// All k channels of the rows that begin at x_at; the next eight are loaded while eight are multiplied.
 template <typename TI, int NT, int MT, bool PARTS>
 __device__ __forceinline__ void mix_products(float (&acc)[MT][NT][4], u32 x_at, int k, u32 w, bool split_w) {
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
     u32 rows[2 * MT];
 #pragma unroll
     for (int m = 0; m < 2 * MT; m++) rows[m] = x_at + ((8 * m + g) * k + t) * sizeof(TI);
-    int left = k;
+    float next[MT][4];
+    mix_load_left<TI, MT>(next, rows, k);
 #pragma unroll 1
-    for (; left >= 8; left -= 8, w += NT * mix_block_bytes(NT)) {
-        mix_product8<TI, NT, MT, PARTS, false>(acc, rows, 8, w, split_w);
+    for (int left = k; left > 0; w += NT * mix_block_bytes(NT, MIX_PLAIN)) {
+        float v[MT][4];
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[m][i] = next[m][i];
 #pragma unroll
         for (int m = 0; m < 2 * MT; m++) rows[m] += 8 * sizeof(TI);
+        left -= 8;
+        if (left > 0) mix_load_left<TI, MT>(next, rows, left);
+        mix_product8<TI, NT, MT, PARTS>(acc, v, w, split_w);
     }
-    if (left) mix_product8<TI, NT, MT, PARTS, true>(acc, rows, left, w, split_w);
+}
+// The same in pairs.  A row of an odd number of 16-bit values begins between words: its pairs are put together.
+template <typename TI, int MT>
+__device__ __forceinline__ void mix_load_pairs(u32 (&v)[MT][4], const u32 (&rows)[2 * MT], int left, bool words) {
+    const int t = threadIdx.x & 3;
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int c = 2 * t + (i & 2 ? 8 : 0);
+            const u32 at = rows[2 * m + (i & 1)] + (i & 2 ? 16 : 0);
+            v[m][i] = 0;   // behind the last channel lies another row, which may hold NaN
+            if (words) {
+                if (c < left) v[m][i] = lds_u32(at);
+            } else {
+                if (c < left) v[m][i] = lds_u16(at);
+                if (c + 1 < left) v[m][i] |= lds_u16(at + 2) << 16;
+            }
+        }
+}
+template <typename TI, int NT, int MT>
+__device__ __forceinline__ void mix_products_of_pairs(float (&acc)[MT][NT][4], u32 x_at, int k, u32 w) {
+    const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+    const bool words = k % 2 == 0;
+    u32 rows[2 * MT];
+#pragma unroll
+    for (int m = 0; m < 2 * MT; m++) rows[m] = x_at + ((8 * m + g) * k + 2 * t) * 2;
+    u32 next[MT][4];
+    mix_load_pairs<TI, MT>(next, rows, k, words);
+#pragma unroll 1
+    for (int left = k; left > 0; w += NT * 256) {
+        u32 v[MT][4];
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[m][i] = next[m][i];
+#pragma unroll
+        for (int m = 0; m < 2 * MT; m++) rows[m] += 32;
+        left -= 16;
+        if (left > 0) mix_load_pairs<TI, MT>(next, rows, left, words);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const uint2 b = lds2(w + 256 * j);
+            const u32 both[2] = {b.x, b.y};
+#pragma unroll
+            for (int m = 0; m < MT; m++) mma16<TI>(acc[m][j], v[m], both);
+        }
+    }
 }
 
-template <typename TI, typename TO, int NT, int MT, bool PARTS>
+// Columns 8 (j / 2) + 2 t + j % 2 of R rows, four lanes a row.  A channel that is not there, of the blocks that may have some: never the
+// largest, nothing in a sum.
+template <int NT>
+__device__ __forceinline__ bool mix_there(int j, int n) {
+    return j / 2 < mix_full_blocks(NT) || 8 * (j / 2) + 2 * (int)(threadIdx.x & 3) + (j & 1) < n;
+}
+template <int R, int NT>
+__device__ __forceinline__ void mix_activate(float (&z)[R][2 * NT], int activation, int n) {
+    if (activation == PL_ACT_SOFTMAX) {
+        constexpr float LOG2_E = 1.4426950408889634f;
+        float top[R], den[R];
+#pragma unroll
+        for (int m = 0; m < R; m++) top[m] = -INFINITY, den[m] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2 * NT; j++)
+#pragma unroll
+            for (int m = 0; m < R; m++) {
+                if (!mix_there<NT>(j, n)) z[m][j] = -INFINITY;
+                top[m] = fmaxf(top[m], z[m][j]);
+            }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1)
+#pragma unroll
+            for (int m = 0; m < R; m++) top[m] = fmaxf(top[m], __shfl_xor_sync(~0u, top[m], o));
+#pragma unroll
+        for (int m = 0; m < R; m++)
+            if (top[m] == -INFINITY) top[m] = 0.f;   // nothing allowed: zeros (a NaN among them stays one)
+#pragma unroll
+        for (int j = 0; j < 2 * NT; j++)
+#pragma unroll
+            for (int m = 0; m < R; m++) {
+                z[m][j] = exp2_approx((z[m][j] - top[m]) * LOG2_E);   // (in one step the type's least value would overflow)
+                den[m] += z[m][j];
+            }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1)
+#pragma unroll
+            for (int m = 0; m < R; m++) den[m] += __shfl_xor_sync(~0u, den[m], o);
+#pragma unroll
+        for (int m = 0; m < R; m++) {
+            const float inv = den[m] == 0.f ? 0.f : __fdividef(1.f, den[m]);   // (1 to 128: the quick quotient is within a step)
+#pragma unroll
+            for (int j = 0; j < 2 * NT; j++) z[m][j] *= inv;
+        }
+    } else if (activation == PL_ACT_RELU) {
+#pragma unroll
+        for (int m = 0; m < R; m++)
+#pragma unroll
+            for (int j = 0; j < 2 * NT; j++) z[m][j] = z[m][j] < 0.f ? 0.f : z[m][j];
+    }
+}
+
+template <typename TI, typename TO, int NT, int MT, int WAY>
 __global__ void __launch_bounds__(128, MIXF_C) mix_forward(MixArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
     constexpr int BLOCK = 16 * MT;
     const int warps = (int)blockDim.x / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tile_rows = BLOCK * a.blocks, k = a.k, k2 = a.k2, n = a.n, stages = a.stages;
-    const MixSmem<TI, TO> at(tile_rows, k, k2, n, NT);
+    const MixSmem<TI, TO> at(tile_rows, k, k2, n, NT, WAY);
     u64* bars = reinterpret_cast<u64*>(smem) + MIX_STAGES * warp;
     float* bias_s = reinterpret_cast<float*>(smem + at.bias);
     unsigned char* stage0 = smem + at.stage0 + at.stage_bytes * stages * warp;
@@ -164,16 +288,18 @@ __global__ void __launch_bounds__(128, MIXF_C) mix_forward(MixArgs a) {
     for (int s = 0; s < stages; s++) fetch(first + s * step, s);
 
     // the weights, zeros behind the last channel of either side, while the first tiles arrive
-    const int kp = up8(k);
-    for (int i = threadIdx.x; i < (kp + up8(k2)) * 8 * NT; i += blockDim.x) {
+    const int kp = up_to(k, mix_step(WAY));
+    for (int i = threadIdx.x; i < (kp + up_to(k2, mix_step(WAY))) * 8 * NT; i += blockDim.x) {
         const int r = i / (8 * NT), c = i - r * (8 * NT);
         const bool second = r >= kp;
         const int j = second ? r - kp : r;
         float v = 0.f;
         if (c < n && j < (second ? k2 : k))
             v = load_weight(second ? a.weight2 : a.weight, a.transposed ? c * k + j : j * n + c, a.weight_dtype);
-        unsigned char* to = smem + at.weights + mix_weight_at(NT, r, c);
-        if constexpr (mix_both_terms(NT)) {
+        unsigned char* to = smem + at.weights + mix_weight_at(NT, WAY, r, c);
+        if constexpr (WAY == MIX_PAIRS) {
+            *reinterpret_cast<TI*>(to) = from_float<TI>(v);
+        } else if constexpr (mix_both_terms(NT, WAY)) {
             u32 hi, lo;
             split(v, hi, lo);
             reinterpret_cast<u32*>(to)[0] = hi, reinterpret_cast<u32*>(to)[2] = lo;
@@ -185,7 +311,7 @@ __global__ void __launch_bounds__(128, MIXF_C) mix_forward(MixArgs a) {
     __syncthreads();
 
     const int g = lane >> 2, t = lane & 3;
-    const u32 w_at = shared_address(smem + at.weights) + lane * (mix_block_bytes(NT) / 32);
+    const u32 w_at = shared_address(smem + at.weights) + lane * (mix_block_bytes(NT, WAY) / 32);
     const bool split_w = a.weight_dtype == PL_F32, bulk_out = aligned16(a.out);
     bool alive = true;
     int s = 0, parity = 0;
@@ -210,59 +336,45 @@ __global__ void __launch_bounds__(128, MIXF_C) mix_forward(MixArgs a) {
                 for (int m = 0; m < MT; m++) acc[m][j][0] = acc[m][j][2] = b.x, acc[m][j][1] = acc[m][j][3] = b.y;
             }
 #pragma unroll 1
-            for (int second = 0; second < (k2 ? 2 : 1); second++)
-                mix_products<TI, NT, MT, PARTS>(acc, second ? stage_at + (u32)at.x2_at + r0 * k2 * sizeof(TI) : stage_at + r0 * k * sizeof(TI), second ? k2 : k,
-                                                second ? w_at + kp / 8 * NT * mix_block_bytes(NT) : w_at, split_w);
+            for (int second = 0; second < (k2 ? 2 : 1); second++) {
+                const int width = second ? k2 : k;
+                const u32 x_at = stage_at + (second ? (u32)at.x2_at : 0) + r0 * width * sizeof(TI);
+                const u32 w = w_at + (second ? kp / mix_step(WAY) * NT * mix_block_bytes(NT, WAY) : 0);
+                if constexpr (WAY == MIX_PAIRS) mix_products_of_pairs<TI, NT, MT>(acc, x_at, width, w);
+                else mix_products<TI, NT, MT, WAY == MIX_PARTED>(acc, x_at, width, w, split_w);
+            }
+            // The lane's 2 MT rows, 8 m + g of the block: z[m].
+            constexpr int R = 2 * MT;
+            const int row = (r0 + g) * n + 2 * t;
+            const u32 r_at = stage_at + (u32)at.r_at + row * sizeof(TI), to = stage_at + (u32)at.r_at + row * sizeof(TO);
+            float z[R][2 * NT];
 #pragma unroll
-            for (int m = 0; m < MT; m++)
+            for (int m = 0; m < R; m++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) {   // rows g and g + 8 of the sixteen
-                    // A channel that is not there, of the blocks that may have some: never the largest, nothing in a sum.
-                    auto there = [&](int j) { return j / 2 < mix_full_blocks(NT) || 8 * (j / 2) + 2 * t + (j & 1) < n; };
-                    const int row = (r0 + 16 * m + 8 * h + g) * n + 2 * t;
-                    const u32 r_at = stage_at + (u32)at.r_at + row * sizeof(TI), to = stage_at + (u32)at.r_at + row * sizeof(TO);
-                    float z[2 * NT];
+                for (int j = 0; j < 2 * NT; j++) z[m][j] = acc[m / 2][j / 2][2 * (m & 1) + (j & 1)];
+            if (residual) {
 #pragma unroll
-                    for (int j = 0; j < 2 * NT; j++) z[j] = acc[m][j / 2][2 * h + (j & 1)];
-                    if (residual) {
+                for (int j = 0; j < 2 * NT; j++)
+                    if (mix_there<NT>(j, n)) {
 #pragma unroll
-                        for (int j = 0; j < 2 * NT; j++)
-                            if (there(j)) z[j] = fmaf(a.scale, lds_value<TI>(r_at + (8 * (j / 2) + (j & 1)) * sizeof(TI)), z[j]);
+                        for (int m = 0; m < R; m++)
+                            z[m][j] = fmaf(a.scale, lds_value<TI>(r_at + (8 * m * n + 8 * (j / 2) + (j & 1)) * sizeof(TI)), z[m][j]);
                     }
-                    if (a.activation == PL_ACT_SOFTMAX) {
-                        constexpr float LOG2_E = 1.4426950408889634f;
-                        float top = -INFINITY, den = 0.f;
+            }
+            mix_activate<R, NT>(z, a.activation, n);
+            if (!alive) {
 #pragma unroll
-                        for (int j = 0; j < 2 * NT; j++) {
-                            if (!there(j)) z[j] = -INFINITY;
-                            top = fmaxf(top, z[j]);
-                        }
-                        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-                        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                        if (top == -INFINITY) top = 0.f;   // nothing allowed: zeros (a NaN among them stays one)
+                for (int m = 0; m < R; m++)
 #pragma unroll
-                        for (int j = 0; j < 2 * NT; j++) {
-                            z[j] = exp2_approx((z[j] - top) * LOG2_E);   // (in one step the type's least value would overflow)
-                            den += z[j];
-                        }
-                        den += __shfl_xor_sync(~0u, den, 1);
-                        den += __shfl_xor_sync(~0u, den, 2);
-                        const float inv = den == 0.f ? 0.f : __fdividef(1.f, den);   // (1 to 128: the quick quotient is within a step)
+                    for (int j = 0; j < 2 * NT; j++) z[m][j] = NAN;   // gave up: nothing that could pass for a result
+            }
+            // The output goes where the residual was: each lane has read the values at the places that it writes.  With an output of
+            // fewer bytes than the input there is no residual.
 #pragma unroll
-                        for (int j = 0; j < 2 * NT; j++) z[j] *= inv;
-                    } else if (a.activation == PL_ACT_RELU) {
+            for (int j = 0; j < 2 * NT; j++)
+                if (mix_there<NT>(j, n)) {
 #pragma unroll
-                        for (int j = 0; j < 2 * NT; j++) z[j] = z[j] < 0.f ? 0.f : z[j];
-                    }
-                    if (!alive) {
-#pragma unroll
-                        for (int j = 0; j < 2 * NT; j++) z[j] = NAN;   // nothing that could pass for a result
-                    }
-                    // The output goes where the residual was.  Each lane has read the values at the places that it writes; with
-                    // an output of fewer bytes than the input there is no residual.
-#pragma unroll
-                    for (int j = 0; j < 2 * NT; j++)
-                        if (there(j)) sts_value<TO>(to + (8 * (j / 2) + (j & 1)) * sizeof(TO), z[j]);
+                    for (int m = 0; m < R; m++) sts_value<TO>(to + (8 * m * n + 8 * (j / 2) + (j & 1)) * sizeof(TO), z[m][j]);
                 }
             if constexpr (MT == 2) {   // whole blocks: 32 rows of any number of channels
                 const long long row0 = tile0 + r0;
@@ -292,6 +404,106 @@ __global__ void __launch_bounds__(128, MIXF_C) mix_forward(MixArgs a) {
     }
     if (!alive)   // gave up once: no copy may be in flight when the CTA ends
         for (int i = 0; i < stages; i++) mbar_wait(&bars[i], 0), mbar_wait(&bars[i], 1);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Many channels out (65 and more) of float rows.  The weights of both inputs take up to 128 KB of shared memory, which leaves too
+// little for whole rows: a warp takes 16 rows, 32 channels at a time, by way of its registers (the next ones are on their way while
+// these are multiplied), reads the residual and writes its rows from registers.  Bound by the tensor cores: three products of 11-bit
+// terms for one of floats, 276 TFLOP/s of them.
+// ---------------------------------------------------------------------------------------------
+constexpr int WIDE_WARPS = 12, WIDE_CHUNK = 32, WIDE_STRIDE = WIDE_CHUNK + 4;   // (rows of 36 floats: 8 rows by 4 channels in 32 banks)
+constexpr int WIDE_NT = 16;
+__host__ __device__ constexpr size_t wide_smem(int k, int k2) {
+    return mix_weight_bytes(WIDE_NT, MIX_PARTED, up8(k) + up8(k2)) + sizeof(float) * (8 * WIDE_NT + WIDE_WARPS * 16 * WIDE_STRIDE);
+}
+template <typename TO>
+__global__ void __launch_bounds__(32 * WIDE_WARPS, 1) mix_forward_wide(MixArgs a) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    constexpr int NT = WIDE_NT;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int k = a.k, k2 = a.k2, n = a.n, kp = up8(k), all_p = kp + up8(k2);
+    float* bias_s = reinterpret_cast<float*>(smem + mix_weight_bytes(NT, MIX_PARTED, all_p));
+    float* rows_s = bias_s + 8 * NT + warp * 16 * WIDE_STRIDE;
+    for (int i = threadIdx.x; i < all_p * 8 * NT; i += blockDim.x) {
+        const int r = i / (8 * NT), c = i - r * (8 * NT);
+        const bool second = r >= kp;
+        const int j = second ? r - kp : r;
+        float v = 0.f;
+        if (c < n && j < (second ? k2 : k))
+            v = load_weight(second ? a.weight2 : a.weight, a.transposed ? c * k + j : j * n + c, a.weight_dtype);
+        *reinterpret_cast<float*>(smem + mix_weight_at(NT, MIX_PARTED, r, c)) = v;
+    }
+    for (int i = threadIdx.x; i < 8 * NT; i += blockDim.x) bias_s[i] = a.bias && i < n ? load_weight(a.bias, i, a.weight_dtype) : 0.f;
+    __syncthreads();
+    const float* x = static_cast<const float*>(a.x);
+    const float* x2 = static_cast<const float*>(a.x2);
+    const float* residual = static_cast<const float*>(a.residual);
+    TO* out = static_cast<TO*>(a.out);
+    const u32 w_at = shared_address(smem) + lane * 8, rows_at = shared_address(rows_s);
+    const bool split_w = a.weight_dtype == PL_F32;
+    const int chunks = (k + WIDE_CHUNK - 1) / WIDE_CHUNK, all = chunks + (k2 + WIDE_CHUNK - 1) / WIDE_CHUNK;
+    const long long tiles = (a.rows + 15) / 16, step = (long long)gridDim.x * WIDE_WARPS;
+    float next[16];
+    auto fetch = [&](long long tile, int chunk) {   // a channel a lane, 16 rows
+        const bool second = chunk >= chunks;
+        const int width = second ? k2 : k, c = (second ? chunk - chunks : chunk) * WIDE_CHUNK + lane;
+        const float* from = (second ? x2 : x) + tile * 16 * width + c;
+        const int here = tile < tiles && c < width ? (int)min(16ll, a.rows - tile * 16) : 0;
+#pragma unroll
+        for (int r = 0; r < 16; r++) next[r] = r < here ? from[(long long)r * width] : 0.f;
+    };
+    long long tile = (long long)blockIdx.x * WIDE_WARPS + warp;
+    fetch(tile, 0);
+    for (; tile < tiles; tile += step) {
+        float acc[1][NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const float2 b = *reinterpret_cast<const float2*>(bias_s + 8 * j + 2 * t);
+            acc[0][j][0] = acc[0][j][2] = b.x, acc[0][j][1] = acc[0][j][3] = b.y;
+        }
+#pragma unroll 1
+        for (int chunk = 0; chunk < all; chunk++) {
+            __syncwarp();
+#pragma unroll
+            for (int r = 0; r < 16; r++) rows_s[r * WIDE_STRIDE + lane] = next[r];
+            __syncwarp();
+            if (chunk + 1 < all) fetch(tile, chunk + 1);
+            else fetch(tile + step, 0);
+            const bool second = chunk >= chunks;
+            const int c0 = (second ? chunk - chunks : chunk) * WIDE_CHUNK, left = (second ? k2 : k) - c0;
+            u32 w = w_at + ((second ? kp : 0) + c0) / 8 * NT * 256;
+            u32 rows[2] = {rows_at + (g * WIDE_STRIDE + t) * 4, rows_at + ((8 + g) * WIDE_STRIDE + t) * 4};
+#pragma unroll 1
+            for (int c = 0; c < min(left, WIDE_CHUNK); c += 8, w += NT * 256) {
+                float v[1][4];
+                mix_load_left<float, 1>(v, rows, 8);   // (zeros behind the last channel)
+                rows[0] += 32, rows[1] += 32;
+                mix_product8<float, NT, 1, true>(acc, v, w, split_w);
+            }
+        }
+        float z[2][2 * NT];
+        const long long row0 = tile * 16 + g;
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            const long long at = (row0 + 8 * m) * n + 2 * t;
+            const bool row_there = row0 + 8 * m < a.rows;
+#pragma unroll
+            for (int j = 0; j < 2 * NT; j++) {
+                z[m][j] = acc[0][j / 2][2 * m + (j & 1)];
+                if (residual && row_there && mix_there<NT>(j, n)) z[m][j] = fmaf(a.scale, residual[at + 8 * (j / 2) + (j & 1)], z[m][j]);
+            }
+        }
+        mix_activate<2, NT>(z, a.activation, n);
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            const long long at = (row0 + 8 * m) * n + 2 * t;
+            if (row0 + 8 * m >= a.rows) continue;
+#pragma unroll
+            for (int j = 0; j < 2 * NT; j++)
+                if (mix_there<NT>(j, n)) out[at + 8 * (j / 2) + (j & 1)] = from_float<TO>(z[m][j]);
+        }
+    }
 }
 
 }  // namespace pl
