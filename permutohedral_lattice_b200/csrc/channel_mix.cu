@@ -19,6 +19,7 @@
 #include "mix_common.cuh"
 #include "mix_forward.cuh"
 #include "mix_backward.cuh"
+#include "mix_tiny.cuh"
 
 namespace pl {
 
@@ -198,8 +199,29 @@ static int launch_forward_wide(const MixArgs& a, cudaStream_t st) {
     PL_CUDA(cudaGetLastError());
     return PL_OK;
 }
+// Channels of every operand where they are the same, 2 or 4, and all rows begin at multiples of their size; else 0.
+static int tiny_channels(int k, int k2, int n, size_t size, const void* const* rows, int count) {
+    if (k != n || (k2 && k2 != n) || (n != 2 && n != 4)) return 0;
+    for (int i = 0; i < count; i++)
+        if (!aligned(rows[i], n * size)) return 0;
+    return n;
+}
+static bool tiny(int k, int k2, int n) { return k <= TINY && k2 <= TINY && n <= TINY; }
 template <typename TI, typename TO>
 static int forward_any(const MixArgs& a, cudaStream_t st) {
+    if constexpr (std::is_same<TI, TO>::value) {
+        if (tiny(a.k, a.k2, a.n)) {
+            const unsigned grid = grid_for(a.rows, 256 * TINY_ROWS, 4);
+            const void* rows[] = {a.x, a.x2, a.residual, a.out};
+            const int v = tiny_channels(a.k, a.k2, a.n, sizeof(TI), rows, 4);
+            if (v == 4) mix_tiny<TI, 4><<<grid, 256, 0, st>>>(a);
+            else if (v == 2) mix_tiny<TI, 2><<<grid, 256, 0, st>>>(a);
+            else mix_tiny<TI, 0><<<grid, 256, 0, st>>>(a);
+            PL_COUNT_LAUNCHES(1);
+            PL_CUDA(cudaGetLastError());
+            return PL_OK;
+        }
+    }
     if constexpr (sizeof(TI) == 4) {
         if (a.n > 64) return launch_forward_wide<TO>(a, st);
     }
@@ -285,6 +307,17 @@ static int launch_wide(const MixBackArgs& a, const pl_mix_gradients& d, cudaStre
 template <typename T>
 static int launch_back(const pl_mix* m, const MixBackArgs& a, const pl_mix_gradients& d, cudaStream_t st) {
     if (!narrow(m)) return launch_wide<T>(a, d, st);
+    if (tiny(a.k, a.k2, a.n)) {
+        const unsigned ctas = grid_for(a.rows, 256 * TINY_BACK_ROWS, 2);
+        const void* rows[] = {a.grad, a.out.full, a.x.full, a.x2.full, a.dx, a.dx2, a.dresidual};
+        const int v = tiny_channels(a.k, a.k2, a.n, sizeof(T), rows, 7);
+        if (v == 4) mix_tiny_backward<T, 4><<<ctas, 256, 0, st>>>(a);
+        else if (v == 2) mix_tiny_backward<T, 2><<<ctas, 256, 0, st>>>(a);
+        else mix_tiny_backward<T, 0><<<ctas, 256, 0, st>>>(a);
+        PL_COUNT_LAUNCHES(1);
+        PL_CUDA(cudaGetLastError());
+        return a.shares ? add_shares(a, d, (int)ctas, st) : PL_OK;
+    }
     return a.out.codes || a.x.codes || a.x2.codes ? narrow_any<T, true>(a, d, st) : narrow_any<T, false>(a, d, st);
 }
 

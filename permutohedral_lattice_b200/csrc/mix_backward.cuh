@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(128, MIXB_C) mix_backward(MixBackArgs a) {
             }
             // dx and dx2, CH blocks of eight channels at a time, to where x and x2 were
             if (a.dx || a.dx2) {
-                constexpr int CH = MB == 3 ? 6 : MB == 1 ? 2 : 5;
+                constexpr int CH = MB == 3 ? (PACKED ? 3 : 6) : MB == 1 ? 2 : 5;
                 const int blocks = all_p / 8;
 #pragma unroll 1
                 for (int c0 = a.dx ? 0 : kp / 8; c0 < (a.dx2 ? blocks : kp / 8); c0 += CH) {
@@ -549,7 +549,10 @@ __global__ void __launch_bounds__(256, 1) mix_backward_weights(MixBackArgs a) {
         }
     const long long tiles = (a.rows + WIDE_ROWS - 1) / WIDE_ROWS;
     const int c = threadIdx.x & 127, r_first = threadIdx.x >> 7;   // this thread's channel, and the first of its rows: every second
+    // In 8 bits, rows of whole words: four channels at a time, of every eighth row.
+    const bool words = from.codes && k % 4 == 0 && (reinterpret_cast<uintptr_t>(from.codes) & 3) == 0;
     float next_d[16], next_x[16];
+    u32 next_c[4], next_h[4];
     auto fetch = [&](long long tile) {
         const long long row0 = tile * WIDE_ROWS + r_first;
 #pragma unroll
@@ -558,9 +561,18 @@ __global__ void __launch_bounds__(256, 1) mix_backward_weights(MixBackArgs a) {
             const bool there = row < a.rows;
             next_d[i] = there && c < n ? a.dz[row * n + c] : 0.f;
             next_x[i] = 0.f;
-            if (there && want && c < k) {
+            if (!words && there && want && c < k) {
                 const long long at = row * k + c;
                 next_x[i] = from.codes ? decode_value(from.codes[at], (u32)(u16)from.scales[at / PACK_BLOCK]) : to_float(static_cast<const T*>(from.full)[at]);
+            }
+        }
+        if (words) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const long long row = tile * WIDE_ROWS + warp + 8 * i, at = row * k + 4 * lane;
+                const bool there = row < a.rows && want && 4 * lane < k;
+                next_c[i] = there ? *reinterpret_cast<const u32*>(from.codes + at) : 0;
+                next_h[i] = there ? (u32)(u16)from.scales[at / PACK_BLOCK] : 1;
             }
         }
     };
@@ -572,7 +584,15 @@ __global__ void __launch_bounds__(256, 1) mix_backward_weights(MixBackArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             dz_s[(r_first + 2 * i) * WIDE_DS + c] = next_d[i];
-            x_s[(r_first + 2 * i) * WIDE_DS + c] = next_x[i];
+            if (!words) x_s[(r_first + 2 * i) * WIDE_DS + c] = next_x[i];
+        }
+        if (words) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float v[4];
+                decode4(v, next_c[i], next_h[i]);
+                store4(x_s + (warp + 8 * i) * WIDE_DS + 4 * lane, v);
+            }
         }
         __syncthreads();   // (nobody writes this buffer again before everybody has passed the next barrier)
         fetch(tile + gridDim.x);
