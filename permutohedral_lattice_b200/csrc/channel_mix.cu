@@ -29,36 +29,26 @@ template <typename T>
 __global__ void __launch_bounds__(256) pack_blocks(uint8_t* __restrict__ codes, int16_t* __restrict__ scales,
                                                    const T* __restrict__ x, long long n, int keep_nonzero, int wide) {
     const int lane = threadIdx.x & 31;
-    int at[2];
-    runs_of_lane(at[0], at[1]);
+    int first, second;
+    runs_of_lane(first, second);
     const long long step = (long long)gridDim.x * 2048;
     for (long long i0 = (long long)blockIdx.x * 2048 + (threadIdx.x >> 5) * 256; i0 < n; i0 += step) {   // (the same for a warp)
-        float v[8];
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const long long i = i0 + at[u];
-            float q[4];
-            if (wide && i + 3 < n) load4(q, x + i);
-            else
-#pragma unroll
-                for (int j = 0; j < 4; j++) q[j] = i + j < n ? to_float(x[i + j]) : 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; j++) v[4 * u + j] = q[j];
+        if (!wide || i0 + 256 > n) {
+            pack_rest(x + i0, (int)min(256ll, n - i0), codes + i0, scales + i0 / PACK_BLOCK, keep_nonzero != 0);
+            continue;
         }
+        float v[8], q[4];
+        load4(q, x + i0 + first);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = q[i];
+        load4(q, x + i0 + second);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[4 + i] = q[i];
         u32 header;
         const uint2 c = encode8(v, header, keep_nonzero != 0);
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const long long i = i0 + at[u];
-            const u32 w = u ? c.y : c.x;
-            if (wide && i + 3 < n) *reinterpret_cast<u32*>(codes + i) = w;
-            else
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (i + j < n) codes[i + j] = (uint8_t)(w >> (8 * j));
-        }
-        const long long b = i0 / PACK_BLOCK + (lane >> 2);
-        if ((lane & 3) == 0 && b * PACK_BLOCK < n) scales[b] = (int16_t)header;
+        *reinterpret_cast<u32*>(codes + i0 + first) = c.x;
+        *reinterpret_cast<u32*>(codes + i0 + second) = c.y;
+        if ((lane & 3) == 0) scales[i0 / PACK_BLOCK + (lane >> 2)] = (int16_t)header;
     }
 }
 

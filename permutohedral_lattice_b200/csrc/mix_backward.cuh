@@ -186,33 +186,37 @@ __global__ void __launch_bounds__(128, MIXB_C) mix_backward(MixBackArgs a) {
 #pragma unroll 1
         for (int r0 = 0; r0 < rows_here; r0 += 32) {
             const int here = min(32, rows_here - r0);
-            // 32 rows from 8 bits to floats; rows that are not there to zeros
+            // 32 rows to floats, from 8 bits eight lanes a block; rows that are not there to zeros.
             auto decode = [&](float* to, const Kept& p, const unsigned char* place, const u32* heads, int most, int c) {
-                const int count = here * c;
-                const T* values = reinterpret_cast<const T*>(place) + r0 * c;
-                for (int i0 = 0; i0 < 32 * c; i0 += 128) {
-                    const int i = i0 + 4 * lane;
-                    if (p.codes) {
-                        const int b = r0 / 32 * c + i / 32;
+                float* w = to + 4 * lane;
+                int left = c - lane / 8;   // blocks, from this lane's on
+                if (p.codes) {
+                    const u32* codes = reinterpret_cast<const u32*>(place + r0 * c) + lane;
+                    int b = r0 / 32 * c + lane / 8;
+                    for (int i = 0; i < c; i += 4, left -= 4, b += 4, w += 128, codes += 32) {
                         u32 head = __shfl_sync(~0u, heads[0], b);
-                        if (most > 1 && a.blocks * c > 32) {
+                        if (most > 1 && c > 32) {
                             const u32 second = __shfl_sync(~0u, heads[most > 1 ? 1 : 0], b), third = __shfl_sync(~0u, heads[most > 2 ? 2 : 0], b);
                             head = b < 32 ? head : b < 64 ? second : third;
                         }
-                        if (i >= 32 * c) continue;
-                        float v[4];
-                        decode4(v, *reinterpret_cast<const u32*>(place + r0 * c + i), head);
-                        if (here < 32) {
-#pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                if (i + e >= count) v[e] = 0.f;
+                        if (left > 0) {
+                            float v[4];
+                            decode4(v, *codes, head);
+                            store4(w, v);
                         }
-                        store4(to + i, v);
-                    } else if (i < 32 * c) {
-                        float v[4];
-                        load4(v, values + i);
-                        store4(to + i, v);
                     }
+                } else {
+                    const T* values = reinterpret_cast<const T*>(place) + r0 * c + 4 * lane;
+                    for (int i = 0; i < c; i += 4, left -= 4, w += 128, values += 128)
+                        if (left > 0) {
+                            float v[4];
+                            load4(v, values);
+                            store4(w, v);
+                        }
+                }
+                if (here < 32) {
+                    __syncwarp();
+                    for (int i = here * c + lane; i < 32 * c; i += 32) to[i] = 0.f;
                 }
             };
             float* work = reinterpret_cast<float*>(own + at.work_at);
