@@ -149,7 +149,7 @@ static MixLaunch mix_launch(long long rows, int block_rows, size_t block_bytes, 
 
 template <typename TI, typename TO, int NT, int MT, int WAY>
 static int launch_forward(MixArgs a, cudaStream_t st) {
-    const MixLaunch l = mix_launch(a.rows, 16 * MT, 16 * MT * (sizeof(TI) * (a.k + a.k2 + (a.residual ? a.n : 0)) + sizeof(TO) * a.n), 6, MIX_STAGES, 8,
+    const MixLaunch l = mix_launch(a.rows, 16 * MT, 16 * MT * (sizeof(TI) * (a.k + a.k2 + (a.residual ? a.n : 0)) + sizeof(TO) * a.n), mix_forward_ctas(NT, WAY), MIX_STAGES, 8,
                                    [&](int warps, int stages, int blocks) {
                                        return MixSmem<TI, TO>(16 * MT * blocks, a.k, a.k2, a.n, NT, WAY).bytes(warps, stages);
                                    });
@@ -223,7 +223,7 @@ static int forward_any(const MixArgs& a, cudaStream_t st) {
     return forward_of<TI, TO, MIX_PARTED>(a, st);
 }
 
-constexpr int BACK_CTAS = 4;   // of an SM, at most: as many shares of dW there may be
+constexpr int BACK_CTAS = 3;   // of an SM, at most: as many shares of dW there may be
 static bool narrow(const pl_mix* m) { return up8(m->k) + up8(m->k2) <= 80 && m->n <= 32; }
 static size_t shares_bytes(const pl_mix* m) {
     return up16(sizeof(float) * (size_t)(m->k + m->k2 + 1) * m->n * num_sms() * BACK_CTAS);
@@ -246,7 +246,7 @@ template <typename T, bool PACKED, int MB, int NB>
 static int launch_narrow(MixBackArgs a, const pl_mix_gradients& d, cudaStream_t st) {
     // in 8 bits: one stage, and as many blocks of rows as give 32 headers of each array (see mix_backward)
     const int widest = std::max(a.n, std::max(a.k, a.k2));
-    const MixLaunch l = mix_launch(a.rows, 32, 32 * sizeof(T) * (2 * a.n + 2 * (a.k + a.k2)), BACK_CTAS, PACKED ? 1 : MIX_STAGES,
+    const MixLaunch l = mix_launch(a.rows, 32, 32 * sizeof(T) * (2 * a.n + 2 * (a.k + a.k2)), MB * NB > 12 ? 2 : BACK_CTAS, PACKED ? 1 : MIX_STAGES,
                                    PACKED ? std::max(1, 32 / widest) : 8, [&](int warps, int stages, int blocks) {
                                        MixBackArgs b = a;
                                        b.blocks = blocks, b.stages = stages;

@@ -14,9 +14,6 @@
 
 namespace pl {
 
-#ifndef MIXB_C
-#define MIXB_C (MB * NB > 12 ? 2 : 3)
-#endif
 struct Kept {   // an activation as it was, or in 8 bits
     const void* full;
     const uint8_t* codes;
@@ -69,7 +66,7 @@ struct MixBackSmem {
 // PACKED: some of the output, x and x2 come in 8 bits; all are then read from floats of the warp's own memory.  One stage, and the
 // headers of its blocks in registers: there are at most 32 of the output and 96 of x or x2 in a tile (see narrow_any).
 template <typename T, bool PACKED, int MB, int NB>
-__global__ void __launch_bounds__(128, MIXB_C) mix_backward(MixBackArgs a) {
+__global__ void __launch_bounds__(32 * MIX_WARPS, MB * NB > 12 ? 2 : 3) mix_backward(MixBackArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
     typedef typename std::conditional<PACKED, float, T>::type TX;   // of the rows that are worked on
     const int warps = (int)blockDim.x / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -235,12 +232,15 @@ __global__ void __launch_bounds__(128, MIXB_C) mix_backward(MixBackArgs a) {
             for (int p = 0; p < 4; p++)
 #pragma unroll
                 for (int j = 0; j < J; j++) {
-                    d[p][j] = y[p][j] = 0.f;
-                    if (4 * j + t < n) {
-                        d[p][j] = lds_value<T>(g_row + (8 * p * n + 4 * j) * sizeof(T));
-                        if (reads_y) y[p][j] = lds_value<TX>(y_row + (8 * p * n + 4 * j) * sizeof(TX));
-                    }
+                    d[p][j] = lds_value_if<T>(4 * j + t < n, g_row + (8 * p * n + 4 * j) * sizeof(T));
+                    y[p][j] = 0.f;
                 }
+            if (reads_y) {
+#pragma unroll
+                for (int p = 0; p < 4; p++)
+#pragma unroll
+                    for (int j = 0; j < J; j++) y[p][j] = lds_value_if<TX>(4 * j + t < n, y_row + (8 * p * n + 4 * j) * sizeof(TX));
+            }
             if (a.activation == PL_ACT_SOFTMAX) {
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -275,15 +275,13 @@ __global__ void __launch_bounds__(128, MIXB_C) mix_backward(MixBackArgs a) {
                 for (int p = 0; p < 4; p++)
 #pragma unroll
                     for (int j = 0; j < J; j++)
-                        sts_value<float>(dz_at + (p * NB + j / 2) * MIX_DZ_BLOCK + (4 * (4 * (j & 1) + t) + (g & 3)) * 8 + 4 * (g >> 2), d[p][j]);
+                        sts(dz_at + (p * NB + j / 2) * MIX_DZ_BLOCK + (4 * (4 * (j & 1) + t) + (g & 3)) * 8 + 4 * (g >> 2), d[p][j]);
             }
             if (a.dresidual) {
 #pragma unroll
                 for (int j = 0; j < J; j++)
-                    if (4 * j + t < n) {
 #pragma unroll
-                        for (int p = 0; p < 4; p++) sts_value<T>(g_row + (8 * p * n + 4 * j) * sizeof(T), a.scale * d[p][j]);   // (where this lane has read)
-                    }
+                    for (int p = 0; p < 4; p++) sts_value_if<T>(4 * j + t < n, g_row + (8 * p * n + 4 * j) * sizeof(T), a.scale * d[p][j]);   // (where this lane has read)
             }
             if constexpr (PACKED) {
                 __syncwarp();
@@ -416,11 +414,9 @@ __global__ void __launch_bounds__(128, MIXB_C) mix_backward(MixBackArgs a) {
                         const u32 to = (second ? x2_at : x_at) + (g * width + c) * sizeof(T);
 #pragma unroll
                         for (int e = 0; e < 2; e++)
-                            if (c + e < width) {
 #pragma unroll
-                                for (int m = 0; m < 4; m++)
-                                    sts_value<T>(to + (8 * m * width + e) * sizeof(T), part[m / 2][j][2 * (m & 1) + e]);
-                            }
+                            for (int m = 0; m < 4; m++)
+                                sts_value_if<T>(c + e < width, to + (8 * m * width + e) * sizeof(T), part[m / 2][j][2 * (m & 1) + e]);
                     }
                 }
             }

@@ -265,15 +265,25 @@ __device__ __forceinline__ float lds(u32 at) {
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
     return v;
 }
-__device__ __forceinline__ u32 lds_u32(u32 at) {
+// The accesses of which some lanes have none are predicated here: as branches around them they took a quarter of all instructions.
+__device__ __forceinline__ u32 lds_u32_if(bool there, u32 at) {
     u32 v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.shared.u32 %0, [%1];\n\t}" : "=&r"(v) : "r"(at), "r"((int)there));
     return v;
 }
-__device__ __forceinline__ u32 lds_u16(u32 at) {
+__device__ __forceinline__ u32 lds_u16_if(bool there, u32 at) {
     u16 v;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b16 %0, 0;\n\t@p ld.shared.u16 %0, [%1];\n\t}" : "=&h"(v) : "r"(at), "r"((int)there));
     return v;
+}
+template <typename T>
+__device__ __forceinline__ float value_of_bits(u32 bits) {
+    if constexpr (sizeof(T) == 4) {
+        return __uint_as_float(bits);
+    } else {
+        const u16 half = (u16)bits;
+        return to_float(*reinterpret_cast<const T*>(&half));
+    }
 }
 template <typename T>
 __device__ __forceinline__ float lds_value(u32 at) {
@@ -282,8 +292,13 @@ __device__ __forceinline__ float lds_value(u32 at) {
     } else {
         u16 bits;
         asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(at));
-        return to_float(*reinterpret_cast<T*>(&bits));
+        return value_of_bits<T>(bits);
     }
+}
+template <typename T>
+__device__ __forceinline__ float lds_value_if(bool there, u32 at) {   // else zero
+    if constexpr (sizeof(T) == 4) return value_of_bits<T>(lds_u32_if(there, at));
+    else return value_of_bits<T>(lds_u16_if(there, at));
 }
 __device__ __forceinline__ uint4 lds4(u32 at) {
     uint4 v;
@@ -296,14 +311,16 @@ __device__ __forceinline__ uint2 lds2(u32 at) {
     return v;
 }
 template <typename T>
-__device__ __forceinline__ void sts_value(u32 at, float v) {
+__device__ __forceinline__ void sts_value_if(bool there, u32 at, float v) {
     if constexpr (sizeof(T) == 4) {
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p st.shared.f32 [%0], %1;\n\t}" ::"r"(at), "f"(v), "r"((int)there) : "memory");
     } else {
         T h = from_float<T>(v);
-        asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(*reinterpret_cast<u16*>(&h)) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p st.shared.u16 [%0], %1;\n\t}" ::"r"(at), "h"(*reinterpret_cast<u16*>(&h)), "r"((int)there) : "memory");
     }
 }
+__device__ __forceinline__ void sts(u32 at, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
+
 // A warp's finished rows from shared to global memory: one bulk copy, or plain stores.  Lane 0 waits later (bulk_wait_read).
 template <typename T>
 __device__ __forceinline__ void copy_out(T* to, const T* from, int count, bool bulk) {

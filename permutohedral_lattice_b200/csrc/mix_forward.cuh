@@ -9,9 +9,6 @@
 
 namespace pl {
 
-#ifndef MIXF_C
-#define MIXF_C (NT <= 4 ? 4 : WAY == MIX_PAIRS ? 3 : 2)
-#endif
 struct MixArgs {
     long long rows;
     int k, k2, n, activation;
@@ -42,6 +39,8 @@ __host__ __device__ constexpr int mix_weight_at(int nt, int way, int r, int c) {
     return way == MIX_PAIRS ? ((r >> 4) * nt + (c >> 3)) * 256 + (4 * (c & 7) + (r >> 1 & 3)) * 8 + 4 * (r >> 3 & 1) + 2 * (r & 1)
                             : ((r >> 3) * nt + (c >> 3)) * mix_block_bytes(nt, way) + (4 * (c & 7) + (r & 3)) * (mix_block_bytes(nt, way) / 32) + 4 * (r >> 2 & 1);
 }
+// CTAs of four warps that an SM's registers have to hold.
+__host__ __device__ constexpr int mix_forward_ctas(int nt, int way) { return nt <= 4 ? 4 : way == MIX_PAIRS ? 3 : 2; }
 // Column blocks all of whose channels are there, whatever n: those of up to 64 channels are compiled one by one.
 __host__ __device__ constexpr int mix_full_blocks(int nt) { return nt <= 8 ? nt - 1 : nt / 2; }
 
@@ -66,10 +65,8 @@ __device__ __forceinline__ void mix_load_left(float (&v)[MT][4], const u32 (&row
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[m][i] = 0.f;   // behind the last channel lies another row, which may hold NaN
-            if (t + (i & 2 ? 4 : 0) < left) v[m][i] = lds_value<TI>(rows[2 * m + (i & 1)] + (i & 2 ? 4 : 0) * sizeof(TI));
-        }
+        for (int i = 0; i < 4; i++)   // (behind the last channel lies another row, which may hold NaN)
+            v[m][i] = lds_value_if<TI>(t + (i & 2 ? 4 : 0) < left, rows[2 * m + (i & 1)] + (i & 2 ? 4 : 0) * sizeof(TI));
 }
 // acc += the left side times eight weight rows, which begin at w.
 // PARTS: the products by themselves, then added to the sums as floats are.  The tensor cores cut what they add to: of
@@ -156,13 +153,8 @@ __device__ __forceinline__ void mix_load_pairs(u32 (&v)[MT][4], const u32 (&rows
         for (int i = 0; i < 4; i++) {
             const int c = 2 * t + (i & 2 ? 8 : 0);
             const u32 at = rows[2 * m + (i & 1)] + (i & 2 ? 16 : 0);
-            v[m][i] = 0;   // behind the last channel lies another row, which may hold NaN
-            if (words) {
-                if (c < left) v[m][i] = lds_u32(at);
-            } else {
-                if (c < left) v[m][i] = lds_u16(at);
-                if (c + 1 < left) v[m][i] |= lds_u16(at + 2) << 16;
-            }
+            if (words) v[m][i] = lds_u32_if(c < left, at);   // (behind the last channel lies another row, which may hold NaN)
+            else v[m][i] = lds_u16_if(c < left, at) | lds_u16_if(c + 1 < left, at + 2) << 16;
         }
 }
 template <typename TI, int NT, int MT>
@@ -248,7 +240,7 @@ __device__ __forceinline__ void mix_activate(float (&z)[R][2 * NT], int activati
 }
 
 template <typename TI, typename TO, int NT, int MT, int WAY>
-__global__ void __launch_bounds__(128, MIXF_C) mix_forward(MixArgs a) {
+__global__ void __launch_bounds__(32 * MIX_WARPS, mix_forward_ctas(NT, WAY)) mix_forward(MixArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
     constexpr int BLOCK = 16 * MT;
     const int warps = (int)blockDim.x / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -355,11 +347,9 @@ __global__ void __launch_bounds__(128, MIXF_C) mix_forward(MixArgs a) {
             if (residual) {
 #pragma unroll
                 for (int j = 0; j < 2 * NT; j++)
-                    if (mix_there<NT>(j, n)) {
 #pragma unroll
-                        for (int m = 0; m < R; m++)
-                            z[m][j] = fmaf(a.scale, lds_value<TI>(r_at + (8 * m * n + 8 * (j / 2) + (j & 1)) * sizeof(TI)), z[m][j]);
-                    }
+                    for (int m = 0; m < R; m++)
+                        z[m][j] = fmaf(a.scale, lds_value_if<TI>(mix_there<NT>(j, n), r_at + (8 * m * n + 8 * (j / 2) + (j & 1)) * sizeof(TI)), z[m][j]);
             }
             mix_activate<R, NT>(z, a.activation, n);
             if (!alive) {
@@ -372,10 +362,8 @@ __global__ void __launch_bounds__(128, MIXF_C) mix_forward(MixArgs a) {
             // fewer bytes than the input there is no residual.
 #pragma unroll
             for (int j = 0; j < 2 * NT; j++)
-                if (mix_there<NT>(j, n)) {
 #pragma unroll
-                    for (int m = 0; m < R; m++) sts_value<TO>(to + (8 * m * n + 8 * (j / 2) + (j & 1)) * sizeof(TO), z[m][j]);
-                }
+                for (int m = 0; m < R; m++) sts_value_if<TO>(mix_there<NT>(j, n), to + (8 * m * n + 8 * (j / 2) + (j & 1)) * sizeof(TO), z[m][j]);
             if constexpr (MT == 2) {   // whole blocks: 32 rows of any number of channels
                 const long long row0 = tile0 + r0;
                 auto keep = [&](const auto* rows, int c, uint8_t* codes, int16_t* scales, bool nonzero) {
