@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, MB * NB > 12 ? 2 : 3) mix_back
 #pragma unroll
     for (int j = 0; j < NB; j++) sums[j] = 0.f;
 
-    constexpr int J = 2 * NB;   // channels of a row that a lane looks at: every fourth
+    constexpr int J = 2 * NB, FULL = 2 * NB - 2;   // channels of a row that a lane looks at: every fourth; those that are there whatever n is
     bool alive = true;
     int s = 0, parity = 0;
     for (long long tile = first; tile < tiles; tile += step) {
@@ -232,14 +232,18 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, MB * NB > 12 ? 2 : 3) mix_back
             for (int p = 0; p < 4; p++)
 #pragma unroll
                 for (int j = 0; j < J; j++) {
-                    d[p][j] = lds_value_if<T>(4 * j + t < n, g_row + (8 * p * n + 4 * j) * sizeof(T));
+                    const u32 at = g_row + (8 * p * n + 4 * j) * sizeof(T);
+                    d[p][j] = j < FULL ? lds_value<T>(at) : lds_value_if<T>(4 * j + t < n, at);
                     y[p][j] = 0.f;
                 }
             if (reads_y) {
 #pragma unroll
                 for (int p = 0; p < 4; p++)
 #pragma unroll
-                    for (int j = 0; j < J; j++) y[p][j] = lds_value_if<TX>(4 * j + t < n, y_row + (8 * p * n + 4 * j) * sizeof(TX));
+                    for (int j = 0; j < J; j++) {
+                        const u32 at = y_row + (8 * p * n + 4 * j) * sizeof(TX);
+                        y[p][j] = j < FULL ? lds_value<TX>(at) : lds_value_if<TX>(4 * j + t < n, at);
+                    }
             }
             if (a.activation == PL_ACT_SOFTMAX) {
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -281,7 +285,11 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, MB * NB > 12 ? 2 : 3) mix_back
 #pragma unroll
                 for (int j = 0; j < J; j++)
 #pragma unroll
-                    for (int p = 0; p < 4; p++) sts_value_if<T>(4 * j + t < n, g_row + (8 * p * n + 4 * j) * sizeof(T), a.scale * d[p][j]);   // (where this lane has read)
+                    for (int p = 0; p < 4; p++) {   // (where this lane has read)
+                        const u32 at = g_row + (8 * p * n + 4 * j) * sizeof(T);
+                        if (j < FULL) sts_value<T>(at, a.scale * d[p][j]);
+                        else sts_value_if<T>(4 * j + t < n, at, a.scale * d[p][j]);
+                    }
             }
             if constexpr (PACKED) {
                 __syncwarp();
@@ -371,7 +379,7 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, MB * NB > 12 ? 2 : 3) mix_back
             }
             // dx and dx2, CH blocks of eight channels at a time, to where x and x2 were
             if (a.dx || a.dx2) {
-                constexpr int CH = MB == 3 ? (PACKED ? 3 : 6) : MB == 1 ? 2 : 5;
+                constexpr int CH = MB == 3 ? 3 : MB == 1 ? 2 : 5;
                 const int blocks = all_p / 8;
 #pragma unroll 1
                 for (int c0 = a.dx ? 0 : kp / 8; c0 < (a.dx2 ? blocks : kp / 8); c0 += CH) {

@@ -200,33 +200,29 @@ __device__ __noinline__ void pack_rest(const T* values, int count, uint8_t* code
     const int lane = threadIdx.x & 31;
     if ((lane & 3) == 0 && (lane >> 2) * PACK_BLOCK < count) scales[lane >> 2] = (int16_t)header;
 }
-// `count` values in shared memory, whole blocks from the first one on, to 8 bits by one warp.  wide: codes is 4-byte aligned.
-// (All cases in one loop took 150 instructions for 256 values, whole blocks by themselves take 60.)
-template <typename T>
-__device__ __forceinline__ void pack_by_warp(const T* values, int count, uint8_t* __restrict__ codes, int16_t* __restrict__ scales,
-                                             bool keep_nonzero, bool wide) {
-    if (!wide || count % PACK_BLOCK) {
-        for (int i = 0; i < count; i += 256) pack_rest(values + i, min(256, count - i), codes + i, scales + i / PACK_BLOCK, keep_nonzero);
-        return;
-    }
+// `count` values in shared memory, whole blocks from the first one on, to 8 bits by one warp: where(i) says where the i-th lies (four from
+// a multiple of four on lie together).  wide: codes is 4-byte aligned and the blocks are whole.  (All cases in one loop took 150 instructions
+// for 256 values, whole blocks by themselves take 60.)
+template <typename T, typename Where>
+__device__ __forceinline__ void pack_blocks_of(const T* values, int count, uint8_t* __restrict__ codes, int16_t* __restrict__ scales, bool keep_nonzero,
+                                               Where where) {
     const int lane = threadIdx.x & 31;
     int first, second;
     runs_of_lane(first, second);
-    const T *v0 = values + first, *v1 = values + second;
     uint8_t *c0 = codes + first, *c1 = codes + second;
     int16_t* head = scales + (lane >> 2);
     int left = count / PACK_BLOCK - (lane >> 2);   // blocks, from this lane's on
-    for (int b = 0; b < count / PACK_BLOCK; b += 8, left -= 8, v0 += 256, v1 += 256, c0 += 256, c1 += 256, head += 8) {
+    for (int i = 0; i < count; i += 256, left -= 8, c0 += 256, c1 += 256, head += 8) {
         float v[8], q[4];
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = 0.f;
+        for (int e = 0; e < 8; e++) v[e] = 0.f;
         if (left > 0) {
-            load4(q, v0);
+            load4(q, values + where(i + first));
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = q[i];
-            load4(q, v1);
+            for (int e = 0; e < 4; e++) v[e] = q[e];
+            load4(q, values + where(i + second));
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[4 + i] = q[i];
+            for (int e = 0; e < 4; e++) v[4 + e] = q[e];
         }
         u32 header;
         const uint2 c = encode8(v, header, keep_nonzero);
@@ -237,16 +233,56 @@ __device__ __forceinline__ void pack_by_warp(const T* values, int count, uint8_t
         }
     }
 }
+template <typename T>
+__device__ __forceinline__ void pack_by_warp(const T* values, int count, uint8_t* __restrict__ codes, int16_t* __restrict__ scales,
+                                             bool keep_nonzero, bool wide) {
+    if (wide && count % PACK_BLOCK == 0) pack_blocks_of(values, count, codes, scales, keep_nonzero, [](int i) { return i; });
+    else
+        for (int i = 0; i < count; i += 256) pack_rest(values + i, min(256, count - i), codes + i, scales + i / PACK_BLOCK, keep_nonzero);
+}
 
 // ---------------------------------------------------------------------------------------------
 // Tiles.  Every warp has its own: some rows of every operand, contiguous in memory whatever the number of channels, in a stage
 // of shared memory of its own, fetched and sent out by bulk copies (one lane asks for them), the results in the place of what
 // has been read.  Warps share the weights of their CTA and nothing else, and meet nobody at a tile.  What does not start on a
 // 16-byte boundary, and the last rows, are copied by the lanes.
+//
+// Rows of 32, 64, ... 512 bytes would begin in the same few banks, and eight of them are read together (64 channels of 16 bits: up
+// to 8 accesses for one, 259 us a forward pass over a million rows, so 113).  They lie 16 bytes further apart and are copied by the lanes,
+// 16 bytes each.
 // ---------------------------------------------------------------------------------------------
 constexpr int MIX_WARPS = 4, MIX_STAGES = 2;   // of a CTA and of a warp, at most
 
 __device__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Values of `c` channels from one row to the next in shared memory: whether rows lie apart (RowsApart) is asked for by the caller, who knows
+// that they are 16-byte aligned in memory.
+struct RowsApart {
+    int stride, shift;   // elements; log2 of the channels, or -1: one after another
+    __host__ __device__ RowsApart(int c, int size, bool aligned) : stride(c), shift(-1) {
+        const int bytes = c * size;
+        if (!aligned || bytes < 32 || (bytes & (bytes - 1))) return;
+        stride = c + 16 / size;
+        shift = 0;
+        while (1 << shift < c) shift++;
+    }
+    __host__ __device__ bool apart() const { return shift >= 0; }
+    __device__ __forceinline__ int at(int i) const { return shift < 0 ? i : i + (i >> shift) * (stride - (1 << shift)); }   // of element i
+};
+template <typename T>
+__device__ __forceinline__ void copy_rows_in(T* to, const T* from, int rows, const RowsApart& r) {   // there after the group's wait
+    constexpr int PER = 16 / sizeof(T);
+    const int lane = threadIdx.x & 31, count = rows << r.shift;
+    for (int i = lane * PER; i < count; i += 32 * PER) cp_async16(to + r.at(i), from + i);
+}
+template <typename T>
+__device__ __forceinline__ void copy_rows_out(T* to, const T* from, int rows, const RowsApart& r) {
+    constexpr int PER = 16 / sizeof(T);
+    const int lane = threadIdx.x & 31, count = rows << r.shift;
+    for (int i = lane * PER; i < count; i += 32 * PER) *reinterpret_cast<uint4*>(to + i) = *reinterpret_cast<const uint4*>(from + r.at(i));
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_async_wait_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }   // one group may be on its way
 
 // A warp copies `count` elements to shared memory; they are there after cp_async_wait_all and __syncwarp.
 template <typename E>
@@ -317,6 +353,15 @@ __device__ __forceinline__ void sts_value_if(bool there, u32 at, float v) {
     } else {
         T h = from_float<T>(v);
         asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p st.shared.u16 [%0], %1;\n\t}" ::"r"(at), "h"(*reinterpret_cast<u16*>(&h)), "r"((int)there) : "memory");
+    }
+}
+template <typename T>
+__device__ __forceinline__ void sts_value(u32 at, float v) {
+    if constexpr (sizeof(T) == 4) {
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+    } else {
+        T h = from_float<T>(v);
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(*reinterpret_cast<u16*>(&h)) : "memory");
     }
 }
 __device__ __forceinline__ void sts(u32 at, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }

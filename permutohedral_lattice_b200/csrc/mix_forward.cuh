@@ -16,7 +16,8 @@ struct MixArgs {
     const void *x, *x2, *weight, *weight2, *bias, *residual;
     void* out;
     int weight_dtype, transposed;      // transposed: weight is [n][k] (no second input)
-    int stages, blocks;                // blocks of 16 MT rows in a tile
+    int blocks;                        // of 16 MT rows in a tile
+    int x_apart, x2_apart, out_apart;  // rows may lie apart in shared memory (see RowsApart): x, x2, residual and out
     uint8_t *x_codes, *x2_codes, *out_codes;
     int16_t *x_scales, *x2_scales, *out_scales;
 };
@@ -45,43 +46,51 @@ __host__ __device__ constexpr int mix_forward_ctas(int nt, int way) { return nt 
 __host__ __device__ constexpr int mix_full_blocks(int nt) { return nt <= 8 ? nt - 1 : nt / 2; }
 
 template <typename TI, typename TO>
-struct MixSmem {   // byte offsets; a stage holds `rows` rows of x, x2 and of the residual, in whose place the output leaves
+struct MixSmem {   // byte offsets; a stage holds the tile's rows of x, x2 and of the residual, in whose place the output leaves
+    RowsApart x, x2, out;
     size_t weights, bias, stage0, x2_at, r_at, stage_bytes;
-    __host__ __device__ MixSmem(int rows, int k, int k2, int n, int nt, int way) {
-        weights = up16(sizeof(u64) * MIX_WARPS * MIX_STAGES);   // barriers before
-        bias = up16(weights + mix_weight_bytes(nt, way, up_to(k, mix_step(way)) + up_to(k2, mix_step(way))));
+    __host__ __device__ MixSmem(const MixArgs& a, int rows, int nt, int way)
+        : x(a.k, sizeof(TI), a.x_apart), x2(a.k2, sizeof(TI), a.x2_apart), out(a.n, sizeof(TO), a.out_apart) {
+        weights = up16(sizeof(u64) * 2 * MIX_WARPS);   // barriers before
+        bias = up16(weights + mix_weight_bytes(nt, way, up_to(a.k, mix_step(way)) + up_to(a.k2, mix_step(way))));
         stage0 = up16(bias + sizeof(float) * 8 * nt);
-        x2_at = up16(sizeof(TI) * (size_t)rows * k);
-        r_at = x2_at + up16(sizeof(TI) * (size_t)rows * k2);
-        stage_bytes = up16(r_at + (sizeof(TI) > sizeof(TO) ? sizeof(TI) : sizeof(TO)) * (size_t)rows * n);
+        x2_at = up16(sizeof(TI) * (size_t)rows * x.stride);
+        r_at = x2_at + up16(sizeof(TI) * (size_t)rows * x2.stride);
+        stage_bytes = up16(r_at + sizeof(TO) * (size_t)rows * out.stride);   // (a residual has the output's type)
     }
-    __host__ __device__ size_t bytes(int warps, int stages) const { return stage0 + stage_bytes * stages * warps; }
+    __host__ __device__ size_t bytes(int warps) const { return stage0 + stage_bytes * warps; }
 };
 
-// The left side of a product of eight channels, as it is: those of the lane's 2 MT rows, which begin (at its channel) at rows[].
-template <typename TI, int MT>
+// The left side of a product of eight channels: those of the lane's 2 MT rows, which begin (at its channel) at rows[].  EDGE: fewer are left;
+// behind them lies another row, which may hold NaN.
+template <typename TI, int MT, bool EDGE>
 __device__ __forceinline__ void mix_load_left(float (&v)[MT][4], const u32 (&rows)[2 * MT], int left) {
     const int t = threadIdx.x & 3;
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)   // (behind the last channel lies another row, which may hold NaN)
-            v[m][i] = lds_value_if<TI>(t + (i & 2 ? 4 : 0) < left, rows[2 * m + (i & 1)] + (i & 2 ? 4 : 0) * sizeof(TI));
+        for (int i = 0; i < 4; i++) {
+            const u32 at = rows[2 * m + (i & 1)] + (i & 2 ? 4 : 0) * sizeof(TI);
+            if constexpr (EDGE) v[m][i] = lds_value_if<TI>(t + (i & 2 ? 4 : 0) < left, at);
+            else v[m][i] = lds_value<TI>(at);
+        }
+}
+template <typename TI, int MT>
+__device__ __forceinline__ void mix_split_left(u32 (&hi)[MT][4], u32 (&lo)[MT][4], const float (&v)[MT][4]) {
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (sizeof(TI) == 4) split(v[m][i], hi[m][i], lo[m][i]);
+            else hi[m][i] = __float_as_uint(v[m][i]);
+        }
 }
 // acc += the left side times eight weight rows, which begin at w.
 // PARTS: the products by themselves, then added to the sums as floats are.  The tensor cores cut what they add to: of
 // sums of more than a hundred terms that cancel (128 labels: dz W^T) it cost 1.6 bits.
 template <typename TI, int NT, int MT, bool PARTS>
-__device__ __forceinline__ void mix_product8(float (&acc)[MT][NT][4], const float (&v)[MT][4], u32 w, bool split_w) {
+__device__ __forceinline__ void mix_product8(float (&acc)[MT][NT][4], const u32 (&a_hi)[MT][4], const u32 (&a_lo)[MT][4], u32 w, bool split_w) {
     constexpr int JG = NT % 4 == 0 ? 4 : NT % 3 == 0 ? 3 : NT % 2 == 0 ? 2 : NT == 1 ? 1 : NT;
-    u32 a_hi[MT][4], a_lo[MT][4];
-#pragma unroll
-    for (int m = 0; m < MT; m++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if constexpr (sizeof(TI) == 4) split(v[m][i], a_hi[m][i], a_lo[m][i]);
-            else a_hi[m][i] = __float_as_uint(v[m][i]);
-        }
 #pragma unroll
     for (int j0 = 0; j0 < NT; j0 += JG) {
         u32 b_hi[JG][2], b_lo[JG][2];
@@ -122,25 +131,24 @@ __device__ __forceinline__ void mix_product8(float (&acc)[MT][NT][4], const floa
 }
 // All k channels of the rows that begin at x_at; the next eight are loaded while eight are multiplied.
 template <typename TI, int NT, int MT, bool PARTS>
-__device__ __forceinline__ void mix_products(float (&acc)[MT][NT][4], u32 x_at, int k, u32 w, bool split_w) {
+__device__ __forceinline__ void mix_products(float (&acc)[MT][NT][4], u32 x_at, int k, int stride, u32 w, bool split_w) {
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
     u32 rows[2 * MT];
 #pragma unroll
-    for (int m = 0; m < 2 * MT; m++) rows[m] = x_at + ((8 * m + g) * k + t) * sizeof(TI);
+    for (int m = 0; m < 2 * MT; m++) rows[m] = x_at + ((8 * m + g) * stride + t) * sizeof(TI);
     float next[MT][4];
-    mix_load_left<TI, MT>(next, rows, k);
+    if (k >= 8) mix_load_left<TI, MT, false>(next, rows, k);
+    else mix_load_left<TI, MT, true>(next, rows, k);
 #pragma unroll 1
     for (int left = k; left > 0; w += NT * mix_block_bytes(NT, MIX_PLAIN)) {
-        float v[MT][4];
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[m][i] = next[m][i];
+        u32 a_hi[MT][4], a_lo[MT][4];
+        mix_split_left<TI, MT>(a_hi, a_lo, next);
 #pragma unroll
         for (int m = 0; m < 2 * MT; m++) rows[m] += 8 * sizeof(TI);
         left -= 8;
-        if (left > 0) mix_load_left<TI, MT>(next, rows, left);
-        mix_product8<TI, NT, MT, PARTS>(acc, v, w, split_w);
+        if (left >= 8) mix_load_left<TI, MT, false>(next, rows, left);
+        else if (left > 0) mix_load_left<TI, MT, true>(next, rows, left);
+        mix_product8<TI, NT, MT, PARTS>(acc, a_hi, a_lo, w, split_w);
     }
 }
 // The same in pairs.  A row of an odd number of 16-bit values begins between words: its pairs are put together.
@@ -158,12 +166,12 @@ __device__ __forceinline__ void mix_load_pairs(u32 (&v)[MT][4], const u32 (&rows
         }
 }
 template <typename TI, int NT, int MT>
-__device__ __forceinline__ void mix_products_of_pairs(float (&acc)[MT][NT][4], u32 x_at, int k, u32 w) {
+__device__ __forceinline__ void mix_products_of_pairs(float (&acc)[MT][NT][4], u32 x_at, int k, int stride, u32 w) {
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
-    const bool words = k % 2 == 0;
+    const bool words = k % 2 == 0;   // (then the stride is even, too)
     u32 rows[2 * MT];
 #pragma unroll
-    for (int m = 0; m < 2 * MT; m++) rows[m] = x_at + ((8 * m + g) * k + 2 * t) * 2;
+    for (int m = 0; m < 2 * MT; m++) rows[m] = x_at + ((8 * m + g) * stride + 2 * t) * 2;
     u32 next[MT][4];
     mix_load_pairs<TI, MT>(next, rows, k, words);
 #pragma unroll 1
@@ -239,45 +247,58 @@ __device__ __forceinline__ void mix_activate(float (&z)[R][2 * NT], int activati
     }
 }
 
-template <typename TI, typename TO, int NT, int MT, int WAY>
+// KEEP: the activations go to 8 bits, too (a kernel of its own: as a branch it cost the others a tenth of their time).
+// A warp has one stage.  Its rows of x and x2 are fetched again as soon as they have been multiplied, while the rows of the tile are
+// finished, those of the residual when the output has left.
+template <typename TI, typename TO, int NT, int MT, int WAY, bool KEEP>
 __global__ void __launch_bounds__(32 * MIX_WARPS, mix_forward_ctas(NT, WAY)) mix_forward(MixArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
     constexpr int BLOCK = 16 * MT;
     const int warps = (int)blockDim.x / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tile_rows = BLOCK * a.blocks, k = a.k, k2 = a.k2, n = a.n, stages = a.stages;
-    const MixSmem<TI, TO> at(tile_rows, k, k2, n, NT, WAY);
-    u64* bars = reinterpret_cast<u64*>(smem) + MIX_STAGES * warp;
+    const int tile_rows = BLOCK * a.blocks, k = a.k, k2 = a.k2, n = a.n;
+    const MixSmem<TI, TO> at(a, tile_rows, NT, WAY);
+    u64* bars = reinterpret_cast<u64*>(smem) + 2 * warp;   // of x and x2, of the residual
     float* bias_s = reinterpret_cast<float*>(smem + at.bias);
-    unsigned char* stage0 = smem + at.stage0 + at.stage_bytes * stages * warp;
+    unsigned char* stage = smem + at.stage0 + at.stage_bytes * warp;
     const TI* x = static_cast<const TI*>(a.x);
     const TI* x2 = static_cast<const TI*>(a.x2);
     const TI* residual = static_cast<const TI*>(a.residual);
     const long long tiles = (a.rows + tile_rows - 1) / tile_rows, step = (long long)gridDim.x * warps;
     const long long first = (long long)blockIdx.x * warps + warp;
-    if (lane == 0)
-        for (int s = 0; s < stages; s++) mbar_init(&bars[s], 1);
+    if (lane == 0) mbar_init(&bars[0], 1), mbar_init(&bars[1], 1);
     __syncwarp();
-    const bool bulk_in = aligned16(x) && (!k2 || aligned16(x2)) && (!residual || aligned16(residual));
-    const u32 tile_bytes = (u32)(tile_rows * (k + k2 + (residual ? n : 0)) * sizeof(TI));
-    auto fetch = [&](long long tile, int s) {
-        unsigned char* stage = stage0 + at.stage_bytes * s;
-        const long long row0 = tile * tile_rows;
-        if (bulk_in && row0 + tile_rows <= a.rows) {
-            if (lane == 0) {
-                mbar_expect_tx(&bars[s], tile_bytes);
-                bulk_load(stage, x + row0 * k, (u32)(tile_rows * k * sizeof(TI)), &bars[s]);
-                if (k2) bulk_load(stage + at.x2_at, x2 + row0 * k2, (u32)(tile_rows * k2 * sizeof(TI)), &bars[s]);
-                if (residual) bulk_load(stage + at.r_at, residual + row0 * n, (u32)(tile_rows * n * sizeof(TI)), &bars[s]);
-            }
-        } else if (row0 < a.rows) {
-            const int here = (int)min((long long)tile_rows, a.rows - row0);
-            copy_in(stage, x + row0 * k, here * k);
-            if (k2) copy_in(stage + at.x2_at, x2 + row0 * k2, here * k2);
-            if (residual) copy_in(stage + at.r_at, residual + row0 * n, here * n);
-            if (lane == 0) mbar_expect_tx(&bars[s], 0);
-        }
+    const bool bulk_x = (at.x.apart() || aligned16(x)) && (!k2 || at.x2.apart() || aligned16(x2)), bulk_r = at.out.apart() || aligned16(residual);
+    const u32 x_bytes = (u32)(tile_rows * sizeof(TI)) * ((at.x.apart() ? 0 : k) + (at.x2.apart() ? 0 : k2));
+    const u32 r_bytes = (u32)(tile_rows * sizeof(TI)) * (at.out.apart() ? 0 : n);
+    auto rows_in = [&](size_t place, const TI* from, int c, const RowsApart& r, int here, bool bulk, u64* bar) {
+        TI* to = reinterpret_cast<TI*>(stage + place);
+        if (r.apart()) copy_rows_in(to, from, here, r);
+        else if (!bulk) copy_in(to, from, here * c);
+        else if (lane == 0) bulk_load(to, from, (u32)(tile_rows * c * sizeof(TI)), bar);
     };
-    for (int s = 0; s < stages; s++) fetch(first + s * step, s);
+    auto fetch_x = [&](long long tile) {
+        const long long row0 = tile * tile_rows;
+        const int here = (int)max(0ll, min((long long)tile_rows, a.rows - row0));
+        const bool bulk = bulk_x && here == tile_rows;
+        if (here) {
+            if (lane == 0) mbar_expect_tx(&bars[0], bulk ? x_bytes : 0);
+            rows_in(0, x + row0 * k, k, at.x, here, bulk, &bars[0]);
+            if (k2) rows_in(at.x2_at, x2 + row0 * k2, k2, at.x2, here, bulk, &bars[0]);
+        }
+        cp_async_commit();
+    };
+    auto fetch_r = [&](long long tile) {
+        const long long row0 = tile * tile_rows;
+        const int here = residual ? (int)max(0ll, min((long long)tile_rows, a.rows - row0)) : 0;
+        const bool bulk = bulk_r && here == tile_rows;
+        if (here) {
+            if (lane == 0) mbar_expect_tx(&bars[1], bulk ? r_bytes : 0);
+            rows_in(at.r_at, residual + row0 * n, n, at.out, here, bulk, &bars[1]);
+        }
+        cp_async_commit();
+    };
+    fetch_x(first);
+    fetch_r(first);
 
     // the weights, zeros behind the last channel of either side, while the first tiles arrive
     const int kp = up_to(k, mix_step(WAY));
@@ -305,18 +326,23 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, mix_forward_ctas(NT, WAY)) mix
     const int g = lane >> 2, t = lane & 3;
     const u32 w_at = shared_address(smem + at.weights) + lane * (mix_block_bytes(NT, WAY) / 32);
     const bool split_w = a.weight_dtype == PL_F32, bulk_out = aligned16(a.out);
+    TO* o_s = reinterpret_cast<TO*>(stage + at.r_at);
+    const u32 stage_at = shared_address(stage);
+    // What has been asked for is there for all lanes; false once it did not come.  (The copies of x and x2 and those of a residual are
+    // committed in turn: one group may be on its way behind the one that is waited for.)
+    auto arrived = [&](u64* bar, int parity, bool before) {
+        cp_async_wait_one();
+        const bool there = before && mbar_wait(bar, parity);
+        const bool all = __all_sync(~0u, there);
+        __syncwarp();
+        return all;
+    };
     bool alive = true;
-    int s = 0, parity = 0;
-    for (long long tile = first; tile < tiles; tile += step) {
-        unsigned char* stage = stage0 + at.stage_bytes * s;
-        cp_async_wait_all();
-        alive = alive && mbar_wait(&bars[s], parity);
-        alive = __all_sync(~0u, alive);
-        __syncwarp();   // what the lanes copied is there for all
+    int parity = 0;
+    for (long long tile = first; tile < tiles; tile += step, parity ^= 1) {
+        alive = arrived(&bars[0], parity, alive);
         const long long tile0 = tile * tile_rows;
         const int rows_here = (int)min((long long)tile_rows, a.rows - tile0);
-        TO* o_s = reinterpret_cast<TO*>(stage + at.r_at);
-        const u32 stage_at = shared_address(stage);
 #pragma unroll 1
         for (int r0 = 0; r0 < rows_here; r0 += BLOCK) {
             const int here = min(BLOCK, rows_here - r0);
@@ -330,14 +356,33 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, mix_forward_ctas(NT, WAY)) mix
 #pragma unroll 1
             for (int second = 0; second < (k2 ? 2 : 1); second++) {
                 const int width = second ? k2 : k;
-                const u32 x_at = stage_at + (second ? (u32)at.x2_at : 0) + r0 * width * sizeof(TI);
+                const int stride = second ? at.x2.stride : at.x.stride;
+                const u32 x_at = stage_at + (second ? (u32)at.x2_at : 0) + r0 * stride * sizeof(TI);
                 const u32 w = w_at + (second ? kp / mix_step(WAY) * NT * mix_block_bytes(NT, WAY) : 0);
-                if constexpr (WAY == MIX_PAIRS) mix_products_of_pairs<TI, NT, MT>(acc, x_at, width, w);
-                else mix_products<TI, NT, MT, WAY == MIX_PARTED>(acc, x_at, width, w, split_w);
+                if constexpr (WAY == MIX_PAIRS) mix_products_of_pairs<TI, NT, MT>(acc, x_at, width, stride, w);
+                else mix_products<TI, NT, MT, WAY == MIX_PARTED>(acc, x_at, width, stride, w, split_w);
             }
+            const long long row0 = tile0 + r0;
+            auto keep = [&](const auto* rows, int c, const RowsApart& r, uint8_t* codes, int16_t* scales, bool nonzero) {
+                const long long from = row0 * c;
+                const bool wide = (reinterpret_cast<uintptr_t>(codes) & 3) == 0;
+                if (!r.apart()) pack_by_warp(rows + r0 * c, here * c, codes + from, scales + from / PACK_BLOCK, nonzero, wide);
+                else   // (see launch_forward: rows lie apart only where the codes are aligned and blocks whole)
+                    pack_blocks_of(rows + r0 * r.stride, here * c, codes + from, scales + from / PACK_BLOCK, nonzero, [&](int i) { return r.at(i); });
+            };
+            if constexpr (KEEP) {   // whole blocks: 32 rows of any number of channels
+                static_assert(MT == 2);
+                if (a.x_codes) keep(reinterpret_cast<const TI*>(stage), k, at.x, a.x_codes, a.x_scales, false);
+                if (a.x2_codes) keep(reinterpret_cast<const TI*>(stage + at.x2_at), k2, at.x2, a.x2_codes, a.x2_scales, false);
+            }
+            if (r0 + BLOCK >= rows_here) {
+                __syncwarp();
+                if (alive) fetch_x(tile + step);
+            }
+            if (r0 == 0 && residual) alive = arrived(&bars[1], parity, alive);
             // The lane's 2 MT rows, 8 m + g of the block: z[m].
             constexpr int R = 2 * MT;
-            const int row = (r0 + g) * n + 2 * t;
+            const int ns = at.out.stride, row = (r0 + g) * ns + 2 * t;
             const u32 r_at = stage_at + (u32)at.r_at + row * sizeof(TI), to = stage_at + (u32)at.r_at + row * sizeof(TO);
             float z[R][2 * NT];
 #pragma unroll
@@ -349,7 +394,10 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, mix_forward_ctas(NT, WAY)) mix
                 for (int j = 0; j < 2 * NT; j++)
 #pragma unroll
                     for (int m = 0; m < R; m++)
-                        z[m][j] = fmaf(a.scale, lds_value_if<TI>(mix_there<NT>(j, n), r_at + (8 * m * n + 8 * (j / 2) + (j & 1)) * sizeof(TI)), z[m][j]);
+                    {
+                        const u32 at = r_at + (8 * m * ns + 8 * (j / 2) + (j & 1)) * sizeof(TI);
+                        z[m][j] = fmaf(a.scale, j / 2 < mix_full_blocks(NT) ? lds_value<TI>(at) : lds_value_if<TI>(mix_there<NT>(j, n), at), z[m][j]);
+                    }
             }
             mix_activate<R, NT>(z, a.activation, n);
             if (!alive) {
@@ -363,35 +411,31 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, mix_forward_ctas(NT, WAY)) mix
 #pragma unroll
             for (int j = 0; j < 2 * NT; j++)
 #pragma unroll
-                for (int m = 0; m < R; m++) sts_value_if<TO>(mix_there<NT>(j, n), to + (8 * m * n + 8 * (j / 2) + (j & 1)) * sizeof(TO), z[m][j]);
-            if constexpr (MT == 2) {   // whole blocks: 32 rows of any number of channels
-                const long long row0 = tile0 + r0;
-                auto keep = [&](const auto* rows, int c, uint8_t* codes, int16_t* scales, bool nonzero) {
-                    const long long from = row0 * c;
-                    pack_by_warp(rows + r0 * c, here * c, codes + from, scales + from / PACK_BLOCK, nonzero,
-                                 (reinterpret_cast<uintptr_t>(codes) & 3) == 0);
-                };
-                if (a.x_codes) keep(reinterpret_cast<const TI*>(stage), k, a.x_codes, a.x_scales, false);
-                if (a.x2_codes) keep(reinterpret_cast<const TI*>(stage + at.x2_at), k2, a.x2_codes, a.x2_scales, false);
+                for (int m = 0; m < R; m++) {
+                    const u32 at = to + (8 * m * ns + 8 * (j / 2) + (j & 1)) * sizeof(TO);
+                    if (j / 2 < mix_full_blocks(NT)) sts_value<TO>(at, z[m][j]);
+                    else sts_value_if<TO>(mix_there<NT>(j, n), at, z[m][j]);
+                }
+            if constexpr (KEEP) {
                 if (a.out_codes) {
                     __syncwarp();
-                    keep(o_s, n, a.out_codes, a.out_scales, a.activation == PL_ACT_RELU);
+                    keep(o_s, n, at.out, a.out_codes, a.out_scales, a.activation == PL_ACT_RELU);
                 }
             }
         }
         fence_async_proxy();
         __syncwarp();
-        copy_out(static_cast<TO*>(a.out) + tile0 * n, o_s, rows_here * n, bulk_out && rows_here == tile_rows);
+        if (at.out.apart()) copy_rows_out(static_cast<TO*>(a.out) + tile0 * n, o_s, rows_here, at.out);
+        else copy_out(static_cast<TO*>(a.out) + tile0 * n, o_s, rows_here * n, bulk_out && rows_here == tile_rows);
         if (lane == 0) {
             bulk_commit();
             bulk_wait_read();
         }
         __syncwarp();
-        if (alive) fetch(tile + stages * step, s);
-        if (++s == stages) s = 0, parity ^= 1;
+        if (alive) fetch_r(tile + step);
     }
     if (!alive)   // gave up once: no copy may be in flight when the CTA ends
-        for (int i = 0; i < stages; i++) mbar_wait(&bars[i], 0), mbar_wait(&bars[i], 1);
+        for (int i = 0; i < 2; i++) mbar_wait(&bars[i], 0), mbar_wait(&bars[i], 1);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -465,9 +509,11 @@ __global__ void __launch_bounds__(32 * WIDE_WARPS, 1) mix_forward_wide(MixArgs a
 #pragma unroll 1
             for (int c = 0; c < min(left, WIDE_CHUNK); c += 8, w += NT * 256) {
                 float v[1][4];
-                mix_load_left<float, 1>(v, rows, 8);   // (zeros behind the last channel)
+                u32 a_hi[1][4], a_lo[1][4];
+                mix_load_left<float, 1, false>(v, rows, 8);   // (zeros behind the last channel)
+                mix_split_left<float, 1>(a_hi, a_lo, v);
                 rows[0] += 32, rows[1] += 32;
-                mix_product8<float, NT, 1, true>(acc, v, w, split_w);
+                mix_product8<float, NT, 1, true>(acc, a_hi, a_lo, w, split_w);
             }
         }
         float z[2][2 * NT];

@@ -1,0 +1,35 @@
+// Channel products of float rows.
+#include "mix_launch.cuh"
+
+namespace pl {
+
+template <typename TO>
+static int launch_forward_wide(const MixArgs& a, cudaStream_t st) {
+    const size_t smem = wide_smem(a.k, a.k2);
+    PL_TRY((ensure_dynamic_smem<mix_forward_wide<TO>>(smem)));
+    const long long tiles = (a.rows + 15) / 16;
+    const unsigned ctas = (unsigned)std::min<long long>((tiles + WIDE_WARPS - 1) / WIDE_WARPS, num_sms());
+    mix_forward_wide<TO><<<ctas, 32 * WIDE_WARPS, smem, st>>>(a);
+    PL_COUNT_LAUNCHES(1);
+    PL_CUDA(cudaGetLastError());
+    return PL_OK;
+}
+
+template <typename TO>
+static int forward_floats(const MixArgs& a, cudaStream_t st) {
+    if constexpr (std::is_same<TO, float>::value) {
+        if (tiny(a.k, a.k2, a.n)) return launch_tiny<float>(a, st);
+    }
+    if (a.n > 64) return launch_forward_wide<TO>(a, st);
+    // few products to a sum: what the tensor cores cut stays below 2^-21 of it
+    if (a.k + a.k2 <= 96 && a.n <= 32) return forward_of<float, TO, MIX_PLAIN>(a, st);
+    return forward_of<float, TO, MIX_PARTED>(a, st);
+}
+
+int mix_forward_floats(const MixArgs& a, int out_dtype, cudaStream_t st) {
+    return out_dtype == PL_F32   ? forward_floats<float>(a, st)
+           : out_dtype == PL_F16 ? forward_floats<__half>(a, st)
+                                 : forward_floats<__nv_bfloat16>(a, st);
+}
+
+}  // namespace pl

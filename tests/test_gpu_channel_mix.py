@@ -43,7 +43,8 @@ def needs_of(a):
 
 SHAPES = [(1, 1, 0, 1), (1, 21, 21, 21), (2, 2, 2, 2), (31, 3, 1, 5), (32, 8, 8, 8), (33, 75, 0, 16), (257, 21, 21, 21),
           (1000, 33, 17, 40), (64, 128, 128, 128), (63, 127, 1, 128), (130, 128, 0, 1), (129, 1, 128, 127), (500, 64, 64, 64),
-          (4099, 9, 7, 24), (20011, 21, 21, 21), (12345, 2, 2, 2), (3001, 64, 0, 96), (777, 16, 32, 48), (2051, 100, 100, 10)]
+          (4099, 9, 7, 24), (20011, 21, 21, 21), (12345, 2, 2, 2), (3001, 64, 0, 96), (777, 16, 32, 48), (2051, 100, 100, 10),
+          (900, 32, 32, 32), (333, 4, 4, 4), (70, 4, 0, 3), (5000, 16, 16, 16), (257, 40, 40, 24), (260, 24, 56, 32), (100, 72, 8, 8)]
 
 
 @pytest.mark.parametrize("dtype,weight_dtype", [(F32, F32), (F16, F16), (BF16, BF16), (BF16, F32), (F16, F32)])
@@ -246,7 +247,8 @@ def test_8_bit_blocks_of_extreme_values(plb):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("rows,k,k2,n", [(1, 1, 0, 1), (33, 21, 21, 21), (1000, 75, 0, 16), (257, 128, 128, 128), (4099, 2, 2, 2),
-                                         (515, 5, 9, 31), (100, 128, 7, 3)])
+                                         (515, 5, 9, 31), (100, 128, 7, 3), (512, 64, 64, 64), (300, 32, 16, 64), (4097, 16, 0, 8),
+                                         (1600, 32, 32, 32), (95, 8, 8, 16), (1, 64, 0, 64)])
 def test_activations_in_8_bits(plb, rows, k, k2, n, dtype):
     """What the forward pass keeps is what pack_activations makes of the same tensors, and the gradients are those at the
     values that the codes stand for."""
