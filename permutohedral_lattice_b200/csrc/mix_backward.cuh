@@ -139,17 +139,13 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, MB * NB > 12 ? 2 : 3) mix_back
 
     // W^T: a row an input channel, zeros behind the last channel of either side
     const int kp = up8(k), all_p = kp + up8(k2);
-    for (int i = threadIdx.x; i < all_p * 8 * NB; i += blockDim.x) {
-        const int r = i / (8 * NB), c = i - r * (8 * NB);
-        const bool second = r >= kp;
-        const int j = second ? r - kp : r;
-        const void* w = second ? a.weight2 : a.weight;
+    for_weights<8 * NB>(all_p, kp, k, k2, n, a.weight, a.weight2, 0, a.weight_dtype, [&](int r, int c, float v) {
         u32 hi, lo;
-        split(c < n && j < (second ? k2 : k) && w ? load_weight(w, j * n + c, a.weight_dtype) : 0.f, hi, lo);
+        split(v, hi, lo);
         // the product's rows are the output channels c, its columns the input channels r
         u32* to = reinterpret_cast<u32*>(smem + at.weights + ((r >> 3) * NB + (c >> 3)) * MIX_BLOCK + (4 * (r & 7) + (c & 3)) * 16 + 4 * (c >> 2 & 1));
         to[0] = hi, to[2] = lo;
-    }
+    });
     __syncthreads();
 
     const int g = lane >> 2, t = lane & 3;

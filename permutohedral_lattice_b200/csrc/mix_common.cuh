@@ -27,6 +27,31 @@ __device__ __forceinline__ float load_weight(const void* w, int i, int dtype) {
                              : __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
 }
 
+// put(r, c, weight of input channel r (those of a second input from first_rows on) and output channel c) for a grid of rows x columns, zeros
+// where there is no such channel.  Four at a time: in a small call this is half of what a CTA does, and each is a trip to L2.
+// transposed: the (first and only) weight is [n][k].
+template <int COLUMNS, typename Put>
+__device__ __forceinline__ void for_weights(int rows, int first_rows, int k, int k2, int n, const void* weight, const void* weight2, int transposed,
+                                            int dtype, Put put) {
+    constexpr int U = 4;
+    for (int i0 = threadIdx.x; i0 < rows * COLUMNS; i0 += U * blockDim.x) {
+        float v[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = i0 + u * (int)blockDim.x, r = i / COLUMNS, c = i - r * COLUMNS;
+            const bool second = r >= first_rows;
+            const int j = second ? r - first_rows : r;
+            const void* w = second ? weight2 : weight;
+            v[u] = i < rows * COLUMNS && c < n && j < (second ? k2 : k) && w ? load_weight(w, transposed ? c * k + j : j * n + c, dtype) : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = i0 + u * (int)blockDim.x;
+            if (i < rows * COLUMNS) put(i / COLUMNS, i % COLUMNS, v[u]);
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------------------
 // Products: m16n8k8 on numbers of 11 significant bits (tf32), sums in float.  A float is the sum of two such numbers up to
 // 2^-23 of it: v = hi + lo, hi the nearest one, lo what is left cut to 11 bits; a product of two floats is then hi hi + hi lo +

@@ -302,13 +302,7 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, mix_forward_ctas(NT, WAY)) mix
 
     // the weights, zeros behind the last channel of either side, while the first tiles arrive
     const int kp = up_to(k, mix_step(WAY));
-    for (int i = threadIdx.x; i < (kp + up_to(k2, mix_step(WAY))) * 8 * NT; i += blockDim.x) {
-        const int r = i / (8 * NT), c = i - r * (8 * NT);
-        const bool second = r >= kp;
-        const int j = second ? r - kp : r;
-        float v = 0.f;
-        if (c < n && j < (second ? k2 : k))
-            v = load_weight(second ? a.weight2 : a.weight, a.transposed ? c * k + j : j * n + c, a.weight_dtype);
+    for_weights<8 * NT>(kp + up_to(k2, mix_step(WAY)), kp, k, k2, n, a.weight, a.weight2, a.transposed, a.weight_dtype, [&](int r, int c, float v) {
         unsigned char* to = smem + at.weights + mix_weight_at(NT, WAY, r, c);
         if constexpr (WAY == MIX_PAIRS) {
             *reinterpret_cast<TI*>(to) = from_float<TI>(v);
@@ -319,7 +313,7 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, mix_forward_ctas(NT, WAY)) mix
         } else {
             *reinterpret_cast<float*>(to) = v;
         }
-    }
+    });
     for (int i = threadIdx.x; i < 8 * NT; i += blockDim.x) bias_s[i] = a.bias && i < n ? load_weight(a.bias, i, a.weight_dtype) : 0.f;
     __syncthreads();
 
@@ -457,15 +451,8 @@ __global__ void __launch_bounds__(32 * WIDE_WARPS, 1) mix_forward_wide(MixArgs a
     const int k = a.k, k2 = a.k2, n = a.n, kp = up8(k), all_p = kp + up8(k2);
     float* bias_s = reinterpret_cast<float*>(smem + mix_weight_bytes(NT, MIX_PARTED, all_p));
     float* rows_s = bias_s + 8 * NT + warp * 16 * WIDE_STRIDE;
-    for (int i = threadIdx.x; i < all_p * 8 * NT; i += blockDim.x) {
-        const int r = i / (8 * NT), c = i - r * (8 * NT);
-        const bool second = r >= kp;
-        const int j = second ? r - kp : r;
-        float v = 0.f;
-        if (c < n && j < (second ? k2 : k))
-            v = load_weight(second ? a.weight2 : a.weight, a.transposed ? c * k + j : j * n + c, a.weight_dtype);
-        *reinterpret_cast<float*>(smem + mix_weight_at(NT, MIX_PARTED, r, c)) = v;
-    }
+    for_weights<8 * NT>(all_p, kp, k, k2, n, a.weight, a.weight2, a.transposed, a.weight_dtype,
+                        [&](int r, int c, float v) { *reinterpret_cast<float*>(smem + mix_weight_at(NT, MIX_PARTED, r, c)) = v; });
     for (int i = threadIdx.x; i < 8 * NT; i += blockDim.x) bias_s[i] = a.bias && i < n ? load_weight(a.bias, i, a.weight_dtype) : 0.f;
     __syncthreads();
     const float* x = static_cast<const float*>(a.x);

@@ -37,12 +37,12 @@ template <typename Smem>
 static MixLaunch mix_launch(long long rows, int block_rows, size_t block_bytes, int most_ctas, int most_stages, int most_blocks, Smem smem) {
     MixLaunch l;
     const long long all = (rows + block_rows - 1) / block_rows;
-    // A tile of some 4 KB, as long as there are tiles for four warps of every SM; a CTA of four warps, as long as there are tiles for
-    // every SM.
+    // A tile of some 4 KB, as long as there are tiles for four warps of every SM.  (Four warps a CTA however few rows there are: they share
+    // the work of reading the weights.)
     l.blocks = (int)std::max<size_t>(1, std::min<size_t>(most_blocks, 4096 / block_bytes));
     while (l.blocks > 1 && all < (long long)l.blocks * 4 * num_sms()) l.blocks--;
     const long long tiles = (all + l.blocks - 1) / l.blocks;
-    l.warps = (int)std::max(1ll, std::min((long long)MIX_WARPS, tiles / num_sms()));
+    l.warps = MIX_WARPS;
     // Two stages where three CTAs of an SM have room for them: what a warp waits for a tile is otherwise better hidden by other warps
     // (the gradients of 21 labels: 700 us with two stages and eight warps an SM, 602 with one and twelve).
     l.stages = tiles > (long long)l.warps * num_sms() ? most_stages : 1;
