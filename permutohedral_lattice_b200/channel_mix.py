@@ -13,6 +13,7 @@ that share a power of two, a quarter of float32's memory, half a step (1/510 to 
 negative values in the block 1/254 to 1/127) off at most.
 """
 import ctypes
+import functools
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -56,33 +57,36 @@ class MixGradients(NamedTuple):
 def _check_values(t, name, dtype=None):
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a tensor" % name)
-    if t.dtype not in _DTYPES:
-        raise TypeError("%s must be float32, float16 or bfloat16" % name)
-    if dtype is not None and t.dtype != dtype:
+    if dtype is None:
+        if t.dtype not in _DTYPES:
+            raise TypeError("%s must be float32, float16 or bfloat16" % name)
+    elif t.dtype is not dtype:
         raise TypeError("%s must have dtype %s like the other operand" % (name, dtype))
 
 
 def _check_device(tensors):
     """All on one GPU, which is returned."""
-    device = None
+    index = None
     for name, t in tensors:
         if t is None:
             continue
         if not t.is_cuda:
             raise ValueError("%s must be a CUDA tensor (there is no CPU path in this package)" % name)
-        if device is not None and t.device != device:
-            raise ValueError("%s is on %s, the other operands are on %s" % (name, t.device, device))
-        device = t.device
-    return device
+        at = t.get_device()
+        if index is not None and at != index:
+            raise ValueError("%s is on device %d, the other operands are on %d" % (name, at, index))
+        index, device_of = at, t
+    return device_of.device
 
 
 def _check_weight(w, name, x_dtype, dtype, k, n):
     _check_values(w, name, dtype)
-    if w.dtype not in (torch.float32, x_dtype):
+    if w.dtype is not torch.float32 and w.dtype is not x_dtype:
         raise TypeError("%s must be float32 or of the input's dtype" % name)
-    if w.dim() != 2 or (k is not None and w.shape[0] != k) or (n is not None and w.shape[1] != n):
+    shape = w.shape
+    if len(shape) != 2 or (k is not None and shape[0] != k) or (n is not None and shape[1] != n):
         raise ValueError("%s must be [channels of its input, channels of the output]" % name)
-    if not 1 <= w.shape[0] <= MOST_CHANNELS or not 1 <= w.shape[1] <= MOST_CHANNELS:
+    if not 1 <= shape[0] <= MOST_CHANNELS or not 1 <= shape[1] <= MOST_CHANNELS:
         raise ValueError("%s: 1 to %d channels are supported" % (name, MOST_CHANNELS))
 
 
@@ -123,14 +127,17 @@ def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
 
+_NOT_PACKED = capi.PlPacked(0, 0)
+
+
 def _packed(p):
-    return capi.PlPacked(0, 0) if p is None else capi.PlPacked(p.codes.data_ptr(), p.scales.data_ptr())
+    return _NOT_PACKED if p is None else capi.PlPacked(p.codes.data_ptr(), p.scales.data_ptr())
 
 
 def _kept(a):
     if isinstance(a, PackedActivations):
         return capi.PlKept(0, _packed(a))
-    return capi.PlKept(_ptr(a), capi.PlPacked(0, 0))
+    return capi.PlKept(_ptr(a), _NOT_PACKED)
 
 
 def _contiguous(t):
@@ -145,8 +152,17 @@ def _empty_packed(shape, dtype, device):
                              torch.empty(-(-count // BLOCK), dtype=torch.int16, device=device), tuple(shape), dtype)
 
 
+@functools.lru_cache(maxsize=1024)
 def _shape_of(rows, k, k2, n, activation, dtype, weight_dtype, residual_scale):
-    return capi.PlMix(rows, k, k2, n, _ACTIVATIONS[activation], _DTYPES[dtype], _DTYPES[weight_dtype], residual_scale)
+    """The C structure of a call, which the library only reads (building it takes a tenth of a small call's time on the host)."""
+    return ctypes.byref(capi.PlMix(rows, k, k2, n, _ACTIVATIONS[activation], _DTYPES[dtype], _DTYPES[weight_dtype], residual_scale))
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*shape):
+    nbytes = ctypes.c_size_t(0)
+    capi.check(capi.lib().pl_channel_mix_workspace_bytes(_shape_of(*shape), ctypes.byref(nbytes)), "pl_channel_mix_workspace_bytes")
+    return max(1, nbytes.value)
 
 
 def pack_activations(x):
@@ -196,17 +212,21 @@ def unpack_activations(packed, dtype=None):
 def _forward(device, x, weight, bias, residual, x2, weight2, activation, residual_scale, keep):
     """The call itself on checked arguments; keep: which of "x", "x2" and "out" to put into 8 bits too.
     Returns out and {name: PackedActivations}."""
-    x, weight, bias, residual, x2, weight2 = map(_contiguous, (x, weight, bias, residual, x2, weight2))
+    x, weight = x.contiguous(), weight.contiguous()
+    bias, residual, x2, weight2 = _contiguous(bias), _contiguous(residual), _contiguous(x2), _contiguous(weight2)
     k, k2, n = x.shape[-1], 0 if x2 is None else x2.shape[-1], weight.shape[1]
-    out = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=device)
-    like = {"x": x, "x2": x2, "out": out}
-    packs = {name: _empty_packed(like[name].shape, x.dtype, device) for name in keep if like[name] is not None}
+    out = x.new_empty(x.shape[:-1] + (n,)) if residual is None else torch.empty_like(residual)
+    packs = {}
+    if keep:
+        like = {"x": x, "x2": x2, "out": out}
+        packs = {name: _empty_packed(like[name].shape, x.dtype, device) for name in keep if like[name] is not None}
     m = _shape_of(out.numel() // n, k, k2, n, activation, x.dtype, weight.dtype, residual_scale)
     with _OnDevice(device):
-        capi.check(capi.lib().pl_channel_mix(
-            ctypes.byref(m), out.data_ptr(), x.data_ptr(), _ptr(x2), weight.data_ptr(), _ptr(weight2), _ptr(bias),
-            _ptr(residual), _packed(packs.get("x")), _packed(packs.get("x2")), _packed(packs.get("out")),
-            _stream_handle(device)), "pl_channel_mix")
+        rc = capi.lib().pl_channel_mix(
+            m, out.data_ptr(), x.data_ptr(), _ptr(x2), weight.data_ptr(), _ptr(weight2), _ptr(bias), _ptr(residual),
+            _packed(packs.get("x")), _packed(packs.get("x2")), _packed(packs.get("out")), _stream_handle(device))
+        if rc != capi.PL_OK:
+            capi.check(rc, "pl_channel_mix")
     return out, packs
 
 
@@ -288,16 +308,15 @@ def _backward(device, grad_out, out, x, x2, weight, weight2, activation, residua
               "residual": (head + (n,), grad_out.dtype), "weight": ((k, n), weight.dtype),
               "weight2": ((k2, n), weight.dtype), "bias": ((n,), weight.dtype)}
     made = {name: torch.empty(shapes[name][0], dtype=shapes[name][1], device=device) for name in needs}
-    m = _shape_of(grad_out.numel() // n, k, k2, n, activation, grad_out.dtype, weight.dtype, residual_scale)
-    L = capi.lib()
-    nbytes = ctypes.c_size_t(0)
+    shape = (grad_out.numel() // n, k, k2, n, activation, grad_out.dtype, weight.dtype, residual_scale)
     with _OnDevice(device):
-        capi.check(L.pl_channel_mix_workspace_bytes(ctypes.byref(m), ctypes.byref(nbytes)), "pl_channel_mix_workspace_bytes")
-        workspace = torch.empty(max(1, nbytes.value), dtype=torch.uint8, device=device)
+        workspace = torch.empty(_workspace_bytes(*shape), dtype=torch.uint8, device=device)
         d = capi.PlMixGradients(**{name: t.data_ptr() for name, t in made.items()})
-        capi.check(L.pl_channel_mix_backward(
-            ctypes.byref(m), grad_out.data_ptr(), _kept(out), _kept(x), _kept(x2), weight.data_ptr(), _ptr(weight2), d,
-            workspace.data_ptr(), workspace.numel(), _stream_handle(device)), "pl_channel_mix_backward")
+        rc = capi.lib().pl_channel_mix_backward(
+            _shape_of(*shape), grad_out.data_ptr(), _kept(out), _kept(x), _kept(x2), weight.data_ptr(), _ptr(weight2), d,
+            workspace.data_ptr(), workspace.numel(), _stream_handle(device))
+        if rc != capi.PL_OK:
+            capi.check(rc, "pl_channel_mix_backward")
     return MixGradients(**made)
 
 
