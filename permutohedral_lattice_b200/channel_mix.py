@@ -299,9 +299,8 @@ def channel_mix_backward(grad_out, saved, weight, weight2=None, activation=None,
 
 
 def _backward(device, grad_out, out, x, x2, weight, weight2, activation, residual_scale, needs):
-    grad_out, weight, weight2 = grad_out.detach().contiguous(), weight.detach().contiguous(), (
-        None if weight2 is None else weight2.detach().contiguous())
-    out, x, x2 = (a if a is None or isinstance(a, PackedActivations) else a.detach().contiguous() for a in (out, x, x2))
+    grad_out, weight, weight2 = grad_out.contiguous(), weight.contiguous(), _contiguous(weight2)
+    out, x, x2 = (a if a is None or isinstance(a, PackedActivations) else a.contiguous() for a in (out, x, x2))
     head, n = tuple(grad_out.shape[:-1]), grad_out.shape[-1]
     k, k2 = weight.shape[0], 0 if weight2 is None else weight2.shape[0]
     shapes = {"x": (head + (k,), grad_out.dtype), "x2": (head + (k2,), grad_out.dtype),
