@@ -43,23 +43,52 @@ __global__ void __launch_bounds__(256) pack_blocks(uint8_t* __restrict__ codes, 
     }
 }
 
+// 16 bytes of values a thread, four times on the way at once.
+constexpr int UNPACK_AT_ONCE = 4;
+template <typename T>
+__host__ __device__ constexpr int unpack_values() { return 256 * UNPACK_AT_ONCE * 16 / (int)sizeof(T); }   // of a CTA at a time
 template <typename T>
 __global__ void __launch_bounds__(256) unpack_blocks(T* __restrict__ x, const uint8_t* __restrict__ codes,
                                                      const int16_t* __restrict__ scales, long long n, int wide) {
-    const long long step = (long long)gridDim.x * 1024;
-    for (long long i = (long long)blockIdx.x * 1024 + threadIdx.x * 4; i < n; i += step) {
-        const u32 header = (u32)(u16)scales[i / PACK_BLOCK];
-        u32 c = 0;
-        float v[4];
-        if (wide && i + 3 < n) c = *reinterpret_cast<const u32*>(codes + i);
-        else
-            for (int j = 0; j < 4; j++)
-                if (i + j < n) c |= (u32)codes[i + j] << (8 * j);
-        decode4(v, c, header);
-        if (wide && i + 3 < n) store4(x + i, v);
-        else
-            for (int j = 0; j < 4; j++)
-                if (i + j < n) x[i + j] = from_float<T>(v[j]);
+    constexpr int PER = 16 / sizeof(T), U = UNPACK_AT_ONCE;
+    const long long step = (long long)gridDim.x * unpack_values<T>();
+    for (long long i0 = (long long)blockIdx.x * unpack_values<T>() + threadIdx.x * PER; i0 < n; i0 += step) {
+        u32 c[U][PER / 4], header[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long long i = i0 + u * 256 * PER;
+            header[u] = i < n ? (u32)(u16)scales[i / PACK_BLOCK] : 0;
+#pragma unroll
+            for (int w = 0; w < PER / 4; w++) {
+                c[u][w] = 0;
+                if (wide && i + PER <= n) c[u][w] = reinterpret_cast<const u32*>(codes + i)[w];
+                else
+                    for (int j = 0; j < 4; j++)
+                        if (i + 4 * w + j < n) c[u][w] |= (u32)codes[i + 4 * w + j] << (8 * j);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long long i = i0 + u * 256 * PER;
+            if (i >= n) break;
+            float v[PER / 4][4];
+#pragma unroll
+            for (int w = 0; w < PER / 4; w++) decode4(v[w], c[u][w], header[u]);
+            if (wide && i + PER <= n) {
+                if constexpr (PER == 4) {
+                    store4(x + i, v[0]);
+                } else {
+                    uint4 q;
+                    T* h = reinterpret_cast<T*>(&q);
+#pragma unroll
+                    for (int j = 0; j < PER; j++) h[j] = from_float<T>(v[j / 4][j & 3]);
+                    *reinterpret_cast<uint4*>(x + i) = q;
+                }
+            } else {
+                for (int j = 0; j < PER; j++)
+                    if (i + j < n) x[i + j] = from_float<T>(v[j / 4][j & 3]);
+            }
+        }
     }
 }
 
@@ -90,8 +119,8 @@ static int pack_any(pl_packed to, const void* x, int64_t n, int dtype, bool keep
 }
 template <typename T>
 static int launch_unpack(void* x, const pl_packed& from, int64_t n, cudaStream_t st) {
-    const bool wide = aligned(x, 4 * sizeof(T)) && aligned(from.codes, 4);
-    unpack_blocks<T><<<grid_for(n, 1024, 8), 256, 0, st>>>(static_cast<T*>(x), from.codes, from.scales, n, wide);
+    const bool wide = aligned(x, 16) && aligned(from.codes, 4);
+    unpack_blocks<T><<<grid_for(n, unpack_values<T>(), 8), 256, 0, st>>>(static_cast<T*>(x), from.codes, from.scales, n, wide);
     PL_COUNT_LAUNCHES(1);
     PL_CUDA(cudaGetLastError());
     return PL_OK;

@@ -90,7 +90,7 @@ __device__ __forceinline__ void mix_split_left(u32 (&hi)[MT][4], u32 (&lo)[MT][4
 // sums of more than a hundred terms that cancel (128 labels: dz W^T) it cost 1.6 bits.
 template <typename TI, int NT, int MT, bool PARTS>
 __device__ __forceinline__ void mix_product8(float (&acc)[MT][NT][4], const u32 (&a_hi)[MT][4], const u32 (&a_lo)[MT][4], u32 w, bool split_w) {
-    constexpr int JG = NT % 4 == 0 ? 4 : NT % 3 == 0 ? 3 : NT % 2 == 0 ? 2 : NT == 1 ? 1 : NT;
+    constexpr int JG = NT % 16 == 0 ? 8 : NT % 4 == 0 ? 4 : NT % 3 == 0 ? 3 : NT % 2 == 0 ? 2 : NT == 1 ? 1 : NT;
 #pragma unroll
     for (int j0 = 0; j0 < NT; j0 += JG) {
         u32 b_hi[JG][2], b_lo[JG][2];
