@@ -5,6 +5,10 @@
 // that last for the whole kernel, dx into the place where x came in.  At the end a CTA's warps add their shares of dW up,
 // mix_add_shares those of the CTAs, in double and in a fixed order.
 //
+// 16 x 512x512 rows of 21 + 21 channels to 21, floats: 503 us, 4.9 TB/s of what has to be moved (356 without dW); from activations in 8
+// bits 667, a quarter of it their decoding.  Three CTAs of four warps an SM, 168 registers: bound by issue slots (2080 instructions for 32
+// rows, in 8 bits 2900, at 2 of 4 a cycle).
+//
 // Beyond that dW does not fit a warp's registers: mix_dz writes dz to the workspace, mix_forward multiplies it by the
 // transposed weights, mix_backward_weights gives a CTA's warps blocks of dW to sum over all its rows.
 #pragma once
@@ -179,32 +183,39 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, MB * NB > 12 ? 2 : 3) mix_back
 #pragma unroll 1
         for (int r0 = 0; r0 < rows_here; r0 += 32) {
             const int here = min(32, rows_here - r0);
-            // 32 rows to floats, from 8 bits eight lanes a block; rows that are not there to zeros.
+            // 32 rows to floats, four lanes a block; rows that are not there to zeros.  Every other block's lanes take their two halves the
+            // other way round, so that lanes which write together write to different banks.
             auto decode = [&](float* to, const Kept& p, const unsigned char* place, const u32* heads, int most, int c) {
-                float* w = to + 4 * lane;
-                int left = c - lane / 8;   // blocks, from this lane's on
+                const int from = 32 * (lane >> 2) + 8 * (lane & 3), swap = lane & 4;
+                float* w = to + from;
+                int left = c - (lane >> 2);   // blocks, from this lane's on
                 if (p.codes) {
-                    const u32* codes = reinterpret_cast<const u32*>(place + r0 * c) + lane;
-                    int b = r0 / 32 * c + lane / 8;
-                    for (int i = 0; i < c; i += 4, left -= 4, b += 4, w += 128, codes += 32) {
+                    const uint2* codes = reinterpret_cast<const uint2*>(place + r0 * c + from);
+                    int b = r0 / 32 * c + (lane >> 2);
+                    for (int i = 0; i < c; i += 8, left -= 8, b += 8, w += 256, codes += 32) {
                         u32 head = __shfl_sync(~0u, heads[0], b);
                         if (most > 1 && c > 32) {
                             const u32 second = __shfl_sync(~0u, heads[most > 1 ? 1 : 0], b), third = __shfl_sync(~0u, heads[most > 2 ? 2 : 0], b);
                             head = b < 32 ? head : b < 64 ? second : third;
                         }
                         if (left > 0) {
+                            const uint2 q = *codes;
                             float v[4];
-                            decode4(v, *codes, head);
-                            store4(w, v);
+                            decode4(v, swap ? q.y : q.x, head);
+                            store4(w + swap, v);
+                            decode4(v, swap ? q.x : q.y, head);
+                            store4(w + 4 - swap, v);
                         }
                     }
                 } else {
-                    const T* values = reinterpret_cast<const T*>(place) + r0 * c + 4 * lane;
-                    for (int i = 0; i < c; i += 4, left -= 4, w += 128, values += 128)
+                    const T* values = reinterpret_cast<const T*>(place) + r0 * c + from;
+                    for (int i = 0; i < c; i += 8, left -= 8, w += 256, values += 256)
                         if (left > 0) {
                             float v[4];
-                            load4(v, values);
-                            store4(w, v);
+                            load4(v, values + swap);
+                            store4(w + swap, v);
+                            load4(v, values + 4 - swap);
+                            store4(w + 4 - swap, v);
                         }
                 }
                 if (here < 32) {
@@ -529,7 +540,8 @@ __global__ void __launch_bounds__(256) mix_dz(MixBackArgs a) {
 }
 
 // dW of one input (blockIdx.y: x or x2) and, with the first, dbias: a CTA's eight warps each sum blocks of 64 x 32 of it over all the
-// CTA's rows, 32 rows at a time through shared memory; the next 32 are on their way in registers meanwhile.
+// CTA's rows, 32 rows at a time through shared memory; the next 32 are on their way in registers meanwhile.  154 401 rows of 128 + 128 x
+// 128: 329 us, the tensor cores busy a third of them (110 us is their floor); 680 with loads and products in turn.
 constexpr int WIDE_ROWS = 32, WIDE_DS = MIX_MOST + 8;   // (rows of 136 floats: 4 rows by 8 channels in 32 banks)
 constexpr size_t WIDE_SMEM = sizeof(float) * 2 * 2 * WIDE_ROWS * WIDE_DS;
 template <typename T>

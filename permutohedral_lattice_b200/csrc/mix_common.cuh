@@ -59,7 +59,7 @@ __device__ __forceinline__ void for_weights(int rows, int first_rows, int k, int
 //   a: (g, t), (g + 8, t), (g, t + 4), (g + 8, t + 4)    b: (t, g), (t + 4, g)    c: (g, 2t), (g, 2t + 1), (g + 8, 2t), (g + 8, 2t + 1)
 // and wants each of them in registers that follow one another.  So b's that are read more than once lie in shared memory as the
 // lanes take them, 16 bytes a lane: the high terms of both, then the low ones.  (Lying row by row as pairs of terms they took two accesses
-// and four moves: a third of all instructions of the gradients at 21 labels.)
+// and four moves: a quarter of all instructions of the gradients at 21 labels.)
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ void mma8(float (&c)[4], const u32 (&a)[4], const u32 (&b)[2]) {
     asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -273,7 +273,7 @@ __device__ __forceinline__ void pack_by_warp(const T* values, int count, uint8_t
 // 16-byte boundary, and the last rows, are copied by the lanes.
 //
 // Rows of 32, 64, ... 512 bytes would begin in the same few banks, and eight of them are read together (64 channels of 16 bits: up
-// to 8 accesses for one, 259 us a forward pass over a million rows, so 113).  They lie 16 bytes further apart and are copied by the lanes,
+// to 8 accesses for one, 259 us a forward pass over a million rows, so 160).  They lie 16 bytes further apart and are copied by the lanes,
 // 16 bytes each.
 // ---------------------------------------------------------------------------------------------
 constexpr int MIX_WARPS = 4, MIX_STAGES = 2;   // of a CTA and of a warp, at most
@@ -326,7 +326,7 @@ __device__ __forceinline__ float lds(u32 at) {
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
     return v;
 }
-// The accesses of which some lanes have none are predicated here: as branches around them they took a quarter of all instructions.
+// The accesses of which some lanes have none are predicated here: as branches around them they took a seventh of all instructions.
 __device__ __forceinline__ u32 lds_u32_if(bool there, u32 at) {
     u32 v;
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.shared.u32 %0, [%1];\n\t}" : "=&r"(v) : "r"(at), "r"((int)there));

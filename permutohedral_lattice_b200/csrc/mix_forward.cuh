@@ -4,6 +4,10 @@
 // all tiles of a CTA, a warp takes 16 MT rows at a time through the tensor cores and finishes them in registers (a row's logits lie in
 // the registers of four lanes: the maximum and the sum of a softmax take two shuffles each); the output leaves from where the
 // residual came in.
+//
+// 16 x 512x512 rows of 21 + 21 channels to 21, floats: 270 us, 5.2 TB/s of what has to be moved.  Half of them: 143 us with four CTAs of
+// four warps an SM (three 148, five 141, six, which spill, 153), 117 without the products, 113 without the softmax too, 101 for
+// torch's addcmul, which reads three tensors and writes one.  What is left are issue slots: IPC 2 of 4.
 #pragma once
 #include "mix_common.cuh"
 
@@ -435,8 +439,10 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, mix_forward_ctas(NT, WAY)) mix
 // ---------------------------------------------------------------------------------------------
 // Many channels out (65 and more) of float rows.  The weights of both inputs take up to 128 KB of shared memory, which leaves too
 // little for whole rows: a warp takes 16 rows, 32 channels at a time, by way of its registers (the next ones are on their way while
-// these are multiplied), reads the residual and writes its rows from registers.  Bound by the tensor cores: three products of 11-bit
-// terms for one of floats, 276 TFLOP/s of them.
+// these are multiplied), reads the residual and writes its rows from registers.  154 401 rows of 128 + 128 channels to 128: 269 us (558
+// with whole rows in shared memory and four warps an SM; 8, 12 and 14 warps 289, 269 and 306; four blocks of columns at once in place
+// of eight 285).  Its floor is the tensor cores' 110 us, three products of 11-bit terms for one of floats at 276 TFLOP/s: they are
+// busy 43 % of the time, warps wait for products that they depend on.
 // ---------------------------------------------------------------------------------------------
 constexpr int WIDE_WARPS = 12, WIDE_CHUNK = 32, WIDE_STRIDE = WIDE_CHUNK + 4;   // (rows of 36 floats: 8 rows by 4 channels in 32 banks)
 constexpr int WIDE_NT = 16;

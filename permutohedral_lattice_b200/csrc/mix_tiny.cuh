@@ -1,6 +1,6 @@
 // The channel products with up to four channels of each input and of the output (two or three classes, a grey image): a thread
 // a row, weights and sums in registers.  A row is some tens of bytes: bound by memory, and as matrix products of 8 x 8 blocks most of the
-// work was on channels that are not there (volumes of two classes, 3.4 million rows, float: forward 93 -> 34 us, gradients 130 -> 45).
+// work was on channels that are not there (volumes of two classes, 3.4 million rows, float: forward 93 -> 37 us, gradients 130 -> 47).
 #pragma once
 #include "mix_backward.cuh"
 
