@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, MB * NB > 12 ? 2 : 3) mix_back
                     from[i] = second ? x2_at + (t * k2 + g + 8 * i - kp) * sizeof(TX) : x_at + (t * k + g + (8 * i < kp ? 8 * i : 0)) * sizeof(TX);
                 }
                 u32 dz_from = dz_at + lane * 8;
-#pragma unroll 1
+#pragma unroll (LONG ? 4 : 1)
                 for (int r = 0; r < 32; r += 8, dz_from += NB * MIX_DZ_BLOCK) {
                     u32 b_hi[NB][2], b_lo[NB][2];
 #pragma unroll
