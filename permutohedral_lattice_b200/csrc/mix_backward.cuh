@@ -5,9 +5,9 @@
 // that last for the whole kernel, dx into the place where x came in.  At the end a CTA's warps add their shares of dW up,
 // mix_add_shares those of the CTAs, in double and in a fixed order.
 //
-// 16 x 512x512 rows of 21 + 21 channels to 21, floats: 503 us, 4.9 TB/s of what has to be moved (356 without dW); from activations in 8
-// bits 667, a quarter of it their decoding.  Three CTAs of four warps an SM, 168 registers: bound by issue slots (2080 instructions for 32
-// rows, in 8 bits 2900, at 2 of 4 a cycle).
+// 16 x 512x512 rows of 21 + 21 channels to 21, floats: 496 us, 5.0 TB/s of what has to be moved (358 without dW); from activations in 8
+// bits 618, a fifth of it their decoding.  Three CTAs of four warps an SM, 168 registers: bound by issue slots (1920 instructions for 32
+// rows, in 8 bits 2530, at 2 of 4 a cycle).
 //
 // Beyond that dW does not fit a warp's registers: mix_dz writes dz to the workspace, mix_forward multiplies it by the
 // transposed weights, mix_backward_weights gives a CTA's warps blocks of dW to sum over all its rows.

@@ -5,9 +5,9 @@
 // the registers of four lanes: the maximum and the sum of a softmax take two shuffles each); the output leaves from where the
 // residual came in.
 //
-// 16 x 512x512 rows of 21 + 21 channels to 21, floats: 270 us, 5.2 TB/s of what has to be moved.  Half of them: 143 us with four CTAs of
-// four warps an SM (three 148, five 141, six, which spill, 153), 117 without the products, 113 without the softmax too, 101 for
-// torch's addcmul, which reads three tensors and writes one.  What is left are issue slots: IPC 2 of 4.
+// 16 x 512x512 rows of 21 + 21 channels to 21, floats: 252 us, 5.6 TB/s of what has to be moved.  Half of them: 133 us; without the products
+// 117, without the softmax too 113, and 101 for torch's addcmul, which reads three tensors and writes one.  Four CTAs of four warps an SM:
+// three, five and six (which spill) took 148, 141 and 153 where four took 143.  What is left are issue slots: IPC 2 of 4.
 #pragma once
 #include "mix_common.cuh"
 
