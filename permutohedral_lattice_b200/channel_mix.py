@@ -196,7 +196,7 @@ def _check_packed(p, name):
 
 def unpack_activations(packed, dtype=None):
     """The values of a PackedActivations, in `dtype` (default: that of the tensor that was packed).  float32 and bfloat16
-    hold each exactly, float16 those between 2^-16 and 65504 that are."""
+    hold each exactly; float16 rounds, and takes those beyond 65504 for infinities."""
     count = _check_packed(packed, "packed")
     dtype = packed.dtype if dtype is None else dtype
     if dtype not in _DTYPES:
@@ -366,7 +366,9 @@ def channel_mix(x, weight, bias=None, residual=None, x2=None, weight2=None, acti
     weight2 [K2, N] and bias [N] in float32 or the input's dtype; up to 128 channels each.  activation: None, "relu" or
     "softmax" over the channels; a row whose channels are all forbidden by an infinite residual gives zeros and has no
     gradient.  checkpoint="8bit" keeps the activations that the backward pass needs in 8 bits: their gradients are those
-    at the rounded activations, and x, x2 and the output may be freed in between."""
+    at the rounded activations, and x, x2 and the output may be freed in between.  x, x2 and the weights have to be finite
+    (a row that is not comes out NaN).  In a CUDA graph: one ordinary call before the capture, which sets the kernel up; forward
+    and backward together, on leaves made inside it."""
     device = _check_mix(x, weight, bias, residual, x2, weight2, activation, checkpoint)
     args = (x, weight, bias, residual, x2, weight2)
     if not _watched_by_torch() and not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args)):

@@ -441,3 +441,73 @@ def test_values_beyond_32_bit_offsets(plb):
     grads = ref.gradients(g[-1000:], y, kept, w, None, None, "softmax", 1.0)
     ref.assert_within(d.x[-1000:], *grads["x"])
     ref.assert_within(d.weight, *grads["weight"])
+
+
+def test_wide_rows_beyond_32_bit_offsets(plb):
+    """2.15 billion floats: rows behind the 2^31st value in the kernels of wide rows, forward and backward."""
+    rows, k, n = 16_800_001, 128, 128
+    x = torch.zeros((rows, k), device="cuda")
+    w = torch.randn((k, n), generator=torch.Generator().manual_seed(0)).cuda()
+    tail = torch.randn((50, k), generator=torch.Generator().manual_seed(1)).cuda()
+    x[-50:] = tail
+    out, saved = plb.channel_mix_raw(x, w, activation="softmax")
+    want, bound = ref.forward(tail, w, None, None, None, None, "softmax", 1.0)
+    ref.assert_within(out[-50:], want, bound)
+    assert bool((out[-51] == 1 / 128).all())
+    g = torch.zeros_like(out)
+    g[-50:] = torch.randn((50, n), generator=torch.Generator().manual_seed(2)).cuda()
+    d = plb.channel_mix_backward(g, saved, w, activation="softmax", needs=("x", "weight"))
+    assert not bool(d.x[:-50].any())
+    grads = ref.gradients(g[-50:], out[-50:], tail, w, None, None, "softmax", 1.0)
+    ref.assert_within(d.x[-50:], *grads["x"])
+    ref.assert_within(d.weight, *grads["weight"])
+
+
+def test_a_single_row_without_other_dimensions(plb):
+    a, g = make(1, 9, 4, 6)
+    flat = {m: (t[0, 0] if t is not None and t.dim() == 3 else t) for m, t in a.items()}
+    out, saved = plb.channel_mix_raw(**flat, activation="softmax", checkpoint="8bit")
+    assert out.shape == (6,) and torch.equal(out, plb.channel_mix(**a, activation="softmax")[0, 0])
+    d = plb.channel_mix_backward(g[0, 0], saved, a["weight"], a["weight2"], "softmax", 1.0, needs_of(a))
+    assert d.x.shape == (9,) and d.x2.shape == (4,) and d.residual.shape == (6,)
+    assert plb.channel_mix_backward(g[0, 0], saved, a["weight"], a["weight2"], "softmax", needs=()) == plb.MixGradients()
+
+
+def test_two_host_threads_on_streams_of_their_own(plb):
+    import threading
+    cases = [make(4000 + 37 * i, 21 + i, 10, 21, seed=i) for i in range(4)]
+
+    def work(a, g):
+        out, saved = plb.channel_mix_raw(**a, activation="softmax", checkpoint="8bit")
+        d = plb.channel_mix_backward(g, saved, a["weight"], a["weight2"], "softmax", 1.0, needs_of(a))
+        return [out] + [getattr(d, m) for m in needs_of(a)]
+
+    want = [work(*c) for c in cases]
+    torch.cuda.synchronize()
+    got = [None] * len(cases)
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got[i] = work(*cases[i])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for one, other in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(one, other))
+
+
+def test_the_largest_finite_values(plb):
+    """Values up to 3.4e38 and down to the least ones: nothing becomes NaN that is not."""
+    for dtype in (F32, BF16, F16):
+        big = torch.finfo(dtype).max * 0.99
+        x = torch.tensor([[big, 0, 0], [0, big, -big], [torch.finfo(dtype).tiny, 1, 0], [0, 0, 0]], dtype=dtype, device="cuda")
+        w = torch.tensor([[0.5, 0.0], [0.25, 0.25], [0.25, -0.125]], dtype=dtype, device="cuda")
+        out = plb.channel_mix(x, w)
+        want = x.double() @ w.double()
+        assert bool(torch.isfinite(out).all())
+        assert float(((out.double() - want).abs() / (x.double().abs() @ w.double().abs() + 1e-30)).max()) <= ref.PRODUCT + ref.half_step(dtype)
