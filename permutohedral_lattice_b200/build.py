@@ -19,7 +19,7 @@ SOURCES = [os.path.join(CSRC, "pl_lattice.cu"), os.path.join(CSRC, "channel_mix.
 HEADERS = [os.path.join(CSRC, h) for h in ("simplex.cuh", "common.cuh", "lattice_build.cuh", "splat.cuh",
                                              "blur_slice.cuh", "small.cuh", "export.cuh", "fp64.cuh", "direct_index.cuh", "direct_bounds.h", "crf.cuh",
                                              "smem_limit.h", "host_calls.h", "mix_common.cuh",
-                                             "mix_forward.cuh", "mix_backward.cuh", "mix_tiny.cuh",
+                                             "mix_forward.cuh", "mix_backward.cuh", "mix_tensor.cuh", "mix_tiny.cuh",
                                              "mix_host.h", "mix_launch.cuh", "mix_back_launch.cuh")] + [
     os.path.join(ROOT, "include", "pl_lattice.h")]
 

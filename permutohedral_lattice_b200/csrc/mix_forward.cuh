@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, mix_forward_ctas(NT, WAY)) mix
 }
 
 // ---------------------------------------------------------------------------------------------
-// Many channels out (65 and more) of float rows.  The weights of both inputs take up to 128 KB of shared memory, which leaves too
+// Many channels out (65 and more) of float rows, what mix_forward_tensor does not take (see tensor_pays).  The weights of both inputs take up to 128 KB of shared memory, which leaves too
 // little for whole rows: a warp takes 16 rows, 32 channels at a time, by way of its registers (the next ones are on their way while
 // these are multiplied), reads the residual and writes its rows from registers.  154 401 rows of 128 + 128 channels to 128: 269 us (558
 // with whole rows in shared memory and four warps an SM; 8, 12 and 14 warps 289, 269 and 306; four blocks of columns at once in place

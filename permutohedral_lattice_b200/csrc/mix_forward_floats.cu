@@ -1,5 +1,6 @@
 // Channel products of float rows.
 #include "mix_launch.cuh"
+#include "mix_tensor.cuh"
 
 namespace pl {
 
@@ -15,10 +16,25 @@ static int launch_forward_wide(const MixArgs& a, cudaStream_t st) {
     return PL_OK;
 }
 
+template <typename TO, typename W>
+static int launch_forward_tensor(const MixArgs& a, cudaStream_t st) {
+    PL_TRY((ensure_dynamic_smem<mix_forward_tensor<TO, W>>(TC_SMEM)));
+    mix_forward_tensor<TO, W><<<grid_for(a.rows, TC_ROWS, 1), TC_THREADS, TC_SMEM, st>>>(a);
+    PL_COUNT_LAUNCHES(1);
+    PL_CUDA(cudaGetLastError());
+    return PL_OK;
+}
+
 template <typename TO>
 static int forward_floats(const MixArgs& a, cudaStream_t st) {
     if constexpr (std::is_same<TO, float>::value) {
         if (tiny(a.k, a.k2, a.n)) return launch_tiny<float>(a, st);
+    }
+    if (a.n > 64 && tensor_pays(a)) {
+        if constexpr (!std::is_same<TO, float>::value) {
+            if (a.weight_dtype != PL_F32) return launch_forward_tensor<TO, TO>(a, st);   // (the other weights are of the output's type)
+        }
+        return launch_forward_tensor<TO, float>(a, st);
     }
     if (a.n > 64) return launch_forward_wide<TO>(a, st);
     // Few products to a sum: what the tensor cores cut stays below 2^-21 of it (75 channels of one sign: 0.9e-6 off in all, so 0.2e-6).

@@ -511,3 +511,72 @@ def test_the_largest_finite_values(plb):
         want = x.double() @ w.double()
         assert bool(torch.isfinite(out).all())
         assert float(((out.double() - want).abs() / (x.double().abs() @ w.double().abs() + 1e-30)).max()) <= ref.PRODUCT + ref.half_step(dtype)
+
+
+@pytest.mark.parametrize("dtype,weight_dtype", [(F32, F32), (BF16, BF16), (F16, F32)])
+@pytest.mark.parametrize("rows,k,k2,n", [(1, 64, 0, 68), (127, 67, 67, 68), (128, 32, 32, 100), (129, 61, 3, 128), (20011, 128, 4, 128),
+                                         (38000, 97, 31, 72), (19000, 33, 31, 67), (257, 63, 0, 128), (500, 68, 128, 21)])
+def test_many_labels(plb, rows, k, k2, n, dtype, weight_dtype):
+    """One tile a CTA and several, widths of whole float4 and others, as many channels in as the tensor-memory kernel takes and fewer."""
+    for activation in ("softmax", "relu"):
+        a, g = make(rows, k, k2, n, dtype, weight_dtype)
+        out, saved = plb.channel_mix_raw(**a, activation=activation, residual_scale=-1.0)
+        want, bound = ref.forward(a["x"], a["weight"], a["bias"], a["residual"], a["x2"], a["weight2"], activation, -1.0)
+        ref.assert_within(out, want, bound, activation)
+        needs = needs_of(a)
+        d = plb.channel_mix_backward(g, saved, a["weight"], a["weight2"], activation, -1.0, needs)
+        gradients = ref.gradients(g, out, a["x"], a["weight"], a["x2"], a["weight2"], activation, -1.0)
+        for m in needs:
+            ref.assert_within(getattr(d, m), *gradients[m], "%s of %s" % (m, activation))
+
+
+@pytest.mark.parametrize("moved", ["x", "x2", "weight", "weight2", "bias", "residual"])
+def test_many_labels_at_addresses_of_any_alignment(plb, moved):
+    a, _ = make(700, 128, 64, 128)
+    want, bound = ref.forward(a["x"], a["weight"], a["bias"], a["residual"], a["x2"], a["weight2"], "softmax", -1.0)
+    t = a[moved]
+    store = torch.empty(t.numel() + 1, device="cuda")
+    a[moved] = store[1:].view(t.shape).copy_(t)
+    assert a[moved].data_ptr() % 16 == 4
+    out = plb.channel_mix(**a, activation="softmax", residual_scale=-1.0)
+    ref.assert_within(out, want, bound, moved)
+    assert torch.equal(out, plb.channel_mix(**{**a, moved: t}, activation="softmax", residual_scale=-1.0))
+
+
+def test_bad_values_of_many_labels_stay_in_their_row(plb):
+    a, _ = make(300, 128, 70, 128)
+    clean = plb.channel_mix(**a, activation="softmax", residual_scale=-1.0)
+    a["x"][0, 7, 127] = math.nan
+    a["x2"][0, 129, 69] = math.inf
+    a["residual"][0, 299, 127] = math.nan
+    out = plb.channel_mix(**a, activation="softmax", residual_scale=-1.0)
+    bad = [7, 129, 299]
+    assert bool(torch.isnan(out[0, bad]).all())
+    keep = [r for r in range(300) if r not in bad]
+    assert torch.equal(out[0, keep], clean[0, keep])
+
+
+def test_many_labels_on_several_streams_and_in_graphs(plb):
+    """Kernels that take all of an SM's tensor memory, on four streams at once and replayed beside each other, with a library product
+    on a fifth."""
+    cases = [make(40000 + 131 * i, 128, 0, 128, seed=i)[0] for i in range(4)]
+    want = [plb.channel_mix(**a, activation="softmax") for a in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    graphs, results = [], []
+    for s, a in zip(streams, cases):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            results.append(plb.channel_mix(**a, activation="softmax"))
+        graphs.append(graph)
+    square = torch.randn((2048, 2048), device="cuda", dtype=BF16)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        torch.cuda.synchronize()
+        eager = []
+        for s, a, graph in zip(streams, cases, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+                eager.append(plb.channel_mix(**a, activation="softmax"))
+        square @ square
+        torch.cuda.synchronize()
+        assert all(torch.equal(r, w) for r, w in zip(results, want)) and all(torch.equal(r, w) for r, w in zip(eager, want))
