@@ -81,20 +81,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1) mix_forward_tensor(MixArgs a) {
     const int chunks = (k + TC_CHUNK - 1) / TC_CHUNK, all = chunks + (k2 + TC_CHUNK - 1) / TC_CHUNK;
     const long long tiles = (a.rows + TC_ROWS - 1) / TC_ROWS;
     const bool quads = k % 4 == 0 && aligned16(x), quads2 = k2 % 4 == 0 && aligned16(x2), quads_out = aligned16(residual) && aligned16(out);
-    // What a thread fetches of 32 channels: four channels of rows i / 8 (i = its number, and so on), and of columns i % 128 of the weights.
+    // What a thread fetches of 32 channels: four channels of rows i / 8 (i = its number, and so on), and of the weights.
     // (What is not there is read elsewhere and made zero when it is stored: nothing waits for a load before then, and no branch parts them.)
     float4 next_x[TC_U];
     W next_w[TC_U][4];
-    const int my_c = 4 * (threadIdx.x & 7), my_row = threadIdx.x >> 3, my_cw = 4 * (threadIdx.x >> 7), my_col = threadIdx.x & 127;
+    const int my_c = 4 * (threadIdx.x & 7), my_row = threadIdx.x >> 3;
+    // (A row of the weights is one of columns, or of channels where they are transposed: threads side by side read along it.  dz and
+    // two dz W^T of 154 401 rows and 128 + 128 labels: 228 us, 337 where they read across.)
+    const int my_cw = a.transposed ? my_c : 4 * (threadIdx.x >> 7), my_col = a.transposed ? my_row : threadIdx.x & 127;
+    const int next_cw = a.transposed ? 0 : 4 * TC_PARTS, next_col = a.transposed ? TC_THREADS / 8 : 0;   // from one piece to the next
     auto fetch = [&](long long tile, int chunk) {
         const bool second = chunk >= chunks;
         const int width = second ? k2 : k, c0 = (second ? chunk - chunks : chunk) * TC_CHUNK;
-        const W* w = static_cast<const W*>(second ? a.weight2 : a.weight) + min(my_col, n - 1) * (a.transposed ? k : 1);
-        const int of_row = a.transposed ? 1 : n;
+        const W* w = static_cast<const W*>(second ? a.weight2 : a.weight);
+        const int of_channel = a.transposed ? 1 : n, of_column = a.transposed ? k : 1;
 #pragma unroll
         for (int u = 0; u < TC_U; u++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) next_w[u][e] = w[min(c0 + my_cw + 4 * TC_PARTS * u + e, width - 1) * of_row];
+            for (int e = 0; e < 4; e++) next_w[u][e] = w[min(c0 + my_cw + next_cw * u + e, width - 1) * of_channel + min(my_col + next_col * u, n - 1) * of_column];
         const float* rows = second ? x2 : x;
         const int c = c0 + my_c;
 #pragma unroll
@@ -122,8 +126,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) mix_forward_tensor(MixArgs a) {
             const float4 q = next_x[u];
             store_terms(buffer, my_c / 4 * TC_CHANNEL_BLOCKS + (row >> 3) * TC_ROW_BLOCKS + (row & 7) * 16, have > 0 ? q.x : 0.f, have > 1 ? q.y : 0.f,
                         have > 2 ? q.z : 0.f, have > 3 ? q.w : 0.f);
-            const int cw = my_cw + 4 * TC_PARTS * u, have_w = my_col < n ? width - c0 - cw : 0;
-            store_terms(buffer + 2 * TC_OPERAND, cw / 4 * TC_CHANNEL_BLOCKS + (my_col >> 3) * TC_ROW_BLOCKS + (my_col & 7) * 16,
+            const int cw = my_cw + next_cw * u, col = my_col + next_col * u, have_w = col < n ? width - c0 - cw : 0;
+            store_terms(buffer + 2 * TC_OPERAND, cw / 4 * TC_CHANNEL_BLOCKS + (col >> 3) * TC_ROW_BLOCKS + (col & 7) * 16,
                         have_w > 0 ? to_float(next_w[u][0]) : 0.f, have_w > 1 ? to_float(next_w[u][1]) : 0.f, have_w > 2 ? to_float(next_w[u][2]) : 0.f,
                         have_w > 3 ? to_float(next_w[u][3]) : 0.f);
         }
