@@ -324,8 +324,8 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, mix_forward_ctas(NT, WAY)) mix
     const bool split_w = a.weight_dtype == PL_F32, bulk_out = aligned16(a.out);
     TO* o_s = reinterpret_cast<TO*>(stage + at.r_at);
     const u32 stage_at = shared_address(stage);
-    // What has been asked for is there for all lanes; false once it did not come.  (The copies of x and x2 and those of a residual are
-    // committed in turn: one group may be on its way behind the one that is waited for.)
+    // What has been asked for is there for all lanes; false once it did not come.  (One group of copies has to be committed behind the one
+    // that is waited for: a tile's residual behind its x and x2, the next x and x2 behind a residual.)
     auto arrived = [&](u64* bar, int parity, bool before) {
         cp_async_wait_one();
         const bool there = before && mbar_wait(bar, parity);
@@ -371,11 +371,15 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, mix_forward_ctas(NT, WAY)) mix
                 if (a.x_codes) keep(reinterpret_cast<const TI*>(stage), k, at.x, a.x_codes, a.x_scales, false);
                 if (a.x2_codes) keep(reinterpret_cast<const TI*>(stage + at.x2_at), k2, at.x2, a.x2_codes, a.x2_scales, false);
             }
-            if (r0 + BLOCK >= rows_here) {
+            const bool last = r0 + BLOCK >= rows_here;
+            if (last) {
                 __syncwarp();
                 if (alive) fetch_x(tile + step);
             }
-            if (r0 == 0 && residual) alive = arrived(&bars[1], parity, alive);
+            if (r0 == 0 && residual) {
+                if (!last) cp_async_commit();   // in a tile of several blocks the next x is not on its way yet: an empty group in its place
+                alive = arrived(&bars[1], parity, alive);
+            }
             // The lane's 2 MT rows, 8 m + g of the block: z[m].
             constexpr int R = 2 * MT;
             const int ns = at.out.stride, row = (r0 + g) * ns + 2 * t;
