@@ -28,3 +28,21 @@ def test_residuals_of_tiles_of_several_blocks(plb, rows, k, k2, n, offset):
         for checkpoint in (None, "8bit"):
             out, _ = plb.channel_mix_raw(**a, activation=activation, residual_scale=-1.0, checkpoint=checkpoint)
             ref.assert_within(out, want, bound, "%s %s" % (activation, checkpoint))
+
+
+@pytest.mark.parametrize("dtype,weight_dtype", [(F32, F32), (F16, F16), (BF16, BF16), (BF16, F32)])
+@pytest.mark.parametrize("rows,k,k2,n", [(700, 3, 100, 3), (701, 100, 2, 4), (130, 4, 73, 2), (1025, 128, 4, 4), (33, 2, 128, 2)])
+def test_gradients_of_a_narrow_input_beside_a_wide_one(plb, rows, k, k2, n, dtype, weight_dtype):
+    """Up to four channels of one input and of the output, and another input too wide for one pass."""
+    for activation, scale in ((None, 0.25), ("relu", 1.0), ("softmax", -1.0)):
+        a, g = make(rows, k, k2, n, dtype, weight_dtype)
+        for checkpoint in (None, "8bit"):
+            out, saved = plb.channel_mix_raw(**a, activation=activation, residual_scale=scale, checkpoint=checkpoint)
+            y, x, x2 = (plb.unpack_activations(t, F32) if isinstance(t, plb.PackedActivations) else t
+                        for t in (saved.out, saved.x, saved.x2))
+            want = ref.gradients(g, y, x, a["weight"], x2, a["weight2"], activation, scale)
+            d = plb.channel_mix_backward(g, saved, a["weight"], a["weight2"], activation, scale, needs_of(a))
+            for m in needs_of(a):
+                ref.assert_within(getattr(d, m), *want[m], "%s of %s" % (m, activation))
+                one = plb.channel_mix_backward(g, saved, a["weight"], a["weight2"], activation, scale, (m,))
+                assert torch.equal(getattr(one, m), getattr(d, m))
