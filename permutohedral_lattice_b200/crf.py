@@ -86,8 +86,9 @@ class DenseCRF:
                  bilateral_weight=1.0, spatial_weight=1.0, compatibility=None, label_bias=None, checkpoint=None):
         """image [B, *S, R] float32 on the GPU; compatibility [L, L] (default: Potts, 1 - identity).
         bilateral_weight, spatial_weight: numbers, or tensors of one value or [L] (a weight for each label that sends
-        messages); label_bias: None or [L].  Tensors that require grad are learned.  checkpoint: None or "8bit", how the
-        steps keep what their backward pass needs."""
+        messages); label_bias: None or [L].  Tensors that require grad are learned: every step takes them as they are then,
+        whatever their device, type or order; other tensors are constants, taken now.  checkpoint: None or "8bit", how the steps
+        keep what their backward pass needs."""
         shape = tuple(image.shape[:-1])
         self.n_labels = int(n_labels)
         self.bilateral = Lattice(image, None, True, theta_alpha, theta_beta, 1.0, max_channels=n_labels)
@@ -97,22 +98,31 @@ class DenseCRF:
         self.checkpoint = checkpoint
         self.bilateral_weight = self._weight(bilateral_weight, "bilateral_weight", image.device)
         self.spatial_weight = self._weight(spatial_weight, "spatial_weight", image.device)
-        self.label_bias = None if label_bias is None else label_bias.to(device=image.device, dtype=torch.float32)
+        self.label_bias = None if label_bias is None else self._parameter(label_bias, image.device)
         if label_bias is not None and tuple(label_bias.shape) != (self.n_labels,):
             raise ValueError("label_bias must be [n_labels]")
         # None: Potts model (1 - identity), which the kernel evaluates without the L x L product
-        self.compatibility = None if compatibility is None else compatibility.to(
-            device=image.device, dtype=torch.float32).contiguous()
+        self.compatibility = None if compatibility is None else self._parameter(compatibility, image.device)
         if self.compatibility is not None and tuple(self.compatibility.shape) != (self.n_labels, self.n_labels):
             raise ValueError("compatibility must be [n_labels, n_labels]")
 
     def _weight(self, w, name, device):
-        """A number where nothing can be learned, else a float32 tensor of one value or [n_labels]."""
+        """A number where nothing can be learned, else a tensor of one value or [n_labels]."""
         if not isinstance(w, torch.Tensor) or (w.numel() == 1 and not w.requires_grad):
             return float(w)
         if tuple(w.shape) not in ((), (1,), (self.n_labels,)):
             raise ValueError("%s must be a number, or a tensor of one value or [n_labels]" % name)
-        return w.to(device=device, dtype=torch.float32)
+        return self._parameter(w, device)
+
+    @staticmethod
+    def _parameter(t, device):
+        """What to keep of a tensor: one that is learned as it was given, since a copy would not follow its optimizer; a constant
+        as the kernels take it."""
+        return t if t.requires_grad else DenseCRF._as_taken(t, device)
+
+    @staticmethod
+    def _as_taken(t, device):
+        return t.to(device=device, dtype=torch.float32).contiguous()
 
     def _by_channel_mix(self):
         """Whether a step has parameters that pl_crf_update_f32 does not take, or has to know their gradients."""
@@ -124,10 +134,11 @@ class DenseCRF:
         return 1.0 - torch.eye(self.n_labels, device=device)
 
     def _mix_weights(self, device):
-        """What a step's `channel_mix` multiplies the filtered distributions with: minus weight times compatibility."""
-        compatibility = self._potts(device) if self.compatibility is None else self.compatibility
-        return tuple(-(w.reshape(-1, 1) if isinstance(w, torch.Tensor) else w) * compatibility
-                     for w in (self.bilateral_weight, self.spatial_weight))
+        """What a step's `channel_mix` multiplies the filtered distributions with, minus weight times compatibility, and its bias."""
+        compatibility = self._potts(device) if self.compatibility is None else self._as_taken(self.compatibility, device)
+        return tuple(-(self._as_taken(w, device).reshape(-1, 1) if isinstance(w, torch.Tensor) else w) * compatibility
+                     for w in (self.bilateral_weight, self.spatial_weight)) + (
+                         None if self.label_bias is None else self._as_taken(self.label_bias, device),)
 
     def step(self, q, unaries):
         """Q after one mean-field update."""
@@ -138,12 +149,12 @@ class DenseCRF:
         grad = torch.is_grad_enabled()
         if self._by_channel_mix():
             self._check_step(q, unaries)
-            wb, ws = self._mix_weights(q.device) if mix_weights is None else mix_weights
+            wb, ws, bias = self._mix_weights(q.device) if mix_weights is None else mix_weights
             if grad and q.requires_grad:
                 qb, qs = (_LatticeApplyFunction.apply(lattice, q) for lattice in (self.bilateral, self.spatial))
             else:
                 qb, qs = self.bilateral.apply(q), self.spatial.apply(q)
-            return channel_mix(qb, wb, self.label_bias, unaries, qs, ws, "softmax", -1.0, self.checkpoint)
+            return channel_mix(qb, wb, bias, unaries, qs, ws, "softmax", -1.0, self.checkpoint)
         if grad and (q.requires_grad or unaries.requires_grad):
             self._check_step(q, unaries)
             return _CrfStepFunction.apply(self, q, unaries)
@@ -166,11 +177,12 @@ class DenseCRF:
         qs = self.spatial.apply(q)
         out = torch.empty_like(qb)
         n_points = out.numel() // self.n_labels
+        compatibility = None if self.compatibility is None else self._as_taken(self.compatibility, out.device)
         with torch.cuda.device(out.device):
             capi.check(capi.lib().pl_crf_update_f32(
                 out.data_ptr(), unaries.data_ptr(), qb.data_ptr(), qs.data_ptr(),
-                0 if self.compatibility is None else self.compatibility.data_ptr(), self.bilateral_weight,
-                self.spatial_weight, n_points, self.n_labels, _stream_handle(out.device)), "pl_crf_update_f32")
+                0 if compatibility is None else compatibility.data_ptr(), self.bilateral_weight, self.spatial_weight,
+                n_points, self.n_labels, _stream_handle(out.device)), "pl_crf_update_f32")
         return out
 
     def _fused_step(self, q, unaries):
