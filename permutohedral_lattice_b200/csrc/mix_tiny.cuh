@@ -72,7 +72,7 @@ __device__ __forceinline__ void store_tiny_row(T* rows, const float (&v)[TINY], 
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(256) mix_tiny(MixArgs a) {
+__global__ void __launch_bounds__(256, 2) mix_tiny(MixArgs a) {
     __shared__ __align__(16) T pack_s[8][32 * TINY_ROWS * TINY];   // a warp's rows on their way to 8 bits
     const int k = a.k, k2 = a.k2, n = a.n, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     TinyWeights v;
