@@ -200,6 +200,7 @@ int pl_profile_next_call(void** stage_events);
  * q_bilateral / q_spatial are the current label distributions filtered through the appearance and the
  * smoothness kernel (pl_lattice_apply_f32 on two lattices built once per image); compatibility is
  * [n_labels][n_labels] row-major, or NULL for the Potts model (1 - identity).  n_labels <= 128.
+ * A point whose unaries are all +infinity (no label is allowed: padding) comes out as zeros, here and in the two calls below.
  * q_out must not overlap the inputs.  No counterpart in the reference: it ships no CRF code, its README
  * (README.md:15-16) names CRF-as-RNN as the user the filter was written for; this is the step either
  * side of the filter in that user. */

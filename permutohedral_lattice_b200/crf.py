@@ -30,6 +30,7 @@ from torch.autograd.function import once_differentiable
 
 from . import capi
 from .channel_mix import MixSaved, PackedActivations, channel_mix, channel_mix_backward, pack_activations
+from .channel_mix import _backward as _mix_backward
 from .lattice_filter import Lattice, _OnDevice, _check_tensor, _float32_only, _stream_handle, _watched_by_torch
 
 
@@ -45,6 +46,32 @@ class _LatticeApplyFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         return None, ctx.lattice.apply(grad, reverse=True)
+
+
+def _start_kernel(unaries):
+    u = unaries.contiguous()
+    q = torch.empty_like(u)
+    with _OnDevice(u.device):
+        capi.check(capi.lib().pl_crf_start_f32(q.data_ptr(), u.data_ptr(), u.numel() // u.shape[-1], u.shape[-1],
+                                               _stream_handle(u.device)), "pl_crf_start_f32")
+    return q
+
+
+class _CrfStartFunction(torch.autograd.Function):
+    """softmax(-unaries) by the kernel that inference starts with.  Its gradient is a step's, without messages."""
+
+    @staticmethod
+    def forward(ctx, unaries):
+        out = _start_kernel(unaries)
+        ctx.save_for_backward(out)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        (out,) = ctx.saved_tensors
+        weight = out.new_empty((1, out.shape[-1]))       # of no input: this gradient does not depend on it
+        return _mix_backward(out.device, grad, out, None, None, weight, None, "softmax", -1.0, ("residual",)).residual
 
 
 class _CrfStepFunction(torch.autograd.Function):
@@ -210,18 +237,16 @@ class DenseCRF:
 
     @staticmethod
     def _start(unaries):
-        """softmax(-unaries), in one kernel where pl_crf_start_f32 takes them and torch does not follow them: a tracer,
-        a transform or a tensor of another class would not see the kernel, torch's softmax they do."""
+        """softmax(-unaries), zeros where every label is forbidden, in one kernel where pl_crf_start_f32 takes them and torch
+        does not follow them: a tracer, a transform or a tensor of another class would not see the kernel, torch's operations
+        they do."""
         if type(unaries) is not torch.Tensor or _watched_by_torch() or not unaries.is_cuda \
-                or unaries.dtype != torch.float32 or unaries.requires_grad or unaries.dim() < 1 \
-                or not 1 <= unaries.shape[-1] <= 128:
-            return torch.softmax(-unaries, dim=-1)
-        u = unaries.contiguous()
-        q = torch.empty_like(u)
-        with _OnDevice(u.device):
-            capi.check(capi.lib().pl_crf_start_f32(q.data_ptr(), u.data_ptr(), u.numel() // u.shape[-1], u.shape[-1],
-                                                   _stream_handle(u.device)), "pl_crf_start_f32")
-        return q
+                or unaries.dtype != torch.float32 or unaries.dim() < 1 or not 1 <= unaries.shape[-1] <= 128:
+            nothing = torch.isposinf(unaries).all(-1, keepdim=True)
+            return torch.softmax(-unaries.masked_fill(nothing, 0.0), dim=-1).masked_fill(nothing, 0.0)
+        if torch.is_grad_enabled() and unaries.requires_grad:
+            return _CrfStartFunction.apply(unaries)
+        return _start_kernel(unaries)
 
     def infer(self, unaries, iterations=5):
         """Q after `iterations` mean-field updates, starting from softmax(-unaries)."""

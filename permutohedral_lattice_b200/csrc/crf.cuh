@@ -18,6 +18,9 @@ __host__ __forceinline__ size_t crf_smem_bytes(int tpb, int L) {
     return sizeof(float) * ((size_t)2 * tpb * crf_row_stride(L) + (size_t)L * L);
 }
 
+__device__ __forceinline__ float crf_shift(float largest) { return largest == -INFINITY ? 0.f : largest; }
+__device__ __forceinline__ float crf_factor(float den) { return den == 0.f ? 0.f : PL_FDIV(1.f, den); }   // 1 at least, where there is a label
+
 // One CTA per TPB consecutive points, whose [point][label] blocks are contiguous in memory: the block is
 // loaded with coalesced accesses (message and negated unaries formed on the way), then one thread per
 // point does the L x L product, the softmax, and the block leaves the same way it came.
@@ -27,6 +30,8 @@ __host__ __forceinline__ size_t crf_smem_bytes(int tpb, int L) {
 // shared memory).
 // qb == nullptr: no message yet, the distributions that an inference starts from (softmax of -unaries; as torch
 // operations a negation and a softmax, 21 us on 375x500 x 21, so 11).
+// A point whose logits are all -infinity (unaries that forbid every label: padding) comes out as zeros: as NaN it would
+// spread through the next filter to all points that share a vertex with it.
 template <int TPB, int LT>
 __global__ void __launch_bounds__(TPB)
 crf_update(float* __restrict__ q_out, const float* __restrict__ unaries, const float* __restrict__ qb,
@@ -78,13 +83,14 @@ crf_update(float* __restrict__ q_out, const float* __restrict__ unaries, const f
                 zr[k] = PL_FADD(zr[k], -PL_FADD(sum, -mr[k]));
                 mx = fmaxf(mx, zr[k]);
             }
+            mx = crf_shift(mx);
             float den = 0.f;
 #pragma unroll
             for (int k = 0; k < LT; k++) {
                 zr[k] = expf(PL_FADD(zr[k], -mx));
                 den = PL_FADD(den, zr[k]);
             }
-            const float inv = PL_FDIV(1.f, den);
+            const float inv = crf_factor(den);
 #pragma unroll
             for (int k = 0; k < LT; k++) m[k] = PL_FMUL(zr[k], inv);
         } else {
@@ -106,13 +112,14 @@ crf_update(float* __restrict__ q_out, const float* __restrict__ unaries, const f
                     mx = fmaxf(mx, zk);
                 }
             }
+            mx = crf_shift(mx);
             float den = 0.f;
             for (int k = 0; k < L; k++) {
                 const float ex = expf(PL_FADD(z[k], -mx));
                 m[k] = ex;
                 den = PL_FADD(den, ex);
             }
-            const float inv = PL_FDIV(1.f, den);
+            const float inv = crf_factor(den);
             for (int k = 0; k < L; k++) m[k] = PL_FMUL(m[k], inv);
         }
     }
@@ -314,13 +321,14 @@ crf_slices(Geom g, float* __restrict__ q_out, const float* __restrict__ unaries,
                 m[j] = PL_FADD(-u[j], -PL_FADD(sum, -m[j]));
                 mx = fmaxf(mx, m[j]);
             }
+        mx = crf_shift(mx);
 #pragma unroll
         for (int j = 0; j < VP; j++)
             if (j < C) {
                 m[j] = expf(PL_FADD(m[j], -mx));
                 den = PL_FADD(den, m[j]);
             }
-        const float inv = PL_FDIV(1.f, den);
+        const float inv = crf_factor(den);
         float* o = rows_s + tid * C;
 #pragma unroll
         for (int j = 0; j < VP; j++)

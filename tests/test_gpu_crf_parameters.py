@@ -1,8 +1,10 @@
 """DenseCRF's learned parameters and its points without any label."""
+import math
+
 import pytest
 import torch
 
-from test_gpu_crf_training import plb  # noqa: F401
+from test_gpu_crf_training import FULL, PACKED, _assert_near, _Filter, _matrix, _rounded, _Update, plb  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +48,96 @@ def test_learned_parameters_are_followed(plb, learned, kind):
     assert float((results[0] - results[1]).abs().max()) > 1e-2
     assert float((crf.step(results[1], u).detach() - plb.DenseCRF(image, labels, 4.0, 0.4, 1.5, **{
         learned: p.detach().to("cuda", torch.float32).contiguous()}).step(results[1], u)).abs().max()) <= 1e-4
+
+
+class _PaddedUpdate(_Update):
+    """A step in 64 bits in which a point without a label comes out as zeros (its gradient, through its output, is zero then)."""
+
+    @staticmethod
+    def forward(ctx, qb, qs, wb, ws, bias, u, keep):
+        z = bias - u + qb @ wb + qs @ ws
+        nothing = (z == -math.inf).all(-1, keepdim=True)
+        y = torch.softmax(z.masked_fill(nothing, 0.0), -1).masked_fill(nothing, 0.0)
+        ctx.save_for_backward(keep(qb), keep(qs), keep(y), wb, ws)
+        return y
+
+
+ITERATIONS = 3
+
+
+@pytest.mark.parametrize("checkpoint", [None, "8bit"])
+@pytest.mark.parametrize("learned", [False, True])
+@pytest.mark.parametrize("shape,labels,compatible", [((2, 7, 9), 5, False), ((1, 11, 6), 21, False), ((1, 11, 6), 21, True), ((1, 4, 5, 6), 3, False),
+                                                     ((1, 9, 5), 40, False), ((1, 5, 9), 34, True)])
+def test_points_without_a_label(plb, shape, labels, compatible, learned, checkpoint):
+    """Padding (every label forbidden) comes out as zeros, sends nothing, and takes no gradient; forbidden labels get nothing."""
+    g = torch.Generator().manual_seed(sum(shape) + labels)
+    image = torch.rand(shape + (3 if len(shape) == 3 else 1,), generator=g).cuda()
+    u = 2.0 * torch.randn(shape + (labels,), generator=g)
+    u = torch.where(torch.rand(u.shape, generator=g) < 0.2, math.inf, u)
+    padding = torch.rand(shape, generator=g) < 0.15
+    padding.view(-1)[0] = True
+    u[padding] = math.inf
+    u, padding = u.cuda(), torch.isinf(u).all(-1).cuda()      # (of three labels some points have all forbidden one by one)
+    grad = torch.randn(shape + (labels,), generator=g).cuda()
+    compatibility = torch.rand((labels, labels), generator=g) if compatible else 1.0 - torch.eye(labels)
+    params = [torch.tensor(1.5), torch.tensor(0.75), compatibility, torch.randn(labels, generator=g) if learned else torch.zeros(labels)]
+    if learned:
+        leaves = [p.cuda().requires_grad_(True) for p in params]
+        crf = plb.DenseCRF(image, labels, 4.0, 0.4, 1.5, *leaves, checkpoint=checkpoint)
+    else:
+        leaves = []
+        crf = plb.DenseCRF(image, labels, 4.0, 0.4, 1.5, 1.5, 0.75, compatibility if compatible else None, checkpoint=checkpoint)
+    with torch.no_grad():
+        plain = crf.infer(u, ITERATIONS)
+    u.requires_grad_(True)
+    out = crf.infer(u, ITERATIONS)
+    got = torch.autograd.grad(out, [u] + leaves, grad)
+
+    b, n = crf.bilateral.call.batch, crf.bilateral.call.n
+    mats = [[_matrix(lat, labels, r) for r in (False, True)] for lat in (crf.bilateral, crf.spatial)]
+    wide = u.detach().double().cpu().view(b, n, labels).requires_grad_(True)
+    wp = [p.double().requires_grad_(True) for p in params]
+    keep = _rounded if checkpoint else (lambda t: t)
+    nothing = torch.isinf(wide.detach()).all(-1, keepdim=True)
+    q = torch.softmax(-wide.masked_fill(nothing, 0.0), -1).masked_fill(nothing, 0.0)
+    for _ in range(ITERATIONS):
+        q = _PaddedUpdate.apply(_Filter.apply(q, *mats[0]), _Filter.apply(q, *mats[1]), -wp[0] * wp[2], -wp[1] * wp[2], wp[3], wide, keep)
+    want = torch.autograd.grad(q, [wide] + wp[:len(leaves)], grad.double().cpu().view(b, n, labels))
+
+    for o in (plain, out.detach(), crf.infer(u.detach(), 0), crf.infer(u, 0).detach()):
+        assert bool(torch.isfinite(o).all()) and bool((o[padding] == 0).all()) and bool((o[torch.isinf(u.detach())] == 0).all())
+        assert float((o.sum(-1) - (~padding).float()).abs().max()) <= 1e-5
+    _assert_near(plain, q.detach().reshape(out.shape), FULL, "q")
+    _assert_near(out, q.detach().reshape(out.shape), FULL, "q")
+    assert bool((got[0][torch.isinf(u.detach())] == 0).all())
+    for name, a, w in zip(("unaries", "bilateral_weight", "spatial_weight", "compatibility", "label_bias"), got, want):
+        _assert_near(a, w, PACKED if checkpoint else FULL, name)
+
+
+@pytest.mark.parametrize("labels", [1, 2, 5, 33, 128])
+def test_the_start_of_an_inference(plb, labels):
+    """The kernel's softmax and its gradient; torch's where torch follows the unaries or the kernel does not take them."""
+    g = torch.Generator().manual_seed(labels)
+    u = 3.0 * torch.randn((2, 50, labels), generator=g)
+    u[torch.rand(u.shape, generator=g) < 0.3] = math.inf
+    u[0, 3] = math.inf
+    u[:, 7] = 1.0
+    grad = torch.randn(u.shape, generator=g)
+    nothing = torch.isinf(u).all(-1, keepdim=True)
+    wide = u.double().requires_grad_(True)
+    want = torch.softmax(-wide.masked_fill(nothing, 0.0), -1).masked_fill(nothing, 0.0)
+    (want_du,) = torch.autograd.grad(want, [wide], grad.double())
+    for x in (u.cuda(), u, u.cuda().double(), u.cuda().transpose(0, 1).contiguous().transpose(0, 1)):
+        leaf = x.clone().requires_grad_(True) if x.is_contiguous() else x.detach().requires_grad_(True)
+        q = plb.DenseCRF._start(leaf)
+        (du,) = torch.autograd.grad(q, [leaf], grad.to(q))
+        # an exponential, a quotient and a sum of up to 128 terms: 1e-6 as elsewhere; the gradient's sum of up to 128 products of
+        # values and upstream gradients of up to 5 again
+        assert float((q.detach().cpu().double() - want.detach()).abs().max()) <= 1e-6
+        assert float((du.cpu().double() - want_du).abs().max()) <= 1e-5
+        assert not bool(q.detach().cpu()[nothing.expand(u.shape)].any()) and not bool(du.cpu()[torch.isinf(u)].any())
+        with torch.no_grad():
+            assert float((plb.DenseCRF._start(leaf) - q).abs().max()) <= 1e-6
+    padded = torch.func.vmap(plb.DenseCRF._start)(u.cuda())
+    assert float((padded.cpu().double() - want.detach()).abs().max()) <= 1e-6
