@@ -82,12 +82,13 @@ class _CrfStepFunction(torch.autograd.Function):
         out = crf._constant_step(q, unaries)
         ctx.crf, ctx.weights = crf, (crf.bilateral_weight, crf.spatial_weight)
         ctx.packed = None
+        compatibility = None if crf.compatibility is None else crf._as_taken(crf.compatibility, out.device)
         if crf.checkpoint:
             packed = pack_activations(out)
             ctx.packed = packed.shape, packed.dtype
-            ctx.save_for_backward(crf.compatibility, packed.codes, packed.scales)
+            ctx.save_for_backward(compatibility, packed.codes, packed.scales)
         else:
-            ctx.save_for_backward(crf.compatibility, out)
+            ctx.save_for_backward(compatibility, out)
         return out
 
     @staticmethod
@@ -149,6 +150,7 @@ class DenseCRF:
 
     @staticmethod
     def _as_taken(t, device):
+        """A kept parameter as the kernels take it: whether or not it is still learned."""
         return t.to(device=device, dtype=torch.float32).contiguous()
 
     def _by_channel_mix(self):

@@ -50,6 +50,26 @@ def test_learned_parameters_are_followed(plb, learned, kind):
         learned: p.detach().to("cuda", torch.float32).contiguous()}).step(results[1], u)).abs().max()) <= 1e-4
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("learned", ["bilateral_weight", "compatibility", "label_bias"])
+def test_parameters_that_are_learned_no_longer(plb, learned, kind):
+    """Frozen after the CRF was made: constants from then on, the unaries still have their gradient."""
+    labels = 5
+    image, u = _image_and_unaries(labels=labels)
+    g = torch.Generator().manual_seed(2)
+    p = KINDS[kind](torch.rand((labels, labels) if learned == "compatibility" else (labels,), generator=g)).detach().requires_grad_(True)
+    crf = plb.DenseCRF(image, labels, 4.0, 0.4, 1.5, **{learned: p})
+    p.requires_grad_(False)
+    fresh = plb.DenseCRF(image, labels, 4.0, 0.4, 1.5, **{learned: p})
+    u.requires_grad_(True)
+    results = []
+    for c in (crf, fresh):
+        q = c.infer(u, 2)
+        results.append((q.detach(), *torch.autograd.grad((q * q).sum(), [u])))
+    for a, b in zip(*results):
+        assert float((a - b).abs().max()) <= 1e-4 * max(1.0, float(b.abs().max()))
+
+
 class _PaddedUpdate(_Update):
     """A step in 64 bits in which a point without a label comes out as zeros (its gradient, through its output, is zero then)."""
 
