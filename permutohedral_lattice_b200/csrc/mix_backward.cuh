@@ -262,6 +262,23 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, MB * NB > 12 ? 2 : 3) mix_back
                 for (int o = 1; o < 4; o <<= 1)
 #pragma unroll
                     for (int p = 0; p < 4; p++) sum[p] += __shfl_xor_sync(~0u, sum[p], o);
+                // A row that came out as zeros has no gradient, whatever comes from above: -1 / 0 of a logarithm, say.  (One vote, where all
+                // sums are finite.)
+                bool odd = false;
+#pragma unroll
+                for (int p = 0; p < 4; p++) odd |= !(fabsf(sum[p]) < INFINITY);
+                if (__any_sync(~0u, odd)) {
+#pragma unroll
+                    for (int p = 0; p < 4; p++) {
+                        bool any = false;
+#pragma unroll
+                        for (int j = 0; j < J; j++) any |= y[p][j] != 0.f;
+                        if (__ballot_sync(~0u, any) >> (lane & 28) & 15u) continue;
+                        sum[p] = 0.f;
+#pragma unroll
+                        for (int j = 0; j < J; j++) d[p][j] = 0.f;
+                    }
+                }
 #pragma unroll
                 for (int p = 0; p < 4; p++)
 #pragma unroll
@@ -528,6 +545,8 @@ __global__ void __launch_bounds__(256) mix_dz(MixBackArgs a) {
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+        if (a.activation == PL_ACT_SOFTMAX && !__any_sync(~0u, y[0] != 0.f || y[1] != 0.f || y[2] != 0.f || y[3] != 0.f))
+            s = g[0] = g[1] = g[2] = g[3] = 0.f;   // a row of zeros has no gradient (see mix_backward)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int c = lane + 32 * j;

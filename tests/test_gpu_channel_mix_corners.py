@@ -46,3 +46,31 @@ def test_gradients_of_a_narrow_input_beside_a_wide_one(plb, rows, k, k2, n, dtyp
                 ref.assert_within(getattr(d, m), *want[m], "%s of %s" % (m, activation))
                 one = plb.channel_mix_backward(g, saved, a["weight"], a["weight2"], activation, scale, (m,))
                 assert torch.equal(getattr(one, m), getattr(d, m))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("checkpoint", [None, "8bit"])
+@pytest.mark.parametrize("rows,k,k2,n", [(700, 21, 21, 21), (1001, 2, 2, 2), (333, 3, 0, 4), (97, 8, 8, 8), (300, 75, 0, 16), (130, 64, 64, 64),
+                                         (257, 128, 128, 128), (41, 100, 5, 33)])
+def test_rows_of_zeros_have_no_gradient_whatever_comes_from_above(plb, rows, k, k2, n, dtype, checkpoint):
+    """The gradient of a logarithm of the output is infinite, or NaN, in a row without a label: nothing of it goes further."""
+    a, g = make(rows, k, k2, n, dtype, masked=True)
+    out, saved = plb.channel_mix_raw(**a, activation="softmax", residual_scale=-1.0, checkpoint=checkpoint)
+    empty = torch.isinf(a["residual"]).all(-1)
+    assert bool(empty[0, 0]) and not bool(empty.all())
+    bad = torch.tensor([math.nan, math.inf, -math.inf, 1.0], dtype=dtype, device="cuda")
+    place = torch.arange(rows * n, device="cuda").view(1, rows, n)
+    above = torch.where(empty[..., None], bad[place % 4], g)
+    needs = needs_of(a)
+    d = plb.channel_mix_backward(above, saved, a["weight"], a["weight2"], "softmax", -1.0, needs)
+    y, x, x2 = (plb.unpack_activations(t, F32) if isinstance(t, plb.PackedActivations) else t for t in (saved.out, saved.x, saved.x2))
+    want = ref.gradients(torch.where(empty[..., None], torch.zeros_like(g), g), y, x, a["weight"], x2, a["weight2"], "softmax", -1.0)
+    for m in needs:
+        ref.assert_within(getattr(d, m), *want[m], m)
+    assert not bool(d.residual[empty].any()) and not bool(d.x[empty].any())
+    # a row with a label passes on what is not finite
+    row = int((~empty[0]).nonzero()[0])
+    above = g.clone()
+    above[0, row] = math.nan
+    d = plb.channel_mix_backward(above, saved, a["weight"], a["weight2"], "softmax", -1.0, ("x", "residual"))
+    assert bool(torch.isnan(d.x[0, row]).all()) and bool(torch.isfinite(d.x[0, row + 1:]).all())
