@@ -28,7 +28,7 @@ static int launch_forward_tensor(const MixArgs& a, cudaStream_t st) {
 template <typename TO>
 static int forward_floats(const MixArgs& a, cudaStream_t st) {
     if constexpr (std::is_same<TO, float>::value) {
-        if (tiny(a.k, a.k2, a.n)) return launch_tiny<float>(a, st);
+        if (tiny(a.k, a.k2, a.n) && !a.transposed) return launch_tiny<float>(a, st);   // (which takes weights as they are)
     }
     if (a.n > 64 && tensor_pays(a)) {
         if constexpr (!std::is_same<TO, float>::value) {

@@ -11,13 +11,12 @@ constexpr int TINY = 4, TINY_ROWS = 4, TINY_BACK_ROWS = 2;   // channels; rows t
 struct TinyWeights {
     float w[TINY][TINY], w2[TINY][TINY];
 };
-// transposed: the (first and only) weight is [n][k].
-__device__ __forceinline__ void load_tiny_weights(TinyWeights& v, const void* weight, const void* weight2, int k, int k2, int n, int transposed, int dtype) {
+__device__ __forceinline__ void load_tiny_weights(TinyWeights& v, const void* weight, const void* weight2, int k, int k2, int n, int dtype) {
 #pragma unroll
     for (int j = 0; j < TINY; j++)
 #pragma unroll
         for (int c = 0; c < TINY; c++) {
-            v.w[j][c] = weight && j < k && c < n ? load_weight(weight, transposed ? c * k + j : j * n + c, dtype) : 0.f;
+            v.w[j][c] = weight && j < k && c < n ? load_weight(weight, j * n + c, dtype) : 0.f;
             v.w2[j][c] = weight2 && j < k2 && c < n ? load_weight(weight2, j * n + c, dtype) : 0.f;
         }
 }
@@ -76,7 +75,7 @@ __global__ void __launch_bounds__(256, 2) mix_tiny(MixArgs a) {
     __shared__ __align__(16) T pack_s[8][32 * TINY_ROWS * TINY];   // a warp's rows on their way to 8 bits
     const int k = a.k, k2 = a.k2, n = a.n, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     TinyWeights v;
-    load_tiny_weights(v, a.weight, a.weight2, k, k2, n, a.transposed, a.weight_dtype);
+    load_tiny_weights(v, a.weight, a.weight2, k, k2, n, a.weight_dtype);
     float bias[TINY];
 #pragma unroll
     for (int c = 0; c < TINY; c++) bias[c] = a.bias && c < n ? load_weight(a.bias, c, a.weight_dtype) : 0.f;
@@ -147,7 +146,7 @@ __global__ void __launch_bounds__(256, 2) mix_tiny_backward(MixBackArgs a) {
     __shared__ float sums_s[8][SUMS];
     const int k = a.k, k2 = a.k2, n = a.n, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     TinyWeights v;
-    load_tiny_weights(v, a.weight, a.weight2, k, k2, n, 0, a.weight_dtype);
+    load_tiny_weights(v, a.weight, a.weight2, k, k2, n, a.weight_dtype);
     float sums[2 * TINY + 1][TINY];   // dW, dW2, dbias
 #pragma unroll
     for (int j = 0; j <= 2 * TINY; j++)
