@@ -67,6 +67,9 @@ struct MixBackSmem {
     __host__ __device__ size_t bytes(int warps) const { return own0 + own_bytes * warps + 128; }   // (reads of eight channels pass the last one)
 };
 
+// 0 where the output is zero, NaN where it is: of a block in 8 bits that held an infinity nothing is known but that.
+__device__ __forceinline__ float relu_gradient(float y, float g) { return y > 0.f ? g : y * 0.f; }
+
 // PACKED: some of the output, x and x2 come in 8 bits; all are then read from floats of the warp's own memory.  One stage, and the
 // headers of its blocks in registers: there are at most 32 of the output and 96 of x or x2 in a tile (see narrow_any).
 template <typename T, bool PACKED, int MB, int NB>
@@ -287,7 +290,7 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, MB * NB > 12 ? 2 : 3) mix_back
 #pragma unroll
                 for (int p = 0; p < 4; p++)
 #pragma unroll
-                    for (int j = 0; j < J; j++) d[p][j] = y[p][j] > 0.f ? d[p][j] : 0.f;
+                    for (int j = 0; j < J; j++) d[p][j] = relu_gradient(y[p][j], d[p][j]);
             }
             if (!alive || here < 32) {
 #pragma unroll
@@ -551,7 +554,7 @@ __global__ void __launch_bounds__(256) mix_dz(MixBackArgs a) {
         for (int j = 0; j < 4; j++) {
             const int c = lane + 32 * j;
             if (c >= n) continue;
-            const float dz = a.activation == PL_ACT_SOFTMAX ? y[j] * (g[j] - s) : a.activation == PL_ACT_RELU ? (y[j] > 0.f ? g[j] : 0.f) : g[j];
+            const float dz = a.activation == PL_ACT_SOFTMAX ? y[j] * (g[j] - s) : a.activation == PL_ACT_RELU ? relu_gradient(y[j], g[j]) : g[j];
             a.dz[row * n + c] = dz;
             if (a.dresidual) static_cast<T*>(a.dresidual)[row * n + c] = from_float<T>(a.scale * dz);
         }

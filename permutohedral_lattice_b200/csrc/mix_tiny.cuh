@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(256, 2) mix_tiny_backward(MixBackArgs a) {
             const bool empty = y[u][0] == 0.f && y[u][1] == 0.f && y[u][2] == 0.f && y[u][3] == 0.f;   // of a softmax: no gradient (see mix_backward)
 #pragma unroll
             for (int c = 0; c < TINY; c++) {
-                dz[c] = a.activation == PL_ACT_SOFTMAX ? (empty ? 0.f : y[u][c] * (g[u][c] - s)) : a.activation == PL_ACT_RELU ? (y[u][c] > 0.f ? g[u][c] : 0.f) : g[u][c];
+                dz[c] = a.activation == PL_ACT_SOFTMAX ? (empty ? 0.f : y[u][c] * (g[u][c] - s)) : a.activation == PL_ACT_RELU ? relu_gradient(y[u][c], g[u][c]) : g[u][c];
                 dr[c] = a.scale * dz[c];
                 sums[2 * TINY][c] += dz[c];
             }

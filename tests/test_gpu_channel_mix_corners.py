@@ -74,3 +74,24 @@ def test_rows_of_zeros_have_no_gradient_whatever_comes_from_above(plb, rows, k, 
     above[0, row] = math.nan
     d = plb.channel_mix_backward(above, saved, a["weight"], a["weight2"], "softmax", -1.0, ("x", "residual"))
     assert bool(torch.isnan(d.x[0, row]).all()) and bool(torch.isfinite(d.x[0, row + 1:]).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,k,k2,n", [(300, 21, 21, 21), (301, 2, 2, 2), (95, 3, 0, 4), (130, 64, 0, 70), (260, 8, 8, 8)])
+def test_relu_of_what_is_not_finite(plb, rows, k, k2, n, dtype):
+    """An infinite output passes its gradient on; as a block in 8 bits, which comes back as NaN, the block's gradients are NaN:
+    no zeros that would pass for a mask.  A row that is NaN has gradients that are."""
+    a, g = make(rows, k, k2, n, dtype)
+    a["residual"][0, 40, 1] = math.inf
+    a["x"][0, 90, 0] = math.nan
+    for checkpoint in (None, "8bit"):
+        out, saved = plb.channel_mix_raw(**a, activation="relu", checkpoint=checkpoint)
+        assert bool(torch.isinf(out[0, 40, 1])) and bool(torch.isnan(out[0, 90]).all())
+        d = plb.channel_mix_backward(g, saved, a["weight"], a["weight2"], "relu", 1.0, ("x", "residual"))
+        y = out if checkpoint is None else plb.unpack_activations(saved.out, dtype)
+        bad = torch.isnan(y)
+        assert bool(bad[0, 90].all()) and bool(bad[0, 40, 1]) == (checkpoint is not None)
+        assert torch.equal(torch.isnan(d.residual), bad)
+        assert torch.equal(d.residual[~bad], torch.where(out > 0, g, torch.zeros_like(g))[~bad])
+        rows_bad = bad.any(-1)
+        assert torch.equal(torch.isnan(d.x).any(-1), rows_bad)
