@@ -324,8 +324,9 @@ typedef struct pl_kept {
  * dtype: of x, x2, residual, out and their gradients; weight_dtype: of weights, bias and their gradients, PL_F32 or dtype.
  * Products and sums are float or better whatever the types; every result is rounded once.  A row of a softmax whose z
  * are all -infinity (a residual that forbids every channel: a padded point) comes out as zeros, with zero gradients.  x and
- * the weights have to be finite, and below 3.402e38: a row of x that is not makes its row of out NaN.  Where out is NaN its
- * gradients are; so are those of a whole block of 32 values in 8 bits that holds an infinite value of out. */
+ * the weights have to be finite, and below 3.402e38: of a row of x that is not, each value of out is NaN or what the formula
+ * gives, infinities and what the activation makes of them.  Where out is NaN its gradients are; so are those of a
+ * whole block of 32 values in 8 bits that holds an infinite value of out. */
 typedef struct pl_mix {
     int64_t rows;
     int k, k2, n;

@@ -367,8 +367,9 @@ def channel_mix(x, weight, bias=None, residual=None, x2=None, weight2=None, acti
     "softmax" over the channels; a row whose channels are all forbidden by an infinite residual gives zeros and has no
     gradient.  checkpoint="8bit" keeps the activations that the backward pass needs in 8 bits: their gradients are those
     at the rounded activations, and x, x2 and the output may be freed in between.  x, x2 and the weights have to be finite
-    (a row that is not comes out NaN).  In a CUDA graph: one ordinary call before the capture, which sets the kernel up; forward
-    and backward together, on leaves made inside it."""
+    (of a row that is not, each value comes out NaN or as the formula gives it; other rows are as they would be).  In a CUDA
+    graph: one ordinary call before the capture, which sets the kernel up; forward and backward together, on leaves made inside
+    it."""
     device = _check_mix(x, weight, bias, residual, x2, weight2, activation, checkpoint)
     args = (x, weight, bias, residual, x2, weight2)
     if not _watched_by_torch() and not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args)):

@@ -95,3 +95,27 @@ def test_relu_of_what_is_not_finite(plb, rows, k, k2, n, dtype):
         assert torch.equal(d.residual[~bad], torch.where(out > 0, g, torch.zeros_like(g))[~bad])
         rows_bad = bad.any(-1)
         assert torch.equal(torch.isnan(d.x).any(-1), rows_bad)
+
+
+@pytest.mark.parametrize("dtype,weight_dtype", [(F32, F32), (BF16, BF16), (F16, F16), (BF16, F32)])
+@pytest.mark.parametrize("rows,k,k2,n", [(200, 2, 2, 2), (200, 3, 0, 4), (200, 4, 1, 3), (200, 21, 21, 21), (200, 64, 0, 16), (200, 40, 40, 40),
+                                         (200, 33, 0, 67), (200, 64, 64, 128)])
+def test_rows_that_are_not_finite(plb, rows, k, k2, n, dtype, weight_dtype):
+    """NaN in a row of x: all of its output is NaN, of relu too.  An infinity: each value is NaN or what the formula gives.
+    Other rows have the same bits."""
+    a, _ = make(rows, k, k2, n, dtype, weight_dtype)
+    bad = {7: math.nan, 40: math.inf, 41: -math.inf}
+    other = [r for r in range(rows) if r not in bad]
+    for activation in (None, "relu", "softmax"):
+        clean = plb.channel_mix(**a, activation=activation)
+        for name in ("x", "x2") if k2 else ("x",):
+            dirty = {**a, name: a[name].clone()}
+            for row, value in bad.items():
+                dirty[name][0, row, -1] = value
+            out = plb.channel_mix(**dirty, activation=activation)
+            assert torch.equal(out[0, other], clean[0, other])
+            assert bool(torch.isnan(out[0, 7]).all())
+            want, _ = ref.forward(dirty["x"], a["weight"], a["bias"], a["residual"], dirty["x2"], a["weight2"], activation, 1.0)
+            for row in (40, 41):
+                nan = torch.isnan(out[0, row])
+                assert torch.equal(out[0, row].double()[~nan], want[0, row][~nan]), (activation, name, row)
