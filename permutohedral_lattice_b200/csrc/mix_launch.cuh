@@ -34,7 +34,7 @@ static int launch_forward(MixArgs a, cudaStream_t st) {
     return PL_OK;
 }
 // Output channels in steps of 8: the accumulators of a warp's rows are in registers.  From 65 channels on a warp takes
-// 16 rows in place of 32.
+// 16 rows in place of 32, of 16-bit values: rows of floats have kernels of their own there (see forward_floats).
 template <typename TI, typename TO, int WAY>
 static int forward_of(const MixArgs& a, cudaStream_t st) {
     if (a.n <= 8) return launch_forward<TI, TO, 1, 2, WAY>(a, st);
@@ -42,11 +42,11 @@ static int forward_of(const MixArgs& a, cudaStream_t st) {
     if (a.n <= 24) return launch_forward<TI, TO, 3, 2, WAY>(a, st);
     if (a.n <= 32) return launch_forward<TI, TO, 4, 2, WAY>(a, st);
     if constexpr (WAY != MIX_PLAIN) {
-        return a.n <= 40   ? launch_forward<TI, TO, 5, 2, WAY>(a, st)
-               : a.n <= 48 ? launch_forward<TI, TO, 6, 2, WAY>(a, st)
-               : a.n <= 56 ? launch_forward<TI, TO, 7, 2, WAY>(a, st)
-               : a.n <= 64 ? launch_forward<TI, TO, 8, 2, WAY>(a, st)
-                           : launch_forward<TI, TO, 16, 1, WAY>(a, st);
+        if (a.n <= 40) return launch_forward<TI, TO, 5, 2, WAY>(a, st);
+        if (a.n <= 48) return launch_forward<TI, TO, 6, 2, WAY>(a, st);
+        if (a.n <= 56) return launch_forward<TI, TO, 7, 2, WAY>(a, st);
+        if (a.n <= 64) return launch_forward<TI, TO, 8, 2, WAY>(a, st);
+        if constexpr (sizeof(TI) == 2) return launch_forward<TI, TO, 16, 1, WAY>(a, st);
     }
     return PL_INTERNAL_ERROR;
 }
