@@ -24,6 +24,9 @@ parameters is
 
 as two filters and one `channel_mix`, whose backward pass gives every gradient in one pass over the points; the filters'
 gradients are the lattices' applied in reverse.  checkpoint="8bit" keeps a step's distributions in 8 bits until then.
+
+A label is forbidden by an infinite unary; a point without any (padding) has zeros from the start on, sends nothing and takes
+no gradient.
 """
 import torch
 from torch.autograd.function import once_differentiable

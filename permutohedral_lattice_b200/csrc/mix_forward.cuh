@@ -441,10 +441,11 @@ __global__ void __launch_bounds__(32 * MIX_WARPS, mix_forward_ctas(NT, WAY)) mix
 // ---------------------------------------------------------------------------------------------
 // Many channels out (65 and more) of float rows, what mix_forward_tensor does not take (see tensor_pays).  The weights of both inputs take up to 128 KB of shared memory, which leaves too
 // little for whole rows: a warp takes 16 rows, 32 channels at a time, by way of its registers (the next ones are on their way while
-// these are multiplied), reads the residual and writes its rows from registers.  154 401 rows of 128 + 128 channels to 128: 269 us (558
-// with whole rows in shared memory and four warps an SM; 8, 12 and 14 warps 289, 269 and 306; four blocks of columns at once in place
-// of eight 285).  Its floor is the tensor cores' 110 us, three products of 11-bit terms for one of floats at 276 TFLOP/s: they are
-// busy 43 % of the time, warps wait for products that they depend on.
+// these are multiplied), reads the residual and writes its rows from registers.  154 401 rows with a softmax: 101 + 101 channels to 101 210 us,
+// 67 + 67 to 67 150, 32 to 96 59, 16 to 68 41.  All columns are computed, up to 128 of them.  Its shape was chosen on 128 + 128 channels to 128,
+// which mix_forward_tensor has taken since: 269 us (558 with whole rows in shared memory and four warps an SM; 8, 12 and 14 warps 289, 269
+// and 306; four blocks of columns at once in place of eight 285), the tensor cores busy 43 % of the time (110 us, three products of 11-bit terms
+// for one of floats at 276 TFLOP/s), warps waiting for products that they depend on.
 // ---------------------------------------------------------------------------------------------
 constexpr int WIDE_WARPS = 12, WIDE_CHUNK = 32, WIDE_STRIDE = WIDE_CHUNK + 4;   // (rows of 36 floats: 8 rows by 4 channels in 32 banks)
 constexpr int WIDE_NT = 16;

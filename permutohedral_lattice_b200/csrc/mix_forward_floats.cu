@@ -37,7 +37,8 @@ static int forward_floats(const MixArgs& a, cudaStream_t st) {
         return launch_forward_tensor<TO, float>(a, st);
     }
     if (a.n > 64) return launch_forward_wide<TO>(a, st);
-    // Few products to a sum: what the tensor cores cut stays below 2^-21 of it (75 channels of one sign: 0.9e-6 off in all, so 0.2e-6).
+    // Few products to a sum: what the tensor cores cut stays below 2^-21 of it.  Two million rows of 75 channels of one sign to 16: 138 us
+    // and 7.3e-7 of the norm off, in parts 141 and 1.1e-7; 64 to 32 183 and 5.6e-7, in parts 189 and 1.2e-7.
     if (a.k + a.k2 <= 48 && a.n <= 32) return forward_of<float, TO, MIX_PLAIN>(a, st);
     return forward_of<float, TO, MIX_PARTED>(a, st);
 }
