@@ -245,7 +245,7 @@ class DenseCRF:
         """softmax(-unaries), zeros where every label is forbidden, in one kernel where pl_crf_start_f32 takes them and torch
         does not follow them: a tracer, a transform or a tensor of another class would not see the kernel, torch's operations
         they do."""
-        if type(unaries) is not torch.Tensor or _watched_by_torch() or not unaries.is_cuda \
+        if type(unaries) not in (torch.Tensor, torch.nn.Parameter) or _watched_by_torch() or not unaries.is_cuda \
                 or unaries.dtype != torch.float32 or unaries.dim() < 1 or not 1 <= unaries.shape[-1] <= 128:
             nothing = torch.isposinf(unaries).all(-1, keepdim=True)
             return torch.softmax(-unaries.masked_fill(nothing, 0.0), dim=-1).masked_fill(nothing, 0.0)

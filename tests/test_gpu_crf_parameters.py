@@ -161,3 +161,18 @@ def test_the_start_of_an_inference(plb, labels):
             assert float((plb.DenseCRF._start(leaf) - q).abs().max()) <= 1e-6
     padded = torch.func.vmap(plb.DenseCRF._start)(u.cuda())
     assert float((padded.cpu().double() - want.detach()).abs().max()) <= 1e-6
+
+
+def test_unaries_that_are_a_parameter_start_in_the_kernel(plb):
+    from permutohedral_lattice_b200 import capi
+    u = torch.nn.Parameter(torch.randn((1, 30, 5), generator=torch.Generator().manual_seed(1)).cuda())
+    want = torch.softmax(-u.detach().double(), -1)
+    for enabled in (True, False):
+        with torch.set_grad_enabled(enabled):
+            before = capi.lib().pl_launch_count()
+            q = plb.DenseCRF._start(u)
+            assert capi.lib().pl_launch_count() == before + 1 and type(q) is torch.Tensor and q.requires_grad == enabled
+            assert float((q.detach() - want).abs().max()) <= 1e-6
+    (du,) = torch.autograd.grad((plb.DenseCRF._start(u) ** 2).sum(), [u])
+    d = want * (2 * want - (2 * want * want).sum(-1, keepdim=True))
+    assert float((du + d).abs().max()) <= 1e-5
