@@ -37,8 +37,9 @@ static int forward_floats(const MixArgs& a, cudaStream_t st) {
         return launch_forward_tensor<TO, float>(a, st);
     }
     if (a.n > 64) return launch_forward_wide<TO>(a, st);
-    // Few products to a sum: what the tensor cores cut stays below 2^-21 of it.  Two million rows of 75 channels of one sign to 16: 138 us
-    // and 7.3e-7 of the norm off, in parts 141 and 1.1e-7; 64 to 32 183 and 5.6e-7, in parts 189 and 1.2e-7.
+    // Few products to a sum: what the tensor cores cut stays below 2^-21 of it.  Sums of one sign, off by parts of the norm: 16 x 512x512 rows of
+    // 21 + 21 channels to 21 with a softmax 227 us and 4.7e-7, in parts 248 and 1.3e-7; 8 to 8 67 and 1.4e-7 either way; two million rows of
+    // 75 channels to 16 138 and 7.3e-7, in parts 141 and 1.1e-7; 64 to 32 183 and 5.6e-7, in parts 189 and 1.2e-7.
     if (a.k + a.k2 <= 48 && a.n <= 32) return forward_of<float, TO, MIX_PLAIN>(a, st);
     return forward_of<float, TO, MIX_PARTED>(a, st);
 }
