@@ -26,8 +26,12 @@ def test_residuals_of_tiles_of_several_blocks(plb, rows, k, k2, n, offset):
     for activation in (None, "softmax"):
         want, bound = ref.forward(a["x"], a["weight"], a["bias"], a["residual"], a["x2"], a["weight2"], activation, -1.0)
         for checkpoint in (None, "8bit"):
-            out, _ = plb.channel_mix_raw(**a, activation=activation, residual_scale=-1.0, checkpoint=checkpoint)
+            out, saved = plb.channel_mix_raw(**a, activation=activation, residual_scale=-1.0, checkpoint=checkpoint)
             ref.assert_within(out, want, bound, "%s %s" % (activation, checkpoint))
+            for kept, t in ((saved.x, a["x"]), (saved.x2, a["x2"]), (saved.out, out)) if checkpoint else ():
+                if kept is not None:
+                    alone = plb.pack_activations(t)
+                    assert torch.equal(kept.codes, alone.codes) and torch.equal(kept.scales, alone.scales)
 
 
 @pytest.mark.parametrize("dtype,weight_dtype", [(F32, F32), (F16, F16), (BF16, BF16), (BF16, F32)])
