@@ -362,6 +362,64 @@ int pl_pack_activations(pl_packed packed, const void* x, int64_t n, int dtype, i
 /* No counterpart in the reference. */
 int pl_unpack_activations(void* x, pl_packed packed, int64_t n, int dtype, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------------
+ * What a network's blocks of features take besides: norms, dropout, the gated feed-forward block.  Rows are points, channels
+ * last, as above; dtype: of rows and their gradients.  The reference ships none of it. */
+
+typedef enum pl_norm_kind { PL_NORM_NONE = 0, PL_NORM_LAYER = 1, PL_NORM_RMS = 2 } pl_norm_kind;
+
+/* (x - mean) / sqrt(variance + eps) * weight + bias over a row's channels (layer), x / sqrt(mean of squares + eps) * weight + bias
+ * (rms); weight and bias (device) of the channels, NULL: ones, zeros. */
+typedef struct pl_norm {
+    int kind;   /* pl_norm_kind */
+    float eps;  /* > 0 */
+    const void *weight, *bias;
+} pl_norm;
+
+/* Value i of a tensor (in memory's order) is dropped where word i % 4 of Philox4x32-10 (Salmon et al. 2011) of the counter
+ * (i / 4, offset), 64 bits each, under `key` is below round(p 2^32); others are multiplied by 1 / (1 - p).  seed (device, NULL: the
+ * two numbers here): key and offset as two 64-bit integers, read when the kernel runs.  p = 0: nothing is dropped. */
+typedef struct pl_dropout {
+    double p;   /* 0 <= p < 1 */
+    uint64_t key, offset;
+    const int64_t* seed;
+} pl_dropout;
+
+/* h = residual_scale * residual + gate * dropout(after(x)),  y = before(h).  Each part may be missing: a norm of kind
+ * PL_NORM_NONE, a NULL residual or gate.  gate: a value a channel, or (gate_of_values) one for each of x.  vector_dtype: of norms' weights and
+ * biases, of a gate of the channels, and of their gradients, PL_F32 or dtype.  1 to 512 channels. */
+typedef struct pl_channel_norm_shape {
+    int64_t rows;
+    int channels;
+    int dtype, vector_dtype;   /* pl_dtype */
+    int gate_of_values;
+    float residual_scale;
+    pl_norm after, before;
+    pl_dropout dropout;
+} pl_channel_norm_shape;
+
+/* The gradients to compute, NULL for those that are not wanted; gate: of its own form. */
+typedef struct pl_norm_gradients {
+    void *x, *residual, *gate, *after_weight, *after_bias, *before_weight, *before_bias;
+} pl_norm_gradients;
+
+/* y where and only where there is a norm before; h may then be NULL.  Statistics, and h on its way to y, are float.  Outputs overlap
+ * neither each other nor the inputs.  No counterpart in the reference. */
+int pl_channel_norm(const pl_channel_norm_shape* m, void* h, void* y, const void* x, const void* residual, const void* gate, void* stream);
+
+/* Bytes of workspace that pl_channel_norm_backward takes.  No counterpart in the reference. */
+int pl_channel_norm_workspace_bytes(const pl_channel_norm_shape* m, size_t* bytes);
+
+/* The gradients of pl_channel_norm from those of h (NULL: zeros) and y (there where y was), with its own inputs; residual is read with a norm before
+ * only.  Sums over rows in a fixed order: the same inputs give the same bits.  No counterpart in the reference. */
+int pl_channel_norm_backward(const pl_channel_norm_shape* m, const void* dh, const void* dy, const void* x, const void* residual,
+                             const void* gate, pl_norm_gradients d, void* workspace, size_t workspace_bytes, void* stream);
+
+/* out = residual_scale * residual (NULL: nothing) + dropout(x) of n values; scaled (or NULL) = residual_scale * x: with the gradient of out
+ * as x, out and scaled are those of x and residual.  No counterpart in the reference. */
+int pl_channel_dropout(void* out, void* scaled, const void* x, const void* residual, int64_t n, int dtype, float residual_scale,
+                       const pl_dropout* dropout, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

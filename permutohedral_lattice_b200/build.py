@@ -7,6 +7,7 @@ round every operation separately to select the same simplices as the reference C
 by side, each when it or a header is newer than its object.
 """
 import os
+import re
 import subprocess
 import sys
 
@@ -15,12 +16,14 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libpl_lattice.so")
 SOURCES = [os.path.join(CSRC, "pl_lattice.cu"), os.path.join(CSRC, "channel_mix.cu")] + [
-    os.path.join(CSRC, "mix_%s.cu" % part) for part in ("forward_floats", "forward_halves", "backward_floats", "backward_halves")]
+    os.path.join(CSRC, "mix_%s.cu" % part) for part in ("forward_floats", "forward_halves", "backward_floats", "backward_halves")] + [
+    os.path.join(CSRC, s) for s in ("channel_norm.cu", "norm_floats.cu", "norm_halves.cu")]
 HEADERS = [os.path.join(CSRC, h) for h in ("simplex.cuh", "common.cuh", "lattice_build.cuh", "splat.cuh",
                                              "blur_slice.cuh", "small.cuh", "export.cuh", "fp64.cuh", "direct_index.cuh", "direct_bounds.h", "crf.cuh",
                                              "smem_limit.h", "host_calls.h", "mix_common.cuh",
                                              "mix_forward.cuh", "mix_backward.cuh", "mix_tensor.cuh", "mix_tiny.cuh",
-                                             "mix_host.h", "mix_launch.cuh", "mix_back_launch.cuh")] + [
+                                             "mix_host.h", "mix_launch.cuh", "mix_back_launch.cuh",
+                                             "philox.cuh", "channel_norm.cuh", "norm_launch.cuh")] + [
     os.path.join(ROOT, "include", "pl_lattice.h")]
 
 
@@ -29,6 +32,18 @@ def nvcc_path():
         if cand and os.path.exists(os.path.join(cand, "bin", "nvcc")):
             return os.path.join(cand, "bin", "nvcc")
     return "nvcc"
+
+
+def _with_headers(src):
+    """src and the headers that it includes, theirs included."""
+    found, todo = [], [src]
+    while todo:
+        path = os.path.normpath(todo.pop())
+        if path not in found and os.path.exists(path):
+            found.append(path)
+            with open(path) as f:
+                todo += [os.path.join(os.path.dirname(path), name) for name in re.findall(r'^#include "([^"]+)"', f.read(), re.M)]
+    return found
 
 
 def build(force=False, verbose=False):
@@ -42,7 +57,7 @@ def build(force=False, verbose=False):
     for src in SOURCES:
         obj = src[:-3] + ".o"
         objects.append(obj)
-        if not force and os.path.exists(obj) and all(os.path.getmtime(obj) >= os.path.getmtime(d) for d in [src] + HEADERS):
+        if not force and os.path.exists(obj) and all(os.path.getmtime(obj) >= os.path.getmtime(d) for d in _with_headers(src)):
             continue
         own = ["-fmad=false"] if os.path.basename(src) == "pl_lattice.cu" else []
         running.append((obj, subprocess.Popen([nvcc_path()] + flags + own + ["-c", "-o", obj, src])))

@@ -29,7 +29,8 @@ EXPORTED_SYMBOLS = [
     "pl_export_lattice_f64", "pl_debug_direct_index", "pl_crf_update_f32", "pl_crf_step_f32", "pl_crf_start_f32", "pl_launch_count",
     "pl_direct_index_min_entries", "pl_watch_next_call", "pl_cancel_watch", "pl_await_watched_call",
     "pl_watched_calls_status", "pl_channel_mix", "pl_channel_mix_workspace_bytes", "pl_channel_mix_backward",
-    "pl_pack_activations", "pl_unpack_activations",
+    "pl_pack_activations", "pl_unpack_activations", "pl_channel_norm", "pl_channel_norm_workspace_bytes",
+    "pl_channel_norm_backward", "pl_channel_dropout",
 ]
 STATIC_SCRATCH_BYTES = 64 << 20
 NUM_STAGE_EVENTS = 6
@@ -62,6 +63,28 @@ class PlMix(ctypes.Structure):
 
 class PlMixGradients(ctypes.Structure):
     _fields_ = [(name, ctypes.c_void_p) for name in ("x", "x2", "weight", "weight2", "bias", "residual")]
+
+
+PL_NORM_NONE, PL_NORM_LAYER, PL_NORM_RMS = 0, 1, 2
+
+
+class PlNorm(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int), ("eps", ctypes.c_float), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p)]
+
+
+class PlDropout(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_double), ("key", ctypes.c_uint64), ("offset", ctypes.c_uint64), ("seed", ctypes.c_void_p)]
+
+
+class PlChannelNorm(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("channels", ctypes.c_int), ("dtype", ctypes.c_int), ("vector_dtype", ctypes.c_int),
+                ("gate_of_values", ctypes.c_int), ("residual_scale", ctypes.c_float), ("after", PlNorm), ("before", PlNorm),
+                ("dropout", PlDropout)]
+
+
+class PlNormGradients(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("x", "residual", "gate", "after_weight", "after_bias", "before_weight",
+                                                     "before_bias")]
 
 
 class PlError(RuntimeError):
@@ -128,6 +151,11 @@ def lib():
         L.pl_channel_mix_backward.argtypes = [mix, vp, PlKept, PlKept, PlKept, vp, vp, PlMixGradients, vp, ctypes.c_size_t, vp]
         L.pl_pack_activations.argtypes = [PlPacked, vp, i64, i, i, vp]
         L.pl_unpack_activations.argtypes = [vp, PlPacked, i64, i, vp]
+        norm = ctypes.POINTER(PlChannelNorm)
+        L.pl_channel_norm.argtypes = [norm, vp, vp, vp, vp, vp, vp]
+        L.pl_channel_norm_workspace_bytes.argtypes = [norm, ctypes.POINTER(ctypes.c_size_t)]
+        L.pl_channel_norm_backward.argtypes = [norm, vp, vp, vp, vp, vp, PlNormGradients, vp, ctypes.c_size_t, vp]
+        L.pl_channel_dropout.argtypes = [vp, vp, vp, vp, i64, i, f, ctypes.POINTER(PlDropout), vp]
         _lib = L
     return _lib
 
