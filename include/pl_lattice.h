@@ -416,9 +416,43 @@ int pl_channel_norm_backward(const pl_channel_norm_shape* m, const void* dh, con
                              const void* gate, pl_norm_gradients d, void* workspace, size_t workspace_bytes, void* stream);
 
 /* out = residual_scale * residual (NULL: nothing) + dropout(x) of n values; scaled (or NULL) = residual_scale * x: with the gradient of out
- * as x, out and scaled are those of x and residual.  No counterpart in the reference. */
+ * as x, out and scaled are those of x and residual.  Either may be NULL.  No counterpart in the reference. */
 int pl_channel_dropout(void* out, void* scaled, const void* x, const void* residual, int64_t n, int dtype, float residual_scale,
                        const pl_dropout* dropout, void* stream);
+
+typedef enum pl_gate { PL_GATE_SILU = 0, PL_GATE_GELU = 1, PL_GATE_SIGMOID = 2, PL_GATE_RELU = 3 } pl_gate;   /* GELU: by erf */
+
+/* out[rows, n] = (act(x @ gate_weight + gate_bias) * (x @ up_weight + up_bias)) @ down_weight + down_bias + residual_scale * residual,
+ * x [rows, k], gate_weight and up_weight [k, h], down_weight [h, n]; biases and residual may be NULL.  Up to 128 channels in and out, 512
+ * in between; everything of one type.  Products and sums are float or better; of 16-bit types the values in between are
+ * rounded once on their way to the next product.  Values and weights have to be finite, and below 3.38e38. */
+typedef struct pl_gated_shape {
+    int64_t rows;
+    int k, h, n;
+    int activation;   /* pl_gate */
+    int dtype;        /* pl_dtype */
+    float residual_scale;
+} pl_gated_shape;
+
+typedef struct pl_gated_weights {
+    const void *gate_weight, *up_weight, *down_weight, *gate_bias, *up_bias, *down_bias;
+} pl_gated_weights;
+
+/* The gradients to compute, NULL for those that are not wanted. */
+typedef struct pl_gated_gradients {
+    void *x, *residual, *gate_weight, *up_weight, *down_weight, *gate_bias, *up_bias, *down_bias;
+} pl_gated_gradients;
+
+/* out must not overlap the inputs.  No counterpart in the reference. */
+int pl_gated_mix(const pl_gated_shape* m, void* out, const void* x, const pl_gated_weights* w, const void* residual, void* stream);
+
+/* Bytes of workspace that pl_gated_mix_backward takes for gradients of weights or biases.  No counterpart in the reference. */
+int pl_gated_mix_workspace_bytes(const pl_gated_shape* m, size_t* bytes);
+
+/* The gradients of pl_gated_mix from that of its output and its own inputs: the values in between are made again.  Sums over rows in a
+ * fixed order: the same inputs give the same bits.  The outputs overlap neither each other nor the inputs.  No counterpart in the reference. */
+int pl_gated_mix_backward(const pl_gated_shape* m, const void* grad_out, const void* x, const pl_gated_weights* w, pl_gated_gradients d,
+                          void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

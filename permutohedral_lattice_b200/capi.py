@@ -30,7 +30,7 @@ EXPORTED_SYMBOLS = [
     "pl_direct_index_min_entries", "pl_watch_next_call", "pl_cancel_watch", "pl_await_watched_call",
     "pl_watched_calls_status", "pl_channel_mix", "pl_channel_mix_workspace_bytes", "pl_channel_mix_backward",
     "pl_pack_activations", "pl_unpack_activations", "pl_channel_norm", "pl_channel_norm_workspace_bytes",
-    "pl_channel_norm_backward", "pl_channel_dropout",
+    "pl_channel_norm_backward", "pl_channel_dropout", "pl_gated_mix", "pl_gated_mix_workspace_bytes", "pl_gated_mix_backward",
 ]
 STATIC_SCRATCH_BYTES = 64 << 20
 NUM_STAGE_EVENTS = 6
@@ -85,6 +85,23 @@ class PlChannelNorm(ctypes.Structure):
 class PlNormGradients(ctypes.Structure):
     _fields_ = [(name, ctypes.c_void_p) for name in ("x", "residual", "gate", "after_weight", "after_bias", "before_weight",
                                                      "before_bias")]
+
+
+PL_GATE_SILU, PL_GATE_GELU, PL_GATE_SIGMOID, PL_GATE_RELU = 0, 1, 2, 3
+
+
+class PlGated(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("k", ctypes.c_int), ("h", ctypes.c_int), ("n", ctypes.c_int), ("activation", ctypes.c_int),
+                ("dtype", ctypes.c_int), ("residual_scale", ctypes.c_float)]
+
+
+class PlGatedWeights(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("gate_weight", "up_weight", "down_weight", "gate_bias", "up_bias", "down_bias")]
+
+
+class PlGatedGradients(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("x", "residual", "gate_weight", "up_weight", "down_weight", "gate_bias", "up_bias",
+                                                     "down_bias")]
 
 
 class PlError(RuntimeError):
@@ -156,6 +173,10 @@ def lib():
         L.pl_channel_norm_workspace_bytes.argtypes = [norm, ctypes.POINTER(ctypes.c_size_t)]
         L.pl_channel_norm_backward.argtypes = [norm, vp, vp, vp, vp, vp, PlNormGradients, vp, ctypes.c_size_t, vp]
         L.pl_channel_dropout.argtypes = [vp, vp, vp, vp, i64, i, f, ctypes.POINTER(PlDropout), vp]
+        gated, weights = ctypes.POINTER(PlGated), ctypes.POINTER(PlGatedWeights)
+        L.pl_gated_mix.argtypes = [gated, vp, vp, weights, vp, vp]
+        L.pl_gated_mix_workspace_bytes.argtypes = [gated, ctypes.POINTER(ctypes.c_size_t)]
+        L.pl_gated_mix_backward.argtypes = [gated, vp, vp, weights, PlGatedGradients, vp, ctypes.c_size_t, vp]
         _lib = L
     return _lib
 

@@ -109,7 +109,7 @@ int pl_channel_dropout(void* out, void* scaled, const void* x, const void* resid
                        const pl_dropout* dropout, void* stream) {
     if (n < 0 || dtype < PL_F32 || dtype > PL_BF16 || !dropout || !(dropout->p >= 0.0 && dropout->p < 1.0)) return PL_INVALID_ARGUMENT;
     if (n == 0) return PL_OK;
-    if (!out || !x) return PL_INVALID_ARGUMENT;
+    if ((!out && !scaled) || !x) return PL_INVALID_ARGUMENT;
     const DropArgs a = {n, x, residual, out, scaled, residual_scale, dropout_of(*dropout)};
     const cudaStream_t st = (cudaStream_t)stream;
     return dtype == PL_F32 ? launch_drop<float>(a, st) : dtype == PL_F16 ? launch_drop<__half>(a, st) : launch_drop<__nv_bfloat16>(a, st);

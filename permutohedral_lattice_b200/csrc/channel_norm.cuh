@@ -394,7 +394,7 @@ static __global__ void __launch_bounds__(NORM_THREADS) norm_sums(const __grid_co
     store_weight(a.to[which], i, a.dtype, t);
 }
 
-// out = s residual + x keep / (1 - p), value by value; scaled: s x besides (the residual's gradient, where x is that of out).
+// out = s residual + x keep / (1 - p), value by value; scaled: s x besides (the residual's gradient, where x is that of out).  Either may be NULL.
 struct DropArgs {
     long long n;
     const void *x, *residual;
@@ -433,6 +433,7 @@ __global__ void __launch_bounds__(256) drop_values(const __grid_constant__ DropA
                 for (int j = 0; j < V; j++)
                     if (j < count) scaled[i + j] = from_float<T>(t[j]);
         }
+        if (!out) continue;
 #pragma unroll
         for (int j = 0; j < V; j += 4) {
             const uint4 w = random.words((u64)(i + j) >> 2);

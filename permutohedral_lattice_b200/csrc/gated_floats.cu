@@ -1,0 +1,8 @@
+// The gated feed-forward block of rows of floats.
+#include "gated_launch.cuh"
+
+namespace pl {
+
+int gated_floats(GatedArgs p, GatedPass pass, cudaStream_t st) { return gated_of<float>(p, pass, st); }
+
+}  // namespace pl

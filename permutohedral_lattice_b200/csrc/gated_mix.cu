@@ -1,0 +1,108 @@
+// The gated feed-forward block: the C entry points (see gated.cuh).
+#include "gated_launch.cuh"
+
+namespace pl {
+
+static int check_gated(const pl_gated_shape* m) {
+    if (!m || m->rows < 0 || m->rows > ((long long)1 << 40) || m->k < 1 || m->h < 1 || m->n < 1) return PL_INVALID_ARGUMENT;
+    if (m->activation < PL_GATE_SILU || m->activation > PL_GATE_RELU || m->dtype < PL_F32 || m->dtype > PL_BF16) return PL_INVALID_ARGUMENT;
+    return m->k > MIX_MOST || m->n > MIX_MOST || m->h > GATED_HIDDEN ? PL_UNSUPPORTED_DIMS : PL_OK;
+}
+static int chunk_of(const pl_gated_shape* m) { return m->dtype == PL_F32 ? gated_chunk<float>() : gated_chunk<__half>(); }
+static bool gated_aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+static GatedArgs gated_args(const pl_gated_shape* m, const void* x, const pl_gated_weights* w) {
+    GatedArgs p = {};
+    p.rows = m->rows, p.k = m->k, p.h = m->h, p.n = m->n, p.activation = m->activation, p.scale = m->residual_scale;
+    p.x = x;
+    p.gate_weight = w->gate_weight, p.up_weight = w->up_weight, p.down_weight = w->down_weight;
+    p.gate_bias = w->gate_bias, p.up_bias = w->up_bias, p.down_bias = w->down_bias;
+    p.biased = p.gate_bias || p.up_bias;
+    p.np = (p.n + 15) / 16 * 16;
+    p.wide_x = p.k % 8 == 0 && gated_aligned(x);
+    p.wide_hidden = p.h % 8 == 0 && gated_aligned(p.gate_weight) && gated_aligned(p.up_weight);
+    p.wide_down = p.n % 8 == 0 && gated_aligned(p.down_weight);
+    return p;
+}
+static void set_kp(GatedArgs& p) { p.kp = (p.k + (p.biased ? 1 : 0) + 15) / 16 * 16; }
+static int run_gated(const GatedArgs& p, int dtype, GatedPass pass, cudaStream_t st) {
+    return dtype == PL_F32 ? gated_floats(p, pass, st) : gated_halves(p, dtype, pass, st);
+}
+
+}  // namespace pl
+
+using namespace pl;
+
+extern "C" {
+
+int pl_gated_mix(const pl_gated_shape* m, void* out, const void* x, const pl_gated_weights* w, const void* residual, void* stream) {
+    PL_TRY(check_gated(m));
+    if (m->rows == 0) return PL_OK;
+    if (!out || !x || !w || !w->gate_weight || !w->up_weight || !w->down_weight) return PL_INVALID_ARGUMENT;
+    GatedArgs p = gated_args(m, x, w);
+    set_kp(p);
+    p.out = out, p.residual = residual;
+    p.wide_out = p.n % (m->dtype == PL_F32 ? 4 : 8) == 0 && gated_aligned(out) && gated_aligned(residual);
+    return run_gated(p, m->dtype, GATED_OUT, (cudaStream_t)stream);
+}
+
+int pl_gated_mix_workspace_bytes(const pl_gated_shape* m, size_t* bytes) {
+    PL_TRY(check_gated(m));
+    if (!bytes) return PL_INVALID_ARGUMENT;
+    const int chunk = chunk_of(m), chunks = (m->h + chunk - 1) / chunk;
+    const size_t columns = (m->k + 16) / 16 * 16 + chunk + 16;   // with all biases
+    *bytes = sizeof(float) * 128 * columns * chunks * gated_splits(chunks, m->rows, num_sms());
+    return PL_OK;
+}
+
+int pl_gated_mix_backward(const pl_gated_shape* m, const void* grad_out, const void* x, const pl_gated_weights* w, pl_gated_gradients d,
+                          void* workspace, size_t workspace_bytes, void* stream) {
+    size_t need = 0;
+    PL_TRY(pl_gated_mix_workspace_bytes(m, &need));
+    const cudaStream_t st = (cudaStream_t)stream;
+    const size_t size = m->dtype == PL_F32 ? 4 : 2;
+    const bool sums = d.gate_weight || d.up_weight || d.down_weight || d.gate_bias || d.up_bias || d.down_bias;
+    if (m->rows == 0) {   // sums of nothing
+        const struct { void* to; size_t count; } all[] = {{d.gate_weight, (size_t)m->k * m->h}, {d.up_weight, (size_t)m->k * m->h}, {d.down_weight, (size_t)m->h * m->n},
+                                                          {d.gate_bias, (size_t)m->h}, {d.up_bias, (size_t)m->h}, {d.down_bias, (size_t)m->n}};
+        for (const auto& a : all)
+            if (a.to) PL_CUDA(cudaMemsetAsync(a.to, 0, size * a.count, st));
+        return PL_OK;
+    }
+    if (!grad_out || !x || !w || !w->gate_weight || !w->up_weight || !w->down_weight) return PL_INVALID_ARGUMENT;
+    if (sums && (!workspace || workspace_bytes < need)) return PL_WORKSPACE_TOO_SMALL;
+    if (sums && !gated_aligned(workspace)) return PL_INVALID_ARGUMENT;
+    GatedArgs p = gated_args(m, x, w);
+    p.grad = grad_out;
+    p.wide_grad = p.n % 8 == 0 && gated_aligned(grad_out);
+    if (d.x) {
+        set_kp(p);
+        p.out = d.x, p.dresidual = d.residual;
+        p.wide_out = p.k % (m->dtype == PL_F32 ? 4 : 8) == 0 && gated_aligned(d.x);
+        p.wide_dresidual = p.n % (m->dtype == PL_F32 ? 4 : 8) == 0 && gated_aligned(grad_out) && gated_aligned(d.residual);
+        PL_TRY(run_gated(p, m->dtype, GATED_DX, st));
+    } else if (d.residual) {
+        const pl_dropout none = {};
+        PL_TRY(pl_channel_dropout(nullptr, d.residual, grad_out, nullptr, m->rows * m->n, m->dtype, m->residual_scale, &none, stream));
+    }
+    if (!sums) return PL_OK;
+    p.biased = p.biased || d.gate_bias || d.up_bias;   // (the ones' column sums dg and du)
+    set_kp(p);
+    p.down_bias_wanted = d.down_bias != nullptr;
+    p.shares = static_cast<float*>(workspace);
+    PL_TRY(run_gated(p, m->dtype, GATED_DW, st));
+    GatedSums s = {};
+    s.shares = p.shares, s.k = p.k, s.h = p.h, s.n = p.n, s.kp = p.kp, s.chunk = chunk_of(m);
+    s.chunks = (p.h + s.chunk - 1) / s.chunk, s.splits = gated_splits(s.chunks, m->rows, num_sms());
+    s.down = p.kp, s.bias = s.down + s.chunk, s.columns = s.bias + (p.down_bias_wanted ? 16 : 0);
+    s.gate_weight = d.gate_weight, s.up_weight = d.up_weight, s.down_weight = d.down_weight;
+    s.gate_bias = d.gate_bias, s.up_bias = d.up_bias, s.down_bias = d.down_bias;
+    const dim3 grid((std::max(p.h, p.n) + 255) / 256, 2 * (p.k + 1) + p.h + 1);
+    if (m->dtype == PL_F32) gated_sums<float><<<grid, 256, 0, st>>>(s);
+    else if (m->dtype == PL_F16) gated_sums<__half><<<grid, 256, 0, st>>>(s);
+    else gated_sums<__nv_bfloat16><<<grid, 256, 0, st>>>(s);
+    PL_COUNT_LAUNCHES(1);
+    PL_CUDA(cudaGetLastError());
+    return PL_OK;
+}
+
+}  // extern "C"

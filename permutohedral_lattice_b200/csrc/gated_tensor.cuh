@@ -1,0 +1,121 @@
+// Fifth-generation tensor cores for the gated feed-forward block: 16-bit operands in shared memory, sums in tensor memory.
+//
+// Operands.  A tile of rows x columns lies as blocks of 8 rows by 8 columns, 16 bytes a row and 128 a block, blocks of the same columns
+// one after another, 16 bytes more between those of other columns (so that eight threads with the columns of one row write to different
+// banks).  The same bytes serve as an operand whose sums run over the columns (K-major) and as one whose sums run over the rows
+// (MN-major): nothing is ever transposed, the weights lie as they do in memory, x and its products' operands both ways.
+//
+// Terms.  A float is the sum of three bfloat16 numbers up to 2^-27 of it, each the nearest to what is left, and a product of two
+// floats that of the six pairs whose orders of magnitude are above 2^-24 of it: as many steps as three products of tf32 numbers would
+// take, 2^-22 off then, from 6 bytes a value in place of 8, and either major.  16-bit values are their own only term.
+//
+// Sums.  The tensor cores cut what they add to, a part in 2^24 a step of 16 on average toward zero.  Small products come first, or (over more
+// than 128 terms) have sums of their own.
+#pragma once
+#include "mix_common.cuh"
+
+namespace pl {
+
+template <typename T>
+struct Tensor {
+    static constexpr int TERMS = sizeof(T) == 4 ? 3 : 1;
+    static constexpr u32 FORMAT = std::is_same<T, __half>::value ? 0 : 1;   // of an operand: float16, bfloat16
+    using Term = typename std::conditional<sizeof(T) == 4, __nv_bfloat16, T>::type;
+};
+
+// Bytes from one block of columns to the next, of a tile of so many rows.
+__host__ __device__ constexpr int column_blocks(int rows) { return rows * 16 + 16; }
+__host__ __device__ constexpr int tile_bytes(int rows, int columns) { return columns / 8 * column_blocks(rows); }   // of a term
+
+struct Operand {   // of a product: where its first 16 terms of the sum lie, bytes to the next 16, and to the next term
+    u32 at, step, plane;
+    u64 strides;
+    u32 transposed;
+    __device__ __forceinline__ u64 descriptor(int s, int term) const {
+        return strides | (u64)(((at + s * step + term * plane) >> 4) & 0x3FFF) | 1ull << 46;
+    }
+};
+// The tile's rows are the operand's rows, sums run over its columns.
+__device__ __forceinline__ Operand over_columns(u32 at, int rows, int columns) {
+    const u32 cb = column_blocks(rows);
+    return {at, 2 * cb, (u32)tile_bytes(rows, columns), (u64)(cb >> 4) << 16 | (u64)(128 >> 4) << 32, 0};
+}
+// The tile's columns are the operand's rows, sums run over its rows.
+__device__ __forceinline__ Operand over_rows(u32 at, int rows, int columns) {
+    const u32 cb = column_blocks(rows);
+    return {at, 256, (u32)tile_bytes(rows, columns), (u64)(128 >> 4) << 16 | (u64)(cb >> 4) << 32, 1};
+}
+__device__ __forceinline__ void tensor_product(u32 d, u64 a, u64 b, u32 shape, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+                 "r"(shape), "r"((u32)add)
+                 : "memory");
+}
+// d (+)= a b^T over 16 `steps` terms, 128 x n; small: where products with a term but the first go (may be d).  add, add_small: to what
+// is there.
+template <typename T>
+__device__ __forceinline__ void products(u32 d, u32 small, const Operand& a, const Operand& b, int n, int steps, bool add, bool add_small) {
+    const u32 shape = 1u << 4 | Tensor<T>::FORMAT << 7 | Tensor<T>::FORMAT << 10 | a.transposed << 15 | b.transposed << 16 | (u32)(n / 8) << 17 | 8u << 24;
+    if constexpr (Tensor<T>::TERMS == 3) {
+        bool more = add_small;
+        for (int order = 2; order >= 1; order--)
+            for (int i = 0; i <= order; i++)
+                for (int s = 0; s < steps; s++) {
+                    tensor_product(small, a.descriptor(s, i), b.descriptor(s, order - i), shape, more);
+                    more = true;
+                }
+        if (small == d) add = true;
+    }
+    for (int s = 0; s < steps; s++) tensor_product(d, a.descriptor(s, 0), b.descriptor(s, 0), shape, add || s > 0);
+}
+__device__ __forceinline__ void tensor_commit(u64* bar) {   // the barrier's phase ends when all products asked for so far are done
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_address(bar)) : "memory");
+}
+__device__ __forceinline__ void tensor_load16(float (&v)[16], u32 at) {   // 16 columns of the lane's row; there after tensor_loaded
+    u32* r = reinterpret_cast<u32*>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at));
+}
+__device__ __forceinline__ void tensor_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tensor_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tensor_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void mbar_arrive(u64* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(bar)) : "memory");
+}
+
+__device__ __forceinline__ bool mbar_done(u64* bar, u32 parity) {   // waits a little
+    u32 done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done)
+                 : "r"(shared_address(bar)), "r"(parity)
+                 : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ u64 global_timer() {   // nanoseconds
+    u64 t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+
+// Eight values as terms to a row of a block, 16 bytes each.
+template <typename T>
+__device__ __forceinline__ void store_terms8(unsigned char* to, int plane, const float (&v)[8]) {
+    using Term = typename Tensor<T>::Term;
+    float left[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) left[i] = v[i];
+#pragma unroll
+    for (int t = 0; t < Tensor<T>::TERMS; t++) {
+        uint4 q;
+        Term* e = reinterpret_cast<Term*>(&q);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            e[i] = from_float<Term>(left[i]);
+            if (t + 1 < Tensor<T>::TERMS) left[i] -= to_float(e[i]);
+        }
+        *reinterpret_cast<uint4*>(to + t * plane) = q;
+    }
+}
+
+}  // namespace pl

@@ -1,0 +1,137 @@
+"""A gated feed-forward block of points' features, the nonlinear map beside `channel_mix`'s linear one:
+
+    out = (act(x @ gate_weight + gate_bias) * (x @ up_weight + up_bias)) @ down_weight + down_bias + residual_scale * residual
+
+over channels-last tensors [*, K], in one kernel: the hidden channels' values are neither written nor kept, the backward pass makes them
+again from x.  The reference ships no such operator; the networks that give CRF-as-RNN (its README.md:15-16) its unaries do.
+"""
+import ctypes
+import functools
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import capi
+from .channel_mix import MOST_CHANNELS, _DTYPES, _check_device, _check_values, _contiguous, _ptr
+from .channel_norm import _follows
+from .lattice_filter import _OnDevice, _stream_handle
+
+MOST_HIDDEN = 512
+_ACTIVATIONS = {"silu": capi.PL_GATE_SILU, "gelu": capi.PL_GATE_GELU, "sigmoid": capi.PL_GATE_SIGMOID, "relu": capi.PL_GATE_RELU}
+# What _GatedMix takes gradients of, in its order; the weights in that of the C structure.
+_WEIGHTS = ("gate_weight", "up_weight", "down_weight", "gate_bias", "up_bias", "down_bias")
+_NAMES = ("x", "residual") + _WEIGHTS
+
+
+class _Shape(NamedTuple):
+    rows: int
+    k: int
+    h: int
+    n: int
+    activation: str
+    dtype: torch.dtype
+    residual_scale: float
+
+
+@functools.lru_cache(maxsize=1024)
+def _structure(s):
+    return ctypes.byref(capi.PlGated(s.rows, s.k, s.h, s.n, _ACTIVATIONS[s.activation], _DTYPES[s.dtype], s.residual_scale))
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(s):
+    nbytes = ctypes.c_size_t(0)
+    capi.check(capi.lib().pl_gated_mix_workspace_bytes(_structure(s), ctypes.byref(nbytes)), "pl_gated_mix_workspace_bytes")
+    return nbytes.value
+
+
+def _check(x, residual, weights, activation):
+    if activation not in _ACTIVATIONS:
+        raise ValueError('activation must be "silu", "gelu", "sigmoid" or "relu"')
+    _check_values(x, "x")
+    if x.dim() < 1:
+        raise ValueError("x must be [*, channels]")
+    gate, up, down = weights[:3]
+    for name, w in zip(_WEIGHTS, weights):
+        if w is None and name.endswith("bias"):
+            continue
+        _check_values(w, name, x.dtype)
+    k = x.shape[-1]
+    if gate.dim() != 2 or gate.shape[0] != k:
+        raise ValueError("gate_weight must be [channels of x, hidden channels]")
+    if up.shape != gate.shape:
+        raise ValueError("up_weight must have gate_weight's shape")
+    h = gate.shape[1]
+    if down.dim() != 2 or down.shape[0] != h:
+        raise ValueError("down_weight must be [hidden channels, channels of the output]")
+    n = down.shape[1]
+    if not 1 <= k <= MOST_CHANNELS or not 1 <= n <= MOST_CHANNELS or not 1 <= h <= MOST_HIDDEN:
+        raise ValueError("1 to %d channels in and out, and 1 to %d in between, are supported" % (MOST_CHANNELS, MOST_HIDDEN))
+    for name, b, size in zip(_WEIGHTS[3:], weights[3:], (h, h, n)):
+        if b is not None and tuple(b.shape) != (size,):
+            raise ValueError("%s must be [%d]" % (name, size))
+    if residual is not None:
+        _check_values(residual, "residual", x.dtype)
+        if tuple(residual.shape) != tuple(x.shape[:-1]) + (n,):
+            raise ValueError("residual must have the output's shape")
+    device = _check_device((("x", x), ("residual", residual)) + tuple(zip(_WEIGHTS, weights)))
+    return device, h, n
+
+
+def _forward(device, s, x, residual, weights):
+    out = x.new_empty(x.shape[:-1] + (s.n,))
+    with _OnDevice(device):
+        capi.check(capi.lib().pl_gated_mix(_structure(s), out.data_ptr(), x.data_ptr(), ctypes.byref(capi.PlGatedWeights(*map(_ptr, weights))),
+                                           _ptr(residual), _stream_handle(device)), "pl_gated_mix")
+    return out
+
+
+class _GatedMix(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, device, s, x, residual, *weights):
+        ctx.args = device, s
+        ctx.save_for_backward(x, *weights)
+        return _forward(device, s, x, residual, weights)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, *weights = ctx.saved_tensors
+        device, s = ctx.args
+        grad = grad.contiguous()
+        like = dict(zip(_NAMES, (x, grad, *weights)))
+        made = {name: torch.empty(like[name].shape, dtype=x.dtype, device=device)
+                for name, wanted in zip(_NAMES, ctx.needs_input_grad[2:]) if wanted}
+        with _OnDevice(device):
+            workspace = None
+            if any(name in made for name in _WEIGHTS):
+                workspace = torch.empty(_workspace_bytes(s), dtype=torch.uint8, device=device)
+            capi.check(capi.lib().pl_gated_mix_backward(
+                _structure(s), grad.data_ptr(), x.data_ptr(), ctypes.byref(capi.PlGatedWeights(*map(_ptr, weights))),
+                capi.PlGatedGradients(**{name: t.data_ptr() for name, t in made.items()}), _ptr(workspace),
+                0 if workspace is None else workspace.numel(), _stream_handle(device)), "pl_gated_mix_backward")
+        return (None, None) + tuple(made.get(name) for name in _NAMES)
+
+
+def gated_mix(x, gate_weight, up_weight, down_weight, gate_bias=None, up_bias=None, down_bias=None, residual=None, activation="silu",
+              residual_scale=1.0):
+    """(act(x @ gate_weight + gate_bias) * (x @ up_weight + up_bias)) @ down_weight + down_bias + residual_scale * residual, with
+    gradients for all tensors.
+
+    x [*, K], gate_weight and up_weight [K, H], down_weight [H, N], biases [H], [H], [N], residual and the output [*, N]: all of one type,
+    float32, float16 or bfloat16; up to 128 channels in and out and 512 in between.  activation: "silu", "gelu" (by erf),
+    "sigmoid" or "relu".  Products of floats are off by some 2^-24, sums are float32; of 16-bit types the hidden values (and, in the
+    backward pass, their gradients) are rounded once to that type on their way to the next product.  Gradients' sums over rows have
+    a fixed order.  x, the weights and hidden values have to be finite, and below 3.38e38 (of float16
+    all of them below 65504): of a row that is not, values come out infinite or NaN, other rows are as
+    they would be; the weights' gradients are then not finite.  In a CUDA graph: one ordinary call of the same sizes before the
+    capture, forward and backward, which sets the kernels up; forward and backward together, on leaves made inside it."""
+    weights = (gate_weight, up_weight, down_weight, gate_bias, up_bias, down_bias)
+    device, h, n = _check(x, residual, weights, activation)
+    k = x.shape[-1]
+    s = _Shape(x.numel() // k, k, h, n, activation, x.dtype, float(residual_scale))
+    tensors = tuple(_contiguous(t) for t in (x, residual) + weights)
+    if not _follows(tensors):
+        return _forward(device, s, tensors[0], tensors[1], tensors[2:])
+    return _GatedMix.apply(device, s, *tensors)
