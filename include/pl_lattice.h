@@ -443,11 +443,12 @@ typedef struct pl_gated_gradients {
     void *x, *residual, *gate_weight, *up_weight, *down_weight, *gate_bias, *up_bias, *down_bias;
 } pl_gated_gradients;
 
-/* out must not overlap the inputs.  No counterpart in the reference. */
-int pl_gated_mix(const pl_gated_shape* m, void* out, const void* x, const pl_gated_weights* w, const void* residual, void* stream);
+/* Bytes of workspace that pl_gated_mix takes, or (backward) pl_gated_mix_backward.  No counterpart in the reference. */
+int pl_gated_mix_workspace_bytes(const pl_gated_shape* m, int backward, size_t* bytes);
 
-/* Bytes of workspace that pl_gated_mix_backward takes for gradients of weights or biases.  No counterpart in the reference. */
-int pl_gated_mix_workspace_bytes(const pl_gated_shape* m, size_t* bytes);
+/* out must not overlap the inputs.  No counterpart in the reference. */
+int pl_gated_mix(const pl_gated_shape* m, void* out, const void* x, const pl_gated_weights* w, const void* residual, void* workspace,
+                 size_t workspace_bytes, void* stream);
 
 /* The gradients of pl_gated_mix from that of its output and its own inputs: the values in between are made again.  Sums over rows in a
  * fixed order: the same inputs give the same bits.  The outputs overlap neither each other nor the inputs.  No counterpart in the reference. */

@@ -174,8 +174,8 @@ def lib():
         L.pl_channel_norm_backward.argtypes = [norm, vp, vp, vp, vp, vp, PlNormGradients, vp, ctypes.c_size_t, vp]
         L.pl_channel_dropout.argtypes = [vp, vp, vp, vp, i64, i, f, ctypes.POINTER(PlDropout), vp]
         gated, weights = ctypes.POINTER(PlGated), ctypes.POINTER(PlGatedWeights)
-        L.pl_gated_mix.argtypes = [gated, vp, vp, weights, vp, vp]
-        L.pl_gated_mix_workspace_bytes.argtypes = [gated, ctypes.POINTER(ctypes.c_size_t)]
+        L.pl_gated_mix.argtypes = [gated, vp, vp, weights, vp, vp, ctypes.c_size_t, vp]
+        L.pl_gated_mix_workspace_bytes.argtypes = [gated, i, ctypes.POINTER(ctypes.c_size_t)]
         L.pl_gated_mix_backward.argtypes = [gated, vp, vp, weights, PlGatedGradients, vp, ctypes.c_size_t, vp]
         _lib = L
     return _lib

@@ -6,58 +6,73 @@
 //
 // The hidden values (g, u, a and their gradients) never leave the SM: a CTA takes a tile of rows through the hidden channels a chunk
 // at a time.  A chunk's g and u (and da) are products in tensor memory, its a (dg, du) go to shared memory as the next products' operand.
-// The biases are a row more of the weights beside a one in every row of x.  The backward pass makes g and u again, in two kernels: gated_kernel<DX>
-// sums dx over the chunks of a tile as the forward pass does out, gated_kernel<DW> sums the weights' gradients over the tiles of a
-// chunk, a chunk a CTA, and adds them to a share of its own in the workspace now and then (`drain`, see gated_launch.cuh); gated_sums adds up the
-// shares in order.
+// The biases of g and u are a row more of the weights beside a one in every row of x.  The backward pass makes g and u again, in two
+// kernels: gated_kernel<DX> sums dx over the chunks of a tile as the forward pass does out, gated_kernel<DW> sums the weights' gradients
+// over the tiles of a chunk, a chunk a CTA, and adds them to a share of its own in the workspace now and then (`drain`, see
+// gated_launch.cuh); gated_sums adds up the shares in order.  gated_pack first lays out the weights as the products read them.
 //
-// Warps: eight turn the first products into the second's operand, and take out the sums; one asks for products; four fetch rows and
-// weights.  They meet at barriers in shared memory; every wait is bounded.  If one runs out, all give up and the results are NaN.
+// Warps: workers turn the first products into the second's operand, and take out the sums; two warps ask for the first and the second
+// products, and for the weights that only theirs read; loaders fetch rows.  They meet at barriers in shared memory; every wait is bounded.
+// If one runs out, all give up and the results are NaN.
 #pragma once
 #include "gated_tensor.cuh"
 
 namespace pl {
 
 constexpr int GATED_HIDDEN = 512;   // channels in between, at most
-constexpr int GATED_WORKERS = 8, GATED_LOADERS = 4, GATED_THREADS = 32 * (GATED_WORKERS + 1 + GATED_LOADERS);
 enum GatedPass { GATED_OUT, GATED_DX, GATED_DW };
+// Warps: 20 leave 96 registers a thread, 16 leave 128.  Floats, whose products are six, need fewer workers, and more loaders: three terms of every value.
+template <typename T>
+struct GatedWarps {
+    static constexpr int WORKERS = sizeof(T) == 4 ? 8 : 16, LOADERS = sizeof(T) == 4 ? 6 : 2, THREADS = 32 * (WORKERS + 2 + LOADERS);
+};
 
 struct GatedArgs {
     long long rows;
     int k, h, n, activation;
     int kp, np;                      // columns of a tile of x (with the ones, if there are biases of g or u) and of out
     int chunks, splits;              // of the hidden channels; CTAs of a chunk (DW)
-    int x_buffers, w_buffers, a_buffers, s_buffers, d_buffers, drain;
+    int x_buffers, w_buffers[2], a_buffers, s_buffers, d_buffers, io_buffers, drain;
     float scale;
     const void *x, *gate_weight, *up_weight, *down_weight, *gate_bias, *up_bias, *down_bias, *residual, *grad;
-    int biased, wide_x, wide_grad, wide_hidden, wide_down, wide_out;   // wide: rows of whole 16 bytes on 16-byte boundaries
-    int wide_dresidual, down_bias_wanted;   // (DX, DW)
+    int biased, wide_x, wide_grad, wide_out;   // wide: rows of whole 16 bytes on 16-byte boundaries
+    int wide_dresidual, down_bias_wanted;      // (DX, DW)
+    unsigned char* packed;           // the weights, a chunk after another: Wd, Wg and Wu as tiles
     void *out, *dresidual;           // out: or dx
     float* shares;                   // [chunks][splits][columns of sums][128]
 };
 
 template <typename T>
 __host__ __device__ constexpr int gated_chunk() { return sizeof(T) == 4 ? 32 : 64; }   // hidden channels
+// Bytes of a chunk's Wd, and of its Wg and Wu (side by side in one tile).
+template <typename T>
+__host__ __device__ inline int gated_down_bytes(int np) { return Tensor<T>::TERMS * tile_bytes(gated_chunk<T>(), np); }
+template <typename T>
+__host__ __device__ inline int gated_up_bytes(int kp) { return Tensor<T>::TERMS * tile_bytes(kp, 2 * gated_chunk<T>()); }
 
 // Where things lie in shared memory: offsets, bytes of a buffer, in all.
 template <typename T, GatedPass PASS, int ROWS>
 struct GatedSmem {
     static constexpr int C = gated_chunk<T>(), TERMS = Tensor<T>::TERMS;
     static constexpr int A = TERMS * tile_bytes(ROWS, PASS == GATED_OUT ? C : 2 * C), ACT = PASS == GATED_DW ? TERMS * tile_bytes(ROWS, C) : 0;
-    static constexpr int BARRIERS = 1024;
-    int grad, x, down, w;            // bytes: a tile of dout, of x with it, of Wd, of all weights of a chunk
-    int at_x, at_w, at_a, at_ones, total;
+    static constexpr int BARRIERS = 2048;
+    int grad, x, io_stride;          // bytes: a tile of dout, of x with it; a row on its way out
+    int w[2];                        // of the weights that the first products alone read (OUT: Wg and Wu, DX and DW: Wd), and of the others
+    int at_x, at_w[2], at_a, at_io, at_ones, total;
     __host__ __device__ GatedSmem(const GatedArgs& p) {
         grad = PASS == GATED_OUT ? 0 : TERMS * tile_bytes(ROWS, p.np);
         x = grad + TERMS * tile_bytes(ROWS, p.kp);
-        down = TERMS * tile_bytes(C, p.np);
-        w = down + TERMS * tile_bytes(p.kp, 2 * C);
+        const int down = gated_down_bytes<T>(p.np), up = gated_up_bytes<T>(p.kp);
+        w[0] = PASS == GATED_OUT ? up : down, w[1] = PASS == GATED_OUT ? down : up;
         at_x = BARRIERS;
-        at_w = at_x + p.x_buffers * x;
-        at_a = at_w + p.w_buffers * w;
-        at_ones = at_a + p.a_buffers * (A + ACT);
+        at_w[0] = at_x + p.x_buffers * x;
+        at_w[1] = at_w[0] + p.w_buffers[0] * w[0];
+        at_a = at_w[1] + p.w_buffers[1] * w[1];
+        at_io = at_a + p.a_buffers * (A + ACT);
+        io_stride = ((PASS == GATED_OUT ? p.n : p.k) * (int)sizeof(T) + 15) / 16 * 16 + 16;   // (threads of different rows in different banks)
+        at_ones = at_io + p.io_buffers * ROWS * io_stride;
         // (products of 128 rows read on behind a tile of 64, and of 128 columns behind one of fewer: what they make of it nobody takes)
-        total = at_ones + (PASS == GATED_DW ? tile_bytes(ROWS, 16) : 0) + 2048;
+        total = at_ones + (PASS == GATED_DW ? tile_bytes(ROWS, 16) : 0) + 1024;
     }
 };
 // Columns of tensor memory.  DW: of the sums of dWg and dWu, dWd, and dbd.
@@ -80,84 +95,176 @@ struct GatedColumns {
     }
 };
 
-__device__ __forceinline__ float gated_sigmoid(float g) { return __fdividef(1.f, 1.f + exp2_approx(-1.4426950408889634f * g)); }
-// act(g); slope: act'(g)
-template <int ACT, bool SLOPE>
-__device__ __forceinline__ float gated_act(float g, float& slope) {
-    if constexpr (ACT == PL_GATE_SILU) {
-        const float s = gated_sigmoid(g);
-        if (SLOPE) slope = s * fmaf(g, 1.f - s, 1.f);
-        return g * s;
-    } else if constexpr (ACT == PL_GATE_SIGMOID) {
-        const float s = gated_sigmoid(g);
-        if (SLOPE) slope = s * (1.f - s);
-        return s;
-    } else if constexpr (ACT == PL_GATE_GELU) {
-        const float cdf = fmaf(0.5f, erff(0.70710678118654752f * g), 0.5f);
-        if (SLOPE) slope = fmaf(g, 0.3989422804014327f * exp2_approx(-0.72134752044448170f * g * g), cdf);
-        return g * cdf;
+// Eight sigmoids, e: eight values of g, then of the sigmoid.  A quarter of the reciprocals, the other three by products: with 16-bit types the
+// exponentials and reciprocals of all, two an element, took longer than their other instructions.  2^31 in place of larger exponentials (of -g above
+// 21.5) keeps the product of four in range; 2^-31 is then off by no more than itself.  Floats, whose products take longer, do without.
+template <typename T>
+__device__ __forceinline__ void gated_sigmoids(float2 (&e)[4]) {
+    const float2 minus = make_float2(-1.4426950408889634f, -1.4426950408889634f), one = make_float2(1.f, 1.f);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        e[i] = mul2(e[i], minus);
+        if constexpr (sizeof(T) == 2) {
+            asm("min.NaN.f32 %0, %0, 0f41F80000;" : "+f"(e[i].x));
+            asm("min.NaN.f32 %0, %0, 0f41F80000;" : "+f"(e[i].y));
+        }
+        e[i].x = exp2_approx(e[i].x), e[i].y = exp2_approx(e[i].y);
+        e[i] = add2(e[i], one);
+    }
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const float2 pairs = mul2(e[i], e[i + 1]);                     // x, y: of two each
+            float all;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(all) : "f"(pairs.x * pairs.y));
+            const float2 of_pairs = mul2(make_float2(all, all), make_float2(pairs.y, pairs.x));
+            const float2 first = mul2(of_pairs, e[i + 1]);
+            e[i + 1] = mul2(of_pairs, e[i]);
+            e[i] = first;
+        }
     } else {
-        if (SLOPE) slope = g > 0.f ? 1.f : g <= 0.f ? 0.f : g;   // (NaN: itself)
-        return g < 0.f ? 0.f : g;
+#pragma unroll
+        for (int i = 0; i < 4; i++) e[i].x = __fdividef(1.f, e[i].x), e[i].y = __fdividef(1.f, e[i].y);
+    }
+}
+// act(g) of eight values; SLOPE: act'(g) too
+template <typename T, int ACT, bool SLOPE>
+__device__ __forceinline__ void gated_act(const float2 (&g)[4], float2 (&act)[4], float2 (&slope)[4]) {
+    const float2 one = make_float2(1.f, 1.f), minus = make_float2(-1.f, -1.f);
+    if constexpr (ACT == PL_GATE_SILU || ACT == PL_GATE_SIGMOID) {
+        float2 s[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[i] = g[i];
+        gated_sigmoids<T>(s);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            act[i] = ACT == PL_GATE_SILU ? mul2(g[i], s[i]) : s[i];
+            if constexpr (SLOPE) {   // s (1 + g (1 - s)) or s (1 - s)
+                const float2 rest = fma2(s[i], minus, one);
+                slope[i] = ACT == PL_GATE_SILU ? fma2(act[i], rest, s[i]) : mul2(s[i], rest);
+            }
+        }
+    } else if constexpr (ACT == PL_GATE_GELU) {
+        const float2 half = make_float2(0.5f, 0.5f);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 z = mul2(g[i], make_float2(0.70710678118654752f, 0.70710678118654752f));
+            const float2 cdf = fma2(half, make_float2(erff(z.x), erff(z.y)), half);
+            act[i] = mul2(g[i], cdf);
+            if constexpr (SLOPE) {
+                const float2 q = mul2(mul2(g[i], g[i]), make_float2(-0.72134752044448170f, -0.72134752044448170f));
+                slope[i] = fma2(mul2(g[i], make_float2(0.3989422804014327f, 0.3989422804014327f)), make_float2(exp2_approx(q.x), exp2_approx(q.y)), cdf);
+            }
+        }
+    } else {
+        auto relu = [](float v) { return v < 0.f ? 0.f : v; };
+        auto step = [](float v) { return v > 0.f ? 1.f : v <= 0.f ? 0.f : v; };   // (NaN: itself)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            act[i] = make_float2(relu(g[i].x), relu(g[i].y));
+            if constexpr (SLOPE) slope[i] = make_float2(step(g[i].x), step(g[i].y));
+        }
     }
 }
 
-// rows x columns values to those of a tile of so many rows by the loaders: row r of `valid` from src + r stride, `valid_columns` of them;
-// zeros elsewhere, but for `last`, the row after the valid ones if it is given, and ones in column `ones` of the valid rows.  wide: by 16
-// bytes.  plane: bytes from a term to the next.
-template <typename T>
-__device__ __forceinline__ void stage(unsigned char* to, int rows, int columns, int plane, const T* src, long long stride, int valid, int valid_columns,
-                                      const T* last, int ones, bool wide, int thread) {
-    constexpr int U = 4, STEP = 32 * GATED_LOADERS;
-    const int blocks = columns / 8, cb = column_blocks(rows), items = rows * blocks;
-    for (int i0 = thread; i0 < items; i0 += U * STEP) {
-        float v[U][8];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int i = i0 + u * STEP, r = i / blocks, c = 8 * (i - r * blocks);
-            const T* from = r < valid ? src + r * stride + c : last && r == valid ? last + c : nullptr;
-            if (i >= items || c >= valid_columns) from = nullptr;
-            if (sizeof(T) == 2 && wide && from && r < valid) {
-                cp_async16(to + c / 8 * cb + r * 16, from);
-                continue;
+// Rows of `width` values to a tile by some warps: `valid` of them, zeros behind.  wide: by 16 bytes; the columns behind the last whole block have been
+// written once for all.  Else all of `blocks` blocks are, with ones in column `ones`.  Eight rows of four blocks a warp at a time: whole sectors of
+// memory, all banks of shared memory.
+template <typename T, int ROWS>
+__device__ __forceinline__ void stage(unsigned char* to, int blocks, const T* src, int width, int valid, int ones, bool wide, int warp, int warps) {
+    const int lane = threadIdx.x & 31, r8 = lane & 7, b0 = lane >> 3, plane = tile_bytes(ROWS, 8 * blocks);
+    if (sizeof(T) == 2 && wide) {
+        const int whole = width / 8;
+#pragma unroll 4
+        for (int g = warp; g < ROWS / 8; g += warps) {
+            const int r = 8 * g + r8;
+            unsigned char* there = to + 16 * r + b0 * column_blocks(ROWS);
+            const T* from = src + (long long)r * width + 8 * b0;
+            if (r < valid) {
+                for (int b = b0; b < whole; b += 4, there += 4 * column_blocks(ROWS), from += 32) cp_async16(there, from);
+            } else {
+                for (int b = b0; b < whole; b += 4, there += 4 * column_blocks(ROWS)) *reinterpret_cast<uint4*>(there) = make_uint4(0, 0, 0, 0);
             }
+        }
+        return;
+    }
+    const int end = wide ? width / 8 : blocks;
+    for (int b = b0; b < (end + 3) / 4 * 4; b += 4) {
+        constexpr int U = 4;
+        for (int g0 = warp; g0 < ROWS / 8; g0 += U * warps) {
+            float v[U][8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[u][e] = 0.f;
-            if (from) {
-                if (wide && r < valid) {
-                    float q[4];
-                    load4(q, from);
+            for (int i = 0; i < U; i++) {
+                const int r = 8 * (g0 + i * warps) + r8;
+                const T* from = src + (long long)r * width + 8 * b;
+                const bool there = r < valid && r < ROWS && b < end;
+                if (sizeof(T) == 4 && wide) {
+                    float q[4] = {0.f, 0.f, 0.f, 0.f};
+                    if (there) load4(q, from);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[u][e] = q[e];
-                    load4(q, from + 4);
+                    for (int e = 0; e < 4; e++) v[i][e] = q[e], q[e] = 0.f;
+                    if (there) load4(q, from + 4);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[u][4 + e] = q[e];
+                    for (int e = 0; e < 4; e++) v[i][4 + e] = q[e];
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (c + e < valid_columns) v[u][e] = to_float(from[e]);
+                    for (int e = 0; e < 8; e++) v[i][e] = there && 8 * b + e < width ? to_float(from[e]) : there && 8 * b + e == ones ? 1.f : 0.f;
                 }
             }
-        }
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int i = i0 + u * STEP, r = i / blocks, c = 8 * (i - r * blocks);
-            if (i >= items || (sizeof(T) == 2 && wide && r < valid && c < valid_columns)) continue;
-            if (ones >= c && ones < c + 8 && r < valid) {
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (c + e == ones) v[u][e] = 1.f;
+            for (int i = 0; i < U; i++) {
+                const int r = 8 * (g0 + i * warps) + r8;
+                if (r < ROWS && b < end) store_terms8<T>(to + b * column_blocks(ROWS) + 16 * r, plane, v[i]);
             }
-            store_terms8<T>(to + c / 8 * cb + r * 16, plane, v[u]);
         }
     }
+}
+// The columns behind the last whole block of a tile that `stage` fills by 16 bytes: zeros, but for the ones.  By all threads, once.
+template <typename T, int ROWS>
+__device__ __forceinline__ void stage_rest(unsigned char* to, int blocks, int width, int ones) {
+    const int first = width / 8, rest = blocks - first;
+    for (int i = threadIdx.x; i < rest * ROWS; i += GatedWarps<T>::THREADS) {
+        const int b = first + i / ROWS, r = i % ROWS;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = 8 * b + e == ones ? 1.f : 0.f;
+        store_terms8<T>(to + b * column_blocks(ROWS) + 16 * r, tile_bytes(ROWS, 8 * blocks), v);
+    }
+}
+
+// The weights of all chunks as the products' operands, terms made: a row's eight columns a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) gated_pack(const __grid_constant__ GatedArgs p) {
+    constexpr int C = gated_chunk<T>();
+    const int down_items = C * (p.np / 8), up_items = p.kp * (2 * C / 8), items = down_items + up_items;
+    const int down_bytes = gated_down_bytes<T>(p.np), up_bytes = gated_up_bytes<T>(p.kp);
+    const int chunk = blockIdx.y, h0 = chunk * C;
+    unsigned char* to = p.packed + (long long)chunk * (down_bytes + up_bytes);
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= items) return;
+    const bool down = i < down_items;
+    const int blocks = down ? p.np / 8 : 2 * C / 8, j = down ? i : i - down_items, r = j / blocks, b = j - r * blocks;
+    const bool up = !down && b >= C / 8;
+    const int c0 = down ? 8 * b : h0 + 8 * (up ? b - C / 8 : b), width = down ? p.n : p.h, row = down ? h0 + r : r, rows = down ? p.h : p.k;
+    const T* from = static_cast<const T*>(down ? p.down_weight : up ? p.up_weight : p.gate_weight) + (long long)row * width + c0;
+    bool there = row < rows;
+    if (!down && row == p.k) {   // the biases' row
+        const T* bias = static_cast<const T*>(up ? p.up_bias : p.gate_bias);
+        there = p.biased && bias;
+        from = bias + c0;
+    }
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = there && c0 + e < width ? to_float(from[e]) : 0.f;
+    const int tile_rows = down ? C : p.kp;
+    store_terms8<T>(to + (down ? 0 : down_bytes) + b * column_blocks(tile_rows) + 16 * r, tile_bytes(tile_rows, 8 * blocks), v);
 }
 
 struct GatedBarriers {
-    u64 x_full[2], x_free[2], w_full[16], w_free[16], s_full[2], s_free[2], a_full[2], a_free[2], d_full[2], d_free[2], end;
+    u64 x_full[2], x_free[2], w_full[2][16], w_free[2][16], s_full[2], s_free[2], a_full[2], a_free[2], d_full[2], d_free[2], io_full, io_free, met[4], end[2];
     u32 tensor, dead;
 };
-static_assert(sizeof(GatedBarriers) <= 512);
+static_assert(sizeof(GatedBarriers) <= 1024);
 
 // Where one of a ring of buffers is in its turns.
 struct Turn {
@@ -226,203 +333,331 @@ __device__ __forceinline__ void load16(float (&v)[16], const T* from, int left, 
     static_assert(V >= 4);
 }
 
-// 16 hidden channels of a row: from g, u (and da) to what the second products take.
-template <typename T, GatedPass PASS, int ACT, int ROWS>
-__device__ __forceinline__ void gated_work(const float (&g)[16], const float (&u)[16], const float (&da)[16], unsigned char* a, int row, int column) {
+// Some hidden channels of a row: from g, u (and da) to what the second products take.
+template <typename T, GatedPass PASS, int ACT, int ROWS, int W>
+__device__ __forceinline__ void gated_work(const float (&g)[W], const float (&u)[W], const float (&da)[W], unsigned char* a, int row, int column) {
     constexpr int C = gated_chunk<T>(), CB = column_blocks(ROWS), PLANE = tile_bytes(ROWS, PASS == GATED_OUT ? C : 2 * C);
 #pragma unroll
-    for (int j = 0; j < 16; j += 8) {
-        float v[8], w[8], z[8];
+    for (int j = 0; j < W; j += 8) {
+        float2 g2[4], u2[4], d2[4], act[4], slope[4];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            float slope;
-            const float act = gated_act<ACT, PASS != GATED_OUT>(g[j + e], slope);
-            if constexpr (PASS == GATED_OUT) {
-                v[e] = act * u[j + e];
-            } else {
-                v[e] = da[j + e] * u[j + e] * slope;
-                w[e] = da[j + e] * act;
-                z[e] = act * u[j + e];
-            }
+        for (int i = 0; i < 4; i++) {
+            g2[i] = make_float2(g[j + 2 * i], g[j + 2 * i + 1]);
+            u2[i] = make_float2(u[j + 2 * i], u[j + 2 * i + 1]);
+            if (PASS != GATED_OUT) d2[i] = make_float2(da[j + 2 * i], da[j + 2 * i + 1]);
         }
+        gated_act<T, ACT, PASS != GATED_OUT>(g2, act, slope);
         unsigned char* to = a + (column + j) / 8 * CB + row * 16;
-        store_terms8<T>(to, PLANE, v);
-        if constexpr (PASS != GATED_OUT) store_terms8<T>(to + C / 8 * CB, PLANE, w);
-        if constexpr (PASS == GATED_DW) store_terms8<T>(to + Tensor<T>::TERMS * PLANE, tile_bytes(ROWS, C), z);
+        auto put = [&](unsigned char* where, int plane, auto value) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float2 q = value(i);
+                v[2 * i] = q.x, v[2 * i + 1] = q.y;
+            }
+            store_terms8<T>(where, plane, v);
+        };
+        if constexpr (PASS == GATED_OUT) {
+            put(to, PLANE, [&](int i) { return mul2(act[i], u2[i]); });
+        } else {
+            put(to, PLANE, [&](int i) { return mul2(mul2(d2[i], u2[i]), slope[i]); });
+            put(to + C / 8 * CB, PLANE, [&](int i) { return mul2(d2[i], act[i]); });
+            if constexpr (PASS == GATED_DW) put(to + Tensor<T>::TERMS * PLANE, tile_bytes(ROWS, C), [&](int i) { return mul2(act[i], u2[i]); });
+        }
     }
 }
 
+// The weights that one of the two warps of products fetches for itself: a chunk of one kind for every step, or (all of them there) once.
+struct WeightRing {
+    unsigned char* buffers;
+    const unsigned char* from;   // of the first chunk
+    u64 *full, *free;
+    int count, bytes, chunks, chunk0;
+    long long pitch;             // from a chunk to the next in memory
+    bool resident;
+    long long asked = 0, all;
+    Turn use, load, freed;
+    __device__ __forceinline__ void ask() {
+        mbar_expect_tx(&full[load.at], bytes);
+        bulk_load(buffers + load.at * bytes, from + (chunk0 + (int)(asked % chunks)) * pitch, bytes, &full[load.at]);
+        load.next(count);
+        asked++;
+    }
+    __device__ __forceinline__ void begin() {
+        if (resident) all = min(all, (long long)chunks);
+        while (asked < min(all, (long long)count)) ask();
+    }
+    // After the products of step q have been asked for: the buffer of the step before (or, of one buffer, its own) gets what comes next.
+    __device__ __forceinline__ void used(Waits& wait, long long q) {
+        if (resident) return;
+        tensor_commit(&free[use.at]);
+        use.next(count);
+        if ((q == 0 && count > 1) || asked == all) return;
+        if (!wait.on(&free[freed.at], freed.turns)) return;
+        freed.next(count);
+        ask();
+    }
+    __device__ __forceinline__ void end(Waits& wait) {   // nothing on its way when others have given up
+        if (wait.alive && !*wait.dead) return;
+        for (long long i = max(0ll, asked - count); i < asked; i++) Waits{wait.dead}.on(&full[i % count], (int)(i / count), true);
+    }
+};
+
 template <typename T, GatedPass PASS, int ROWS>
-__global__ void __launch_bounds__(GATED_THREADS, 1) gated_kernel(const __grid_constant__ GatedArgs p) {
+__global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const __grid_constant__ GatedArgs p) {
     extern __shared__ __align__(128) unsigned char smem[];
     using Smem = GatedSmem<T, PASS, ROWS>;
     using Columns = GatedColumns<T, PASS>;
     constexpr int C = gated_chunk<T>(), TERMS = Tensor<T>::TERMS;
+    constexpr int WORKERS = GatedWarps<T>::WORKERS, LOADERS = GatedWarps<T>::LOADERS, THREADS = GatedWarps<T>::THREADS;
     const Smem at(p);
     const Columns col(p);
     GatedBarriers& b = *reinterpret_cast<GatedBarriers*>(smem);
-    float* bias_s = reinterpret_cast<float*>(smem + 512);   // of out
+    float* bias_s = reinterpret_cast<float*>(smem + 1024);   // of out
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // One of the loaders brings the residual, or takes dout to the residual's gradient.
+    const bool beside = (PASS == GATED_OUT && p.residual && p.io_buffers) || (PASS == GATED_DX && p.dresidual);
+    const int row_loaders = LOADERS - (beside ? 1 : 0);
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&b.x_full[i], 32 * GATED_LOADERS), mbar_init(&b.x_free[i], 1);
-            mbar_init(&b.s_full[i], 1), mbar_init(&b.s_free[i], GATED_WORKERS);
-            mbar_init(&b.a_full[i], GATED_WORKERS), mbar_init(&b.a_free[i], 1);
-            mbar_init(&b.d_full[i], 1), mbar_init(&b.d_free[i], GATED_WORKERS);
+            mbar_init(&b.x_full[i], 32 * row_loaders), mbar_init(&b.x_free[i], 1);
+            mbar_init(&b.s_full[i], 1), mbar_init(&b.s_free[i], WORKERS);
+            mbar_init(&b.a_full[i], WORKERS), mbar_init(&b.a_free[i], 1);
+            mbar_init(&b.d_full[i], 1), mbar_init(&b.d_free[i], WORKERS);
+            for (int j = 0; j < p.w_buffers[i]; j++) mbar_init(&b.w_full[i][j], 1), mbar_init(&b.w_free[i][j], 1);
+            mbar_init(&b.end[i], 1);
         }
-        for (int i = 0; i < p.w_buffers; i++) mbar_init(&b.w_full[i], 32 * GATED_LOADERS), mbar_init(&b.w_free[i], 1);
-        mbar_init(&b.end, 1);
+        mbar_init(&b.io_full, 32), mbar_init(&b.io_free, WORKERS);
+        for (int i = 0; i < 4; i++) mbar_init(&b.met[i], WORKERS / 4);
         b.dead = 0;
     }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(shared_address(&b.tensor)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    if constexpr (PASS == GATED_OUT)
-        for (int i = threadIdx.x; i < p.np; i += GATED_THREADS) bias_s[i] = p.down_bias && i < p.n ? to_float(static_cast<const T*>(p.down_bias)[i]) : 0.f;
     if constexpr (PASS == GATED_DW) {   // a column of ones
-        for (int i = threadIdx.x; i < tile_bytes(ROWS, 16) / 4; i += GATED_THREADS) reinterpret_cast<u32*>(smem + at.at_ones)[i] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < ROWS; i += GATED_THREADS)
-            *reinterpret_cast<typename Tensor<T>::Term*>(smem + at.at_ones + 16 * i) = from_float<typename Tensor<T>::Term>(1.f);
-        fence_async_proxy();
+        float one[8] = {1.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, none[8] = {};
+        unsigned char* to = smem + at.at_ones;
+        using Term = typename Tensor<T>::Term;
+        for (int i = threadIdx.x; i < 2 * ROWS; i += THREADS) store_terms8<Term>(to + 16 * i, 0, i < ROWS ? one : none);
     }
+    for (int i = 0; i < p.x_buffers; i++) {
+        unsigned char* x = smem + at.at_x + i * at.x;
+        if (PASS != GATED_OUT && p.wide_grad) stage_rest<T, ROWS>(x, p.np / 8, p.n, -1);
+        if (p.wide_x) stage_rest<T, ROWS>(x + at.grad, p.kp / 8, p.k, p.biased ? p.k : -1);
+    }
+    fence_async_proxy();
+    wait_for_previous_kernel();
+    if constexpr (PASS == GATED_OUT)
+        for (int i = threadIdx.x; i < p.np; i += THREADS) bias_s[i] = p.down_bias && i < p.n ? to_float(static_cast<const T*>(p.down_bias)[i]) : 0.f;
     tensor_before_sync();
     __syncthreads();
     tensor_after_sync();
     const u32 tensor = b.tensor;
     Waits wait{&b.dead};
 
-    // What this CTA does: tiles from `first` on, every `step`-th, each through `chunks` chunks from `chunk0` on.
+    // What this CTA does: tiles from `split` on, every `step`-th, each through `chunks` chunks from `chunk0` on.
     const long long tiles = (p.rows + ROWS - 1) / ROWS;
     const int split = PASS == GATED_DW ? blockIdx.x / p.chunks : blockIdx.x, step = PASS == GATED_DW ? p.splits : gridDim.x;
     const int chunk0 = PASS == GATED_DW ? blockIdx.x % p.chunks : 0, chunks = PASS == GATED_DW ? 1 : p.chunks;
     const long long mine = split < tiles ? (tiles - split + step - 1) / step : 0;
     const long long all = mine * chunks;                                  // steps: chunks of tiles
     const int group = PASS == GATED_DW ? p.drain : chunks;                // steps whose sums are one
-    const bool resident = p.w_buffers >= chunks;
+    auto ring = [&](int which) {
+        const bool down = (which == 0) != (PASS == GATED_OUT);
+        const int down_bytes = gated_down_bytes<T>(p.np);
+        WeightRing r{smem + at.at_w[which], p.packed + (down ? 0 : down_bytes), b.w_full[which], b.w_free[which], p.w_buffers[which], at.w[which], chunks,
+                     chunk0, (long long)down_bytes + gated_up_bytes<T>(p.kp), p.w_buffers[which] >= chunks};
+        r.all = all;
+        return r;
+    };
 
-    if (warp > GATED_WORKERS) {   // loaders
-        const int thread = threadIdx.x - 32 * (GATED_WORKERS + 1);
-        Turn xt, wt;
-        for (long long t = 0; t < mine && wait.alive; t++) {
-            const long long row0 = (split + t * step) * ROWS;
-            const int valid = (int)min((long long)ROWS, p.rows - row0);
-            if (!wait.free(b.x_free, xt)) break;
-            unsigned char* x = smem + at.at_x + xt.at * at.x;
-            if constexpr (PASS != GATED_OUT)
-                stage<T>(x, ROWS, p.np, tile_bytes(ROWS, p.np), static_cast<const T*>(p.grad) + row0 * p.n, p.n, valid, p.n, nullptr, -1, p.wide_grad, thread);
-            stage<T>(x + at.grad, ROWS, p.kp, tile_bytes(ROWS, p.kp), static_cast<const T*>(p.x) + row0 * p.k, p.k, valid, p.k, nullptr,
-                     p.biased ? p.k : -1, p.wide_x, thread);
-            if (sizeof(T) == 2) cp_async_wait_all();
-            fence_async_proxy();
-            mbar_arrive(&b.x_full[xt.at]);
-            xt.next(p.x_buffers);
-            if (t > 0 && resident) continue;
-            for (int c = 0; c < chunks; c++) {
-                if (!wait.free(b.w_free, wt)) break;
-                unsigned char* w = smem + at.at_w + wt.at * at.w;
-                const int h0 = (chunk0 + c) * C, have = min(C, p.h - h0);
-                const T *wg = static_cast<const T*>(p.gate_weight) + h0, *wu = static_cast<const T*>(p.up_weight) + h0;
-                const T *bg = static_cast<const T*>(p.gate_bias), *bu = static_cast<const T*>(p.up_bias);
-                stage<T>(w, C, p.np, tile_bytes(C, p.np), static_cast<const T*>(p.down_weight) + (long long)h0 * p.n, p.n, have, p.n, nullptr, -1, p.wide_down,
-                         thread);
-                // gate and up side by side in one tile
-                const int plane = tile_bytes(p.kp, 2 * C);
-                stage<T>(w + at.down, p.kp, C, plane, wg, p.h, p.k, have, bg ? bg + h0 : nullptr, -1, p.wide_hidden, thread);
-                stage<T>(w + at.down + tile_bytes(p.kp, C), p.kp, C, plane, wu, p.h, p.k, have, bu ? bu + h0 : nullptr, -1, p.wide_hidden, thread);
-                if (sizeof(T) == 2) cp_async_wait_all();
+    if (warp >= WORKERS + 2) {   // loaders
+        const int loader = warp - WORKERS - 2;
+        if (beside && loader == LOADERS - 1) {
+            for (long long t = 0; t < mine && wait.alive; t++) {
+                const long long row0 = (split + t * step) * ROWS;
+                const int valid = (int)min((long long)ROWS, p.rows - row0);
+                if constexpr (PASS == GATED_OUT) {   // the residual to where the output leaves from
+                    if (t > 0 && !wait.on(&b.io_free, (int)(t - 1))) break;
+                    const T* from = static_cast<const T*>(p.residual) + row0 * p.n;
+                    unsigned char* to = smem + at.at_io;
+                    if (p.wide_out) {
+                        const int pieces = p.n * (int)sizeof(T) / 16;
+                        for (int i = lane; i < valid * pieces; i += 32) {
+                            const int r = i / pieces;
+                            cp_async16(to + r * at.io_stride + 16 * (i - r * pieces), reinterpret_cast<const unsigned char*>(from) + 16 * i);
+                        }
+                        cp_async_wait_all();
+                    } else {
+                        for (int i = lane; i < valid * p.n; i += 32) {
+                            const int r = i / p.n;
+                            reinterpret_cast<T*>(to + r * at.io_stride)[i - r * p.n] = from[i];
+                        }
+                    }
+                    mbar_arrive(&b.io_full);
+                } else {
+                    const T* from = static_cast<const T*>(p.grad) + row0 * p.n;
+                    T* to = static_cast<T*>(p.dresidual) + row0 * p.n;
+                    const int count = valid * p.n;
+                    if (p.wide_dresidual) {
+                        constexpr int V = 16 / sizeof(T);
+#pragma unroll 4
+                        for (int i = V * lane; i < count; i += 32 * V) {
+                            float v[V];
+#pragma unroll
+                            for (int e = 0; e < V; e += 4) {
+                                float q[4];
+                                load4(q, from + i + e);
+#pragma unroll
+                                for (int f = 0; f < 4; f++) v[e + f] = p.scale * q[f];
+                            }
+#pragma unroll
+                            for (int e = 0; e < V; e += 4) {
+                                const float q[4] = {v[e], v[e + 1], v[e + 2], v[e + 3]};
+                                store4(to + i + e, q);
+                            }
+                        }
+                    } else {
+                        for (int i = lane; i < count; i += 32) to[i] = from_float<T>(p.scale * to_float(from[i]));
+                    }
+                }
+            }
+        } else {
+            // By cp.async where nothing has to be made of the values: then a tile is on its way while the one before it arrives.
+            const bool lag = sizeof(T) == 2 && p.x_buffers == 2;
+            Turn xt, arrived;
+            for (long long t = 0; t < mine && wait.alive; t++) {
+                const long long row0 = (split + t * step) * ROWS;
+                const int valid = (int)min((long long)ROWS, p.rows - row0);
+                if (!wait.free(b.x_free, xt)) break;
+                unsigned char* x = smem + at.at_x + xt.at * at.x;
+                if constexpr (PASS != GATED_OUT)
+                    stage<T, ROWS>(x, p.np / 8, static_cast<const T*>(p.grad) + row0 * p.n, p.n, valid, -1, p.wide_grad, loader, row_loaders);
+                stage<T, ROWS>(x + at.grad, p.kp / 8, static_cast<const T*>(p.x) + row0 * p.k, p.k, valid, p.biased ? p.k : -1, p.wide_x, loader, row_loaders);
+                xt.next(p.x_buffers);
+                if (lag) {
+                    cp_async_commit();
+                    if (t == 0) continue;
+                    cp_async_wait_one();
+                } else if (sizeof(T) == 2) {
+                    cp_async_wait_all();
+                }
                 fence_async_proxy();
-                mbar_arrive(&b.w_full[wt.at]);
-                wt.next(p.w_buffers);
+                mbar_arrive(&b.x_full[arrived.at]);
+                arrived.next(p.x_buffers);
+            }
+            if (sizeof(T) == 2) cp_async_wait_all();
+            if (lag && wait.alive && mine > 0) {
+                fence_async_proxy();
+                mbar_arrive(&b.x_full[arrived.at]);
             }
         }
-    } else if (warp == GATED_WORKERS) {   // products
+    } else if (warp == WORKERS) {   // the first products: g, u (, da) of a step
         if (lane == 0) {
-            Turn x1, w1, s1, w2, x2, a2, d2;   // of the first and the second products
-            int c1 = 0, in_group = 0;
-            long long q1 = 0;
-            const int k_steps = p.kp / 16, n_steps = p.np / 16;
-            auto first = [&]() {   // g, u (, da) of the next step
-                if (q1 >= all) return;
-                if (c1 == 0 && !wait.full(b.x_full, x1)) return;
-                if (!(resident && q1 >= chunks) && !wait.full(b.w_full, w1)) return;
-                if (!wait.free(b.s_free, s1)) return;
+            WeightRing w = ring(0);
+            w.begin();
+            Turn xt, wt, w2t, st;
+            int c = 0;
+            for (long long q = 0; q < all; q++) {
+                if (c == 0 && !wait.full(b.x_full, xt)) break;
+                if (!(w.resident && q >= chunks) && !wait.full(b.w_full[0], wt)) break;
+                if (PASS != GATED_OUT && !(p.w_buffers[1] >= chunks && q >= chunks) && !wait.full(b.w_full[1], w2t)) break;
+                if (!wait.free(b.s_free, st)) break;
                 tensor_after_sync();
-                const u32 x = shared_address(smem + at.at_x + x1.at * at.x), w = shared_address(smem + at.at_w + w1.at * at.w);
-                const u32 s = tensor + s1.at * Columns::WIDE;
-                products<T>(s, s, over_columns(x + at.grad, ROWS, p.kp), over_rows(w + at.down, p.kp, 2 * C), 2 * C, k_steps, false, false);
-                if constexpr (PASS != GATED_OUT) products<T>(s + 2 * C, s + 2 * C, over_columns(x, ROWS, p.np), over_columns(w, C, p.np), C, n_steps, false, false);
-                tensor_commit(&b.s_full[s1.at]);
-                s1.next(p.s_buffers), w1.next(p.w_buffers);
-                q1++;
-                if (++c1 == chunks) {
-                    c1 = 0;
-                    if (PASS != GATED_DW) tensor_commit(&b.x_free[x1.at]);
-                    x1.next(p.x_buffers);
+                const u32 x = shared_address(smem + at.at_x + xt.at * at.x), s = tensor + st.at * Columns::WIDE;
+                const u32 w0 = shared_address(w.buffers + wt.at * w.bytes), w1 = shared_address(smem + at.at_w[1] + w2t.at * at.w[1]);
+                products<T>(s, s, over_columns(x + at.grad, ROWS, p.kp), over_rows(PASS == GATED_OUT ? w0 : w1, p.kp, 2 * C), 2 * C, p.kp / 16, false);
+                if constexpr (PASS != GATED_OUT) products<T>(s + 2 * C, s + 2 * C, over_columns(x, ROWS, p.np), over_columns(w0, C, p.np), C, p.np / 16, false);
+                tensor_commit(&b.s_full[st.at]);
+                st.next(p.s_buffers), wt.next(w.count), w2t.next(p.w_buffers[1]);
+                if (++c == chunks) {
+                    c = 0;
+                    if (PASS != GATED_DW) tensor_commit(&b.x_free[xt.at]);
+                    xt.next(p.x_buffers);
                 }
-            };
-            // One step ahead, where there is room for it: its weights', and in DW (where the second products read x too) its rows'.
-            const bool ahead = (resident || p.w_buffers >= 2) && (PASS != GATED_DW || p.x_buffers == 2);
-            if (ahead) first();
-            for (long long q = 0; q < all && wait.alive; q++) {
-                first();
-                if (!wait.alive || !wait.full(b.a_full, a2)) break;
-                if (in_group == 0 && !wait.free(b.d_free, d2)) break;
+                w.used(wait, q);
+                if (!wait.alive) break;
+            }
+            w.end(wait);
+            tensor_commit(&b.end[0]);
+        }
+    } else if (warp == WORKERS + 1) {   // the second products
+        if (lane == 0) {
+            WeightRing w = ring(1);
+            w.begin();
+            Turn wt, xt, act, dt;
+            int in_group = 0;
+            for (long long q = 0; q < all; q++) {
+                if (PASS == GATED_OUT && !(w.resident && q >= chunks) && !wait.full(b.w_full[1], wt)) break;   // (the first products have waited for the others)
+                if (!wait.full(b.a_full, act)) break;
+                if (in_group == 0 && !wait.free(b.d_free, dt)) break;
                 tensor_after_sync();
-                const u32 x = shared_address(smem + at.at_x + x2.at * at.x), w = shared_address(smem + at.at_w + w2.at * at.w);
-                const u32 a = shared_address(smem + at.at_a + a2.at * (Smem::A + Smem::ACT));
-                const u32 d = tensor + col.d + d2.at * Columns::SUMS * col.d_one;
+                const u32 x = shared_address(smem + at.at_x + xt.at * at.x), w1 = shared_address(w.buffers + wt.at * w.bytes);
+                const u32 a = shared_address(smem + at.at_a + act.at * (Smem::A + Smem::ACT));
+                const u32 d = tensor + col.d + dt.at * Columns::SUMS * col.d_one;
                 const bool add = in_group > 0;
                 if constexpr (PASS == GATED_OUT) {
-                    products<T>(d, d + col.low, over_columns(a, ROWS, C), over_rows(w, C, p.np), p.np, C / 16, add, add);
+                    products<T>(d, d + col.low, over_columns(a, ROWS, C), over_rows(w1, C, p.np), p.np, C / 16, add);
                 } else if constexpr (PASS == GATED_DX) {
-                    products<T>(d, d + col.low, over_columns(a, ROWS, 2 * C), over_columns(w + at.down, p.kp, 2 * C), col.d_one, 2 * C / 16, add, add);
+                    products<T>(d, d + col.low, over_columns(a, ROWS, 2 * C), over_columns(w1, p.kp, 2 * C), col.d_one, 2 * C / 16, add);
                 } else {
-                    products<T>(d, d + col.low, over_rows(a, ROWS, 2 * C), over_rows(x + at.grad, ROWS, p.kp), p.kp, ROWS / 16, add, add);
-                    products<T>(d + col.down, d + col.down + col.low, over_rows(x, ROWS, p.np), over_rows(a + Smem::A, ROWS, C), C, ROWS / 16, add, add);
+                    products<T>(d, d + col.low, over_rows(a, ROWS, 2 * C), over_rows(x + at.grad, ROWS, p.kp), p.kp, ROWS / 16, add);
+                    products<T>(d + col.down, d + col.down + col.low, over_rows(x, ROWS, p.np), over_rows(a + Smem::A, ROWS, C), C, ROWS / 16, add);
                     if (p.down_bias_wanted) {   // (a one has one term)
-                        const u32 shape = 1u << 4 | Tensor<T>::FORMAT << 7 | Tensor<T>::FORMAT << 10 | 1u << 15 | 1u << 16 | 2u << 17 | 8u << 24;
                         const Operand rows_of = over_rows(x, ROWS, p.np), one = over_rows(shared_address(smem + at.at_ones), ROWS, 16);
+                        const u32 shape = product_shape<T>(rows_of, one, 16);
                         for (int t = TERMS - 1; t >= 0; t--)
                             for (int s = 0; s < ROWS / 16; s++)
-                                tensor_product(d + col.bias + (t ? col.low : 0), rows_of.descriptor(s, t), one.descriptor(s, 0), shape,
+                                tensor_product(d + col.bias + (t ? col.low : 0), rows_of.at(t * rows_of.plane + s * rows_of.step), one.at(s * one.step), shape,
                                                add || s > 0 || (TERMS == 3 && t == 1));
                     }
-                    tensor_commit(&b.x_free[x2.at]);
-                    x2.next(p.x_buffers);
+                    tensor_commit(&b.x_free[xt.at]);
+                    xt.next(p.x_buffers);
                 }
-                tensor_commit(&b.a_free[a2.at]);
-                if (!resident) tensor_commit(&b.w_free[w2.at]);
-                a2.next(p.a_buffers), w2.next(p.w_buffers);
+                tensor_commit(&b.a_free[act.at]);
+                act.next(p.a_buffers), wt.next(w.count);
                 if (++in_group == group || q + 1 == all) {
                     in_group = 0;
-                    tensor_commit(&b.d_full[d2.at]);
-                    d2.next(p.d_buffers);
+                    tensor_commit(&b.d_full[dt.at]);
+                    dt.next(p.d_buffers);
                 }
+                w.used(wait, q);
+                if (!wait.alive) break;
             }
-            tensor_commit(&b.end);
+            w.end(wait);
+            tensor_commit(&b.end[1]);
         }
     } else {   // workers
-        const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane;
+        constexpr int PARTS = WORKERS / 4, W = C / PARTS;   // warps of 32 rows, hidden channels of each
+        const int quarter = warp & 3, part = warp >> 2, row = 32 * quarter + lane;
         const bool works = 32 * quarter < ROWS;
         const u32 lanes = tensor + ((u32)(32 * quarter) << 16);
         Turn st, act, dt;
-        int in_group = 0;
-        long long group_index = 0;
-        // The finished sums: of tile group_index, or of as many groups of tiles.
+        int in_group = 0, turns = 0, meetings = 0;
+        auto meet = [&]() {   // the warps of the same rows
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b.met[quarter]);
+            return wait.on(&b.met[quarter], meetings++);
+        };
+        // The finished sums: of this CTA's index-th tile, or group of tiles.
         auto take_out = [&](long long index) {
             if (!wait.full(b.d_full, dt)) return;
             tensor_after_sync();
             const u32 d = lanes + col.d + dt.at * Columns::SUMS * col.d_one;
-            const long long at_row = PASS == GATED_DW ? 0 : (split + index * step) * ROWS + row;
-            const bool there = works && at_row < p.rows;
+            const long long row0 = PASS == GATED_DW ? 0 : (split + index * step) * ROWS, at_row = row0 + row;
+            const bool there = works && at_row < p.rows, staged = PASS != GATED_DW && p.io_buffers;
+            const int width = PASS == GATED_OUT ? p.n : p.k;
             float* share = PASS == GATED_DW ? p.shares + ((long long)chunk0 * p.splits + split) * col.d_one * 128 + row : nullptr;
-            for (int c = 16 * half; c < col.d_one; c += 32) {
+            T* mine_s = reinterpret_cast<T*>(smem + at.at_io + row * at.io_stride);
+            if (staged) {
+                if (!(PASS == GATED_OUT && p.residual ? wait.on(&b.io_full, turns) : meet())) return;   // (either way the rows before have left)
+            }
+            for (int c = 16 * part; c < col.d_one; c += 16 * PARTS) {
                 float v[16], low[16];
                 __syncwarp();
-                tensor_load16(v, d + c);
-                if (Columns::SUMS == 2) tensor_load16(low, d + col.low + c);
+                tensor_load(v, d + c);
+                if (Columns::SUMS == 2) tensor_load(low, d + col.low + c);
                 tensor_loaded();
                 if (Columns::SUMS == 2) {
 #pragma unroll
@@ -430,88 +665,94 @@ __global__ void __launch_bounds__(GATED_THREADS, 1) gated_kernel(const __grid_co
                 }
                 if constexpr (PASS == GATED_DW) {
                     float* to = share + (long long)c * 128;
+                    if (index) {
 #pragma unroll
-                    for (int j = 0; j < 16; j++) low[j] = index ? to[j * 128] : 0.f;
+                        for (int j = 0; j < 16; j++) v[j] += to[j * 128];
+                    }
 #pragma unroll
-                    for (int j = 0; j < 16; j++) to[j * 128] = low[j] + v[j];
+                    for (int j = 0; j < 16; j++) to[j * 128] = v[j];
                 } else if (there) {
-                    const int width = PASS == GATED_OUT ? p.n : p.k;
                     if constexpr (PASS == GATED_OUT) {
 #pragma unroll
                         for (int j = 0; j < 16; j++) v[j] += bias_s[c + j];
                         if (p.residual) {
                             float r[16];
-                            load16(r, static_cast<const T*>(p.residual) + at_row * width + c, width - c, p.wide_out);
+                            load16(r, staged ? mine_s + c : static_cast<const T*>(p.residual) + at_row * width + c, width - c, p.wide_out);
 #pragma unroll
                             for (int j = 0; j < 16; j++) v[j] = fmaf(p.scale, r[j], v[j]);
                         }
                     }
-                    store16(static_cast<T*>(p.out) + at_row * width + c, v, width - c, p.wide_out);
+                    store16(staged ? mine_s + c : static_cast<T*>(p.out) + at_row * width + c, v, width - c, p.wide_out);
                 }
-            }
-            if constexpr (PASS == GATED_DX) {   // s dout, which has just been read
-                if (p.dresidual && there)
-                    for (int c = 16 * half; c < p.np; c += 32) {
-                        float v[16];
-                        load16(v, static_cast<const T*>(p.grad) + at_row * p.n + c, p.n - c, p.wide_dresidual);
-#pragma unroll
-                        for (int j = 0; j < 16; j++) v[j] *= p.scale;
-                        store16(static_cast<T*>(p.dresidual) + at_row * p.n + c, v, p.n - c, p.wide_dresidual);
-                    }
-                __syncwarp();
             }
             tensor_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&b.d_free[dt.at]);
             dt.next(p.d_buffers);
-        };
-        for (long long q = 0; q < all && wait.alive; q++) {
-            if (!wait.full(b.s_full, st)) break;
-            if (!wait.free(b.a_free, act)) break;
-            tensor_after_sync();
-            const u32 s = lanes + st.at * Columns::WIDE;
-            unsigned char* a = smem + at.at_a + act.at * (Smem::A + Smem::ACT);
-            if (works) {
-#pragma unroll 1
-                for (int j = 0; j < C / 2; j += 16) {
-                    const int c = half * (C / 2) + j;
-                    float g[16], u[16], da[16];
-                    tensor_load16(g, s + c);
-                    tensor_load16(u, s + C + c);
-                    if (PASS != GATED_OUT) tensor_load16(da, s + 2 * C + c);
-                    tensor_loaded();
-                    if (p.activation == PL_GATE_SILU) gated_work<T, PASS, PL_GATE_SILU, ROWS>(g, u, da, a, row, c);
-                    else if (p.activation == PL_GATE_GELU) gated_work<T, PASS, PL_GATE_GELU, ROWS>(g, u, da, a, row, c);
-                    else if (p.activation == PL_GATE_SIGMOID) gated_work<T, PASS, PL_GATE_SIGMOID, ROWS>(g, u, da, a, row, c);
-                    else gated_work<T, PASS, PL_GATE_RELU, ROWS>(g, u, da, a, row, c);
+            if (!staged) return;
+            // The rows of these warps leave together, side by side.
+            if (!meet()) return;
+            const int valid = (int)max(0ll, min(32ll, p.rows - row0 - 32 * quarter)) * (works ? 1 : 0), thread = 32 * part + lane;
+            const unsigned char* from = smem + at.at_io + 32 * quarter * at.io_stride;
+            T* to = static_cast<T*>(p.out) + (row0 + 32 * quarter) * width;
+            if (p.wide_out) {
+                const int pieces = width * (int)sizeof(T) / 16;
+                for (int i = thread; i < valid * pieces; i += 32 * PARTS) {
+                    const int r = i / pieces;
+                    reinterpret_cast<uint4*>(to)[i] = *reinterpret_cast<const uint4*>(from + r * at.io_stride + 16 * (i - r * pieces));
+                }
+            } else {
+                for (int i = thread; i < valid * width; i += 32 * PARTS) {
+                    const int r = i / width;
+                    to[i] = reinterpret_cast<const T*>(from + r * at.io_stride)[i - r * width];
                 }
             }
-            fence_async_proxy();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b.io_free);
+            turns++;
+        };
+        for (long long q = 0, groups = 0; q < all && wait.alive; q++) {
+            if (!wait.full(b.s_full, st)) break;
+            tensor_after_sync();
+            const u32 s = lanes + st.at * Columns::WIDE + W * part;
+            float g[W], u[W], da[W];
+            tensor_load(g, s);
+            tensor_load(u, s + C);
+            if (PASS != GATED_OUT) tensor_load(da, s + 2 * C);
+            tensor_loaded();
             tensor_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&b.s_free[st.at]), mbar_arrive(&b.a_full[act.at]);
+            if (lane == 0) mbar_arrive(&b.s_free[st.at]);
+            if (!wait.free(b.a_free, act)) break;
+            unsigned char* a = smem + at.at_a + act.at * (Smem::A + Smem::ACT);
+            if (works) {
+                if (p.activation == PL_GATE_SILU) gated_work<T, PASS, PL_GATE_SILU, ROWS>(g, u, da, a, row, W * part);
+                else if (p.activation == PL_GATE_GELU) gated_work<T, PASS, PL_GATE_GELU, ROWS>(g, u, da, a, row, W * part);
+                else if (p.activation == PL_GATE_SIGMOID) gated_work<T, PASS, PL_GATE_SIGMOID, ROWS>(g, u, da, a, row, W * part);
+                else gated_work<T, PASS, PL_GATE_RELU, ROWS>(g, u, da, a, row, W * part);
+            }
+            fence_async_proxy();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b.a_full[act.at]);
             st.next(p.s_buffers), act.next(p.a_buffers);
-            if (in_group == 0 && q > 0) take_out(group_index++);   // of the group before: its last products had this step's time
+            if (in_group == 0 && q > 0) take_out(groups++);   // of the group before: its last products had this step's time
             if (++in_group == group) in_group = 0;
+            if (q + 1 == all) take_out(groups);
         }
-        if (wait.alive && all > 0) take_out(group_index);
     }
     // All products are done, or a wait has run out: then nothing that could pass for a result.
     __syncwarp();
-    if (warp == GATED_WORKERS) Waits{&b.dead}.on(&b.end, 0, true);
+    if (warp == WORKERS || warp == WORKERS + 1) Waits{&b.dead}.on(&b.end[warp - WORKERS], 0, true);
     __syncthreads();
     if (b.dead) {
         if constexpr (PASS == GATED_DW) {
             float* share = p.shares + ((long long)chunk0 * p.splits + split) * col.d_one * 128;
-            for (int i = threadIdx.x; i < col.d_one * 128; i += GATED_THREADS) share[i] = NAN;
+            for (int i = threadIdx.x; i < col.d_one * 128; i += THREADS) share[i] = NAN;
         } else {
             const int width = PASS == GATED_OUT ? p.n : p.k;
             for (long long t = 0; t < mine; t++) {
                 const long long row0 = (split + t * step) * ROWS, count = min((long long)ROWS, p.rows - row0) * width;
-                for (long long i = threadIdx.x; i < count; i += GATED_THREADS) static_cast<T*>(p.out)[row0 * width + i] = from_float<T>(NAN);
-                if (PASS == GATED_DX && p.dresidual)
-                    for (long long i = threadIdx.x; i < min((long long)ROWS, p.rows - row0) * p.n; i += GATED_THREADS)
-                        static_cast<T*>(p.dresidual)[row0 * p.n + i] = from_float<T>(NAN);
+                for (long long i = threadIdx.x; i < count; i += THREADS) static_cast<T*>(p.out)[row0 * width + i] = from_float<T>(NAN);
             }
         }
     }

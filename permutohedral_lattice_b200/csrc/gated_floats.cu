@@ -3,6 +3,6 @@
 
 namespace pl {
 
-int gated_floats(GatedArgs p, GatedPass pass, cudaStream_t st) { return gated_of<float>(p, pass, st); }
+int gated_floats(GatedArgs p, GatedPass pass, bool pack, cudaStream_t st) { return gated_of<float>(p, pass, pack, st); }
 
 }  // namespace pl

@@ -7,33 +7,34 @@
 
 namespace pl {
 
-int gated_floats(GatedArgs p, GatedPass pass, cudaStream_t st);
-int gated_halves(GatedArgs p, int dtype, GatedPass pass, cudaStream_t st);
+int gated_floats(GatedArgs p, GatedPass pass, bool pack, cudaStream_t st);
+int gated_halves(GatedArgs p, int dtype, GatedPass pass, bool pack, cudaStream_t st);
 
 constexpr size_t GATED_SMEM = 227 * 1024;   // of a CTA, at most
 
 // CTAs of a chunk of hidden channels when the weights' gradients are summed up.
 inline int gated_splits(int chunks, long long rows, int sms) { return (int)std::max(1ll, std::min<long long>(std::max(1, sms / chunks), (rows + 127) / 128)); }
 
-// Buffers, as far as there is room: the weights of all chunks where they fit (else they come anew for every tile), of everything else two, so
-// that what comes next is fetched while products run.
+// Buffers, as far as there is room: rows that leave together (or a thread stores its own), the weights of all chunks (else they come anew for every
+// tile), of everything else two, so that what comes next is fetched while products run.
 template <typename T, GatedPass PASS, int ROWS>
 static bool gated_plan(GatedArgs& p) {
     const int chunks = PASS == GATED_DW ? 1 : p.chunks;
-    auto fits = [&](int w) {
-        for (int left : {0, 1, 2, 3}) {
-            p.w_buffers = w, p.x_buffers = left & 2 ? 1 : 2, p.a_buffers = left & 1 ? 1 : 2;
-            if (PASS == GATED_DW && p.a_buffers == 2) continue;   // (its second products take as long as its first: nothing waits for them)
-            if (GatedSmem<T, PASS, ROWS>(p).total <= (int)GATED_SMEM) return true;
-        }
+    auto fits = [&]() {
+        for (int io = PASS == GATED_DW ? 0 : 1; io >= 0; io--)
+            for (int w : {chunks, std::min(2, chunks), 1})
+                for (int left : {0, 1, 2, 3}) {
+                    p.io_buffers = io, p.w_buffers[0] = p.w_buffers[1] = w, p.x_buffers = left & 2 ? 1 : 2, p.a_buffers = left & 1 ? 1 : 2;
+                    if (PASS == GATED_DW && p.a_buffers == 2) continue;   // (its second products take as long as its first: nothing waits for them)
+                    if (GatedSmem<T, PASS, ROWS>(p).total <= (int)GATED_SMEM) return true;
+                }
         return false;
     };
-    if (!fits(chunks) && !fits(std::min(2, chunks)) && !fits(1)) return false;
     auto columns = [&](int s, int d) {
         p.s_buffers = s, p.d_buffers = d;
         return GatedColumns<T, PASS>(p).total <= 512;
     };
-    return (PASS != GATED_DW && columns(2, 2)) || columns(2, 1) || columns(1, 1);
+    return fits() && ((PASS != GATED_DW && columns(2, 2)) || columns(2, 1) || columns(1, 1));
 }
 
 template <typename T, GatedPass PASS, int ROWS>
@@ -42,9 +43,14 @@ static int launch_gated_rows(GatedArgs& p, cudaStream_t st) {
     const long long tiles = (p.rows + ROWS - 1) / ROWS;
     const unsigned grid = PASS == GATED_DW ? p.chunks * p.splits : (unsigned)std::min<long long>(tiles, num_sms());
     PL_TRY((ensure_dynamic_smem<gated_kernel<T, PASS, ROWS>>(smem)));
-    gated_kernel<T, PASS, ROWS><<<grid, GATED_THREADS, smem, st>>>(p);
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(grid), config.blockDim = dim3(GatedWarps<T>::THREADS), config.dynamicSmemBytes = smem, config.stream = st;
+    cudaLaunchAttribute early[1];   // on the SMs, with its barriers set up, when the kernel before it (gated_pack, usually) ends
+    early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = early, config.numAttrs = 1;
+    PL_CUDA(cudaLaunchKernelEx(&config, gated_kernel<T, PASS, ROWS>, (const GatedArgs)p));
     PL_COUNT_LAUNCHES(1);
-    PL_CUDA(cudaGetLastError());
     return PL_OK;
 }
 template <typename T, GatedPass PASS>
@@ -55,10 +61,20 @@ static int launch_gated(GatedArgs& p, cudaStream_t st) {
     return PL_INTERNAL_ERROR;
 }
 template <typename T>
-static int gated_of(GatedArgs& p, GatedPass pass, cudaStream_t st) {
+static int pack_gated(const GatedArgs& p, cudaStream_t st) {
+    const int items = gated_chunk<T>() * (p.np / 8) + p.kp * (2 * gated_chunk<T>() / 8);
+    gated_pack<T><<<dim3((items + 255) / 256, p.chunks), 256, 0, st>>>(p);
+    PL_COUNT_LAUNCHES(1);
+    PL_CUDA(cudaGetLastError());
+    return PL_OK;
+}
+// pack: the weights first (a backward pass packs them once for both of its kernels).
+template <typename T>
+static int gated_of(GatedArgs& p, GatedPass pass, bool pack, cudaStream_t st) {
     p.chunks = (p.h + gated_chunk<T>() - 1) / gated_chunk<T>();
     p.splits = gated_splits(p.chunks, p.rows, num_sms());
     p.drain = sizeof(T) == 4 ? 2 : 64;
+    if (pack) PL_TRY(pack_gated<T>(p, st));
     return pass == GATED_OUT ? launch_gated<T, GATED_OUT>(p, st) : pass == GATED_DX ? launch_gated<T, GATED_DX>(p, st) : launch_gated<T, GATED_DW>(p, st);
 }
 

@@ -19,13 +19,16 @@ static GatedArgs gated_args(const pl_gated_shape* m, const void* x, const pl_gat
     p.biased = p.gate_bias || p.up_bias;
     p.np = (p.n + 15) / 16 * 16;
     p.wide_x = p.k % 8 == 0 && gated_aligned(x);
-    p.wide_hidden = p.h % 8 == 0 && gated_aligned(p.gate_weight) && gated_aligned(p.up_weight);
-    p.wide_down = p.n % 8 == 0 && gated_aligned(p.down_weight);
     return p;
 }
 static void set_kp(GatedArgs& p) { p.kp = (p.k + (p.biased ? 1 : 0) + 15) / 16 * 16; }
-static int run_gated(const GatedArgs& p, int dtype, GatedPass pass, cudaStream_t st) {
-    return dtype == PL_F32 ? gated_floats(p, pass, st) : gated_halves(p, dtype, pass, st);
+static int run_gated(const GatedArgs& p, int dtype, GatedPass pass, bool pack, cudaStream_t st) {
+    return dtype == PL_F32 ? gated_floats(p, pass, pack, st) : gated_halves(p, dtype, pass, pack, st);
+}
+static size_t packed_bytes(const pl_gated_shape* m) {   // with all biases
+    const int chunk = chunk_of(m), chunks = (m->h + chunk - 1) / chunk, kp = (m->k + 16) / 16 * 16, np = (m->n + 15) / 16 * 16;
+    const size_t one = m->dtype == PL_F32 ? gated_down_bytes<float>(np) + gated_up_bytes<float>(kp) : gated_down_bytes<__half>(np) + gated_up_bytes<__half>(kp);
+    return one * chunks;
 }
 
 }  // namespace pl
@@ -34,30 +37,36 @@ using namespace pl;
 
 extern "C" {
 
-int pl_gated_mix(const pl_gated_shape* m, void* out, const void* x, const pl_gated_weights* w, const void* residual, void* stream) {
+int pl_gated_mix_workspace_bytes(const pl_gated_shape* m, int backward, size_t* bytes) {
+    PL_TRY(check_gated(m));
+    if (!bytes) return PL_INVALID_ARGUMENT;
+    *bytes = packed_bytes(m);
+    if (!backward) return PL_OK;
+    const int chunk = chunk_of(m), chunks = (m->h + chunk - 1) / chunk;
+    const size_t columns = (m->k + 16) / 16 * 16 + chunk + 16;   // with all biases
+    *bytes += sizeof(float) * 128 * columns * chunks * gated_splits(chunks, m->rows, num_sms());
+    return PL_OK;
+}
+
+int pl_gated_mix(const pl_gated_shape* m, void* out, const void* x, const pl_gated_weights* w, const void* residual, void* workspace,
+                 size_t workspace_bytes, void* stream) {
     PL_TRY(check_gated(m));
     if (m->rows == 0) return PL_OK;
     if (!out || !x || !w || !w->gate_weight || !w->up_weight || !w->down_weight) return PL_INVALID_ARGUMENT;
+    if (!workspace || workspace_bytes < packed_bytes(m)) return PL_WORKSPACE_TOO_SMALL;
+    if (!gated_aligned(workspace)) return PL_INVALID_ARGUMENT;
     GatedArgs p = gated_args(m, x, w);
     set_kp(p);
+    p.packed = static_cast<unsigned char*>(workspace);
     p.out = out, p.residual = residual;
     p.wide_out = p.n % (m->dtype == PL_F32 ? 4 : 8) == 0 && gated_aligned(out) && gated_aligned(residual);
-    return run_gated(p, m->dtype, GATED_OUT, (cudaStream_t)stream);
-}
-
-int pl_gated_mix_workspace_bytes(const pl_gated_shape* m, size_t* bytes) {
-    PL_TRY(check_gated(m));
-    if (!bytes) return PL_INVALID_ARGUMENT;
-    const int chunk = chunk_of(m), chunks = (m->h + chunk - 1) / chunk;
-    const size_t columns = (m->k + 16) / 16 * 16 + chunk + 16;   // with all biases
-    *bytes = sizeof(float) * 128 * columns * chunks * gated_splits(chunks, m->rows, num_sms());
-    return PL_OK;
+    return run_gated(p, m->dtype, GATED_OUT, true, (cudaStream_t)stream);
 }
 
 int pl_gated_mix_backward(const pl_gated_shape* m, const void* grad_out, const void* x, const pl_gated_weights* w, pl_gated_gradients d,
                           void* workspace, size_t workspace_bytes, void* stream) {
     size_t need = 0;
-    PL_TRY(pl_gated_mix_workspace_bytes(m, &need));
+    PL_TRY(pl_gated_mix_workspace_bytes(m, 1, &need));
     const cudaStream_t st = (cudaStream_t)stream;
     const size_t size = m->dtype == PL_F32 ? 4 : 2;
     const bool sums = d.gate_weight || d.up_weight || d.down_weight || d.gate_bias || d.up_bias || d.down_bias;
@@ -69,27 +78,27 @@ int pl_gated_mix_backward(const pl_gated_shape* m, const void* grad_out, const v
         return PL_OK;
     }
     if (!grad_out || !x || !w || !w->gate_weight || !w->up_weight || !w->down_weight) return PL_INVALID_ARGUMENT;
-    if (sums && (!workspace || workspace_bytes < need)) return PL_WORKSPACE_TOO_SMALL;
-    if (sums && !gated_aligned(workspace)) return PL_INVALID_ARGUMENT;
+    if (!workspace || workspace_bytes < need) return PL_WORKSPACE_TOO_SMALL;
+    if (!gated_aligned(workspace)) return PL_INVALID_ARGUMENT;
     GatedArgs p = gated_args(m, x, w);
     p.grad = grad_out;
     p.wide_grad = p.n % 8 == 0 && gated_aligned(grad_out);
+    p.biased = p.biased || d.gate_bias || d.up_bias;   // (the ones' column sums dg and du)
+    set_kp(p);
+    p.packed = static_cast<unsigned char*>(workspace);
     if (d.x) {
-        set_kp(p);
         p.out = d.x, p.dresidual = d.residual;
         p.wide_out = p.k % (m->dtype == PL_F32 ? 4 : 8) == 0 && gated_aligned(d.x);
         p.wide_dresidual = p.n % (m->dtype == PL_F32 ? 4 : 8) == 0 && gated_aligned(grad_out) && gated_aligned(d.residual);
-        PL_TRY(run_gated(p, m->dtype, GATED_DX, st));
+        PL_TRY(run_gated(p, m->dtype, GATED_DX, true, st));
     } else if (d.residual) {
         const pl_dropout none = {};
         PL_TRY(pl_channel_dropout(nullptr, d.residual, grad_out, nullptr, m->rows * m->n, m->dtype, m->residual_scale, &none, stream));
     }
     if (!sums) return PL_OK;
-    p.biased = p.biased || d.gate_bias || d.up_bias;   // (the ones' column sums dg and du)
-    set_kp(p);
     p.down_bias_wanted = d.down_bias != nullptr;
-    p.shares = static_cast<float*>(workspace);
-    PL_TRY(run_gated(p, m->dtype, GATED_DW, st));
+    p.shares = reinterpret_cast<float*>(p.packed + packed_bytes(m));
+    PL_TRY(run_gated(p, m->dtype, GATED_DW, !d.x, st));
     GatedSums s = {};
     s.shares = p.shares, s.k = p.k, s.h = p.h, s.n = p.n, s.kp = p.kp, s.chunk = chunk_of(m);
     s.chunks = (p.h + s.chunk - 1) / s.chunk, s.splits = gated_splits(s.chunks, m->rows, num_sms());

@@ -1,9 +1,9 @@
 // Fifth-generation tensor cores for the gated feed-forward block: 16-bit operands in shared memory, sums in tensor memory.
 //
 // Operands.  A tile of rows x columns lies as blocks of 8 rows by 8 columns, 16 bytes a row and 128 a block, blocks of the same columns
-// one after another, 16 bytes more between those of other columns (so that eight threads with the columns of one row write to different
-// banks).  The same bytes serve as an operand whose sums run over the columns (K-major) and as one whose sums run over the rows
-// (MN-major): nothing is ever transposed, the weights lie as they do in memory, x and its products' operands both ways.
+// one after another.  The same bytes serve as an operand whose sums run over the columns (K-major) and as one whose sums run over the
+// rows (MN-major): nothing is ever transposed, x and what is made of it are operands both ways.  Threads with eight rows of a block access it
+// together, in all banks.
 //
 // Terms.  A float is the sum of three bfloat16 numbers up to 2^-27 of it, each the nearest to what is left, and a product of two
 // floats that of the six pairs whose orders of magnitude are above 2^-24 of it: as many steps as three products of tf32 numbers would
@@ -23,58 +23,75 @@ struct Tensor {
     using Term = typename std::conditional<sizeof(T) == 4, __nv_bfloat16, T>::type;
 };
 
-// Bytes from one block of columns to the next, of a tile of so many rows.
-__host__ __device__ constexpr int column_blocks(int rows) { return rows * 16 + 16; }
-__host__ __device__ constexpr int tile_bytes(int rows, int columns) { return columns / 8 * column_blocks(rows); }   // of a term
+// Bytes from one block of columns to the next, of a tile of so many rows, and of a tile.
+__host__ __device__ constexpr int column_blocks(int rows) { return rows * 16; }
+__host__ __device__ constexpr int tile_bytes(int rows, int columns) { return rows * columns * 2; }   // of a term
 
-struct Operand {   // of a product: where its first 16 terms of the sum lie, bytes to the next 16, and to the next term
-    u32 at, step, plane;
-    u64 strides;
-    u32 transposed;
-    __device__ __forceinline__ u64 descriptor(int s, int term) const {
-        return strides | (u64)(((at + s * step + term * plane) >> 4) & 0x3FFF) | 1ull << 46;
-    }
+struct Operand {   // of a product: its first 16 terms of the sum, and how far the next 16 are and the next term (in 16 bytes)
+    u64 first;
+    u32 step, plane, transposed;
+    __device__ __forceinline__ u64 at(u32 offset) const { return first + offset; }   // (addresses are below 2^18: nothing is carried)
 };
+__device__ __forceinline__ u64 operand_of(u32 at, u32 along, u32 across) {   // strides of blocks, along the sums and across
+    return (u64)(at >> 4) | (u64)(along >> 4) << 16 | (u64)(across >> 4) << 32 | 1ull << 46;
+}
 // The tile's rows are the operand's rows, sums run over its columns.
 __device__ __forceinline__ Operand over_columns(u32 at, int rows, int columns) {
-    const u32 cb = column_blocks(rows);
-    return {at, 2 * cb, (u32)tile_bytes(rows, columns), (u64)(cb >> 4) << 16 | (u64)(128 >> 4) << 32, 0};
+    return {operand_of(at, column_blocks(rows), 128), (u32)column_blocks(rows) / 8, (u32)tile_bytes(rows, columns) / 16, 0};
 }
 // The tile's columns are the operand's rows, sums run over its rows.
 __device__ __forceinline__ Operand over_rows(u32 at, int rows, int columns) {
-    const u32 cb = column_blocks(rows);
-    return {at, 256, (u32)tile_bytes(rows, columns), (u64)(128 >> 4) << 16 | (u64)(cb >> 4) << 32, 1};
+    return {operand_of(at, 128, column_blocks(rows)), 16, (u32)tile_bytes(rows, columns) / 16, 1};
 }
 __device__ __forceinline__ void tensor_product(u32 d, u64 a, u64 b, u32 shape, bool add) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
                  "r"(shape), "r"((u32)add)
                  : "memory");
 }
-// d (+)= a b^T over 16 `steps` terms, 128 x n; small: where products with a term but the first go (may be d).  add, add_small: to what
-// is there.
 template <typename T>
-__device__ __forceinline__ void products(u32 d, u32 small, const Operand& a, const Operand& b, int n, int steps, bool add, bool add_small) {
-    const u32 shape = 1u << 4 | Tensor<T>::FORMAT << 7 | Tensor<T>::FORMAT << 10 | a.transposed << 15 | b.transposed << 16 | (u32)(n / 8) << 17 | 8u << 24;
+__device__ __forceinline__ u32 product_shape(const Operand& a, const Operand& b, int n) {   // 128 x n
+    return 1u << 4 | Tensor<T>::FORMAT << 7 | Tensor<T>::FORMAT << 10 | a.transposed << 15 | b.transposed << 16 | (u32)(n / 8) << 17 | 8u << 24;
+}
+// d (+)= a b^T over 16 `steps` terms, 128 x n; small: where products with a term but the first go (may be d).  add: to what is there.
+template <typename T>
+__device__ __forceinline__ void products(u32 d, u32 small, const Operand& a, const Operand& b, int n, int steps, bool add) {
+    const u32 shape = product_shape<T>(a, b, n);
     if constexpr (Tensor<T>::TERMS == 3) {
-        bool more = add_small;
+        bool more = add;
+#pragma unroll
         for (int order = 2; order >= 1; order--)
-            for (int i = 0; i <= order; i++)
-                for (int s = 0; s < steps; s++) {
-                    tensor_product(small, a.descriptor(s, i), b.descriptor(s, order - i), shape, more);
+#pragma unroll
+            for (int i = 0; i <= order; i++) {
+                u64 p = a.at(i * a.plane), q = b.at((order - i) * b.plane);
+#pragma unroll 2
+                for (int s = 0; s < steps; s++, p += a.step, q += b.step) {
+                    tensor_product(small, p, q, shape, more);
                     more = true;
                 }
+            }
         if (small == d) add = true;
     }
-    for (int s = 0; s < steps; s++) tensor_product(d, a.descriptor(s, 0), b.descriptor(s, 0), shape, add || s > 0);
+    u64 p = a.first, q = b.first;
+#pragma unroll 4
+    for (int s = 0; s < steps; s++, p += a.step, q += b.step) {
+        tensor_product(d, p, q, shape, add);
+        add = true;
+    }
 }
 __device__ __forceinline__ void tensor_commit(u64* bar) {   // the barrier's phase ends when all products asked for so far are done
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_address(bar)) : "memory");
 }
-__device__ __forceinline__ void tensor_load16(float (&v)[16], u32 at) {   // 16 columns of the lane's row; there after tensor_loaded
+__device__ __forceinline__ void tensor_load(float (&v)[16], u32 at) {   // columns of the lane's row; there after tensor_loaded
     u32* r = reinterpret_cast<u32*>(v);
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
                    "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at));
+}
+__device__ __forceinline__ void tensor_load(float (&v)[8], u32 at) {
+    u32* r = reinterpret_cast<u32*>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(at));
 }
 __device__ __forceinline__ void tensor_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }

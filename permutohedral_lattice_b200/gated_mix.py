@@ -40,10 +40,14 @@ def _structure(s):
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_bytes(s):
+def _workspace_bytes(s, backward):
     nbytes = ctypes.c_size_t(0)
-    capi.check(capi.lib().pl_gated_mix_workspace_bytes(_structure(s), ctypes.byref(nbytes)), "pl_gated_mix_workspace_bytes")
+    capi.check(capi.lib().pl_gated_mix_workspace_bytes(_structure(s), backward, ctypes.byref(nbytes)), "pl_gated_mix_workspace_bytes")
     return nbytes.value
+
+
+def _workspace(s, backward, device):
+    return torch.empty(_workspace_bytes(s, backward), dtype=torch.uint8, device=device)
 
 
 def _check(x, residual, weights, activation):
@@ -82,8 +86,9 @@ def _check(x, residual, weights, activation):
 def _forward(device, s, x, residual, weights):
     out = x.new_empty(x.shape[:-1] + (s.n,))
     with _OnDevice(device):
+        workspace = _workspace(s, False, device)
         capi.check(capi.lib().pl_gated_mix(_structure(s), out.data_ptr(), x.data_ptr(), ctypes.byref(capi.PlGatedWeights(*map(_ptr, weights))),
-                                           _ptr(residual), _stream_handle(device)), "pl_gated_mix")
+                                           _ptr(residual), workspace.data_ptr(), workspace.numel(), _stream_handle(device)), "pl_gated_mix")
     return out
 
 
@@ -104,13 +109,11 @@ class _GatedMix(torch.autograd.Function):
         made = {name: torch.empty(like[name].shape, dtype=x.dtype, device=device)
                 for name, wanted in zip(_NAMES, ctx.needs_input_grad[2:]) if wanted}
         with _OnDevice(device):
-            workspace = None
-            if any(name in made for name in _WEIGHTS):
-                workspace = torch.empty(_workspace_bytes(s), dtype=torch.uint8, device=device)
+            workspace = _workspace(s, True, device)
             capi.check(capi.lib().pl_gated_mix_backward(
                 _structure(s), grad.data_ptr(), x.data_ptr(), ctypes.byref(capi.PlGatedWeights(*map(_ptr, weights))),
-                capi.PlGatedGradients(**{name: t.data_ptr() for name, t in made.items()}), _ptr(workspace),
-                0 if workspace is None else workspace.numel(), _stream_handle(device)), "pl_gated_mix_backward")
+                capi.PlGatedGradients(**{name: t.data_ptr() for name, t in made.items()}), workspace.data_ptr(),
+                workspace.numel(), _stream_handle(device)), "pl_gated_mix_backward")
         return (None, None) + tuple(made.get(name) for name in _NAMES)
 
 

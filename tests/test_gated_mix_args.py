@@ -51,8 +51,8 @@ def test_c_entries_refuse_before_any_launch():
 
     whole = capi.PlGatedWeights(16, 16, 16, 0, 0, 0)
 
-    def forward(m, out=16, x=16, w=whole):
-        return L.pl_gated_mix(m, out, x, None if w is None else ctypes.byref(w), 0, 0)
+    def forward(m, out=16, x=16, w=whole, ws=16, nbytes=1 << 40):
+        return L.pl_gated_mix(m, out, x, None if w is None else ctypes.byref(w), 0, ws, nbytes, 0)
 
     assert forward(None) == capi.PL_INVALID_ARGUMENT
     for bad in ({"rows": -1}, {"rows": (1 << 40) + 1}, {"k": 0}, {"h": 0}, {"n": 0}, {"activation": 4}, {"activation": -1}, {"dtype": 3}):
@@ -61,7 +61,10 @@ def test_c_entries_refuse_before_any_launch():
         assert forward(shape(**bad)) == capi.PL_UNSUPPORTED_DIMS, bad
     for bad in ({"out": 0}, {"x": 0}, {"w": None}, {"w": capi.PlGatedWeights(16, 16, 0, 0, 0, 0)}):
         assert forward(shape(), **bad) == capi.PL_INVALID_ARGUMENT, bad
-    assert forward(shape(rows=0), 0, 0, None) == capi.PL_OK
+    assert forward(shape(rows=0), 0, 0, None, 0, 0) == capi.PL_OK
+    assert forward(shape(), ws=0) == capi.PL_WORKSPACE_TOO_SMALL
+    assert forward(shape(), nbytes=100) == capi.PL_WORKSPACE_TOO_SMALL
+    assert forward(shape(), ws=24) == capi.PL_INVALID_ARGUMENT
 
     def back(m, grad=16, x=16, w=whole, d=None, ws=16, nbytes=1 << 40):
         d = capi.PlGatedGradients(**({"gate_weight": 16} if d is None else d))
@@ -73,4 +76,4 @@ def test_c_entries_refuse_before_any_launch():
     assert back(shape(), ws=0) == capi.PL_WORKSPACE_TOO_SMALL
     assert back(shape(), ws=24) == capi.PL_INVALID_ARGUMENT
     assert back(shape(h=513)) == capi.PL_UNSUPPORTED_DIMS
-    assert L.pl_gated_mix_workspace_bytes(shape(), None) == capi.PL_INVALID_ARGUMENT
+    assert L.pl_gated_mix_workspace_bytes(shape(), 1, None) == capi.PL_INVALID_ARGUMENT
