@@ -6,7 +6,7 @@
 //
 // The hidden values (g, u, a and their gradients) never leave the SM: a CTA takes a tile of rows through the hidden channels a chunk
 // at a time.  A chunk's g and u (and da) are products in tensor memory, its a (dg, du) go to shared memory as the next products' operand.
-// The biases of g and u are a row more of the weights beside a one in every row of x.  The backward pass makes g and u again, in two
+// The biases of g and u are a row more of the weights beside a column of ones.  The backward pass makes g and u again, in two
 // kernels: gated_kernel<DX> sums dx over the chunks of a tile as the forward pass does out, gated_kernel<DW> sums the weights' gradients
 // over the tiles of a chunk, a chunk a CTA, and adds them to a share of its own in the workspace now and then (`drain`, see
 // gated_launch.cuh); gated_sums adds up the shares in order.  gated_pack first lays out the weights as the products read them.
@@ -15,6 +15,7 @@
 // products, and for the weights that only theirs read; loaders fetch rows.  They meet at barriers in shared memory; every wait is bounded.
 // If one runs out, all give up and the results are NaN.
 #pragma once
+#include <cuda.h>
 #include "gated_tensor.cuh"
 
 namespace pl {
@@ -30,16 +31,20 @@ struct GatedWarps {
 struct GatedArgs {
     long long rows;
     int k, h, n, activation;
-    int kp, np;                      // columns of a tile of x (with the ones, if there are biases of g or u) and of out
+    int kx, kp, np;                  // columns of a tile of x, with the ones (if there are biases of g or u), and of out
     int chunks, splits;              // of the hidden channels; CTAs of a chunk (DW)
     int x_buffers, w_buffers[2], a_buffers, s_buffers, d_buffers, io_buffers, drain;
     float scale;
     const void *x, *gate_weight, *up_weight, *down_weight, *gate_bias, *up_bias, *down_bias, *residual, *grad;
-    int biased, wide_x, wide_grad, wide_out;   // wide: rows of whole 16 bytes on 16-byte boundaries
-    int wide_dresidual, down_bias_wanted;      // (DX, DW)
+    int biased, boxes, wide_x, wide_grad, wide_out;   // wide: rows of whole 16 bytes on 16-byte boundaries; boxes: of 16-bit values, what is read
+    int wide_dresidual, down_bias_wanted;             // (DX, DW)
     unsigned char* packed;           // the weights, a chunk after another: Wd, Wg and Wu as tiles
     void *out, *dresidual;           // out: or dx
     float* shares;                   // [chunks][splits][columns of sums][128]
+};
+
+struct GatedMaps {   // of x, dout, the residual and out (or dx) as matrices, where they go by the TMA
+    CUtensorMap x, grad, residual, out;
 };
 
 template <typename T>
@@ -56,23 +61,25 @@ struct GatedSmem {
     static constexpr int C = gated_chunk<T>(), TERMS = Tensor<T>::TERMS;
     static constexpr int A = TERMS * tile_bytes(ROWS, PASS == GATED_OUT ? C : 2 * C), ACT = PASS == GATED_DW ? TERMS * tile_bytes(ROWS, C) : 0;
     static constexpr int BARRIERS = 2048;
-    int grad, x, io_stride;          // bytes: a tile of dout, of x with it; a row on its way out
+    __host__ __device__ static int rows_bytes(int columns) { return TERMS == 1 ? swizzled_bytes(ROWS, 2 * columns) : TERMS * tile_bytes(ROWS, columns); }
+    int grad, x, io;                 // bytes: a tile of dout, of x with it, of rows on their way out
     int w[2];                        // of the weights that the first products alone read (OUT: Wg and Wu, DX and DW: Wd), and of the others
     int at_x, at_w[2], at_a, at_io, at_ones, total;
     __host__ __device__ GatedSmem(const GatedArgs& p) {
-        grad = PASS == GATED_OUT ? 0 : TERMS * tile_bytes(ROWS, p.np);
-        x = grad + TERMS * tile_bytes(ROWS, p.kp);
+        grad = PASS == GATED_OUT ? 0 : rows_bytes(p.np);
+        x = grad + rows_bytes(p.kx);
         const int down = gated_down_bytes<T>(p.np), up = gated_up_bytes<T>(p.kp);
         w[0] = PASS == GATED_OUT ? up : down, w[1] = PASS == GATED_OUT ? down : up;
+        io = swizzled_bytes(ROWS, (PASS == GATED_OUT ? p.n : p.k) * (int)sizeof(T));
         at_x = BARRIERS;
-        at_w[0] = at_x + p.x_buffers * x;
+        at_io = at_x + p.x_buffers * x;
+        at_io = (at_io + 1023) / 1024 * 1024;
+        at_w[0] = at_io + p.io_buffers * io;
         at_w[1] = at_w[0] + p.w_buffers[0] * w[0];
         at_a = at_w[1] + p.w_buffers[1] * w[1];
-        at_io = at_a + p.a_buffers * (A + ACT);
-        io_stride = ((PASS == GATED_OUT ? p.n : p.k) * (int)sizeof(T) + 15) / 16 * 16 + 16;   // (threads of different rows in different banks)
-        at_ones = at_io + p.io_buffers * ROWS * io_stride;
+        at_ones = at_a + p.a_buffers * (A + ACT);
         // (products of 128 rows read on behind a tile of 64, and of 128 columns behind one of fewer: what they make of it nobody takes)
-        total = at_ones + (PASS == GATED_DW ? tile_bytes(ROWS, 16) : 0) + 1024;
+        total = at_ones + tile_bytes(ROWS, 16) + 1024 + 1024;   // (and what lies before the first multiple of 1024)
     }
 };
 // Columns of tensor memory.  DW: of the sums of dWg and dWu, dWd, and dbd.
@@ -88,7 +95,7 @@ struct GatedColumns {
             d_one = bias + (p.down_bias_wanted ? 16 : 0);
         } else {
             down = bias = 0;
-            d_one = PASS == GATED_OUT ? p.np : (p.k + 15) / 16 * 16;
+            d_one = PASS == GATED_OUT ? p.np : p.kx;
         }
         low = SUMS == 2 ? d_one : 0;         // from a sum to that of its small products
         total = d + p.d_buffers * SUMS * d_one;
@@ -167,29 +174,12 @@ __device__ __forceinline__ void gated_act(const float2 (&g)[4], float2 (&act)[4]
     }
 }
 
-// Rows of `width` values to a tile by some warps: `valid` of them, zeros behind.  wide: by 16 bytes; the columns behind the last whole block have been
-// written once for all.  Else all of `blocks` blocks are, with ones in column `ones`.  Eight rows of four blocks a warp at a time: whole sectors of
-// memory, all banks of shared memory.
+// Rows of `width` values to a tile of `blocks` blocks of columns by some warps: `valid` rows, zeros behind and beside.  wide: read by 16 bytes.
+// Eight rows of four blocks a warp at a time: whole sectors of memory, all banks of shared memory.
 template <typename T, int ROWS>
-__device__ __forceinline__ void stage(unsigned char* to, int blocks, const T* src, int width, int valid, int ones, bool wide, int warp, int warps) {
+__device__ __forceinline__ void stage(unsigned char* to, int blocks, const T* src, int width, int valid, bool wide, int warp, int warps) {
     const int lane = threadIdx.x & 31, r8 = lane & 7, b0 = lane >> 3, plane = tile_bytes(ROWS, 8 * blocks);
-    if (sizeof(T) == 2 && wide) {
-        const int whole = width / 8;
-#pragma unroll 4
-        for (int g = warp; g < ROWS / 8; g += warps) {
-            const int r = 8 * g + r8;
-            unsigned char* there = to + 16 * r + b0 * column_blocks(ROWS);
-            const T* from = src + (long long)r * width + 8 * b0;
-            if (r < valid) {
-                for (int b = b0; b < whole; b += 4, there += 4 * column_blocks(ROWS), from += 32) cp_async16(there, from);
-            } else {
-                for (int b = b0; b < whole; b += 4, there += 4 * column_blocks(ROWS)) *reinterpret_cast<uint4*>(there) = make_uint4(0, 0, 0, 0);
-            }
-        }
-        return;
-    }
-    const int end = wide ? width / 8 : blocks;
-    for (int b = b0; b < (end + 3) / 4 * 4; b += 4) {
+    for (int b = b0; b < (blocks + 3) / 4 * 4; b += 4) {
         constexpr int U = 4;
         for (int g0 = warp; g0 < ROWS / 8; g0 += U * warps) {
             float v[U][8];
@@ -197,7 +187,7 @@ __device__ __forceinline__ void stage(unsigned char* to, int blocks, const T* sr
             for (int i = 0; i < U; i++) {
                 const int r = 8 * (g0 + i * warps) + r8;
                 const T* from = src + (long long)r * width + 8 * b;
-                const bool there = r < valid && r < ROWS && b < end;
+                const bool there = r < valid && r < ROWS && 8 * b < width;
                 if (sizeof(T) == 4 && wide) {
                     float q[4] = {0.f, 0.f, 0.f, 0.f};
                     if (there) load4(q, from);
@@ -208,27 +198,15 @@ __device__ __forceinline__ void stage(unsigned char* to, int blocks, const T* sr
                     for (int e = 0; e < 4; e++) v[i][4 + e] = q[e];
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) v[i][e] = there && 8 * b + e < width ? to_float(from[e]) : there && 8 * b + e == ones ? 1.f : 0.f;
+                    for (int e = 0; e < 8; e++) v[i][e] = there && 8 * b + e < width ? to_float(from[e]) : 0.f;
                 }
             }
 #pragma unroll
             for (int i = 0; i < U; i++) {
                 const int r = 8 * (g0 + i * warps) + r8;
-                if (r < ROWS && b < end) store_terms8<T>(to + b * column_blocks(ROWS) + 16 * r, plane, v[i]);
+                if (r < ROWS && b < blocks) store_terms8<T>(to + (sizeof(T) == 2 ? swizzled_at(ROWS, r, b) : b * column_blocks(ROWS) + 16 * r), plane, v[i]);
             }
         }
-    }
-}
-// The columns behind the last whole block of a tile that `stage` fills by 16 bytes: zeros, but for the ones.  By all threads, once.
-template <typename T, int ROWS>
-__device__ __forceinline__ void stage_rest(unsigned char* to, int blocks, int width, int ones) {
-    const int first = width / 8, rest = blocks - first;
-    for (int i = threadIdx.x; i < rest * ROWS; i += GatedWarps<T>::THREADS) {
-        const int b = first + i / ROWS, r = i % ROWS;
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = 8 * b + e == ones ? 1.f : 0.f;
-        store_terms8<T>(to + b * column_blocks(ROWS) + 16 * r, tile_bytes(ROWS, 8 * blocks), v);
     }
 }
 
@@ -248,7 +226,7 @@ __global__ void __launch_bounds__(256) gated_pack(const __grid_constant__ GatedA
     const int c0 = down ? 8 * b : h0 + 8 * (up ? b - C / 8 : b), width = down ? p.n : p.h, row = down ? h0 + r : r, rows = down ? p.h : p.k;
     const T* from = static_cast<const T*>(down ? p.down_weight : up ? p.up_weight : p.gate_weight) + (long long)row * width + c0;
     bool there = row < rows;
-    if (!down && row == p.k) {   // the biases' row
+    if (!down && row == p.kx) {   // the biases' row
         const T* bias = static_cast<const T*>(up ? p.up_bias : p.gate_bias);
         there = p.biased && bias;
         from = bias + c0;
@@ -261,10 +239,11 @@ __global__ void __launch_bounds__(256) gated_pack(const __grid_constant__ GatedA
 }
 
 struct GatedBarriers {
-    u64 x_full[2], x_free[2], w_full[2][16], w_free[2][16], s_full[2], s_free[2], a_full[2], a_free[2], d_full[2], d_free[2], io_full, io_free, met[4], end[2];
+    u64 x_full[2], x_free[2], w_full[2][16], w_free[2][16], s_full[2], s_free[2], a_full[2], a_free[2], d_full[2], d_free[2], io_full, io_done, end[2];
     u32 tensor, dead;
 };
 static_assert(sizeof(GatedBarriers) <= 1024);
+__device__ __forceinline__ bool b_dead(const GatedBarriers& b) { return *static_cast<const volatile u32*>(&b.dead) != 0; }
 
 // Where one of a ring of buffers is in its turns.
 struct Turn {
@@ -291,6 +270,23 @@ struct Waits {
     __device__ __forceinline__ bool free(u64* bars, const Turn& t) { return t.turns == 0 ? alive : on(bars + t.at, t.turns - 1); }
 };
 
+template <typename T>
+struct Piece16 {   // 16 bytes of values
+    static constexpr int V = 16 / sizeof(T);
+    __device__ __forceinline__ static void store(void* to, const float* v) {
+        uint4 q;
+        T* e = reinterpret_cast<T*>(&q);
+#pragma unroll
+        for (int i = 0; i < V; i++) e[i] = from_float<T>(v[i]);
+        *static_cast<uint4*>(to) = q;
+    }
+    __device__ __forceinline__ static void load(float* v, const void* from) {
+        const uint4 q = *static_cast<const uint4*>(from);
+        const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = to_float(e[i]);
+    }
+};
 template <typename T>
 __device__ __forceinline__ void store16(T* to, const float (&v)[16], int left, bool wide) {
     constexpr int V = 16 / sizeof(T);
@@ -331,6 +327,50 @@ __device__ __forceinline__ void load16(float (&v)[16], const T* from, int left, 
         for (int j = 0; j < 16; j++) v[j] = j < left ? to_float(from[j]) : 0.f;
     }
     static_assert(V >= 4);
+}
+
+// 16 columns of a row on its way in or out; pieces of 16 bytes behind the last column are not touched.
+template <typename T, int ROWS>
+__device__ __forceinline__ void io_store16(unsigned char* io, int row, int c, const float (&v)[16], int width) {
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int j = 0; j < 16; j += V)
+        if (c + j < width) Piece16<T>::store(io + swizzled_at(ROWS, row, (c + j) / V), v + j);
+}
+template <typename T, int ROWS>
+__device__ __forceinline__ void io_load16(float (&v)[16], const unsigned char* io, int row, int c, int width) {
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int j = 0; j < 16; j += V) {
+        if (c + j < width) Piece16<T>::load(v + j, io + swizzled_at(ROWS, row, (c + j) / V));
+        else
+#pragma unroll
+            for (int e = 0; e < V; e++) v[j + e] = 0.f;
+    }
+}
+// to = s from, `count` values, by a warp.
+template <typename T>
+__device__ __forceinline__ void scale_rows(T* to, const T* from, int count, float s, bool wide) {
+    constexpr int V = 16 / sizeof(T), U = 8;
+    const int lane = threadIdx.x & 31;
+    if (!wide) {
+        for (int i = lane; i < count; i += 32) to[i] = from_float<T>(s * to_float(from[i]));
+        return;
+    }
+    for (int i0 = V * lane; i0 < count; i0 += 32 * V * U) {
+        uint4 q[U];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (i0 + 32 * V * u < count) q[u] = *reinterpret_cast<const uint4*>(from + i0 + 32 * V * u);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (i0 + 32 * V * u < count) {
+                T* e = reinterpret_cast<T*>(&q[u]);
+#pragma unroll
+                for (int i = 0; i < V; i++) e[i] = from_float<T>(s * to_float(e[i]));
+                *reinterpret_cast<uint4*>(to + i0 + 32 * V * u) = q[u];
+            }
+    }
 }
 
 // Some hidden channels of a row: from g, u (and da) to what the second products take.
@@ -404,8 +444,9 @@ struct WeightRing {
 };
 
 template <typename T, GatedPass PASS, int ROWS>
-__global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const __grid_constant__ GatedArgs p) {
-    extern __shared__ __align__(128) unsigned char smem[];
+__global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const __grid_constant__ GatedArgs p, const __grid_constant__ GatedMaps maps) {
+    extern __shared__ unsigned char unaligned_smem[];
+    unsigned char* smem = unaligned_smem + (-shared_address(unaligned_smem) & 1023);
     using Smem = GatedSmem<T, PASS, ROWS>;
     using Columns = GatedColumns<T, PASS>;
     constexpr int C = gated_chunk<T>(), TERMS = Tensor<T>::TERMS;
@@ -414,37 +455,30 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
     const Columns col(p);
     GatedBarriers& b = *reinterpret_cast<GatedBarriers*>(smem);
     float* bias_s = reinterpret_cast<float*>(smem + 1024);   // of out
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // One of the loaders brings the residual, or takes dout to the residual's gradient.
-    const bool beside = (PASS == GATED_OUT && p.residual && p.io_buffers) || (PASS == GATED_DX && p.dresidual);
+    const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    // The last of the loaders brings the residual and takes the output away, and takes dout to the residual's gradient.
+    const bool beside = p.io_buffers || (PASS == GATED_DX && p.dresidual);
     const int row_loaders = LOADERS - (beside ? 1 : 0);
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&b.x_full[i], 32 * row_loaders), mbar_init(&b.x_free[i], 1);
+            mbar_init(&b.x_full[i], p.boxes ? 1 : 32 * row_loaders), mbar_init(&b.x_free[i], 1);
             mbar_init(&b.s_full[i], 1), mbar_init(&b.s_free[i], WORKERS);
             mbar_init(&b.a_full[i], WORKERS), mbar_init(&b.a_free[i], 1);
             mbar_init(&b.d_full[i], 1), mbar_init(&b.d_free[i], WORKERS);
             for (int j = 0; j < p.w_buffers[i]; j++) mbar_init(&b.w_full[i][j], 1), mbar_init(&b.w_free[i][j], 1);
             mbar_init(&b.end[i], 1);
         }
-        mbar_init(&b.io_full, 32), mbar_init(&b.io_free, WORKERS);
-        for (int i = 0; i < 4; i++) mbar_init(&b.met[i], WORKERS / 4);
+        mbar_init(&b.io_full, 1), mbar_init(&b.io_done, WORKERS);
         b.dead = 0;
     }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(shared_address(&b.tensor)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    if constexpr (PASS == GATED_DW) {   // a column of ones
+    {   // a column of ones
         float one[8] = {1.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, none[8] = {};
-        unsigned char* to = smem + at.at_ones;
         using Term = typename Tensor<T>::Term;
-        for (int i = threadIdx.x; i < 2 * ROWS; i += THREADS) store_terms8<Term>(to + 16 * i, 0, i < ROWS ? one : none);
-    }
-    for (int i = 0; i < p.x_buffers; i++) {
-        unsigned char* x = smem + at.at_x + i * at.x;
-        if (PASS != GATED_OUT && p.wide_grad) stage_rest<T, ROWS>(x, p.np / 8, p.n, -1);
-        if (p.wide_x) stage_rest<T, ROWS>(x + at.grad, p.kp / 8, p.k, p.biased ? p.k : -1);
+        for (int i = threadIdx.x; i < 2 * ROWS; i += THREADS) store_terms8<Term>(smem + at.at_ones + 16 * i, 0, i < ROWS ? one : none);
     }
     fence_async_proxy();
     wait_for_previous_kernel();
@@ -453,7 +487,7 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
     tensor_before_sync();
     __syncthreads();
     tensor_after_sync();
-    const u32 tensor = b.tensor;
+    const u32 tensor = __shfl_sync(~0u, b.tensor, 0);
     Waits wait{&b.dead};
 
     // What this CTA does: tiles from `split` on, every `step`-th, each through `chunks` chunks from `chunk0` on.
@@ -463,6 +497,8 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
     const long long mine = split < tiles ? (tiles - split + step - 1) / step : 0;
     const long long all = mine * chunks;                                  // steps: chunks of tiles
     const int group = PASS == GATED_DW ? p.drain : chunks;                // steps whose sums are one
+    auto rows_over_columns = [](u32 a, int columns) { return TERMS == 1 ? swizzled_over_columns(a, ROWS) : over_columns(a, ROWS, columns); };
+    auto rows_over_rows = [](u32 a, int columns) { return TERMS == 1 ? swizzled_over_rows(a, ROWS) : over_rows(a, ROWS, columns); };
     auto ring = [&](int which) {
         const bool down = (which == 0) != (PASS == GATED_OUT);
         const int down_bytes = gated_down_bytes<T>(p.np);
@@ -477,84 +513,68 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
         if (beside && loader == LOADERS - 1) {
             for (long long t = 0; t < mine && wait.alive; t++) {
                 const long long row0 = (split + t * step) * ROWS;
-                const int valid = (int)min((long long)ROWS, p.rows - row0);
-                if constexpr (PASS == GATED_OUT) {   // the residual to where the output leaves from
-                    if (t > 0 && !wait.on(&b.io_free, (int)(t - 1))) break;
-                    const T* from = static_cast<const T*>(p.residual) + row0 * p.n;
-                    unsigned char* to = smem + at.at_io;
-                    if (p.wide_out) {
-                        const int pieces = p.n * (int)sizeof(T) / 16;
-                        for (int i = lane; i < valid * pieces; i += 32) {
-                            const int r = i / pieces;
-                            cp_async16(to + r * at.io_stride + 16 * (i - r * pieces), reinterpret_cast<const unsigned char*>(from) + 16 * i);
-                        }
-                        cp_async_wait_all();
+                if constexpr (PASS == GATED_DX) {
+                    if (p.dresidual) scale_rows<T>(static_cast<T*>(p.dresidual) + row0 * p.n, static_cast<const T*>(p.grad) + row0 * p.n,
+                                                   (int)min((long long)ROWS, p.rows - row0) * p.n, p.scale, p.wide_dresidual);
+                }
+                if (p.io_buffers && one_of_warp()) {
+                    constexpr int BOX = 128 / sizeof(T);
+                    const int width = PASS == GATED_OUT ? p.n : p.k;
+                    unsigned char* io = smem + at.at_io;
+                    if (PASS == GATED_OUT && p.residual) {
+                        mbar_expect_tx(&b.io_full, at.io);
+                        for (int c = 0; c < width; c += BOX) box_load(io + c / BOX * ROWS * 128, &maps.residual, c, (int)row0, &b.io_full);
                     } else {
-                        for (int i = lane; i < valid * p.n; i += 32) {
-                            const int r = i / p.n;
-                            reinterpret_cast<T*>(to + r * at.io_stride)[i - r * p.n] = from[i];
-                        }
+                        mbar_arrive(&b.io_full);
                     }
-                    mbar_arrive(&b.io_full);
-                } else {
-                    const T* from = static_cast<const T*>(p.grad) + row0 * p.n;
-                    T* to = static_cast<T*>(p.dresidual) + row0 * p.n;
-                    const int count = valid * p.n;
-                    if (p.wide_dresidual) {
-                        constexpr int V = 16 / sizeof(T);
-#pragma unroll 4
-                        for (int i = V * lane; i < count; i += 32 * V) {
-                            float v[V];
-#pragma unroll
-                            for (int e = 0; e < V; e += 4) {
-                                float q[4];
-                                load4(q, from + i + e);
-#pragma unroll
-                                for (int f = 0; f < 4; f++) v[e + f] = p.scale * q[f];
-                            }
-#pragma unroll
-                            for (int e = 0; e < V; e += 4) {
-                                const float q[4] = {v[e], v[e + 1], v[e + 2], v[e + 3]};
-                                store4(to + i + e, q);
-                            }
-                        }
-                    } else {
-                        for (int i = lane; i < count; i += 32) to[i] = from_float<T>(p.scale * to_float(from[i]));
+                    if (wait.on(&b.io_done, (int)t)) {
+                        for (int c = 0; c < width; c += BOX) box_store(&maps.out, c, (int)row0, io + c / BOX * ROWS * 128);
+                        bulk_commit();
+                        bulk_wait_read();
+                    } else if (PASS == GATED_OUT && p.residual) {
+                        wait.alive = true, wait.on(&b.io_full, (int)t, true), wait.alive = false;   // nothing on its way
                     }
                 }
+                wait.alive = __shfl_sync(~0u, (int)!b_dead(b), 0) != 0;
+            }
+            if (p.io_buffers) bulk_wait_all();
+        } else if (p.boxes) {
+            if (loader == 0 && one_of_warp()) {
+                Turn xt;
+                for (long long t = 0; t < mine; t++) {
+                    const int row0 = (int)((split + t * step) * ROWS);
+                    if (!wait.free(b.x_free, xt)) break;
+                    unsigned char* x = smem + at.at_x + xt.at * at.x;
+                    mbar_expect_tx(&b.x_full[xt.at], at.x);
+                    if (PASS != GATED_OUT)
+                        for (int c = 0; c < p.n; c += 64) box_load(x + c * ROWS * 2, &maps.grad, c, row0, &b.x_full[xt.at]);
+                    for (int c = 0; c < p.k; c += 64) box_load(x + at.grad + c * ROWS * 2, &maps.x, c, row0, &b.x_full[xt.at]);
+                    xt.next(p.x_buffers);
+                }
+                // nothing on its way when others have given up
+                if (b_dead(b))
+                    for (int i = 0; i < p.x_buffers; i++) {
+                        const int turns = xt.turns - (i >= xt.at ? 1 : 0);
+                        if (turns >= 0) Waits{&b.dead}.on(&b.x_full[i], turns, true);
+                    }
             }
         } else {
-            // By cp.async where nothing has to be made of the values: then a tile is on its way while the one before it arrives.
-            const bool lag = sizeof(T) == 2 && p.x_buffers == 2;
-            Turn xt, arrived;
+            Turn xt;
             for (long long t = 0; t < mine && wait.alive; t++) {
                 const long long row0 = (split + t * step) * ROWS;
                 const int valid = (int)min((long long)ROWS, p.rows - row0);
                 if (!wait.free(b.x_free, xt)) break;
                 unsigned char* x = smem + at.at_x + xt.at * at.x;
                 if constexpr (PASS != GATED_OUT)
-                    stage<T, ROWS>(x, p.np / 8, static_cast<const T*>(p.grad) + row0 * p.n, p.n, valid, -1, p.wide_grad, loader, row_loaders);
-                stage<T, ROWS>(x + at.grad, p.kp / 8, static_cast<const T*>(p.x) + row0 * p.k, p.k, valid, p.biased ? p.k : -1, p.wide_x, loader, row_loaders);
+                    stage<T, ROWS>(x, p.np / 8, static_cast<const T*>(p.grad) + row0 * p.n, p.n, valid, p.wide_grad, loader, row_loaders);
+                stage<T, ROWS>(x + at.grad, p.kx / 8, static_cast<const T*>(p.x) + row0 * p.k, p.k, valid, p.wide_x, loader, row_loaders);
+                fence_async_proxy();
+                mbar_arrive(&b.x_full[xt.at]);
                 xt.next(p.x_buffers);
-                if (lag) {
-                    cp_async_commit();
-                    if (t == 0) continue;
-                    cp_async_wait_one();
-                } else if (sizeof(T) == 2) {
-                    cp_async_wait_all();
-                }
-                fence_async_proxy();
-                mbar_arrive(&b.x_full[arrived.at]);
-                arrived.next(p.x_buffers);
-            }
-            if (sizeof(T) == 2) cp_async_wait_all();
-            if (lag && wait.alive && mine > 0) {
-                fence_async_proxy();
-                mbar_arrive(&b.x_full[arrived.at]);
             }
         }
     } else if (warp == WORKERS) {   // the first products: g, u (, da) of a step
-        if (lane == 0) {
+        if (one_of_warp()) {
             WeightRing w = ring(0);
             w.begin();
             Turn xt, wt, w2t, st;
@@ -567,8 +587,14 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                 tensor_after_sync();
                 const u32 x = shared_address(smem + at.at_x + xt.at * at.x), s = tensor + st.at * Columns::WIDE;
                 const u32 w0 = shared_address(w.buffers + wt.at * w.bytes), w1 = shared_address(smem + at.at_w[1] + w2t.at * at.w[1]);
-                products<T>(s, s, over_columns(x + at.grad, ROWS, p.kp), over_rows(PASS == GATED_OUT ? w0 : w1, p.kp, 2 * C), 2 * C, p.kp / 16, false);
-                if constexpr (PASS != GATED_OUT) products<T>(s + 2 * C, s + 2 * C, over_columns(x, ROWS, p.np), over_columns(w0, C, p.np), C, p.np / 16, false);
+                const Operand up = over_rows(PASS == GATED_OUT ? w0 : w1, p.kp, 2 * C);
+                if (p.biased) {   // ones times the biases' row
+                    const Operand one = over_columns(shared_address(smem + at.at_ones), ROWS, 16);
+                    const u32 shape = product_shape<T>(one, up, 2 * C);
+                    for (int t = TERMS - 1; t >= 0; t--) tensor_product(s, one.first, up.at(p.kx / 16, t), shape, t < TERMS - 1);
+                }
+                products<T>(s, s, rows_over_columns(x + at.grad, p.kx), up, 2 * C, p.kx / 16, p.biased);
+                if constexpr (PASS != GATED_OUT) products<T>(s + 2 * C, s + 2 * C, rows_over_columns(x, p.np), over_columns(w0, C, p.np), C, p.np / 16, false);
                 tensor_commit(&b.s_full[st.at]);
                 st.next(p.s_buffers), wt.next(w.count), w2t.next(p.w_buffers[1]);
                 if (++c == chunks) {
@@ -583,7 +609,7 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
             tensor_commit(&b.end[0]);
         }
     } else if (warp == WORKERS + 1) {   // the second products
-        if (lane == 0) {
+        if (one_of_warp()) {
             WeightRing w = ring(1);
             w.begin();
             Turn wt, xt, act, dt;
@@ -602,16 +628,19 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                 } else if constexpr (PASS == GATED_DX) {
                     products<T>(d, d + col.low, over_columns(a, ROWS, 2 * C), over_columns(w1, p.kp, 2 * C), col.d_one, 2 * C / 16, add);
                 } else {
-                    products<T>(d, d + col.low, over_rows(a, ROWS, 2 * C), over_rows(x + at.grad, ROWS, p.kp), p.kp, ROWS / 16, add);
-                    products<T>(d + col.down, d + col.down + col.low, over_rows(x, ROWS, p.np), over_rows(a + Smem::A, ROWS, C), C, ROWS / 16, add);
-                    if (p.down_bias_wanted) {   // (a one has one term)
-                        const Operand rows_of = over_rows(x, ROWS, p.np), one = over_rows(shared_address(smem + at.at_ones), ROWS, 16);
-                        const u32 shape = product_shape<T>(rows_of, one, 16);
+                    const Operand hidden = over_rows(a, ROWS, 2 * C), grad = rows_over_rows(x, p.np);
+                    products<T>(d, d + col.low, hidden, rows_over_rows(x + at.grad, p.kx), p.kx, ROWS / 16, add);
+                    products<T>(d + col.down, d + col.down + col.low, grad, over_rows(a + Smem::A, ROWS, C), C, ROWS / 16, add);
+                    // the biases': times ones (which have one term)
+                    const Operand one = over_rows(shared_address(smem + at.at_ones), ROWS, 16);
+                    auto column_sums = [&](const Operand& of, u32 to) {
+                        const u32 shape = product_shape<T>(of, one, 16);
                         for (int t = TERMS - 1; t >= 0; t--)
                             for (int s = 0; s < ROWS / 16; s++)
-                                tensor_product(d + col.bias + (t ? col.low : 0), rows_of.at(t * rows_of.plane + s * rows_of.step), one.at(s * one.step), shape,
-                                               add || s > 0 || (TERMS == 3 && t == 1));
-                    }
+                                tensor_product(to + (t ? col.low : 0), of.at(s, t), one.at(s, 0), shape, add || s > 0 || (TERMS == 3 && t == 1));
+                    };
+                    if (p.biased) column_sums(hidden, d + p.kx);
+                    if (p.down_bias_wanted) column_sums(grad, d + col.bias);
                     tensor_commit(&b.x_free[xt.at]);
                     xt.next(p.x_buffers);
                 }
@@ -634,12 +663,7 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
         const bool works = 32 * quarter < ROWS;
         const u32 lanes = tensor + ((u32)(32 * quarter) << 16);
         Turn st, act, dt;
-        int in_group = 0, turns = 0, meetings = 0;
-        auto meet = [&]() {   // the warps of the same rows
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&b.met[quarter]);
-            return wait.on(&b.met[quarter], meetings++);
-        };
+        int in_group = 0, turns = 0;
         // The finished sums: of this CTA's index-th tile, or group of tiles.
         auto take_out = [&](long long index) {
             if (!wait.full(b.d_full, dt)) return;
@@ -649,10 +673,8 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
             const bool there = works && at_row < p.rows, staged = PASS != GATED_DW && p.io_buffers;
             const int width = PASS == GATED_OUT ? p.n : p.k;
             float* share = PASS == GATED_DW ? p.shares + ((long long)chunk0 * p.splits + split) * col.d_one * 128 + row : nullptr;
-            T* mine_s = reinterpret_cast<T*>(smem + at.at_io + row * at.io_stride);
-            if (staged) {
-                if (!(PASS == GATED_OUT && p.residual ? wait.on(&b.io_full, turns) : meet())) return;   // (either way the rows before have left)
-            }
+            unsigned char* io = smem + at.at_io;
+            if (staged && !wait.on(&b.io_full, turns++)) return;   // the residual is there, and the rows before have left
             for (int c = 16 * part; c < col.d_one; c += 16 * PARTS) {
                 float v[16], low[16];
                 __syncwarp();
@@ -677,12 +699,14 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                         for (int j = 0; j < 16; j++) v[j] += bias_s[c + j];
                         if (p.residual) {
                             float r[16];
-                            load16(r, staged ? mine_s + c : static_cast<const T*>(p.residual) + at_row * width + c, width - c, p.wide_out);
+                            if (staged) io_load16<T, ROWS>(r, io, row, c, width);
+                            else load16(r, static_cast<const T*>(p.residual) + at_row * width + c, width - c, p.wide_out);
 #pragma unroll
                             for (int j = 0; j < 16; j++) v[j] = fmaf(p.scale, r[j], v[j]);
                         }
                     }
-                    store16(staged ? mine_s + c : static_cast<T*>(p.out) + at_row * width + c, v, width - c, p.wide_out);
+                    if (staged) io_store16<T, ROWS>(io, row, c, v, width);
+                    else store16(static_cast<T*>(p.out) + at_row * width + c, v, width - c, p.wide_out);
                 }
             }
             tensor_before_sync();
@@ -690,26 +714,9 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
             if (lane == 0) mbar_arrive(&b.d_free[dt.at]);
             dt.next(p.d_buffers);
             if (!staged) return;
-            // The rows of these warps leave together, side by side.
-            if (!meet()) return;
-            const int valid = (int)max(0ll, min(32ll, p.rows - row0 - 32 * quarter)) * (works ? 1 : 0), thread = 32 * part + lane;
-            const unsigned char* from = smem + at.at_io + 32 * quarter * at.io_stride;
-            T* to = static_cast<T*>(p.out) + (row0 + 32 * quarter) * width;
-            if (p.wide_out) {
-                const int pieces = width * (int)sizeof(T) / 16;
-                for (int i = thread; i < valid * pieces; i += 32 * PARTS) {
-                    const int r = i / pieces;
-                    reinterpret_cast<uint4*>(to)[i] = *reinterpret_cast<const uint4*>(from + r * at.io_stride + 16 * (i - r * pieces));
-                }
-            } else {
-                for (int i = thread; i < valid * width; i += 32 * PARTS) {
-                    const int r = i / width;
-                    to[i] = reinterpret_cast<const T*>(from + r * at.io_stride)[i - r * width];
-                }
-            }
+            fence_async_proxy();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&b.io_free);
-            turns++;
+            if (lane == 0) mbar_arrive(&b.io_done);
         };
         for (long long q = 0, groups = 0; q < all && wait.alive; q++) {
             if (!wait.full(b.s_full, st)) break;
@@ -766,7 +773,7 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
 // consecutive channels out (dWd, dbd) side by side in a share.
 struct GatedSums {
     const float* shares;
-    int k, h, n, kp, chunk, chunks, splits, columns, down, bias;
+    int k, h, n, kx, chunk, chunks, splits, columns, down, bias;
     void *gate_weight, *up_weight, *down_weight, *gate_bias, *up_bias, *down_bias;
 };
 template <typename T>
@@ -784,7 +791,7 @@ __global__ void __launch_bounds__(256) gated_sums(const __grid_constant__ GatedS
         void* weight = up ? p.up_weight : p.gate_weight;
         if (r == p.k ? !bias : !weight) return;
         to = r == p.k ? static_cast<T*>(bias) + i : static_cast<T*>(weight) + (long long)r * p.h + i;
-        chunk = i / p.chunk, column = r, line = i % p.chunk + (up ? p.chunk : 0);
+        chunk = i / p.chunk, column = r == p.k ? p.kx : r, line = i % p.chunk + (up ? p.chunk : 0);
     } else {
         r -= 2 * (p.k + 1);
         if (i >= p.n) return;

@@ -20,8 +20,9 @@ inline int gated_splits(int chunks, long long rows, int sms) { return (int)std::
 template <typename T, GatedPass PASS, int ROWS>
 static bool gated_plan(GatedArgs& p) {
     const int chunks = PASS == GATED_DW ? 1 : p.chunks;
+    p.boxes = sizeof(T) == 2 && p.wide_x && (PASS == GATED_OUT || p.wide_grad);
     auto fits = [&]() {
-        for (int io = PASS == GATED_DW ? 0 : 1; io >= 0; io--)
+        for (int io = PASS != GATED_DW && p.wide_out ? 1 : 0; io >= 0; io--)
             for (int w : {chunks, std::min(2, chunks), 1})
                 for (int left : {0, 1, 2, 3}) {
                     p.io_buffers = io, p.w_buffers[0] = p.w_buffers[1] = w, p.x_buffers = left & 2 ? 1 : 2, p.a_buffers = left & 1 ? 1 : 2;
@@ -37,9 +38,26 @@ static bool gated_plan(GatedArgs& p) {
     return fits() && ((PASS != GATED_DW && columns(2, 2)) || columns(2, 1) || columns(1, 1));
 }
 
+// A matrix of rows as the TMA takes it: boxes of 128 bytes by `box` rows, in shared memory as swizzled_at says.
+int encode_matrix(CUtensorMap& map, const void* p, int dtype, unsigned long long rows, unsigned long long columns, unsigned box_columns, unsigned box_rows);
+template <typename T>
+static int matrix_map(CUtensorMap& map, const void* p, long long rows, int columns, int box) {
+    const int dtype = sizeof(T) == 4 ? PL_F32 : std::is_same<T, __half>::value ? PL_F16 : PL_BF16;
+    return encode_matrix(map, p, dtype, rows, columns, 128 / sizeof(T), box);
+}
+
 template <typename T, GatedPass PASS, int ROWS>
 static int launch_gated_rows(GatedArgs& p, cudaStream_t st) {
     const int smem = GatedSmem<T, PASS, ROWS>(p).total;
+    GatedMaps maps = {};
+    if (p.boxes) {
+        PL_TRY(matrix_map<T>(maps.x, p.x, p.rows, p.k, ROWS));
+        if (PASS != GATED_OUT) PL_TRY(matrix_map<T>(maps.grad, p.grad, p.rows, p.n, ROWS));
+    }
+    if (p.io_buffers) {
+        PL_TRY(matrix_map<T>(maps.out, p.out, p.rows, PASS == GATED_OUT ? p.n : p.k, ROWS));
+        if (PASS == GATED_OUT && p.residual) PL_TRY(matrix_map<T>(maps.residual, p.residual, p.rows, p.n, ROWS));
+    }
     const long long tiles = (p.rows + ROWS - 1) / ROWS;
     const unsigned grid = PASS == GATED_DW ? p.chunks * p.splits : (unsigned)std::min<long long>(tiles, num_sms());
     PL_TRY((ensure_dynamic_smem<gated_kernel<T, PASS, ROWS>>(smem)));
@@ -49,7 +67,7 @@ static int launch_gated_rows(GatedArgs& p, cudaStream_t st) {
     early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early[0].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = early, config.numAttrs = 1;
-    PL_CUDA(cudaLaunchKernelEx(&config, gated_kernel<T, PASS, ROWS>, (const GatedArgs)p));
+    PL_CUDA(cudaLaunchKernelEx(&config, gated_kernel<T, PASS, ROWS>, (const GatedArgs)p, (const GatedMaps)maps));
     PL_COUNT_LAUNCHES(1);
     return PL_OK;
 }

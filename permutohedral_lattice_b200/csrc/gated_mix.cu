@@ -3,6 +3,24 @@
 
 namespace pl {
 
+// The driver's function, asked for by name: the library links against the runtime alone.
+int encode_matrix(CUtensorMap& map, const void* p, int dtype, unsigned long long rows, unsigned long long columns, unsigned box_columns, unsigned box_rows) {
+    static const auto encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) f = nullptr;
+        return reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(f);
+    }();
+    if (!encode) return cuda_fail(cudaErrorNotSupported, "cuTensorMapEncodeTiled");
+    const size_t size = dtype == PL_F32 ? 4 : 2;
+    const cuuint64_t dims[2] = {columns, rows}, strides[1] = {columns * size};
+    const cuuint32_t box[2] = {box_columns, box_rows}, steps[2] = {1, 1};
+    const auto type = dtype == PL_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == PL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const CUresult rc = encode(&map, type, 2, const_cast<void*>(p), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return rc == CUDA_SUCCESS ? PL_OK : cuda_fail(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
+}
+
 static int check_gated(const pl_gated_shape* m) {
     if (!m || m->rows < 0 || m->rows > ((long long)1 << 40) || m->k < 1 || m->h < 1 || m->n < 1) return PL_INVALID_ARGUMENT;
     if (m->activation < PL_GATE_SILU || m->activation > PL_GATE_RELU || m->dtype < PL_F32 || m->dtype > PL_BF16) return PL_INVALID_ARGUMENT;
@@ -18,15 +36,15 @@ static GatedArgs gated_args(const pl_gated_shape* m, const void* x, const pl_gat
     p.gate_bias = w->gate_bias, p.up_bias = w->up_bias, p.down_bias = w->down_bias;
     p.biased = p.gate_bias || p.up_bias;
     p.np = (p.n + 15) / 16 * 16;
-    p.wide_x = p.k % 8 == 0 && gated_aligned(x);
+    p.wide_x = p.k % 8 == 0 && gated_aligned(x) && p.rows < (1ll << 31) - 128;   // (a row's number is 31 bits for the TMA)
     return p;
 }
-static void set_kp(GatedArgs& p) { p.kp = (p.k + (p.biased ? 1 : 0) + 15) / 16 * 16; }
+static void set_columns(GatedArgs& p) { p.kx = (p.k + 15) / 16 * 16, p.kp = p.kx + (p.biased ? 16 : 0); }
 static int run_gated(const GatedArgs& p, int dtype, GatedPass pass, bool pack, cudaStream_t st) {
     return dtype == PL_F32 ? gated_floats(p, pass, pack, st) : gated_halves(p, dtype, pass, pack, st);
 }
 static size_t packed_bytes(const pl_gated_shape* m) {   // with all biases
-    const int chunk = chunk_of(m), chunks = (m->h + chunk - 1) / chunk, kp = (m->k + 16) / 16 * 16, np = (m->n + 15) / 16 * 16;
+    const int chunk = chunk_of(m), chunks = (m->h + chunk - 1) / chunk, kp = (m->k + 15) / 16 * 16 + 16, np = (m->n + 15) / 16 * 16;
     const size_t one = m->dtype == PL_F32 ? gated_down_bytes<float>(np) + gated_up_bytes<float>(kp) : gated_down_bytes<__half>(np) + gated_up_bytes<__half>(kp);
     return one * chunks;
 }
@@ -43,7 +61,7 @@ int pl_gated_mix_workspace_bytes(const pl_gated_shape* m, int backward, size_t* 
     *bytes = packed_bytes(m);
     if (!backward) return PL_OK;
     const int chunk = chunk_of(m), chunks = (m->h + chunk - 1) / chunk;
-    const size_t columns = (m->k + 16) / 16 * 16 + chunk + 16;   // with all biases
+    const size_t columns = (m->k + 15) / 16 * 16 + 16 + chunk + 16;   // with all biases
     *bytes += sizeof(float) * 128 * columns * chunks * gated_splits(chunks, m->rows, num_sms());
     return PL_OK;
 }
@@ -56,10 +74,10 @@ int pl_gated_mix(const pl_gated_shape* m, void* out, const void* x, const pl_gat
     if (!workspace || workspace_bytes < packed_bytes(m)) return PL_WORKSPACE_TOO_SMALL;
     if (!gated_aligned(workspace)) return PL_INVALID_ARGUMENT;
     GatedArgs p = gated_args(m, x, w);
-    set_kp(p);
+    set_columns(p);
     p.packed = static_cast<unsigned char*>(workspace);
     p.out = out, p.residual = residual;
-    p.wide_out = p.n % (m->dtype == PL_F32 ? 4 : 8) == 0 && gated_aligned(out) && gated_aligned(residual);
+    p.wide_out = p.n % (m->dtype == PL_F32 ? 4 : 8) == 0 && gated_aligned(out) && gated_aligned(residual) && p.rows < (1ll << 31) - 128;
     return run_gated(p, m->dtype, GATED_OUT, true, (cudaStream_t)stream);
 }
 
@@ -84,11 +102,11 @@ int pl_gated_mix_backward(const pl_gated_shape* m, const void* grad_out, const v
     p.grad = grad_out;
     p.wide_grad = p.n % 8 == 0 && gated_aligned(grad_out);
     p.biased = p.biased || d.gate_bias || d.up_bias;   // (the ones' column sums dg and du)
-    set_kp(p);
+    set_columns(p);
     p.packed = static_cast<unsigned char*>(workspace);
     if (d.x) {
         p.out = d.x, p.dresidual = d.residual;
-        p.wide_out = p.k % (m->dtype == PL_F32 ? 4 : 8) == 0 && gated_aligned(d.x);
+        p.wide_out = p.k % (m->dtype == PL_F32 ? 4 : 8) == 0 && gated_aligned(d.x) && p.rows < (1ll << 31) - 128;
         p.wide_dresidual = p.n % (m->dtype == PL_F32 ? 4 : 8) == 0 && gated_aligned(grad_out) && gated_aligned(d.residual);
         PL_TRY(run_gated(p, m->dtype, GATED_DX, true, st));
     } else if (d.residual) {
@@ -100,7 +118,7 @@ int pl_gated_mix_backward(const pl_gated_shape* m, const void* grad_out, const v
     p.shares = reinterpret_cast<float*>(p.packed + packed_bytes(m));
     PL_TRY(run_gated(p, m->dtype, GATED_DW, !d.x, st));
     GatedSums s = {};
-    s.shares = p.shares, s.k = p.k, s.h = p.h, s.n = p.n, s.kp = p.kp, s.chunk = chunk_of(m);
+    s.shares = p.shares, s.k = p.k, s.h = p.h, s.n = p.n, s.kx = p.kx, s.chunk = chunk_of(m);
     s.chunks = (p.h + s.chunk - 1) / s.chunk, s.splits = gated_splits(s.chunks, m->rows, num_sms());
     s.down = p.kp, s.bias = s.down + s.chunk, s.columns = s.bias + (p.down_bias_wanted ? 16 : 0);
     s.gate_weight = d.gate_weight, s.up_weight = d.up_weight, s.down_weight = d.down_weight;

@@ -27,22 +27,31 @@ struct Tensor {
 __host__ __device__ constexpr int column_blocks(int rows) { return rows * 16; }
 __host__ __device__ constexpr int tile_bytes(int rows, int columns) { return rows * columns * 2; }   // of a term
 
-struct Operand {   // of a product: its first 16 terms of the sum, and how far the next 16 are and the next term (in 16 bytes)
+struct Operand {   // of a product: its first 16 terms of the sum, how far the next 16 are, the next 64, and the next term (in 16 bytes)
     u64 first;
-    u32 step, plane, transposed;
-    __device__ __forceinline__ u64 at(u32 offset) const { return first + offset; }   // (addresses are below 2^18: nothing is carried)
+    u32 step, jump, plane, transposed;
+    __device__ __forceinline__ u64 at(int s, int term) const {   // (addresses are below 2^18: nothing is carried)
+        return first + (u32)((s & 3) * step + (s >> 2) * jump + term * plane);
+    }
 };
 __device__ __forceinline__ u64 operand_of(u32 at, u32 along, u32 across) {   // strides of blocks, along the sums and across
     return (u64)(at >> 4) | (u64)(along >> 4) << 16 | (u64)(across >> 4) << 32 | 1ull << 46;
 }
 // The tile's rows are the operand's rows, sums run over its columns.
 __device__ __forceinline__ Operand over_columns(u32 at, int rows, int columns) {
-    return {operand_of(at, column_blocks(rows), 128), (u32)column_blocks(rows) / 8, (u32)tile_bytes(rows, columns) / 16, 0};
+    return {operand_of(at, column_blocks(rows), 128), (u32)column_blocks(rows) / 8, (u32)column_blocks(rows) / 2, (u32)tile_bytes(rows, columns) / 16, 0};
 }
 // The tile's columns are the operand's rows, sums run over its rows.
 __device__ __forceinline__ Operand over_rows(u32 at, int rows, int columns) {
-    return {operand_of(at, 128, column_blocks(rows)), 16, (u32)tile_bytes(rows, columns) / 16, 1};
+    return {operand_of(at, 128, column_blocks(rows)), 16, 64, (u32)tile_bytes(rows, columns) / 16, 1};
 }
+// Tiles of rows of 16-bit values, which the TMA brings: 64 columns after another, rows of 128 bytes whose 16-byte pieces lie at their number
+// xor the row's (mod 8).  Either way round as well.
+constexpr u64 SWIZZLED = 2ull << 61;
+__host__ __device__ constexpr int swizzled_bytes(int rows, int row_bytes) { return (row_bytes + 127) / 128 * rows * 128; }
+__device__ __forceinline__ int swizzled_at(int rows, int row, int piece) { return (piece >> 3) * rows * 128 + row * 128 + ((piece & 7) ^ (row & 7)) * 16; }
+__device__ __forceinline__ Operand swizzled_over_columns(u32 at, int rows) { return {operand_of(at, 16, 1024) | SWIZZLED, 2, (u32)rows * 8, 0, 0}; }
+__device__ __forceinline__ Operand swizzled_over_rows(u32 at, int rows) { return {operand_of(at, rows * 128, 1024) | SWIZZLED, 128, 512, 0, 1}; }
 __device__ __forceinline__ void tensor_product(u32 d, u64 a, u64 b, u32 shape, bool add) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
                  "r"(shape), "r"((u32)add)
@@ -61,20 +70,17 @@ __device__ __forceinline__ void products(u32 d, u32 small, const Operand& a, con
 #pragma unroll
         for (int order = 2; order >= 1; order--)
 #pragma unroll
-            for (int i = 0; i <= order; i++) {
-                u64 p = a.at(i * a.plane), q = b.at((order - i) * b.plane);
+            for (int i = 0; i <= order; i++)
 #pragma unroll 2
-                for (int s = 0; s < steps; s++, p += a.step, q += b.step) {
-                    tensor_product(small, p, q, shape, more);
+                for (int s = 0; s < steps; s++) {
+                    tensor_product(small, a.at(s, i), b.at(s, order - i), shape, more);
                     more = true;
                 }
-            }
         if (small == d) add = true;
     }
-    u64 p = a.first, q = b.first;
 #pragma unroll 4
-    for (int s = 0; s < steps; s++, p += a.step, q += b.step) {
-        tensor_product(d, p, q, shape, add);
+    for (int s = 0; s < steps; s++) {
+        tensor_product(d, a.at(s, 0), b.at(s, 0), shape, add);
         add = true;
     }
 }
@@ -114,6 +120,23 @@ __device__ __forceinline__ u64 global_timer() {   // nanoseconds
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
     return t;
 }
+
+__device__ __forceinline__ bool one_of_warp() {   // one lane, known as such to the compiler: what is the same for a warp stays in its uniform registers
+    u32 one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+// Boxes of a matrix in memory to shared memory and back by the TMA: columns from x on, rows from y on; what lies outside comes as zeros and is not
+// written.
+__device__ __forceinline__ void box_load(void* to, const void* map, int x, int y, u64* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(shared_address(to)),
+                 "l"(map), "r"(x), "r"(y), "r"(shared_address(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void box_store(const void* map, int x, int y, const void* from) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(shared_address(from)) : "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // Eight values as terms to a row of a block, 16 bytes each.
 template <typename T>
