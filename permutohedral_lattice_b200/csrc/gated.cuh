@@ -11,7 +11,8 @@
 // over the tiles of a chunk, a chunk a CTA, and adds them to a share of its own in the workspace now and then (`drain`, see
 // gated_launch.cuh); gated_sums adds up the shares in order.  gated_pack first lays out the weights as the products read them.
 //
-// Warps: workers turn the first products into the second's operand, and take out the sums; two warps ask for the first and the second
+// Warps: workers turn the first products into the second's operand, and take out the sums, one half of them every other step, so that one half
+// computes while the other waits, loads or stores; two warps ask for the first and the second
 // products, and for the weights that only theirs read; loaders fetch rows.  They meet at barriers in shared memory; every wait is bounded.
 // If one runs out, all give up and the results are NaN.
 #pragma once
@@ -79,7 +80,7 @@ struct GatedSmem {
         at_a = at_w[1] + p.w_buffers[1] * w[1];
         at_ones = at_a + p.a_buffers * (A + ACT);
         // (products of 128 rows read on behind a tile of 64, and of 128 columns behind one of fewer: what they make of it nobody takes)
-        total = at_ones + tile_bytes(ROWS, 16) + 1024 + 1024;   // (and what lies before the first multiple of 1024)
+        total = at_ones + (p.biased || p.down_bias_wanted ? tile_bytes(ROWS, 16) : 0) + (ROWS < 128 ? 1024 : 0);
     }
 };
 // Columns of tensor memory.  DW: of the sums of dWg and dWu, dWd, and dbd.
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(256) gated_pack(const __grid_constant__ GatedA
 }
 
 struct GatedBarriers {
-    u64 x_full[2], x_free[2], w_full[2][16], w_free[2][16], s_full[2], s_free[2], a_full[2], a_free[2], d_full[2], d_free[2], io_full, io_done, end[2];
+    u64 x_full[4], x_free[4], w_full[2][16], w_free[2][16], s_full[2], s_free[2], a_full[2], a_free[2], d_full[2], d_free[2], io_full[2], io_done[2], end[2];
     u32 tensor, dead;
 };
 static_assert(sizeof(GatedBarriers) <= 1024);
@@ -266,6 +267,8 @@ struct Waits {
             }
         return true;
     }
+    // Barriers of even and of odd steps: one half of the workers meets one of them, and sees each of its phases.
+    __device__ __forceinline__ bool step(u64* bars, long long q) { return on(bars + (q & 1), (int)(q >> 1)); }
     __device__ __forceinline__ bool full(u64* bars, const Turn& t) { return on(bars + t.at, t.turns); }
     __device__ __forceinline__ bool free(u64* bars, const Turn& t) { return t.turns == 0 ? alive : on(bars + t.at, t.turns - 1); }
 };
@@ -346,6 +349,20 @@ __device__ __forceinline__ void io_load16(float (&v)[16], const unsigned char* i
         else
 #pragma unroll
             for (int e = 0; e < V; e++) v[j + e] = 0.f;
+    }
+}
+// to = s times the rows of a tile of 16-bit values (swizzled), by a warp.
+template <typename T, int ROWS, typename = typename std::enable_if<sizeof(T) == 2>::type>
+__device__ __forceinline__ void scale_tile(T* to, const unsigned char* tile, int rows, int pieces, float s) {
+    const int lane = threadIdx.x & 31, count = rows * pieces, per = (65536 + pieces - 1) / pieces;   // (i per >> 16 is i / pieces for i < 2048)
+#pragma unroll 4
+    for (int i = lane; i < count; i += 32) {
+        const int r = i * per >> 16;
+        float v[8];
+        Piece16<T>::load(v, tile + swizzled_at(ROWS, r, i - r * pieces));
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] *= s;
+        Piece16<T>::store(to + 8 * i, v);
     }
 }
 // to = s from, `count` values, by a warp.
@@ -445,8 +462,7 @@ struct WeightRing {
 
 template <typename T, GatedPass PASS, int ROWS>
 __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const __grid_constant__ GatedArgs p, const __grid_constant__ GatedMaps maps) {
-    extern __shared__ unsigned char unaligned_smem[];
-    unsigned char* smem = unaligned_smem + (-shared_address(unaligned_smem) & 1023);
+    extern __shared__ __align__(1024) unsigned char smem[];
     using Smem = GatedSmem<T, PASS, ROWS>;
     using Columns = GatedColumns<T, PASS>;
     constexpr int C = gated_chunk<T>(), TERMS = Tensor<T>::TERMS;
@@ -459,23 +475,24 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
     // The last of the loaders brings the residual and takes the output away, and takes dout to the residual's gradient.
     const bool beside = p.io_buffers || (PASS == GATED_DX && p.dresidual);
     const int row_loaders = LOADERS - (beside ? 1 : 0);
+    const bool scales = PASS == GATED_DX && p.dresidual && p.boxes && p.wide_dresidual;   // from the tile of dout: another that reads it
     if (threadIdx.x == 0) {
+        for (int i = 0; i < p.x_buffers; i++) mbar_init(&b.x_full[i], p.boxes ? 1 : 32 * row_loaders), mbar_init(&b.x_free[i], scales ? 2 : 1);
         for (int i = 0; i < 2; i++) {
-            mbar_init(&b.x_full[i], p.boxes ? 1 : 32 * row_loaders), mbar_init(&b.x_free[i], 1);
-            mbar_init(&b.s_full[i], 1), mbar_init(&b.s_free[i], WORKERS);
-            mbar_init(&b.a_full[i], WORKERS), mbar_init(&b.a_free[i], 1);
+            mbar_init(&b.s_full[i], 1), mbar_init(&b.s_free[i], WORKERS / 2);
+            mbar_init(&b.a_full[i], WORKERS / 2), mbar_init(&b.a_free[i], 1);
             mbar_init(&b.d_full[i], 1), mbar_init(&b.d_free[i], WORKERS);
             for (int j = 0; j < p.w_buffers[i]; j++) mbar_init(&b.w_full[i][j], 1), mbar_init(&b.w_free[i][j], 1);
             mbar_init(&b.end[i], 1);
         }
-        mbar_init(&b.io_full, 1), mbar_init(&b.io_done, WORKERS);
+        for (int i = 0; i < p.io_buffers; i++) mbar_init(&b.io_full[i], 1), mbar_init(&b.io_done[i], WORKERS);
         b.dead = 0;
     }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(shared_address(&b.tensor)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    {   // a column of ones
+    if (p.biased || p.down_bias_wanted) {   // a column of ones
         float one[8] = {1.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, none[8] = {};
         using Term = typename Tensor<T>::Term;
         for (int i = threadIdx.x; i < 2 * ROWS; i += THREADS) store_terms8<Term>(smem + at.at_ones + 16 * i, 0, i < ROWS ? one : none);
@@ -511,33 +528,58 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
     if (warp >= WORKERS + 2) {   // loaders
         const int loader = warp - WORKERS - 2;
         if (beside && loader == LOADERS - 1) {
+            constexpr int BOX = 128 / sizeof(T);
+            const int width = PASS == GATED_OUT ? p.n : p.k;
+            const bool one = one_of_warp(), loads = PASS == GATED_OUT && p.residual;
+            long long arrived = 0;      // tiles whose buffer has been given to the workers
+            Turn xt, out;
+            auto give = [&]() {         // the next tile's, with its residual
+                u64* bar = &b.io_full[arrived % p.io_buffers];
+                unsigned char* io = smem + at.at_io + (int)(arrived % p.io_buffers) * at.io;
+                if (loads) {
+                    mbar_expect_tx(bar, at.io);
+                    for (int c = 0; c < width; c += BOX) box_load(io + c / BOX * ROWS * 128, &maps.residual, c, (int)((split + arrived * step) * ROWS), bar);
+                } else {
+                    mbar_arrive(bar);
+                }
+                arrived++;
+            };
+            if (one)
+                while (arrived < min(mine, (long long)p.io_buffers)) give();
             for (long long t = 0; t < mine && wait.alive; t++) {
                 const long long row0 = (split + t * step) * ROWS;
                 if constexpr (PASS == GATED_DX) {
-                    if (p.dresidual) scale_rows<T>(static_cast<T*>(p.dresidual) + row0 * p.n, static_cast<const T*>(p.grad) + row0 * p.n,
-                                                   (int)min((long long)ROWS, p.rows - row0) * p.n, p.scale, p.wide_dresidual);
-                }
-                if (p.io_buffers && one_of_warp()) {
-                    constexpr int BOX = 128 / sizeof(T);
-                    const int width = PASS == GATED_OUT ? p.n : p.k;
-                    unsigned char* io = smem + at.at_io;
-                    if (PASS == GATED_OUT && p.residual) {
-                        mbar_expect_tx(&b.io_full, at.io);
-                        for (int c = 0; c < width; c += BOX) box_load(io + c / BOX * ROWS * 128, &maps.residual, c, (int)row0, &b.io_full);
-                    } else {
-                        mbar_arrive(&b.io_full);
+                    const int valid = (int)min((long long)ROWS, p.rows - row0);
+                    T* to = static_cast<T*>(p.dresidual) + row0 * p.n;
+                    if (scales) {
+                        if (!wait.full(b.x_full, xt)) break;
+                        if constexpr (sizeof(T) == 2) scale_tile<T, ROWS>(to, smem + at.at_x + xt.at * at.x, valid, p.n / 8, p.scale);
+                        __syncwarp();
+                        if (one) mbar_arrive(&b.x_free[xt.at]);
+                        xt.next(p.x_buffers);
+                    } else if (p.dresidual) {
+                        scale_rows<T>(to, static_cast<const T*>(p.grad) + row0 * p.n, valid * p.n, p.scale, p.wide_dresidual);
                     }
-                    if (wait.on(&b.io_done, (int)t)) {
+                }
+                if (p.io_buffers) {
+                    if (!wait.full(b.io_done, out)) break;
+                    if (one) {
+                        const unsigned char* io = smem + at.at_io + out.at * at.io;
                         for (int c = 0; c < width; c += BOX) box_store(&maps.out, c, (int)row0, io + c / BOX * ROWS * 128);
                         bulk_commit();
                         bulk_wait_read();
-                    } else if (PASS == GATED_OUT && p.residual) {
-                        wait.alive = true, wait.on(&b.io_full, (int)t, true), wait.alive = false;   // nothing on its way
+                        if (arrived < mine) give();
                     }
+                    __syncwarp();
+                    out.next(p.io_buffers);
                 }
-                wait.alive = __shfl_sync(~0u, (int)!b_dead(b), 0) != 0;
             }
-            if (p.io_buffers) bulk_wait_all();
+            if (one) {
+                bulk_wait_all();
+                if (loads && b_dead(b))     // nothing on its way when others have given up
+                    for (long long i = max(0ll, arrived - p.io_buffers); i < arrived; i++)
+                        Waits{&b.dead}.on(&b.io_full[i % p.io_buffers], (int)(i / p.io_buffers), true);
+            }
         } else if (p.boxes) {
             if (loader == 0 && one_of_warp()) {
                 Turn xt;
@@ -577,15 +619,15 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
         if (one_of_warp()) {
             WeightRing w = ring(0);
             w.begin();
-            Turn xt, wt, w2t, st;
+            Turn xt, wt, w2t;
             int c = 0;
             for (long long q = 0; q < all; q++) {
                 if (c == 0 && !wait.full(b.x_full, xt)) break;
                 if (!(w.resident && q >= chunks) && !wait.full(b.w_full[0], wt)) break;
                 if (PASS != GATED_OUT && !(p.w_buffers[1] >= chunks && q >= chunks) && !wait.full(b.w_full[1], w2t)) break;
-                if (!wait.free(b.s_free, st)) break;
+                if (q >= p.s_buffers && !wait.step(b.s_free, q - p.s_buffers)) break;
                 tensor_after_sync();
-                const u32 x = shared_address(smem + at.at_x + xt.at * at.x), s = tensor + st.at * Columns::WIDE;
+                const u32 x = shared_address(smem + at.at_x + xt.at * at.x), s = tensor + ((int)q & (p.s_buffers - 1)) * Columns::WIDE;
                 const u32 w0 = shared_address(w.buffers + wt.at * w.bytes), w1 = shared_address(smem + at.at_w[1] + w2t.at * at.w[1]);
                 const Operand up = over_rows(PASS == GATED_OUT ? w0 : w1, p.kp, 2 * C);
                 if (p.biased) {   // ones times the biases' row
@@ -595,8 +637,8 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                 }
                 products<T>(s, s, rows_over_columns(x + at.grad, p.kx), up, 2 * C, p.kx / 16, p.biased);
                 if constexpr (PASS != GATED_OUT) products<T>(s + 2 * C, s + 2 * C, rows_over_columns(x, p.np), over_columns(w0, C, p.np), C, p.np / 16, false);
-                tensor_commit(&b.s_full[st.at]);
-                st.next(p.s_buffers), wt.next(w.count), w2t.next(p.w_buffers[1]);
+                tensor_commit(&b.s_full[q & 1]);
+                wt.next(w.count), w2t.next(p.w_buffers[1]);
                 if (++c == chunks) {
                     c = 0;
                     if (PASS != GATED_DW) tensor_commit(&b.x_free[xt.at]);
@@ -612,15 +654,15 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
         if (one_of_warp()) {
             WeightRing w = ring(1);
             w.begin();
-            Turn wt, xt, act, dt;
+            Turn wt, xt, dt;
             int in_group = 0;
             for (long long q = 0; q < all; q++) {
                 if (PASS == GATED_OUT && !(w.resident && q >= chunks) && !wait.full(b.w_full[1], wt)) break;   // (the first products have waited for the others)
-                if (!wait.full(b.a_full, act)) break;
+                if (!wait.step(b.a_full, q)) break;
                 if (in_group == 0 && !wait.free(b.d_free, dt)) break;
                 tensor_after_sync();
                 const u32 x = shared_address(smem + at.at_x + xt.at * at.x), w1 = shared_address(w.buffers + wt.at * w.bytes);
-                const u32 a = shared_address(smem + at.at_a + act.at * (Smem::A + Smem::ACT));
+                const u32 a = shared_address(smem + at.at_a + ((int)q & (p.a_buffers - 1)) * (Smem::A + Smem::ACT));
                 const u32 d = tensor + col.d + dt.at * Columns::SUMS * col.d_one;
                 const bool add = in_group > 0;
                 if constexpr (PASS == GATED_OUT) {
@@ -644,8 +686,8 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                     tensor_commit(&b.x_free[xt.at]);
                     xt.next(p.x_buffers);
                 }
-                tensor_commit(&b.a_free[act.at]);
-                act.next(p.a_buffers), wt.next(w.count);
+                tensor_commit(&b.a_free[q & 1]);
+                wt.next(w.count);
                 if (++in_group == group || q + 1 == all) {
                     in_group = 0;
                     tensor_commit(&b.d_full[dt.at]);
@@ -658,12 +700,12 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
             tensor_commit(&b.end[1]);
         }
     } else {   // workers
-        constexpr int PARTS = WORKERS / 4, W = C / PARTS;   // warps of 32 rows, hidden channels of each
-        const int quarter = warp & 3, part = warp >> 2, row = 32 * quarter + lane;
+        constexpr int PARTS = WORKERS / 8, W = C / PARTS;   // of one half: warps of 32 rows, hidden channels of each
+        const int quarter = warp & 3, part = (warp >> 2) % PARTS, half = warp / (WORKERS / 2), row = 32 * quarter + lane;
         const bool works = 32 * quarter < ROWS;
         const u32 lanes = tensor + ((u32)(32 * quarter) << 16);
-        Turn st, act, dt;
-        int in_group = 0, turns = 0;
+        Turn dt;
+        Turn io_turn;
         // The finished sums: of this CTA's index-th tile, or group of tiles.
         auto take_out = [&](long long index) {
             if (!wait.full(b.d_full, dt)) return;
@@ -673,9 +715,9 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
             const bool there = works && at_row < p.rows, staged = PASS != GATED_DW && p.io_buffers;
             const int width = PASS == GATED_OUT ? p.n : p.k;
             float* share = PASS == GATED_DW ? p.shares + ((long long)chunk0 * p.splits + split) * col.d_one * 128 + row : nullptr;
-            unsigned char* io = smem + at.at_io;
-            if (staged && !wait.on(&b.io_full, turns++)) return;   // the residual is there, and the rows before have left
-            for (int c = 16 * part; c < col.d_one; c += 16 * PARTS) {
+            unsigned char* io = smem + at.at_io + io_turn.at * at.io;
+            if (staged && !wait.full(b.io_full, io_turn)) return;   // the residual is there, and the rows before have left
+            for (int c = 16 * (2 * part + half); c < col.d_one; c += 32 * PARTS) {
                 float v[16], low[16];
                 __syncwarp();
                 tensor_load(v, d + c);
@@ -695,8 +737,13 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                     for (int j = 0; j < 16; j++) to[j * 128] = v[j];
                 } else if (there) {
                     if constexpr (PASS == GATED_OUT) {
+                        if (p.down_bias) {
 #pragma unroll
-                        for (int j = 0; j < 16; j++) v[j] += bias_s[c + j];
+                            for (int j = 0; j < 16; j += 4) {
+                                const float4 q = *reinterpret_cast<const float4*>(bias_s + c + j);
+                                v[j] += q.x, v[j + 1] += q.y, v[j + 2] += q.z, v[j + 3] += q.w;
+                            }
+                        }
                         if (p.residual) {
                             float r[16];
                             if (staged) io_load16<T, ROWS>(r, io, row, c, width);
@@ -716,36 +763,50 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
             if (!staged) return;
             fence_async_proxy();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&b.io_done);
+            if (lane == 0) mbar_arrive(&b.io_done[io_turn.at]);
+            io_turn.next(p.io_buffers);
         };
-        for (long long q = 0, groups = 0; q < all && wait.alive; q++) {
-            if (!wait.full(b.s_full, st)) break;
+        // Sums are taken out after the half's next step, when their last products have had time; before it where that step may wait for second
+        // products (for its operand's place, its weights' or, in DW, its rows') which wait for the sums' place.
+        const bool late = p.d_buffers == 2 || (PASS == GATED_OUT && p.a_buffers == 2);
+        long long taken = 0, q = half;
+        for (; q < all && wait.alive; q += 2) {
+            const long long before = q / group;      // groups of steps that are done
+            if (!late)
+                while (taken < before && wait.alive) take_out(taken++);
+            if (!wait.step(b.s_full, q)) break;
             tensor_after_sync();
-            const u32 s = lanes + st.at * Columns::WIDE + W * part;
-            float g[W], u[W], da[W];
-            tensor_load(g, s);
-            tensor_load(u, s + C);
-            if (PASS != GATED_OUT) tensor_load(da, s + 2 * C);
-            tensor_loaded();
-            tensor_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&b.s_free[st.at]);
-            if (!wait.free(b.a_free, act)) break;
-            unsigned char* a = smem + at.at_a + act.at * (Smem::A + Smem::ACT);
-            if (works) {
-                if (p.activation == PL_GATE_SILU) gated_work<T, PASS, PL_GATE_SILU, ROWS>(g, u, da, a, row, W * part);
-                else if (p.activation == PL_GATE_GELU) gated_work<T, PASS, PL_GATE_GELU, ROWS>(g, u, da, a, row, W * part);
-                else if (p.activation == PL_GATE_SIGMOID) gated_work<T, PASS, PL_GATE_SIGMOID, ROWS>(g, u, da, a, row, W * part);
-                else gated_work<T, PASS, PL_GATE_RELU, ROWS>(g, u, da, a, row, W * part);
+            const u32 s = lanes + ((int)q & (p.s_buffers - 1)) * Columns::WIDE + W * part;
+            unsigned char* a = smem + at.at_a + ((int)q & (p.a_buffers - 1)) * (Smem::A + Smem::ACT);
+#pragma unroll 1
+            for (int j = 0; j < W; j += 16) {
+                float g[16], u[16], da[16];
+                tensor_load(g, s + j);
+                tensor_load(u, s + C + j);
+                if (PASS != GATED_OUT) tensor_load(da, s + 2 * C + j);
+                tensor_loaded();
+                if (j + 16 == W) {
+                    tensor_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&b.s_free[half]);
+                }
+                if (j == 0 && q >= p.a_buffers && !wait.step(b.a_free, q - p.a_buffers)) break;
+                if (works) {
+                    if (p.activation == PL_GATE_SILU) gated_work<T, PASS, PL_GATE_SILU, ROWS>(g, u, da, a, row, W * part + j);
+                    else if (p.activation == PL_GATE_GELU) gated_work<T, PASS, PL_GATE_GELU, ROWS>(g, u, da, a, row, W * part + j);
+                    else if (p.activation == PL_GATE_SIGMOID) gated_work<T, PASS, PL_GATE_SIGMOID, ROWS>(g, u, da, a, row, W * part + j);
+                    else gated_work<T, PASS, PL_GATE_RELU, ROWS>(g, u, da, a, row, W * part + j);
+                }
+                __syncwarp();
             }
+            if (!wait.alive) break;
             fence_async_proxy();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&b.a_full[act.at]);
-            st.next(p.s_buffers), act.next(p.a_buffers);
-            if (in_group == 0 && q > 0) take_out(groups++);   // of the group before: its last products had this step's time
-            if (++in_group == group) in_group = 0;
-            if (q + 1 == all) take_out(groups);
+            if (lane == 0) mbar_arrive(&b.a_full[half]);
+            while (taken < before && wait.alive) take_out(taken++);
         }
+        const long long groups = (all + group - 1) / group;
+        while (taken < groups && wait.alive) take_out(taken++);
     }
     // All products are done, or a wait has run out: then nothing that could pass for a result.
     __syncwarp();

@@ -22,13 +22,23 @@ static bool gated_plan(GatedArgs& p) {
     const int chunks = PASS == GATED_DW ? 1 : p.chunks;
     p.boxes = sizeof(T) == 2 && p.wide_x && (PASS == GATED_OUT || p.wide_grad);
     auto fits = [&]() {
-        for (int io = PASS != GATED_DW && p.wide_out ? 1 : 0; io >= 0; io--)
-            for (int w : {chunks, std::min(2, chunks), 1})
-                for (int left : {0, 1, 2, 3}) {
-                    p.io_buffers = io, p.w_buffers[0] = p.w_buffers[1] = w, p.x_buffers = left & 2 ? 1 : 2, p.a_buffers = left & 1 ? 1 : 2;
-                    if (PASS == GATED_DW && p.a_buffers == 2) continue;   // (its second products take as long as its first: nothing waits for them)
-                    if (GatedSmem<T, PASS, ROWS>(p).total <= (int)GATED_SMEM) return true;
+        // Two tiles of rows first (what feeds the rest), then the weights, then rows that leave together, and more of both where there is room.
+        const int io = PASS != GATED_DW && p.wide_out, several = std::min(2, chunks);
+        const int tries[][3] = {{2, chunks, 2 * io}, {2, chunks, io}, {2, several, 2 * io}, {2, several, io}, {2, several, 0}, {1, several, io}, {1, several, 0},
+                                {1, 1, io}, {1, 1, 0}};
+        for (const auto& one : tries)
+            for (int a : {2, 1}) {
+                p.x_buffers = one[0], p.w_buffers[0] = p.w_buffers[1] = one[1], p.io_buffers = one[2], p.a_buffers = a;
+                if (PASS == GATED_DW && a == 2) continue;   // (its second products take as long as its first: nothing waits for them)
+                if (GatedSmem<T, PASS, ROWS>(p).total > (int)GATED_SMEM) continue;
+                while (p.x_buffers >= 2 && p.x_buffers < 4) {
+                    p.x_buffers++;
+                    if (GatedSmem<T, PASS, ROWS>(p).total <= (int)GATED_SMEM) continue;
+                    p.x_buffers--;
+                    break;
                 }
+                return true;
+            }
         return false;
     };
     auto columns = [&](int s, int d) {
@@ -73,10 +83,13 @@ static int launch_gated_rows(GatedArgs& p, cudaStream_t st) {
 }
 template <typename T, GatedPass PASS>
 static int launch_gated(GatedArgs& p, cudaStream_t st) {
-    if (gated_plan<T, PASS, 128>(p)) return launch_gated_rows<T, PASS, 128>(p, st);
-    if constexpr (sizeof(T) == 4)   // three terms of everything, from some 90 channels on: tiles of half as many rows, the other half of a product idle
+    // Tiles of 64 rows, the other half of a product idle, where 128 leave no room: three terms of everything, from some 90 channels on; and the sums
+    // over rows of 16-bit values where two tiles of 128 do not fit.
+    const bool fits = gated_plan<T, PASS, 128>(p);
+    if (fits && (PASS != GATED_DW || p.x_buffers >= 2)) return launch_gated_rows<T, PASS, 128>(p, st);
+    if constexpr (sizeof(T) == 4 || PASS == GATED_DW)
         if (gated_plan<T, PASS, 64>(p)) return launch_gated_rows<T, PASS, 64>(p, st);
-    return PL_INTERNAL_ERROR;
+    return fits && gated_plan<T, PASS, 128>(p) ? launch_gated_rows<T, PASS, 128>(p, st) : PL_INTERNAL_ERROR;
 }
 template <typename T>
 static int pack_gated(const GatedArgs& p, cudaStream_t st) {

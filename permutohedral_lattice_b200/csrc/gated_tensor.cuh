@@ -107,11 +107,11 @@ __device__ __forceinline__ void mbar_arrive(u64* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(bar)) : "memory");
 }
 
-__device__ __forceinline__ bool mbar_done(u64* bar, u32 parity) {   // waits a little
+__device__ __forceinline__ bool mbar_done(u64* bar, u32 parity) {   // sleeps for up to 20 us
     u32 done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(done)
-                 : "r"(shared_address(bar)), "r"(parity)
+                 : "r"(shared_address(bar)), "r"(parity), "r"(20000u)
                  : "memory");
     return done != 0;
 }
@@ -150,9 +150,10 @@ __device__ __forceinline__ void store_terms8(unsigned char* to, int plane, const
         uint4 q;
         Term* e = reinterpret_cast<Term*>(&q);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            e[i] = from_float<Term>(left[i]);
-            if (t + 1 < Tensor<T>::TERMS) left[i] -= to_float(e[i]);
+        for (int i = 0; i < 8; i += 2) {
+            if constexpr (std::is_same<Term, __half>::value) reinterpret_cast<__half2*>(&q)[i / 2] = __floats2half2_rn(left[i], left[i + 1]);
+            else reinterpret_cast<__nv_bfloat162*>(&q)[i / 2] = __floats2bfloat162_rn(left[i], left[i + 1]);
+            if (t + 1 < Tensor<T>::TERMS) left[i] -= to_float(e[i]), left[i + 1] -= to_float(e[i + 1]);
         }
         *reinterpret_cast<uint4*>(to + t * plane) = q;
     }
