@@ -433,12 +433,14 @@ struct WeightRing {
     long long pitch;             // from a chunk to the next in memory
     bool resident;
     long long asked = 0, all;
+    int next = 0;                // the chunk to ask for
     Turn use, load, freed;
     __device__ __forceinline__ void ask() {
         mbar_expect_tx(&full[load.at], bytes);
-        bulk_load(buffers + load.at * bytes, from + (chunk0 + (int)(asked % chunks)) * pitch, bytes, &full[load.at]);
+        bulk_load(buffers + load.at * bytes, from + (chunk0 + next) * pitch, bytes, &full[load.at]);
         load.next(count);
         asked++;
+        if (++next == chunks) next = 0;
     }
     __device__ __forceinline__ void begin() {
         if (resident) all = min(all, (long long)chunks);
@@ -532,10 +534,11 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
             const int width = PASS == GATED_OUT ? p.n : p.k;
             const bool one = one_of_warp(), loads = PASS == GATED_OUT && p.residual;
             long long arrived = 0;      // tiles whose buffer has been given to the workers
-            Turn xt, out;
+            Turn xt, out, given;
             auto give = [&]() {         // the next tile's, with its residual
-                u64* bar = &b.io_full[arrived % p.io_buffers];
-                unsigned char* io = smem + at.at_io + (int)(arrived % p.io_buffers) * at.io;
+                u64* bar = &b.io_full[given.at];
+                unsigned char* io = smem + at.at_io + given.at * at.io;
+                given.next(p.io_buffers);
                 if (loads) {
                     mbar_expect_tx(bar, at.io);
                     for (int c = 0; c < width; c += BOX) box_load(io + c / BOX * ROWS * 128, &maps.residual, c, (int)((split + arrived * step) * ROWS), bar);
@@ -769,9 +772,10 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
         // Sums are taken out after the half's next step, when their last products have had time; before it where that step may wait for second
         // products (for its operand's place, its weights' or, in DW, its rows') which wait for the sums' place.
         const bool late = p.d_buffers == 2 || (PASS == GATED_OUT && p.a_buffers == 2);
-        long long taken = 0, q = half;
-        for (; q < all && wait.alive; q += 2) {
-            const long long before = q / group;      // groups of steps that are done
+        long long taken = 0, before = 0;      // groups of steps: whose sums have been taken out, that are done
+        int in_group = half;
+        for (long long q = half; q < all && wait.alive; q += 2, in_group += 2) {
+            for (; in_group >= group; in_group -= group) before++;
             if (!late)
                 while (taken < before && wait.alive) take_out(taken++);
             if (!wait.step(b.s_full, q)) break;
