@@ -17,7 +17,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libpl_lattice.so")
 SOURCES = [os.path.join(CSRC, "pl_lattice.cu"), os.path.join(CSRC, "channel_mix.cu")] + [
     os.path.join(CSRC, "mix_%s.cu" % part) for part in ("forward_floats", "forward_halves", "backward_floats", "backward_halves")] + [
-    os.path.join(CSRC, s) for s in ("channel_norm.cu", "norm_floats.cu", "norm_halves.cu", "gated_mix.cu", "gated_floats.cu", "gated_halves.cu")]
+    os.path.join(CSRC, s) for s in ("channel_norm.cu", "norm_floats.cu", "norm_halves.cu", "norm_bfloats.cu", "gated_mix.cu", "gated_floats.cu", "gated_halves.cu")]
 HEADERS = [os.path.join(CSRC, h) for h in ("simplex.cuh", "common.cuh", "lattice_build.cuh", "splat.cuh",
                                              "blur_slice.cuh", "small.cuh", "export.cuh", "fp64.cuh", "direct_index.cuh", "direct_bounds.h", "crf.cuh",
                                              "smem_limit.h", "host_calls.h", "mix_common.cuh",

@@ -38,7 +38,7 @@ static NormArgs norm_args(const pl_channel_norm_shape* m, const void* x, const v
 }
 static int run_norm(NormArgs& a, int dtype, bool backward, cudaStream_t st) {
     const int ctas = num_sms() * (backward ? NORM_CTAS : 8);
-    return dtype == PL_F32 ? norm_of_floats(a, backward, ctas, st) : norm_of_halves(a, dtype, backward, ctas, st);
+    return dtype == PL_F32 ? norm_of_floats(a, backward, ctas, st) : dtype == PL_F16 ? norm_of_halves(a, backward, ctas, st) : norm_of_bfloats(a, backward, ctas, st);
 }
 template <typename T>
 static int launch_drop(const DropArgs& a, cudaStream_t st) {

@@ -24,7 +24,7 @@ enum NormVector { NORM_WA, NORM_BA, NORM_WB, NORM_BB, NORM_GATE };
 
 struct NormArgs {
     long long rows;
-    int c, lanes;                      // channels; lanes of a row, a power of two
+    int c;                             // channels
     int after, before;                 // pl_norm_kind
     float eps_after, eps_before, scale;
     const void *x, *residual, *gate;   // gate: of every value
@@ -39,25 +39,28 @@ struct NormArgs {
     int ctas;                          // (host) how many ran
 };
 
-// A row in registers: E values a lane, in pieces of V that follow one another in memory, piece i of lane l the (l + i lanes)-th.
-// V is 16 bytes where rows are whole pieces on 16-byte boundaries, else one value: 21 channels of floats, side by side, take as
-// many sectors either way.
+// Pieces of a row: V values that follow one another in memory, 16 bytes where rows are whole pieces on 16-byte boundaries, else one value (21
+// channels of floats, side by side in their lanes, take as many sectors either way).
 template <typename T, bool WIDE>
 struct Piece {
     static constexpr int V = WIDE ? 16 / (int)sizeof(T) : 1;
-    __device__ __forceinline__ static void load(float* v, const T* p) {
+    using Raw = typename std::conditional<WIDE, uint4, T>::type;   // as it comes
+    __device__ __forceinline__ static Raw nothing() {
+        if constexpr (WIDE) return make_uint4(0, 0, 0, 0);
+        else return from_float<T>(0.f);
+    }
+    __device__ __forceinline__ static void values(float* v, const Raw& q) {
         if constexpr (!WIDE) {
-            v[0] = to_float(*p);
+            v[0] = to_float(q);
         } else if constexpr (sizeof(T) == 4) {
-            const float4 q = *reinterpret_cast<const float4*>(p);
-            v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+            v[0] = __uint_as_float(q.x), v[1] = __uint_as_float(q.y), v[2] = __uint_as_float(q.z), v[3] = __uint_as_float(q.w);
         } else {
-            const uint4 q = *reinterpret_cast<const uint4*>(p);
             const T* e = reinterpret_cast<const T*>(&q);
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = to_float(e[j]);
         }
     }
+    __device__ __forceinline__ static void load(float* v, const T* p) { values(v, *reinterpret_cast<const Raw*>(p)); }
     __device__ __forceinline__ static void store(T* p, const float* v) {
         if constexpr (!WIDE) {
             *p = from_float<T>(v[0]);
@@ -65,9 +68,11 @@ struct Piece {
             *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
             uint4 q;
-            T* e = reinterpret_cast<T*>(&q);
 #pragma unroll
-            for (int j = 0; j < 8; j++) e[j] = from_float<T>(v[j]);
+            for (int j = 0; j < 8; j += 2) {
+                if constexpr (std::is_same<T, __half>::value) reinterpret_cast<__half2*>(&q)[j / 2] = __floats2half2_rn(v[j], v[j + 1]);
+                else reinterpret_cast<__nv_bfloat162*>(&q)[j / 2] = __floats2bfloat162_rn(v[j], v[j + 1]);
+            }
             *reinterpret_cast<uint4*>(p) = q;
         }
     }
@@ -84,30 +89,53 @@ struct Piece {
     }
 };
 
-template <typename T, bool WIDE, int E>
+// Rows in registers: E values a lane at most, piece i of lane l of a row the (l + i LANES)-th.
+template <typename T, bool WIDE, int E, int LANES>
 struct RowLanes {
     using P = Piece<T, WIDE>;
+    using Raw = typename P::Raw;
     static constexpr int V = P::V, N = E / V;
     static_assert(E % V == 0);
-    int lanes, l, c;
-    bool there;
-    long long first;   // the row's first value
-    __device__ __forceinline__ int channel(int i) const { return (l + i * lanes) * V; }
-    __device__ __forceinline__ bool live(int i) const { return there && channel(i) < c; }
-    __device__ __forceinline__ void load(float (&v)[E], const void* from) const {
-        const T* p = static_cast<const T*>(from) + first;
+    int l, c, whole;                   // pieces that all lanes of a row have
+    float per;                         // 1 / c
+    bool tail, there;                  // whether this lane has the piece behind the whole ones; whether its row is
+    long long first;                   // the row's first value
+    __device__ __forceinline__ RowLanes(const NormArgs& a) {
+        l = (threadIdx.x & 31) & (LANES - 1), c = a.c, whole = c / V / LANES;
+        per = 1.f / (float)c;
+        tail = l + whole * LANES < c / V;
+    }
+    __device__ __forceinline__ void at(long long row, long long rows) { there = row < rows, first = row * c; }
+    __device__ __forceinline__ int channel(int i) const { return (l + i * LANES) * V; }
+    __device__ __forceinline__ bool has(int i) const { return i < whole || (i == whole && tail); }
+    __device__ __forceinline__ void fetch(Raw (&q)[N], const void* from) const {
+        const T* p = static_cast<const T*>(from) + first + l * V;
 #pragma unroll
         for (int i = 0; i < N; i++) {
+            q[i] = P::nothing();
+            if (there && has(i)) q[i] = *reinterpret_cast<const Raw*>(p + i * LANES * V);
+        }
+    }
+    __device__ __forceinline__ void values(float (&v)[E], const Raw (&q)[N]) const {
 #pragma unroll
-            for (int j = 0; j < V; j++) v[i * V + j] = 0.f;
-            if (live(i)) P::load(v + i * V, p + channel(i));
+        for (int i = 0; i < N; i++) {
+            P::values(v + i * V, q[i]);
         }
     }
     __device__ __forceinline__ void store(void* to, const float (&v)[E]) const {
-        T* p = static_cast<T*>(to) + first;
+        T* p = static_cast<T*>(to) + first + l * V;
 #pragma unroll
-        for (int i = 0; i < N; i++)
-            if (live(i)) P::store(p + channel(i), v + i * V);
+        for (int i = 0; i < N; i++) {
+            if (there && has(i)) P::store(p + i * LANES * V, v + i * V);
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+#pragma unroll
+            for (int j = 0; j < V; j++) f(i * V + j);
+        }
     }
     // f(element, the vector's value for it); a lane without a channel gets another channel's
     template <typename F>
@@ -121,63 +149,67 @@ struct RowLanes {
         }
     }
     __device__ __forceinline__ float sum(float v) const {   // of the row's lanes, the same in all of them
-        for (int o = lanes >> 1; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+            if (o < LANES) v += __shfl_xor_sync(~0u, v, o);
         return v;
     }
-    // v to its normed form without weight and bias, zero where there is no channel; returns the reciprocal deviation
-    __device__ __forceinline__ float normalise(float (&v)[E], int kind, float eps) const {
-        const float per = 1.f / (float)c;
-        if (kind == PL_NORM_LAYER) {
-            float s = 0.f;
+    // f(element) summed over the row's channels
+    template <typename F>
+    __device__ __forceinline__ float sum_of(F f) const {
+        float s = 0.f;
 #pragma unroll
-            for (int e = 0; e < E; e++) s += v[e];
-            const float mean = sum(s) * per;
+        for (int i = 0; i < N; i++) {
+            float p = 0.f;
 #pragma unroll
-            for (int e = 0; e < E; e++) v[e] = live(e / V) ? v[e] - mean : 0.f;
+            for (int j = 0; j < V; j++) p += f(i * V + j);
+            s += has(i) ? p : 0.f;
         }
-        float q = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; e++) q = fmaf(v[e], v[e], q);
-        const float rstd = rsqrtf(fmaf(sum(q), per, eps));
-#pragma unroll
-        for (int e = 0; e < E; e++) v[e] *= rstd;
+        return sum(s);
+    }
+    // v to its normed form without weight and bias; returns the reciprocal deviation.  (What lanes without a channel hold is never summed nor stored.)
+    __device__ __forceinline__ float normalise(float (&v)[E], int kind, float eps) const {
+        if (kind == PL_NORM_LAYER) {
+            const float mean = sum_of([&](int e) { return v[e]; }) * per;
+            each([&](int e) { v[e] -= mean; });
+        }
+        const float rstd = rsqrtf(fmaf(sum_of([&](int e) { return v[e] * v[e]; }), per, eps));
+        each([&](int e) { v[e] *= rstd; });
         return rstd;
     }
-    // d, the gradient of the normed form (zero where there is no channel), to that of what went in
+    // d, the gradient of the normed form, to that of what went in
     __device__ __forceinline__ void back(float (&d)[E], const float (&hat)[E], float rstd, int kind) const {
-        const float per = 1.f / (float)c;
-        float s = 0.f, q = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; e++) s += d[e], q = fmaf(d[e], hat[e], q);
-        q = sum(q) * per;
-        s = kind == PL_NORM_LAYER ? sum(s) * per : 0.f;
-#pragma unroll
-        for (int e = 0; e < E; e++) d[e] = rstd * (d[e] - s - hat[e] * q);
+        const float q = sum_of([&](int e) { return d[e] * hat[e]; }) * per;
+        const float s = kind == PL_NORM_LAYER ? sum_of([&](int e) { return d[e]; }) * per : 0.f;
+        each([&](int e) { d[e] = rstd * (d[e] - s - hat[e] * q); });
     }
-    // Bit e: element e stays.  Values are counted through the whole tensor.  Single values: the words of the warp's rows, which follow one
-    // another, by way of shared memory (a word for every value by its own lane would make each four times).
-    __device__ __forceinline__ u32 kept(const Philox& random, u32 threshold, long long warp_first, uint4* words_s) const {
-        u32 bits = 0;
+    // mask[e]: all ones where element e stays, else zero.  Values are counted through the whole tensor.  Single values: the words of the warp's
+    // rows, which follow one another, by way of shared memory (a word for every value by its own lane would make each four times).
+    __device__ __forceinline__ void kept(u32 (&mask)[E], const Philox& random, u32 threshold, long long warp_first, uint4* words_s) const {
         if constexpr (WIDE) {
 #pragma unroll
             for (int i = 0; i < N; i++)
 #pragma unroll
                 for (int j = 0; j < V; j += 4) {
                     const uint4 w = random.words((u64)(first + channel(i) + j) >> 2);
-                    bits |= ((u32)(w.x >= threshold) | (u32)(w.y >= threshold) << 1 | (u32)(w.z >= threshold) << 2 | (u32)(w.w >= threshold) << 3) << (i * V + j);
+                    mask[i * V + j] = w.x >= threshold ? ~0u : 0u, mask[i * V + j + 1] = w.y >= threshold ? ~0u : 0u;
+                    mask[i * V + j + 2] = w.z >= threshold ? ~0u : 0u, mask[i * V + j + 3] = w.w >= threshold ? ~0u : 0u;
                 }
         } else {
             const u64 quad = (u64)warp_first >> 2;
-            const int count = (int)(((u64)warp_first + (32 / lanes) * c + 3) / 4 - quad), lane = threadIdx.x & 31;
+            const int count = (int)(((u64)warp_first + (32 / LANES) * c + 3) / 4 - quad), lane = threadIdx.x & 31;
             __syncwarp();   // the last rows' words have been read
             for (int q = lane; q < count; q += 32) words_s[q] = random.words(quad + q);
             __syncwarp();
-            const u32* word = reinterpret_cast<const u32*>(words_s) + (first - (long long)(quad << 2));
+            const u32* word = reinterpret_cast<const u32*>(words_s) + (int)(first - (long long)(quad << 2)) + l;
 #pragma unroll
-            for (int i = 0; i < N; i++)
-                if (live(i)) bits |= (u32)(word[channel(i)] >= threshold) << i;
+            for (int i = 0; i < N; i++) {
+                mask[i] = there && has(i) && word[i * LANES] >= threshold ? ~0u : 0u;
+            }
         }
-        return bits;
+    }
+    __device__ __forceinline__ void drop(float (&v)[E], const u32 (&mask)[E], float scale) const {   // what is dropped is zero, whatever it was
+        each([&](int e) { v[e] = __uint_as_float(__float_as_uint(v[e] * scale) & mask[e]); });
     }
 };
 // Quads of words that the rows of a warp may need: 32 E values at most, not begun at a quad's first one.
@@ -190,45 +222,50 @@ __device__ __forceinline__ void norm_vectors_to(float* vectors_s, const NormArgs
     __syncthreads();
 }
 
-template <typename T, bool WIDE, int E>
+template <typename T, bool WIDE, int E, int LANES>
 __global__ void __launch_bounds__(NORM_THREADS) norm_forward(const __grid_constant__ NormArgs a) {
     __shared__ __align__(16) float vectors_s[NORM_VECTORS * NORM_MOST];
     __shared__ uint4 words_s[WIDE ? 1 : NORM_WARPS * norm_words(E)];
     norm_vectors_to(vectors_s, a);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per_warp = 32 / a.lanes;
+    using Row = RowLanes<T, WIDE, E, LANES>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool drops = a.drop.threshold != 0;
     const Philox random(a.drop);
-    for (long long r0 = ((long long)blockIdx.x * NORM_WARPS + warp) * per_warp; r0 < a.rows; r0 += (long long)gridDim.x * NORM_WARPS * per_warp) {
-        const long long row = r0 + lane / a.lanes;
-        const RowLanes<T, WIDE, E> r{a.lanes, lane & (a.lanes - 1), a.c, row < a.rows, row * a.c};
+    Row r(a);
+    const int per_warp = 32 / LANES, own = lane / LANES;
+    const long long step = (long long)gridDim.x * NORM_WARPS * per_warp;
+    // A warp's next rows are on their way while these are worked on.
+    typename Row::Raw next_x[Row::N], next_residual[Row::N], next_gate[Row::N];
+    auto fetch = [&](long long r0) {
+        r.at(r0 + own, a.rows);
+        r.fetch(next_x, a.x);
+        if (a.residual) r.fetch(next_residual, a.residual);
+        if (a.gate) r.fetch(next_gate, a.gate);
+    };
+    long long r0 = ((long long)blockIdx.x * NORM_WARPS + warp) * per_warp;
+    if (r0 < a.rows) fetch(r0);
+    for (; r0 < a.rows; r0 += step) {
         float v[E], residual[E], gate[E];
-        r.load(v, a.x);
-        if (a.residual) r.load(residual, a.residual);
-        if (a.gate) r.load(gate, a.gate);
+        r.values(v, next_x);
+        if (a.residual) r.values(residual, next_residual);
+        if (a.gate) r.values(gate, next_gate);
+        fetch(r0 + step);
+        r.at(r0 + own, a.rows);
         if (a.after) {
             r.normalise(v, a.after, a.eps_after);
             if (a.vectors[NORM_WA]) r.with(vectors_s + NORM_WA * NORM_MOST, [&](int e, float w) { v[e] *= w; });
             if (a.vectors[NORM_BA]) r.with(vectors_s + NORM_BA * NORM_MOST, [&](int e, float w) { v[e] += w; });
         }
         if (drops) {
-            const u32 kept = r.kept(random, a.drop.threshold, r0 * a.c, words_s + (WIDE ? 0 : warp * norm_words(E)));
-#pragma unroll
-            for (int e = 0; e < E; e++) v[e] = kept >> e & 1 ? v[e] * a.drop.scale : 0.f;
+            u32 mask[E];
+            r.kept(mask, random, a.drop.threshold, r0 * a.c, words_s + (WIDE ? 0 : warp * norm_words(E)));
+            r.drop(v, mask, a.drop.scale);
         }
-        if (a.gate) {
-#pragma unroll
-            for (int e = 0; e < E; e++) v[e] *= gate[e];
-        } else if (a.vectors[NORM_GATE]) {
-            r.with(vectors_s + NORM_GATE * NORM_MOST, [&](int e, float w) { v[e] *= w; });
-        }
-        if (a.residual) {
-#pragma unroll
-            for (int e = 0; e < E; e++) v[e] = fmaf(a.scale, residual[e], v[e]);
-        }
+        if (a.gate) r.each([&](int e) { v[e] *= gate[e]; });
+        else if (a.vectors[NORM_GATE]) r.with(vectors_s + NORM_GATE * NORM_MOST, [&](int e, float w) { v[e] *= w; });
+        if (a.residual) r.each([&](int e) { v[e] = fmaf(a.scale, residual[e], v[e]); });
         if (a.h) r.store(a.h, v);
         if (a.before) {
-#pragma unroll
-            for (int e = 0; e < E; e++) v[e] = r.live(e / r.V) ? v[e] : 0.f;   // (a bias is no channel's there)
             r.normalise(v, a.before, a.eps_before);
             if (a.vectors[NORM_WB]) r.with(vectors_s + NORM_WB * NORM_MOST, [&](int e, float w) { v[e] *= w; });
             if (a.vectors[NORM_BB]) r.with(vectors_s + NORM_BB * NORM_MOST, [&](int e, float w) { v[e] += w; });
@@ -237,104 +274,97 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_forward(const __grid_consta
     }
 }
 
-template <typename T, bool WIDE, int E, bool AFTER, bool BEFORE>
-__global__ void __launch_bounds__(NORM_THREADS) norm_backward(const __grid_constant__ NormArgs a) {
+template <typename T, bool WIDE, int E, int LANES, bool AFTER, bool BEFORE>
+__global__ void __launch_bounds__(NORM_THREADS, E <= 8 ? 2 : 1) norm_backward(const __grid_constant__ NormArgs a) {
     __shared__ __align__(16) float vectors_s[NORM_VECTORS * NORM_MOST];
     __shared__ uint4 words_s[WIDE ? 1 : NORM_WARPS * norm_words(E)];
     norm_vectors_to(vectors_s, a);
-    using Row = RowLanes<T, WIDE, E>;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per_warp = 32 / a.lanes;
+    using Row = RowLanes<T, WIDE, E, LANES>;
+    constexpr bool AHEAD = WIDE && sizeof(T) == 2 && E <= 8;   // room for the next rows as they come
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool drops = a.drop.threshold != 0;
     const Philox random(a.drop);
+    Row r(a);
+    const int per_warp = 32 / LANES, own = lane / LANES;
+    const long long step = (long long)gridDim.x * NORM_WARPS * per_warp;
     float sum_wa[E], sum_ba[E], sum_wb[E], sum_bb[E], sum_gate[E];   // (those without a use take no registers)
 #pragma unroll
     for (int e = 0; e < E; e++) sum_wa[e] = sum_ba[e] = sum_wb[e] = sum_bb[e] = sum_gate[e] = 0.f;
-    for (long long r0 = ((long long)blockIdx.x * NORM_WARPS + warp) * per_warp; r0 < a.rows; r0 += (long long)gridDim.x * NORM_WARPS * per_warp) {
-        const long long row = r0 + lane / a.lanes;
-        const Row r{a.lanes, lane & (a.lanes - 1), a.c, row < a.rows, row * a.c};
-        float x[E], h[E], gate[E], d[E], dy[E], rstd = 0.f;
-        if (a.x) r.load(x, a.x);
-        else {
-#pragma unroll
-            for (int e = 0; e < E; e++) x[e] = 0.f;
-        }
-        if (a.gate) r.load(gate, a.gate);
-        if (a.dh) r.load(d, a.dh);
-        else {
-#pragma unroll
-            for (int e = 0; e < E; e++) d[e] = 0.f;
-        }
+    typename Row::Raw raw_x[Row::N], raw_residual[Row::N], raw_gate[Row::N], raw_dh[Row::N], raw_dy[Row::N];
+    auto fetch = [&](long long r0) {
+        r.at(r0 + own, a.rows);
+        if (a.x) r.fetch(raw_x, a.x);
+        if (a.gate) r.fetch(raw_gate, a.gate);
+        if (a.dh) r.fetch(raw_dh, a.dh);
         if constexpr (BEFORE) {
-            if (a.residual) r.load(h, a.residual);
-            else {
-#pragma unroll
-                for (int e = 0; e < E; e++) h[e] = 0.f;
-            }
-            r.load(dy, a.dy);
+            if (a.residual) r.fetch(raw_residual, a.residual);
+            r.fetch(raw_dy, a.dy);
         }
-        u32 kept = ~0u;
-        if (drops) kept = r.kept(random, a.drop.threshold, r0 * a.c, words_s + (WIDE ? 0 : warp * norm_words(E)));
-        if (!a.gate) {
-#pragma unroll
-            for (int e = 0; e < E; e++) gate[e] = 1.f;
-            if (a.vectors[NORM_GATE]) r.with(vectors_s + NORM_GATE * NORM_MOST, [&](int e, float w) { gate[e] = w; });
+    };
+    long long r0 = ((long long)blockIdx.x * NORM_WARPS + warp) * per_warp;
+    if (AHEAD && r0 < a.rows) fetch(r0);
+    for (; r0 < a.rows; r0 += step) {
+        if (!AHEAD) fetch(r0);
+        float x[E], h[E], gate[E], d[E], dy[E], rstd = 0.f;
+        if (a.x) r.values(x, raw_x);
+        else r.each([&](int e) { x[e] = 0.f; });
+        if (a.dh) r.values(d, raw_dh);
+        else r.each([&](int e) { d[e] = 0.f; });
+        if constexpr (BEFORE) {
+            if (a.residual) r.values(h, raw_residual);
+            else r.each([&](int e) { h[e] = 0.f; });
+            r.values(dy, raw_dy);
         }
+        if (a.gate) r.values(gate, raw_gate);
+        else if (a.vectors[NORM_GATE]) r.with(vectors_s + NORM_GATE * NORM_MOST, [&](int e, float w) { gate[e] = w; });
+        else r.each([&](int e) { gate[e] = 1.f; });
+        if (AHEAD) {
+            fetch(r0 + step);
+            r.at(r0 + own, a.rows);
+        }
+        u32 mask[E];
+        if (drops) r.kept(mask, random, a.drop.threshold, r0 * a.c, words_s + (WIDE ? 0 : warp * norm_words(E)));
         if constexpr (AFTER) rstd = r.normalise(x, a.after, a.eps_after);   // x is x^ from here on
         float v[E];
-#pragma unroll
-        for (int e = 0; e < E; e++) v[e] = x[e];
+        r.each([&](int e) { v[e] = x[e]; });
         if constexpr (AFTER) {
             if (a.vectors[NORM_WA]) r.with(vectors_s + NORM_WA * NORM_MOST, [&](int e, float w) { v[e] *= w; });
             if (a.vectors[NORM_BA]) r.with(vectors_s + NORM_BA * NORM_MOST, [&](int e, float w) { v[e] += w; });
         }
-        if (drops) {
-#pragma unroll
-            for (int e = 0; e < E; e++) v[e] = kept >> e & 1 ? v[e] * a.drop.scale : 0.f;
-        }
+        if (drops) r.drop(v, mask, a.drop.scale);
         if constexpr (BEFORE) {
-#pragma unroll
-            for (int e = 0; e < E; e++) h[e] = r.live(e / Row::V) ? fmaf(a.scale, h[e], v[e] * gate[e]) : 0.f;
+            r.each([&](int e) { h[e] = fmaf(a.scale, h[e], v[e] * gate[e]); });
             const float rstd_h = r.normalise(h, a.before, a.eps_before);
             if (a.shares) {
-#pragma unroll
-                for (int e = 0; e < E; e++) {
+                r.each([&](int e) {
                     sum_wb[e] = fmaf(dy[e], h[e], sum_wb[e]);
                     sum_bb[e] += dy[e];
-                }
+                });
             }
             if (a.vectors[NORM_WB]) r.with(vectors_s + NORM_WB * NORM_MOST, [&](int e, float w) { dy[e] *= w; });
             r.back(dy, h, rstd_h, a.before);
-#pragma unroll
-            for (int e = 0; e < E; e++) d[e] += r.live(e / Row::V) ? dy[e] : 0.f;   // (the mean is no channel's there)
+            r.each([&](int e) { d[e] += dy[e]; });
         }
         if (a.dresidual) {
             float t[E];
-#pragma unroll
-            for (int e = 0; e < E; e++) t[e] = a.scale * d[e];
+            r.each([&](int e) { t[e] = a.scale * d[e]; });
             r.store(a.dresidual, t);
         }
         if (a.dgate) {
             float t[E];
-#pragma unroll
-            for (int e = 0; e < E; e++) t[e] = d[e] * v[e];
+            r.each([&](int e) { t[e] = d[e] * v[e]; });
             r.store(a.dgate, t);
         } else if (a.shares) {
-#pragma unroll
-            for (int e = 0; e < E; e++) sum_gate[e] = fmaf(d[e], v[e], sum_gate[e]);
+            r.each([&](int e) { sum_gate[e] = fmaf(d[e], v[e], sum_gate[e]); });
         }
-#pragma unroll
-        for (int e = 0; e < E; e++) d[e] *= gate[e];
-        if (drops) {
-#pragma unroll
-            for (int e = 0; e < E; e++) d[e] = kept >> e & 1 ? d[e] * a.drop.scale : 0.f;
-        }
+        r.each([&](int e) { d[e] *= gate[e]; });
+        if (drops) r.drop(d, mask, a.drop.scale);
         if constexpr (AFTER) {
             if (a.shares) {
-#pragma unroll
-                for (int e = 0; e < E; e++) {
+                r.each([&](int e) {
                     sum_wa[e] = fmaf(d[e], x[e], sum_wa[e]);
                     sum_ba[e] += d[e];
-                }
+                });
             }
             if (a.vectors[NORM_WA]) r.with(vectors_s + NORM_WA * NORM_MOST, [&](int e, float w) { d[e] *= w; });
             r.back(d, x, rstd, a.after);
@@ -345,15 +375,16 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_backward(const __grid_const
     // The CTA's sums: of the rows of a warp by shuffles, of the warps by way of shared memory, a vector at a time.
     __shared__ float warps_s[NORM_WARPS][NORM_MOST];
     float* share = a.shares + (long long)blockIdx.x * NORM_VECTORS * a.c;
-    const Row r{a.lanes, lane & (a.lanes - 1), a.c, true, 0};
     auto gather = [&](const float (&s)[E], int which) {
         if (!(a.wanted >> which & 1)) return;
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < E; e++) {
             float t = s[e];
-            for (int o = a.lanes; o < 32; o <<= 1) t += __shfl_xor_sync(~0u, t, o);
-            if (lane < a.lanes && r.live(e / Row::V)) warps_s[warp][r.channel(e / Row::V) + e % Row::V] = t;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1)
+                if (o >= LANES) t += __shfl_xor_sync(~0u, t, o);
+            if (lane < LANES && r.has(e / Row::V)) warps_s[warp][r.channel(e / Row::V) + e % Row::V] = t;
         }
         __syncthreads();
         for (int i = threadIdx.x; i < a.c; i += NORM_THREADS) {
