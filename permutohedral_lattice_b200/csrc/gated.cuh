@@ -39,6 +39,7 @@ struct GatedArgs {
     const void *x, *gate_weight, *up_weight, *down_weight, *gate_bias, *up_bias, *down_bias, *residual, *grad;
     int biased, boxes, wide_x, wide_grad, wide_out;   // wide: rows of whole 16 bytes on 16-byte boundaries; boxes: of 16-bit values, what is read
     int wide_dresidual, down_bias_wanted;             // (DX, DW)
+    int stacked;                     // (DW, floats) the terms of a product's second operand side by side: a sum for every order of magnitude
     unsigned char* packed;           // the weights, a chunk after another: Wd, Wg and Wu as tiles
     void *out, *dresidual;           // out: or dx
     float* shares;                   // [chunks][splits][columns of sums][128]
@@ -83,23 +84,37 @@ struct GatedSmem {
         total = at_ones + (p.biased || p.down_bias_wanted ? tile_bytes(ROWS, 16) : 0) + (ROWS < 128 ? 1024 : 0);
     }
 };
-// Columns of tensor memory.  DW: of the sums of dWg and dWu, dWd, and dbd.
+// Columns of tensor memory: of g and u (and da), and of the sums.  Those of DW are, in this order, of dWg and dWu, dbg and dbu, dWd, and dbd.
 template <typename T, GatedPass PASS>
 struct GatedColumns {
     static constexpr int C = gated_chunk<T>(), WIDE = PASS == GATED_OUT ? 2 * C : 3 * C, SUMS = Tensor<T>::TERMS == 3 ? 2 : 1;
-    int d, d_one, low, down, bias, total;
+    int d, d_one, d_all, total;         // from there on; of the values, of all their parts
+    int up_bias, down, down_bias;       // (DW) where those sums begin
+    int up_part, down_part, bias_part;  // from one part of a value (float32: of its products' small terms, by size) to the next
     __host__ __device__ GatedColumns(const GatedArgs& p) {
         d = p.s_buffers * WIDE;
-        if (PASS == GATED_DW) {
-            down = p.kp;
-            bias = down + C;
-            d_one = bias + (p.down_bias_wanted ? 16 : 0);
-        } else {
-            down = bias = 0;
-            d_one = PASS == GATED_OUT ? p.np : p.kx;
+        d_one = PASS == GATED_DW ? p.kp + C + (p.down_bias_wanted ? 16 : 0) : PASS == GATED_OUT ? p.np : p.kx;
+        d_all = SUMS * d_one;
+        up_bias = p.kx, down = p.kp, down_bias = p.kp + C;
+        up_part = down_part = bias_part = SUMS == 2 ? d_one : 0;
+        if (p.stacked) {
+            const int biases = p.kp - p.kx + (p.down_bias_wanted ? 16 : 0);
+            down = 3 * p.kx, up_bias = down + 3 * C, down_bias = up_bias + p.kp - p.kx;
+            up_part = p.kx, down_part = C, bias_part = biases;
+            d_all = up_bias + 2 * biases;
         }
-        low = SUMS == 2 ? d_one : 0;         // from a sum to that of its small products
-        total = d + p.d_buffers * SUMS * d_one;
+        total = d + p.d_buffers * d_all;
+    }
+    // Where value c's first part is, how far the next, and how many.
+    __device__ __forceinline__ int place(const GatedArgs& p, int c, int& part, int& parts) const {
+        part = up_part, parts = PASS == GATED_DW && p.stacked ? 3 : SUMS;
+        if (PASS != GATED_DW || c < p.kx) return c;
+        if (c >= p.kp && c < p.kp + C) {
+            part = down_part;
+            return down + c - p.kp;
+        }
+        part = bias_part, parts = SUMS;
+        return c < p.kp ? up_bias + c - p.kx : down_bias + c - p.kp - C;
     }
 };
 
@@ -666,26 +681,32 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                 tensor_after_sync();
                 const u32 x = shared_address(smem + at.at_x + xt.at * at.x), w1 = shared_address(w.buffers + wt.at * w.bytes);
                 const u32 a = shared_address(smem + at.at_a + ((int)q & (p.a_buffers - 1)) * (Smem::A + Smem::ACT));
-                const u32 d = tensor + col.d + dt.at * Columns::SUMS * col.d_one;
+                const u32 d = tensor + col.d + dt.at * col.d_all;
                 const bool add = in_group > 0;
                 if constexpr (PASS == GATED_OUT) {
-                    products<T>(d, d + col.low, over_columns(a, ROWS, C), over_rows(w1, C, p.np), p.np, C / 16, add);
+                    products<T>(d, d + col.up_part, over_columns(a, ROWS, C), over_rows(w1, C, p.np), p.np, C / 16, add);
                 } else if constexpr (PASS == GATED_DX) {
-                    products<T>(d, d + col.low, over_columns(a, ROWS, 2 * C), over_columns(w1, p.kp, 2 * C), col.d_one, 2 * C / 16, add);
+                    products<T>(d, d + col.up_part, over_columns(a, ROWS, 2 * C), over_columns(w1, p.kp, 2 * C), p.kx, 2 * C / 16, add);
                 } else {
                     const Operand hidden = over_rows(a, ROWS, 2 * C), grad = rows_over_rows(x, p.np);
-                    products<T>(d, d + col.low, hidden, rows_over_rows(x + at.grad, p.kx), p.kx, ROWS / 16, add);
-                    products<T>(d + col.down, d + col.down + col.low, grad, over_rows(a + Smem::A, ROWS, C), C, ROWS / 16, add);
+                    const Operand rows = rows_over_rows(x + at.grad, p.kx), act = over_rows(a + Smem::A, ROWS, C);
+                    if (TERMS == 3 && p.stacked) {
+                        stacked_products<T>(d, hidden, rows, p.kx, ROWS / 16, add);
+                        stacked_products<T>(d + col.down, grad, act, C, ROWS / 16, add);
+                    } else {
+                        products<T>(d, d + col.up_part, hidden, rows, p.kx, ROWS / 16, add);
+                        products<T>(d + col.down, d + col.down + col.down_part, grad, act, C, ROWS / 16, add);
+                    }
                     // the biases': times ones (which have one term)
                     const Operand one = over_rows(shared_address(smem + at.at_ones), ROWS, 16);
                     auto column_sums = [&](const Operand& of, u32 to) {
                         const u32 shape = product_shape<T>(of, one, 16);
                         for (int t = TERMS - 1; t >= 0; t--)
                             for (int s = 0; s < ROWS / 16; s++)
-                                tensor_product(to + (t ? col.low : 0), of.at(s, t), one.at(s, 0), shape, add || s > 0 || (TERMS == 3 && t == 1));
+                                tensor_product(to + (t ? col.bias_part : 0), of.at(s, t), one.at(s, 0), shape, add || s > 0 || (TERMS == 3 && t == 1));
                     };
-                    if (p.biased) column_sums(hidden, d + p.kx);
-                    if (p.down_bias_wanted) column_sums(grad, d + col.bias);
+                    if (p.biased) column_sums(hidden, d + col.up_bias);
+                    if (p.down_bias_wanted) column_sums(grad, d + col.down_bias);
                     tensor_commit(&b.x_free[xt.at]);
                     xt.next(p.x_buffers);
                 }
@@ -713,7 +734,7 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
         auto take_out = [&](long long index) {
             if (!wait.full(b.d_full, dt)) return;
             tensor_after_sync();
-            const u32 d = lanes + col.d + dt.at * Columns::SUMS * col.d_one;
+            const u32 d = lanes + col.d + dt.at * col.d_all;
             const long long row0 = PASS == GATED_DW ? 0 : (split + index * step) * ROWS, at_row = row0 + row;
             const bool there = works && at_row < p.rows, staged = PASS != GATED_DW && p.io_buffers;
             const int width = PASS == GATED_OUT ? p.n : p.k;
@@ -723,10 +744,19 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
             for (int c = 16 * (2 * part + half); c < col.d_one; c += 32 * PARTS) {
                 float v[16], low[16];
                 __syncwarp();
-                tensor_load(v, d + c);
-                if (Columns::SUMS == 2) tensor_load(low, d + col.low + c);
+                int part, parts;
+                const u32 from = d + col.place(p, c, part, parts);
+                tensor_load(v, from);
+                if (Columns::SUMS == 2) tensor_load(low, from + part);
                 tensor_loaded();
                 if (Columns::SUMS == 2) {
+                    if (PASS == GATED_DW && parts == 3) {   // the smallest first
+                        float third[16];
+                        tensor_load(third, from + 2 * part);
+                        tensor_loaded();
+#pragma unroll
+                        for (int j = 0; j < 16; j++) low[j] += third[j];
+                    }
 #pragma unroll
                     for (int j = 0; j < 16; j++) v[j] += low[j];
                 }
@@ -769,16 +799,19 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
             if (lane == 0) mbar_arrive(&b.io_done[io_turn.at]);
             io_turn.next(p.io_buffers);
         };
-        // Sums are taken out after the half's next step, when their last products have had time; before it where that step may wait for second
-        // products (for its operand's place, its weights' or, in DW, its rows') which wait for the sums' place.
+        // Sums are taken out after the half's next step, when their last products have had time; amid it where that step's operand may have to wait for
+        // second products, which wait for the sums' place; before it where its first products may, too (for weights or, in DW, for rows).
         const bool late = p.d_buffers == 2 || (PASS == GATED_OUT && p.a_buffers == 2);
+        const bool amid = !late && (PASS == GATED_DW ? p.x_buffers >= 2 : PASS == GATED_DX && (p.w_buffers[1] >= chunks || p.w_buffers[1] >= 3));
         long long taken = 0, before = 0;      // groups of steps: whose sums have been taken out, that are done
         int in_group = half;
         for (long long q = half; q < all && wait.alive; q += 2, in_group += 2) {
             for (; in_group >= group; in_group -= group) before++;
-            if (!late)
+            if (!late && !amid)
                 while (taken < before && wait.alive) take_out(taken++);
             if (!wait.step(b.s_full, q)) break;
+            if (amid)
+                while (taken < before && wait.alive) take_out(taken++);
             tensor_after_sync();
             const u32 s = lanes + ((int)q & (p.s_buffers - 1)) * Columns::WIDE + W * part;
             unsigned char* a = smem + at.at_a + ((int)q & (p.a_buffers - 1)) * (Smem::A + Smem::ACT);

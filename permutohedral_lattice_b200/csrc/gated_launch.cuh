@@ -22,30 +22,43 @@ static bool gated_plan(GatedArgs& p) {
     const int chunks = PASS == GATED_DW ? 1 : p.chunks;
     p.boxes = sizeof(T) == 2 && p.wide_x && (PASS == GATED_OUT || p.wide_grad);
     auto fits = [&]() {
-        // Two tiles of rows first (what feeds the rest), then the weights, then rows that leave together, and more of both where there is room.
-        const int io = PASS != GATED_DW && p.wide_out, several = std::min(2, chunks);
-        const int tries[][3] = {{2, chunks, 2 * io}, {2, chunks, io}, {2, several, 2 * io}, {2, several, io}, {2, several, 0}, {1, several, io}, {1, several, 0},
-                                {1, 1, io}, {1, 1, 0}};
-        for (const auto& one : tries)
-            for (int a : {2, 1}) {
-                p.x_buffers = one[0], p.w_buffers[0] = p.w_buffers[1] = one[1], p.io_buffers = one[2], p.a_buffers = a;
-                if (PASS == GATED_DW && a == 2) continue;   // (its second products take as long as its first: nothing waits for them)
-                if (GatedSmem<T, PASS, ROWS>(p).total > (int)GATED_SMEM) continue;
-                while (p.x_buffers >= 2 && p.x_buffers < 4) {
-                    p.x_buffers++;
-                    if (GatedSmem<T, PASS, ROWS>(p).total <= (int)GATED_SMEM) continue;
-                    p.x_buffers--;
-                    break;
-                }
-                return true;
+        // The weights of all chunks first, or of three: of a step's first products, of its second ones, and on their way; two tiles of rows, and rows
+        // that leave together; more of all where there is room.  (154 401 rows of 128 to 512 to 128 float16 channels: 109 us with two buffers of weights
+        // and rows that leave together, 119 with three and none.)
+        const int io = PASS != GATED_DW && p.wide_out, two = std::min(2, chunks), three = std::min(3, chunks);
+        const int tries[][4] = {{2, chunks, 2 * io, 2}, {2, chunks, io, 2}, {2, chunks, 2 * io, 1}, {2, chunks, io, 1}, {2, three, io, 2}, {2, three, io, 1},
+                                {2, three, 0, 1}, {1, chunks, io, 1}, {2, two, io, 2}, {2, two, io, 1}, {1, three, io, 2}, {1, three, io, 1}, {2, two, 0, 1},
+                                {1, two, io, 2}, {1, two, io, 1}, {1, two, 0, 1}, {1, 1, io, 1}, {1, 1, 0, 1}};
+        for (const auto& one : tries) {
+            p.x_buffers = one[0], p.w_buffers[0] = p.w_buffers[1] = one[1], p.io_buffers = one[2], p.a_buffers = one[3];
+            if (PASS == GATED_DW && p.a_buffers == 2) continue;   // (its second products take as long as its first: nothing waits for them)
+            if (GatedSmem<T, PASS, ROWS>(p).total > (int)GATED_SMEM) continue;
+            while (p.x_buffers >= 2 && p.x_buffers < 4) {
+                p.x_buffers++;
+                if (GatedSmem<T, PASS, ROWS>(p).total <= (int)GATED_SMEM) continue;
+                p.x_buffers--;
+                break;
             }
+            return true;
+        }
         return false;
     };
     auto columns = [&](int s, int d) {
         p.s_buffers = s, p.d_buffers = d;
         return GatedColumns<T, PASS>(p).total <= 512;
     };
-    return fits() && ((PASS != GATED_DW && columns(2, 2)) || columns(2, 1) || columns(1, 1));
+    // What changes a result's bits (rows of a tile, sums side by side) goes by sizes and biases, not by which gradients are wanted.
+    const int wanted = p.down_bias_wanted;
+    p.down_bias_wanted = PASS == GATED_DW;
+    p.stacked = 0;
+    const bool room = fits();
+    // float32: side by side as far as a product is wide, 256 columns, and as there is room
+    if (PASS == GATED_DW && sizeof(T) == 4 && 3 * p.kx <= 256) {
+        p.stacked = 1;
+        if (!columns(1, 1)) p.stacked = 0;
+    }
+    p.down_bias_wanted = wanted;
+    return room && ((PASS != GATED_DW && columns(2, 2)) || columns(2, 1) || columns(1, 1));
 }
 
 // A matrix of rows as the TMA takes it: boxes of 128 bytes by `box` rows, in shared memory as swizzled_at says.

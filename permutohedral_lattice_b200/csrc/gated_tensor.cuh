@@ -84,6 +84,17 @@ __device__ __forceinline__ void products(u32 d, u32 small, const Operand& a, con
         add = true;
     }
 }
+// The same with b's three terms side by side (as they lie behind one another in a tile whose columns are the operand's rows): three products in place
+// of six, whose first operands, which take as long to read as 64 columns to multiply, are read half as often.  What is n columns further on is a part in 2^8 of it.
+template <typename T>
+__device__ __forceinline__ void stacked_products(u32 d, const Operand& a, const Operand& b, int n, int steps, bool add) {
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+        const u32 shape = product_shape<T>(a, b, (3 - i) * n);
+#pragma unroll 2
+        for (int s = 0; s < steps; s++) tensor_product(d + i * n, a.at(s, i), b.at(s, 0), shape, add || i > 0 || s > 0);
+    }
+}
 __device__ __forceinline__ void tensor_commit(u64* bar) {   // the barrier's phase ends when all products asked for so far are done
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_address(bar)) : "memory");
 }
