@@ -39,6 +39,7 @@ struct GatedArgs {
     const void *x, *gate_weight, *up_weight, *down_weight, *gate_bias, *up_bias, *down_bias, *residual, *grad;
     int biased, boxes, wide_x, wide_grad, wide_out;   // wide: rows of whole 16 bytes on 16-byte boundaries; boxes: of 16-bit values, what is read
     int wide_dresidual, down_bias_wanted;             // (DX, DW)
+    int split;                       // (OUT, DX, floats) the sums of every other chunk apart: over more than 256 hidden channels too much would be cut
     int stacked;                     // (DW, floats) the terms of a product's second operand side by side: a sum for every order of magnitude
     unsigned char* packed;           // the weights, a chunk after another: Wd, Wg and Wu as tiles
     void *out, *dresidual;           // out: or dx
@@ -97,6 +98,7 @@ struct GatedColumns {
         d_all = SUMS * d_one;
         up_bias = p.kx, down = p.kp, down_bias = p.kp + C;
         up_part = down_part = bias_part = SUMS == 2 ? d_one : 0;
+        if (p.split) d_all = 3 * d_one;
         if (p.stacked) {
             const int biases = p.kp - p.kx + (p.down_bias_wanted ? 16 : 0);
             down = 3 * p.kx, up_bias = down + 3 * C, down_bias = up_bias + p.kp - p.kx;
@@ -107,7 +109,7 @@ struct GatedColumns {
     }
     // Where value c's first part is, how far the next, and how many.
     __device__ __forceinline__ int place(const GatedArgs& p, int c, int& part, int& parts) const {
-        part = up_part, parts = PASS == GATED_DW && p.stacked ? 3 : SUMS;
+        part = up_part, parts = p.stacked || p.split ? 3 : SUMS;
         if (PASS != GATED_DW || c < p.kx) return c;
         if (c >= p.kp && c < p.kp + C) {
             part = down_part;
@@ -653,8 +655,8 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                     const u32 shape = product_shape<T>(one, up, 2 * C);
                     for (int t = TERMS - 1; t >= 0; t--) tensor_product(s, one.first, up.at(p.kx / 16, t), shape, t < TERMS - 1);
                 }
-                products<T>(s, s, rows_over_columns(x + at.grad, p.kx), up, 2 * C, p.kx / 16, p.biased);
-                if constexpr (PASS != GATED_OUT) products<T>(s + 2 * C, s + 2 * C, rows_over_columns(x, p.np), over_columns(w0, C, p.np), C, p.np / 16, false);
+                products<T>(s, s, rows_over_columns(x + at.grad, p.kx), up, 2 * C, p.kx / 16, p.biased, p.biased);
+                if constexpr (PASS != GATED_OUT) products<T>(s + 2 * C, s + 2 * C, rows_over_columns(x, p.np), over_columns(w0, C, p.np), C, p.np / 16, false, false);
                 tensor_commit(&b.s_full[q & 1]);
                 wt.next(w.count), w2t.next(p.w_buffers[1]);
                 if (++c == chunks) {
@@ -682,11 +684,12 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                 const u32 x = shared_address(smem + at.at_x + xt.at * at.x), w1 = shared_address(w.buffers + wt.at * w.bytes);
                 const u32 a = shared_address(smem + at.at_a + ((int)q & (p.a_buffers - 1)) * (Smem::A + Smem::ACT));
                 const u32 d = tensor + col.d + dt.at * col.d_all;
-                const bool add = in_group > 0;
+                const bool add = in_group > 0, add_main = p.split ? in_group > 1 : add;
+                const u32 main = d + (p.split ? (in_group & 1) * col.up_part : 0), small = d + (p.split ? 2 : 1) * col.up_part;
                 if constexpr (PASS == GATED_OUT) {
-                    products<T>(d, d + col.up_part, over_columns(a, ROWS, C), over_rows(w1, C, p.np), p.np, C / 16, add);
+                    products<T>(main, small, over_columns(a, ROWS, C), over_rows(w1, C, p.np), p.np, C / 16, add_main, add);
                 } else if constexpr (PASS == GATED_DX) {
-                    products<T>(d, d + col.up_part, over_columns(a, ROWS, 2 * C), over_columns(w1, p.kp, 2 * C), p.kx, 2 * C / 16, add);
+                    products<T>(main, small, over_columns(a, ROWS, 2 * C), over_columns(w1, p.kp, 2 * C), p.kx, 2 * C / 16, add_main, add);
                 } else {
                     const Operand hidden = over_rows(a, ROWS, 2 * C), grad = rows_over_rows(x, p.np);
                     const Operand rows = rows_over_rows(x + at.grad, p.kx), act = over_rows(a + Smem::A, ROWS, C);
@@ -694,8 +697,8 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                         stacked_products<T>(d, hidden, rows, p.kx, ROWS / 16, add);
                         stacked_products<T>(d + col.down, grad, act, C, ROWS / 16, add);
                     } else {
-                        products<T>(d, d + col.up_part, hidden, rows, p.kx, ROWS / 16, add);
-                        products<T>(d + col.down, d + col.down + col.down_part, grad, act, C, ROWS / 16, add);
+                        products<T>(d, d + col.up_part, hidden, rows, p.kx, ROWS / 16, add, add);
+                        products<T>(d + col.down, d + col.down + col.down_part, grad, act, C, ROWS / 16, add, add);
                     }
                     // the biases': times ones (which have one term)
                     const Operand one = over_rows(shared_address(smem + at.at_ones), ROWS, 16);
@@ -750,7 +753,7 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                 if (Columns::SUMS == 2) tensor_load(low, from + part);
                 tensor_loaded();
                 if (Columns::SUMS == 2) {
-                    if (PASS == GATED_DW && parts == 3) {   // the smallest first
+                    if (parts == 3) {   // the smallest first
                         float third[16];
                         tensor_load(third, from + 2 * part);
                         tensor_loaded();

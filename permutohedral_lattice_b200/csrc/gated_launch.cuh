@@ -26,8 +26,8 @@ static bool gated_plan(GatedArgs& p) {
         // that leave together; more of all where there is room.  (154 401 rows of 128 to 512 to 128 float16 channels: 109 us with two buffers of weights
         // and rows that leave together, 119 with three and none.)
         const int io = PASS != GATED_DW && p.wide_out, two = std::min(2, chunks), three = std::min(3, chunks);
-        const int tries[][4] = {{2, chunks, 2 * io, 2}, {2, chunks, io, 2}, {2, chunks, 2 * io, 1}, {2, chunks, io, 1}, {2, three, io, 2}, {2, three, io, 1},
-                                {2, three, 0, 1}, {1, chunks, io, 1}, {2, two, io, 2}, {2, two, io, 1}, {1, three, io, 2}, {1, three, io, 1}, {2, two, 0, 1},
+        const int tries[][4] = {{2, chunks, 2 * io, 2}, {2, chunks, io, 2}, {2, chunks, 2 * io, 1}, {2, chunks, io, 1}, {1, chunks, io, 1}, {2, three, io, 2},
+                                {2, three, io, 1}, {2, three, 0, 1}, {2, two, io, 2}, {2, two, io, 1}, {1, three, io, 2}, {1, three, io, 1}, {2, two, 0, 1},
                                 {1, two, io, 2}, {1, two, io, 1}, {1, two, 0, 1}, {1, 1, io, 1}, {1, 1, 0, 1}};
         for (const auto& one : tries) {
             p.x_buffers = one[0], p.w_buffers[0] = p.w_buffers[1] = one[1], p.io_buffers = one[2], p.a_buffers = one[3];
@@ -50,7 +50,7 @@ static bool gated_plan(GatedArgs& p) {
     // What changes a result's bits (rows of a tile, sums side by side) goes by sizes and biases, not by which gradients are wanted.
     const int wanted = p.down_bias_wanted;
     p.down_bias_wanted = PASS == GATED_DW;
-    p.stacked = 0;
+    p.stacked = 0, p.split = sizeof(T) == 4 && PASS != GATED_DW && p.h > 256;
     const bool room = fits();
     // float32: side by side as far as a product is wide, 256 columns, and as there is room
     if (PASS == GATED_DW && sizeof(T) == 4 && 3 * p.kx <= 256) {
@@ -117,7 +117,7 @@ template <typename T>
 static int gated_of(GatedArgs& p, GatedPass pass, bool pack, cudaStream_t st) {
     p.chunks = (p.h + gated_chunk<T>() - 1) / gated_chunk<T>();
     p.splits = gated_splits(p.chunks, p.rows, num_sms());
-    p.drain = sizeof(T) == 4 ? 2 : 64;
+    p.drain = sizeof(T) == 4 ? 4 : 64;   // tiles: float32 sums of 512 rows are 7e-7 off, of 1024 1.3e-6, of 2048 2.5e-6 (and 1377, 1307, 1272 us a million of 32 to 128 to 32)
     if (pack) PL_TRY(pack_gated<T>(p, st));
     return pass == GATED_OUT ? launch_gated<T, GATED_OUT>(p, st) : pass == GATED_DX ? launch_gated<T, GATED_DX>(p, st) : launch_gated<T, GATED_DW>(p, st);
 }

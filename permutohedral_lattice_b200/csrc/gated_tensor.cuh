@@ -61,12 +61,12 @@ template <typename T>
 __device__ __forceinline__ u32 product_shape(const Operand& a, const Operand& b, int n) {   // 128 x n
     return 1u << 4 | Tensor<T>::FORMAT << 7 | Tensor<T>::FORMAT << 10 | a.transposed << 15 | b.transposed << 16 | (u32)(n / 8) << 17 | 8u << 24;
 }
-// d (+)= a b^T over 16 `steps` terms, 128 x n; small: where products with a term but the first go (may be d).  add: to what is there.
+// d (+)= a b^T over 16 `steps` terms, 128 x n; small: where products with a term but the first go (may be d).  add, add_small: to what is there.
 template <typename T>
-__device__ __forceinline__ void products(u32 d, u32 small, const Operand& a, const Operand& b, int n, int steps, bool add) {
+__device__ __forceinline__ void products(u32 d, u32 small, const Operand& a, const Operand& b, int n, int steps, bool add, bool add_small) {
     const u32 shape = product_shape<T>(a, b, n);
     if constexpr (Tensor<T>::TERMS == 3) {
-        bool more = add;
+        bool more = add_small;
 #pragma unroll
         for (int order = 2; order >= 1; order--)
 #pragma unroll
