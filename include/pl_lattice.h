@@ -369,20 +369,18 @@ int pl_unpack_activations(void* x, pl_packed packed, int64_t n, int dtype, void*
 typedef enum pl_norm_kind { PL_NORM_NONE = 0, PL_NORM_LAYER = 1, PL_NORM_RMS = 2 } pl_norm_kind;
 
 /* (x - mean) / sqrt(variance + eps) * weight + bias over a row's channels (layer), x / sqrt(mean of squares + eps) * weight + bias
- * (rms); weight and bias (device) of the channels, NULL: ones, zeros. */
+ * (rms); weight and bias of the channels, NULL: ones, zeros. */
 typedef struct pl_norm {
     int kind;   /* pl_norm_kind */
     float eps;  /* > 0 */
-    const void *weight, *bias;
 } pl_norm;
 
 /* Value i of a tensor (in memory's order) is dropped where word i % 4 of Philox4x32-10 (Salmon et al. 2011) of the counter
- * (i / 4, offset), 64 bits each, under `key` is below round(p 2^32); others are multiplied by 1 / (1 - p).  seed (device, NULL: the
- * two numbers here): key and offset as two 64-bit integers, read when the kernel runs.  p = 0: nothing is dropped. */
+ * (i / 4, offset), 64 bits each, under `key` is below round(p 2^32); others are multiplied by 1 / (1 - p).  The calls' `seed` (device, NULL:
+ * the two numbers here): key and offset as two 64-bit integers, read when the kernel runs.  p = 0: nothing is dropped. */
 typedef struct pl_dropout {
     double p;   /* 0 <= p < 1 */
     uint64_t key, offset;
-    const int64_t* seed;
 } pl_dropout;
 
 /* h = residual_scale * residual + gate * dropout(after(x)),  y = before(h).  Each part may be missing: a norm of kind
@@ -405,20 +403,22 @@ typedef struct pl_norm_gradients {
 
 /* y where and only where there is a norm before; h may then be NULL.  Statistics, and h on its way to y, are float.  Outputs overlap
  * neither each other nor the inputs.  No counterpart in the reference. */
-int pl_channel_norm(const pl_channel_norm_shape* m, void* h, void* y, const void* x, const void* residual, const void* gate, void* stream);
+int pl_channel_norm(const pl_channel_norm_shape* m, void* h, void* y, const void* x, const void* residual, const void* gate, const void* after_weight,
+                    const void* after_bias, const void* before_weight, const void* before_bias, const int64_t* seed, void* stream);
 
 /* Bytes of workspace that pl_channel_norm_backward takes.  No counterpart in the reference. */
 int pl_channel_norm_workspace_bytes(const pl_channel_norm_shape* m, size_t* bytes);
 
 /* The gradients of pl_channel_norm from those of h (NULL: zeros) and y (there where y was), with its own inputs; residual is read with a norm before
  * only.  Sums over rows in a fixed order: the same inputs give the same bits.  No counterpart in the reference. */
-int pl_channel_norm_backward(const pl_channel_norm_shape* m, const void* dh, const void* dy, const void* x, const void* residual,
-                             const void* gate, pl_norm_gradients d, void* workspace, size_t workspace_bytes, void* stream);
+int pl_channel_norm_backward(const pl_channel_norm_shape* m, const void* dh, const void* dy, const void* x, const void* residual, const void* gate,
+                             const void* after_weight, const void* after_bias, const void* before_weight, const int64_t* seed, pl_norm_gradients d,
+                             void* workspace, size_t workspace_bytes, void* stream);
 
 /* out = residual_scale * residual (NULL: nothing) + dropout(x) of n values; scaled (or NULL) = residual_scale * x: with the gradient of out
  * as x, out and scaled are those of x and residual.  Either may be NULL.  No counterpart in the reference. */
 int pl_channel_dropout(void* out, void* scaled, const void* x, const void* residual, int64_t n, int dtype, float residual_scale,
-                       const pl_dropout* dropout, void* stream);
+                       const pl_dropout* dropout, const int64_t* seed, void* stream);
 
 typedef enum pl_gate { PL_GATE_SILU = 0, PL_GATE_GELU = 1, PL_GATE_SIGMOID = 2, PL_GATE_RELU = 3 } pl_gate;   /* GELU: by erf */
 
@@ -434,10 +434,6 @@ typedef struct pl_gated_shape {
     float residual_scale;
 } pl_gated_shape;
 
-typedef struct pl_gated_weights {
-    const void *gate_weight, *up_weight, *down_weight, *gate_bias, *up_bias, *down_bias;
-} pl_gated_weights;
-
 /* The gradients to compute, NULL for those that are not wanted. */
 typedef struct pl_gated_gradients {
     void *x, *residual, *gate_weight, *up_weight, *down_weight, *gate_bias, *up_bias, *down_bias;
@@ -447,13 +443,15 @@ typedef struct pl_gated_gradients {
 int pl_gated_mix_workspace_bytes(const pl_gated_shape* m, int backward, size_t* bytes);
 
 /* out must not overlap the inputs.  No counterpart in the reference. */
-int pl_gated_mix(const pl_gated_shape* m, void* out, const void* x, const pl_gated_weights* w, const void* residual, void* workspace,
-                 size_t workspace_bytes, void* stream);
+int pl_gated_mix(const pl_gated_shape* m, void* out, const void* x, const void* gate_weight, const void* up_weight, const void* down_weight,
+                 const void* gate_bias, const void* up_bias, const void* down_bias, const void* residual, void* workspace, size_t workspace_bytes,
+                 void* stream);
 
 /* The gradients of pl_gated_mix from that of its output and its own inputs: the values in between are made again.  Sums over rows in a
  * fixed order: the same inputs give the same bits.  The outputs overlap neither each other nor the inputs.  No counterpart in the reference. */
-int pl_gated_mix_backward(const pl_gated_shape* m, const void* grad_out, const void* x, const pl_gated_weights* w, pl_gated_gradients d,
-                          void* workspace, size_t workspace_bytes, void* stream);
+int pl_gated_mix_backward(const pl_gated_shape* m, const void* grad_out, const void* x, const void* gate_weight, const void* up_weight,
+                          const void* down_weight, const void* gate_bias, const void* up_bias, pl_gated_gradients d, void* workspace,
+                          size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

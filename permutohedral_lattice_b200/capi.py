@@ -69,11 +69,11 @@ PL_NORM_NONE, PL_NORM_LAYER, PL_NORM_RMS = 0, 1, 2
 
 
 class PlNorm(ctypes.Structure):
-    _fields_ = [("kind", ctypes.c_int), ("eps", ctypes.c_float), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p)]
+    _fields_ = [("kind", ctypes.c_int), ("eps", ctypes.c_float)]
 
 
 class PlDropout(ctypes.Structure):
-    _fields_ = [("p", ctypes.c_double), ("key", ctypes.c_uint64), ("offset", ctypes.c_uint64), ("seed", ctypes.c_void_p)]
+    _fields_ = [("p", ctypes.c_double), ("key", ctypes.c_uint64), ("offset", ctypes.c_uint64)]
 
 
 class PlChannelNorm(ctypes.Structure):
@@ -93,10 +93,6 @@ PL_GATE_SILU, PL_GATE_GELU, PL_GATE_SIGMOID, PL_GATE_RELU = 0, 1, 2, 3
 class PlGated(ctypes.Structure):
     _fields_ = [("rows", ctypes.c_int64), ("k", ctypes.c_int), ("h", ctypes.c_int), ("n", ctypes.c_int), ("activation", ctypes.c_int),
                 ("dtype", ctypes.c_int), ("residual_scale", ctypes.c_float)]
-
-
-class PlGatedWeights(ctypes.Structure):
-    _fields_ = [(name, ctypes.c_void_p) for name in ("gate_weight", "up_weight", "down_weight", "gate_bias", "up_bias", "down_bias")]
 
 
 class PlGatedGradients(ctypes.Structure):
@@ -169,14 +165,14 @@ def lib():
         L.pl_pack_activations.argtypes = [PlPacked, vp, i64, i, i, vp]
         L.pl_unpack_activations.argtypes = [vp, PlPacked, i64, i, vp]
         norm = ctypes.POINTER(PlChannelNorm)
-        L.pl_channel_norm.argtypes = [norm, vp, vp, vp, vp, vp, vp]
+        L.pl_channel_norm.argtypes = [norm] + [vp] * 11
         L.pl_channel_norm_workspace_bytes.argtypes = [norm, ctypes.POINTER(ctypes.c_size_t)]
-        L.pl_channel_norm_backward.argtypes = [norm, vp, vp, vp, vp, vp, PlNormGradients, vp, ctypes.c_size_t, vp]
-        L.pl_channel_dropout.argtypes = [vp, vp, vp, vp, i64, i, f, ctypes.POINTER(PlDropout), vp]
-        gated, weights = ctypes.POINTER(PlGated), ctypes.POINTER(PlGatedWeights)
-        L.pl_gated_mix.argtypes = [gated, vp, vp, weights, vp, vp, ctypes.c_size_t, vp]
+        L.pl_channel_norm_backward.argtypes = [norm] + [vp] * 9 + [PlNormGradients, vp, ctypes.c_size_t, vp]
+        L.pl_channel_dropout.argtypes = [vp, vp, vp, vp, i64, i, f, ctypes.POINTER(PlDropout), vp, vp]
+        gated = ctypes.POINTER(PlGated)
+        L.pl_gated_mix.argtypes = [gated] + [vp] * 10 + [ctypes.c_size_t, vp]
         L.pl_gated_mix_workspace_bytes.argtypes = [gated, i, ctypes.POINTER(ctypes.c_size_t)]
-        L.pl_gated_mix_backward.argtypes = [gated, vp, vp, weights, PlGatedGradients, vp, ctypes.c_size_t, vp]
+        L.pl_gated_mix_backward.argtypes = [gated] + [vp] * 7 + [PlGatedGradients, vp, ctypes.c_size_t, vp]
         _lib = L
     return _lib
 

@@ -32,20 +32,6 @@ class Norm(NamedTuple):
     eps: float = 1e-5
 
 
-class _Shape(NamedTuple):
-    """What a call's C structure holds besides pointers."""
-    rows: int
-    channels: int
-    dtype: torch.dtype
-    vector_dtype: torch.dtype
-    gate_of_values: bool
-    residual_scale: float
-    after: Optional[tuple]       # kind, eps
-    before: Optional[tuple]
-    p: float
-    seed: Optional[tuple]        # key, offset, where they are numbers
-
-
 def _check_share(p, seed):
     """p as a number, and seed as a tensor or a pair of numbers below 2^64."""
     p = float(p)
@@ -66,8 +52,6 @@ def _check_share(p, seed):
 
 
 def _check_norm(norm, name, channels):
-    if norm is None:
-        return
     if not isinstance(norm, Norm):
         raise TypeError("%s must be a Norm" % name)
     if norm.kind not in _KINDS:
@@ -81,21 +65,27 @@ def _check_norm(norm, name, channels):
                 raise ValueError("%s.%s must be [channels]" % (name, part))
 
 
-def _check(x, residual, gate, after, before, dropout, seed):
-    """Returns the device, p, the seed, and the type of the channels' vectors."""
+def _named(residual, gate, after, before):
+    """The vectors of the channels among the arguments, with their names."""
+    found = [(place + part, t) for place, norm in (("after", after), ("before", before)) if norm is not None
+             for part, t in ((".weight", norm.weight), (".bias", norm.bias)) if t is not None]
+    return found if gate is None or gate.dim() > 1 else found + [("gate", gate)]
+
+
+def _check(x, residual, gate, after, before, p, seed):
+    """Returns the device and the type of the channels' vectors."""
     _check_values(x, "x")
     if x.dim() < 1:
         raise ValueError("x must be [*, channels]")
     channels = x.shape[-1]
     if not 1 <= channels <= MOST_NORM_CHANNELS:
         raise ValueError("x: 1 to %d channels are supported" % MOST_NORM_CHANNELS)
-    _check_norm(after, "after", channels)
-    _check_norm(before, "before", channels)
-    p, seed = _check_share(dropout, seed)
+    if after is not None:
+        _check_norm(after, "after", channels)
+    if before is not None:
+        _check_norm(before, "before", channels)
     if after is None and before is None and residual is None and gate is None and not p:
         raise ValueError("nothing to do: a norm, a residual, a gate or dropout is needed")
-    vectors = [(name, t) for name, norm in (("after", after), ("before", before)) if norm is not None
-               for name, t in ((name + ".weight", norm.weight), (name + ".bias", norm.bias)) if t is not None]
     if residual is not None:
         _check_values(residual, "residual", x.dtype)
         if residual.shape != x.shape:
@@ -104,53 +94,54 @@ def _check(x, residual, gate, after, before, dropout, seed):
         _check_values(gate, "gate")
         if gate.shape == x.shape and gate.dim() > 1:
             _check_values(gate, "gate", x.dtype)
-        elif tuple(gate.shape) == (channels,):
-            vectors.append(("gate", gate))
-        else:
+        elif tuple(gate.shape) != (channels,):
             raise ValueError("gate must be [channels], or of x's shape")
+    vectors = _named(residual, gate, after, before)
     vector_dtype = vectors[0][1].dtype if vectors else x.dtype
+    index = x.get_device()
+    same = index >= 0 and (residual is None or residual.get_device() == index) and (gate is None or gate.get_device() == index) and (
+        not p or not isinstance(seed, torch.Tensor) or seed.get_device() == index)
     for name, t in vectors:
-        if t.dtype not in (torch.float32, x.dtype):
-            raise TypeError("%s must be float32 or of x's dtype" % name)
-        if t.dtype != vector_dtype:
-            raise TypeError("%s must have dtype %s like the other vectors of the channels" % (name, vector_dtype))
-    on = [("x", x), ("residual", residual), ("gate", gate)] + vectors
-    if p and isinstance(seed, torch.Tensor):
-        on.append(("seed", seed))
-    return _check_device(on), p, seed, vector_dtype
+        if t.dtype is not vector_dtype or (vector_dtype is not x.dtype and vector_dtype is not torch.float32):
+            raise TypeError("%s must be float32 or of x's dtype, like all vectors of the channels" % name)
+        same = same and t.get_device() == index
+    if not same:
+        _check_device([("x", x), ("residual", residual), ("gate", gate)] + vectors + [("seed", seed if p and isinstance(seed, torch.Tensor) else None)])
+    return x.device, vector_dtype
 
 
-def _dropout_of(p, seed):
-    if isinstance(seed, torch.Tensor):
-        return capi.PlDropout(p, 0, 0, seed.data_ptr() if p else 0)
-    return capi.PlDropout(p, *(seed or (0, 0)), 0)
+@functools.lru_cache(maxsize=1024)
+def _dropout_of(p, key, offset):
+    return ctypes.byref(capi.PlDropout(p, key, offset))
 
 
-def _structure(s, weights, seed):
-    """weights: after's weight and bias, before's weight and bias."""
-    def norm(of, weight, bias):
-        return capi.PlNorm(_KINDS[of[0]], of[1], _ptr(weight), _ptr(bias)) if of else capi.PlNorm(capi.PL_NORM_NONE, 0.0, 0, 0)
+@functools.lru_cache(maxsize=1024)
+def _structure(rows, channels, dtype, vector_dtype, gate_of_values, residual_scale, after, after_eps, before, before_eps, p, key, offset):
+    """The C structure of a call, which the library only reads: sizes and numbers, no addresses."""
+    def norm(kind, eps):
+        return capi.PlNorm(_KINDS[kind], eps) if kind else capi.PlNorm(capi.PL_NORM_NONE, 0.0)
 
-    return ctypes.byref(capi.PlChannelNorm(
-        s.rows, s.channels, _DTYPES[s.dtype], _DTYPES[s.vector_dtype], int(s.gate_of_values), s.residual_scale,
-        norm(s.after, *weights[:2]), norm(s.before, *weights[2:]), _dropout_of(s.p, s.seed if seed is None else seed)))
-
-
-def _forward(device, s, x, residual, gate, weights, seed, wants_h):
-    h = torch.empty_like(x) if wants_h else None
-    y = torch.empty_like(x) if s.before else None
-    with _OnDevice(device):
-        capi.check(capi.lib().pl_channel_norm(_structure(s, weights, seed), _ptr(h), _ptr(y), x.data_ptr(), _ptr(residual), _ptr(gate),
-                                              _stream_handle(device)), "pl_channel_norm")
-    return h, y
+    return ctypes.byref(capi.PlChannelNorm(rows, channels, _DTYPES[dtype], _DTYPES[vector_dtype], int(gate_of_values), residual_scale,
+                                           norm(after, after_eps), norm(before, before_eps), capi.PlDropout(p, key, offset)))
 
 
 @functools.lru_cache(maxsize=256)
-def _workspace_bytes(s):
+def _workspace_bytes(channels):
     nbytes = ctypes.c_size_t(0)
-    capi.check(capi.lib().pl_channel_norm_workspace_bytes(_structure(s, (None,) * 4, None), ctypes.byref(nbytes)),
-               "pl_channel_norm_workspace_bytes")
+    m = _structure(0, channels, torch.float32, torch.float32, False, 1.0, None, 0.0, None, 0.0, 0.0, 0, 0)
+    capi.check(capi.lib().pl_channel_norm_workspace_bytes(m, ctypes.byref(nbytes)), "pl_channel_norm_workspace_bytes")
     return nbytes.value
+
+
+def _forward(device, m, wants_h, wants_y, seed, x, residual, gate, after_weight, after_bias, before_weight, before_bias):
+    h = torch.empty_like(x) if wants_h else None
+    y = torch.empty_like(x) if wants_y else None
+    with _OnDevice(device):
+        rc = capi.lib().pl_channel_norm(m, _ptr(h), _ptr(y), x.data_ptr(), _ptr(residual), _ptr(gate), _ptr(after_weight), _ptr(after_bias),
+                                        _ptr(before_weight), _ptr(before_bias), _ptr(seed), _stream_handle(device))
+        if rc != capi.PL_OK:
+            capi.check(rc, "pl_channel_norm")
+    return h, y
 
 
 # What _ChannelNorm takes gradients of, in its order.
@@ -159,25 +150,24 @@ _NAMES = ("x", "residual", "gate", "after_weight", "after_bias", "before_weight"
 
 class _ChannelNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, device, s, wants_h, seed, x, residual, gate, *weights):
-        h, y = _forward(device, s, x, residual, gate, weights, seed, wants_h)
+    def forward(ctx, device, m, has_after, wants_h, wants_y, seed, x, residual, gate, *weights):
+        h, y = _forward(device, m, wants_h, wants_y, seed, x, residual, gate, *weights)
         ctx.set_materialize_grads(False)
-        ctx.device, ctx.s, ctx.outputs = device, s, (wants_h, y is not None)
-        needs = dict(zip(_NAMES, ctx.needs_input_grad[4:]))
-        keep_x = s.after is not None or s.before is not None or needs["gate"]
-        ctx.save_for_backward(x if keep_x else None, residual if s.before else None, gate, seed, *weights)
-        return (h, y) if wants_h and y is not None else (y if h is None else h)
+        ctx.device, ctx.m, ctx.outputs = device, m, (wants_h, wants_y)
+        keep_x = has_after or wants_y or ctx.needs_input_grad[8]
+        ctx.save_for_backward(x if keep_x else None, residual if wants_y else None, gate, seed, *weights)
+        return (h, y) if wants_h and wants_y else (y if h is None else h)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
         x, residual, gate, seed, *weights = ctx.saved_tensors
-        s, device = ctx.s, ctx.device
-        needs = [name for name, wanted in zip(_NAMES, ctx.needs_input_grad[4:]) if wanted]
+        m, device = ctx.m, ctx.device
+        needs = [name for name, wanted in zip(_NAMES, ctx.needs_input_grad[6:]) if wanted]
         with_h, with_y = ctx.outputs
         dh, dy = grads if with_h and with_y else (grads[0], None) if with_h else (None, grads[0])
         if dh is None and dy is None:
-            return (None,) * (4 + len(_NAMES))
+            return (None,) * (6 + len(_NAMES))
         if with_y and dy is None:       # nobody used y
             dy = torch.zeros_like(dh)
         dh, dy = _contiguous(dh), _contiguous(dy)
@@ -186,16 +176,21 @@ class _ChannelNorm(torch.autograd.Function):
                   "before_weight": weights[2], "before_bias": weights[3]}
         made = {name: torch.empty(shapes[name].shape, dtype=shapes[name].dtype, device=device) for name in needs}
         with _OnDevice(device):
-            workspace = torch.empty(_workspace_bytes(s._replace(rows=0, p=0.0, seed=(0, 0))), dtype=torch.uint8, device=device)
+            workspace = torch.empty(_workspace_bytes(like.shape[-1]), dtype=torch.uint8, device=device)
             d = capi.PlNormGradients(**{name: t.data_ptr() for name, t in made.items()})
             capi.check(capi.lib().pl_channel_norm_backward(
-                _structure(s, weights, seed), _ptr(dh), _ptr(dy), _ptr(x), _ptr(residual), _ptr(gate), d, workspace.data_ptr(),
-                workspace.numel(), _stream_handle(device)), "pl_channel_norm_backward")
-        return (None,) * 4 + tuple(made.get(name) for name in _NAMES)
+                m, _ptr(dh), _ptr(dy), _ptr(x), _ptr(residual), _ptr(gate), _ptr(weights[0]), _ptr(weights[1]), _ptr(weights[2]), _ptr(seed),
+                d, workspace.data_ptr(), workspace.numel(), _stream_handle(device)), "pl_channel_norm_backward")
+        return (None,) * 6 + tuple(made.get(name) for name in _NAMES)
 
 
 def _follows(tensors):
-    return _watched_by_torch() or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
+    """Whether autograd, or something else that follows tensors, has to know of a call."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return _watched_by_torch()
 
 
 def channel_norm(x, residual=None, gate=None, after=None, before=None, residual_scale=1.0, dropout=0.0, seed=None):
@@ -213,47 +208,49 @@ def channel_norm(x, residual=None, gate=None, after=None, before=None, residual_
 
     Gradients' sums over rows have a fixed order.  A value that is not finite makes its row, and the gradients of the vectors, not
     finite.  In a CUDA graph: forward and backward together, on leaves made inside it."""
-    device, p, seed, vector_dtype = _check(x, residual, gate, after, before, dropout, seed)
+    p, seed = _check_share(dropout, seed)
+    device, vector_dtype = _check(x, residual, gate, after, before, p, seed)
     on_gpu = isinstance(seed, torch.Tensor)
+    key, offset = (0, 0) if on_gpu else seed
     channels = x.shape[-1]
-    of_values = gate is not None and gate.dim() > 1
-    shape = _Shape(x.numel() // channels, channels, x.dtype, vector_dtype, of_values, float(residual_scale),
-                   None if after is None else (after.kind, float(after.eps)), None if before is None else (before.kind, float(before.eps)),
-                   p, None if on_gpu else seed)
+    kind_a, eps_a, wa, ba = (None, 0.0, None, None) if after is None else (after.kind, float(after.eps), after.weight, after.bias)
+    kind_b, eps_b, wb, bb = (None, 0.0, None, None) if before is None else (before.kind, float(before.eps), before.weight, before.bias)
+    m = _structure(x.numel() // channels, channels, x.dtype, vector_dtype, gate is not None and gate.dim() > 1, float(residual_scale),
+                   kind_a, eps_a, kind_b, eps_b, p, key, offset)
     wants_h = before is None or after is not None or residual is not None or gate is not None or p > 0.0
-    weights = tuple(t for norm in (after, before) for t in ((None, None) if norm is None else (norm.weight, norm.bias)))
-    tensors = tuple(_contiguous(t) for t in (x, residual, gate) + weights)
+    tensors = (x.contiguous(), _contiguous(residual), _contiguous(gate), _contiguous(wa), _contiguous(ba), _contiguous(wb), _contiguous(bb))
     seed = seed.contiguous() if on_gpu and p else None
     if not _follows(tensors):
-        h, y = _forward(device, shape, *tensors[:3], tensors[3:], seed, wants_h)
+        h, y = _forward(device, m, wants_h, before is not None, seed, *tensors)
         return (h, y) if wants_h and y is not None else (y if h is None else h)
-    return _ChannelNorm.apply(device, shape, wants_h, seed, *tensors)
+    return _ChannelNorm.apply(device, m, after is not None, wants_h, before is not None, seed, *tensors)
 
 
-def _drop(device, x, residual, p, seed, residual_scale, wants_scaled):
+def _drop(device, x, residual, share, seed, residual_scale, wants_scaled):
     out = torch.empty_like(x)
     scaled = torch.empty_like(x) if wants_scaled else None
     with _OnDevice(device):
-        capi.check(capi.lib().pl_channel_dropout(out.data_ptr(), _ptr(scaled), x.data_ptr(), _ptr(residual), x.numel(), _DTYPES[x.dtype],
-                                                 residual_scale, ctypes.byref(_dropout_of(p, seed)), _stream_handle(device)),
-                   "pl_channel_dropout")
+        rc = capi.lib().pl_channel_dropout(out.data_ptr(), _ptr(scaled), x.data_ptr(), _ptr(residual), x.numel(), _DTYPES[x.dtype],
+                                           residual_scale, share, _ptr(seed), _stream_handle(device))
+        if rc != capi.PL_OK:
+            capi.check(rc, "pl_channel_dropout")
     return out, scaled
 
 
 class _ChannelDropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, device, p, numbers, residual_scale, seed, x, residual):
-        ctx.args = device, p, numbers, residual_scale
+    def forward(ctx, device, share, residual_scale, seed, x, residual):
+        ctx.args = device, share, residual_scale
         ctx.save_for_backward(seed)
-        return _drop(device, x, residual, p, numbers if seed is None else seed, residual_scale, False)[0]
+        return _drop(device, x, residual, share, seed, residual_scale, False)[0]
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         (seed,) = ctx.saved_tensors
-        device, p, numbers, residual_scale = ctx.args
-        dx, dresidual = _drop(device, grad.contiguous(), None, p, numbers if seed is None else seed, residual_scale, ctx.needs_input_grad[6])
-        return None, None, None, None, None, dx if ctx.needs_input_grad[5] else None, dresidual
+        device, share, residual_scale = ctx.args
+        dx, dresidual = _drop(device, grad.contiguous(), None, share, seed, residual_scale, ctx.needs_input_grad[5])
+        return None, None, None, None, dx if ctx.needs_input_grad[4] else None, dresidual
 
 
 def channel_dropout(x, p, seed, residual=None, residual_scale=1.0):
@@ -266,10 +263,12 @@ def channel_dropout(x, p, seed, residual=None, residual_scale=1.0):
         if residual.shape != x.shape:
             raise ValueError("residual must have x's shape")
     on_gpu = isinstance(seed, torch.Tensor)
-    device = _check_device((("x", x), ("residual", residual), ("seed", seed if on_gpu and p else None)))
-    x, residual = x.contiguous(), _contiguous(residual)
-    tensor = seed.contiguous() if on_gpu and p else None
-    numbers = (0, 0) if on_gpu else seed
+    tensor = seed if on_gpu and p else None
+    index = x.get_device()
+    if index < 0 or (residual is not None and residual.get_device() != index) or (tensor is not None and tensor.get_device() != index):
+        _check_device((("x", x), ("residual", residual), ("seed", tensor)))
+    share = _dropout_of(p, 0, 0) if on_gpu else _dropout_of(p, *seed)
+    x, residual, tensor = x.contiguous(), _contiguous(residual), _contiguous(tensor)
     if not _follows((x, residual)):
-        return _drop(device, x, residual, p, numbers if tensor is None else tensor, float(residual_scale), False)[0]
-    return _ChannelDropout.apply(device, p, numbers, float(residual_scale), tensor, x, residual)
+        return _drop(x.device, x, residual, share, tensor, float(residual_scale), False)[0]
+    return _ChannelDropout.apply(x.device, share, float(residual_scale), tensor, x, residual)

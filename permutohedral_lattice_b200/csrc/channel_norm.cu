@@ -16,24 +16,25 @@ static int check_norm(const pl_channel_norm_shape* m) {
     if (!(m->dropout.p >= 0.0 && m->dropout.p < 1.0)) return PL_INVALID_ARGUMENT;
     return m->channels > NORM_MOST ? PL_UNSUPPORTED_DIMS : PL_OK;
 }
-static Dropout dropout_of(const pl_dropout& d) {
+static Dropout dropout_of(const pl_dropout& d, const int64_t* seed) {
     Dropout r = {};
     r.threshold = (u32)std::min(d.p * 4294967296.0 + 0.5, 4294967295.0);
     r.scale = (float)(1.0 / (1.0 - d.p));
-    r.key = d.key, r.offset = d.offset, r.seed = reinterpret_cast<const long long*>(d.seed);
+    r.key = d.key, r.offset = d.offset, r.seed = reinterpret_cast<const long long*>(seed);
     return r;
 }
-static NormArgs norm_args(const pl_channel_norm_shape* m, const void* x, const void* residual, const void* gate) {
+static NormArgs norm_args(const pl_channel_norm_shape* m, const void* x, const void* residual, const void* gate, const void* after_weight,
+                          const void* after_bias, const void* before_weight, const void* before_bias, const int64_t* seed) {
     NormArgs a = {};
     a.rows = m->rows, a.c = m->channels;
     a.after = m->after.kind, a.before = m->before.kind;
     a.eps_after = m->after.eps, a.eps_before = m->before.eps, a.scale = m->residual_scale;
     a.x = x, a.residual = residual, a.gate = m->gate_of_values ? gate : nullptr;
-    if (a.after) a.vectors[NORM_WA] = m->after.weight, a.vectors[NORM_BA] = m->after.bias;
-    if (a.before) a.vectors[NORM_WB] = m->before.weight, a.vectors[NORM_BB] = m->before.bias;
+    if (a.after) a.vectors[NORM_WA] = after_weight, a.vectors[NORM_BA] = after_bias;
+    if (a.before) a.vectors[NORM_WB] = before_weight, a.vectors[NORM_BB] = before_bias;
     a.vectors[NORM_GATE] = m->gate_of_values ? nullptr : gate;
     a.vector_dtype = m->vector_dtype;
-    a.drop = dropout_of(m->dropout);
+    a.drop = dropout_of(m->dropout, seed);
     return a;
 }
 static int run_norm(NormArgs& a, int dtype, bool backward, cudaStream_t st) {
@@ -57,11 +58,12 @@ using namespace pl;
 
 extern "C" {
 
-int pl_channel_norm(const pl_channel_norm_shape* m, void* h, void* y, const void* x, const void* residual, const void* gate, void* stream) {
+int pl_channel_norm(const pl_channel_norm_shape* m, void* h, void* y, const void* x, const void* residual, const void* gate, const void* after_weight,
+                    const void* after_bias, const void* before_weight, const void* before_bias, const int64_t* seed, void* stream) {
     PL_TRY(check_norm(m));
     if (m->rows == 0) return PL_OK;
     if (!x || (!h && !y) || (y != nullptr) != (m->before.kind != PL_NORM_NONE)) return PL_INVALID_ARGUMENT;
-    NormArgs a = norm_args(m, x, residual, gate);
+    NormArgs a = norm_args(m, x, residual, gate, after_weight, after_bias, before_weight, before_bias, seed);
     a.h = h, a.y = y;
     return run_norm(a, m->dtype, false, (cudaStream_t)stream);
 }
@@ -73,8 +75,9 @@ int pl_channel_norm_workspace_bytes(const pl_channel_norm_shape* m, size_t* byte
     return PL_OK;
 }
 
-int pl_channel_norm_backward(const pl_channel_norm_shape* m, const void* dh, const void* dy, const void* x, const void* residual,
-                             const void* gate, pl_norm_gradients d, void* workspace, size_t workspace_bytes, void* stream) {
+int pl_channel_norm_backward(const pl_channel_norm_shape* m, const void* dh, const void* dy, const void* x, const void* residual, const void* gate,
+                             const void* after_weight, const void* after_bias, const void* before_weight, const int64_t* seed, pl_norm_gradients d,
+                             void* workspace, size_t workspace_bytes, void* stream) {
     size_t need = 0;
     PL_TRY(pl_channel_norm_workspace_bytes(m, &need));
     const cudaStream_t st = (cudaStream_t)stream;
@@ -91,7 +94,7 @@ int pl_channel_norm_backward(const pl_channel_norm_shape* m, const void* dh, con
     if (!x && (m->after.kind || m->before.kind || d.gate)) return PL_INVALID_ARGUMENT;
     if (!workspace || workspace_bytes < need) return PL_WORKSPACE_TOO_SMALL;
     if (!norm_aligned(workspace)) return PL_INVALID_ARGUMENT;
-    NormArgs a = norm_args(m, x, residual, gate);
+    NormArgs a = norm_args(m, x, residual, gate, after_weight, after_bias, before_weight, nullptr, seed);
     a.dh = dh, a.dy = dy, a.dx = d.x, a.dresidual = d.residual, a.dgate = values ? d.gate : nullptr;
     for (int v = 0; v < NORM_VECTORS; v++) a.wanted |= vectors[v] ? 1 << v : 0;
     if (a.wanted) a.shares = static_cast<float*>(workspace);
@@ -106,11 +109,11 @@ int pl_channel_norm_backward(const pl_channel_norm_shape* m, const void* dh, con
 }
 
 int pl_channel_dropout(void* out, void* scaled, const void* x, const void* residual, int64_t n, int dtype, float residual_scale,
-                       const pl_dropout* dropout, void* stream) {
+                       const pl_dropout* dropout, const int64_t* seed, void* stream) {
     if (n < 0 || dtype < PL_F32 || dtype > PL_BF16 || !dropout || !(dropout->p >= 0.0 && dropout->p < 1.0)) return PL_INVALID_ARGUMENT;
     if (n == 0) return PL_OK;
     if ((!out && !scaled) || !x) return PL_INVALID_ARGUMENT;
-    const DropArgs a = {n, x, residual, out, scaled, residual_scale, dropout_of(*dropout)};
+    const DropArgs a = {n, x, residual, out, scaled, residual_scale, dropout_of(*dropout, seed)};
     const cudaStream_t st = (cudaStream_t)stream;
     return dtype == PL_F32 ? launch_drop<float>(a, st) : dtype == PL_F16 ? launch_drop<__half>(a, st) : launch_drop<__nv_bfloat16>(a, st);
 }

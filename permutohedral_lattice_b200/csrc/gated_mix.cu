@@ -28,12 +28,13 @@ static int check_gated(const pl_gated_shape* m) {
 }
 static int chunk_of(const pl_gated_shape* m) { return m->dtype == PL_F32 ? gated_chunk<float>() : gated_chunk<__half>(); }
 static bool gated_aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
-static GatedArgs gated_args(const pl_gated_shape* m, const void* x, const pl_gated_weights* w) {
+static GatedArgs gated_args(const pl_gated_shape* m, const void* x, const void* gate_weight, const void* up_weight, const void* down_weight,
+                            const void* gate_bias, const void* up_bias) {
     GatedArgs p = {};
     p.rows = m->rows, p.k = m->k, p.h = m->h, p.n = m->n, p.activation = m->activation, p.scale = m->residual_scale;
     p.x = x;
-    p.gate_weight = w->gate_weight, p.up_weight = w->up_weight, p.down_weight = w->down_weight;
-    p.gate_bias = w->gate_bias, p.up_bias = w->up_bias, p.down_bias = w->down_bias;
+    p.gate_weight = gate_weight, p.up_weight = up_weight, p.down_weight = down_weight;
+    p.gate_bias = gate_bias, p.up_bias = up_bias;
     p.biased = p.gate_bias || p.up_bias;
     p.np = (p.n + 15) / 16 * 16;
     p.wide_x = p.k % 8 == 0 && gated_aligned(x) && p.rows < (1ll << 31) - 128;   // (a row's number is 31 bits for the TMA)
@@ -66,14 +67,16 @@ int pl_gated_mix_workspace_bytes(const pl_gated_shape* m, int backward, size_t* 
     return PL_OK;
 }
 
-int pl_gated_mix(const pl_gated_shape* m, void* out, const void* x, const pl_gated_weights* w, const void* residual, void* workspace,
-                 size_t workspace_bytes, void* stream) {
+int pl_gated_mix(const pl_gated_shape* m, void* out, const void* x, const void* gate_weight, const void* up_weight, const void* down_weight,
+                 const void* gate_bias, const void* up_bias, const void* down_bias, const void* residual, void* workspace, size_t workspace_bytes,
+                 void* stream) {
     PL_TRY(check_gated(m));
     if (m->rows == 0) return PL_OK;
-    if (!out || !x || !w || !w->gate_weight || !w->up_weight || !w->down_weight) return PL_INVALID_ARGUMENT;
+    if (!out || !x || !gate_weight || !up_weight || !down_weight) return PL_INVALID_ARGUMENT;
     if (!workspace || workspace_bytes < packed_bytes(m)) return PL_WORKSPACE_TOO_SMALL;
     if (!gated_aligned(workspace)) return PL_INVALID_ARGUMENT;
-    GatedArgs p = gated_args(m, x, w);
+    GatedArgs p = gated_args(m, x, gate_weight, up_weight, down_weight, gate_bias, up_bias);
+    p.down_bias = down_bias;
     set_columns(p);
     p.packed = static_cast<unsigned char*>(workspace);
     p.out = out, p.residual = residual;
@@ -81,8 +84,9 @@ int pl_gated_mix(const pl_gated_shape* m, void* out, const void* x, const pl_gat
     return run_gated(p, m->dtype, GATED_OUT, true, (cudaStream_t)stream);
 }
 
-int pl_gated_mix_backward(const pl_gated_shape* m, const void* grad_out, const void* x, const pl_gated_weights* w, pl_gated_gradients d,
-                          void* workspace, size_t workspace_bytes, void* stream) {
+int pl_gated_mix_backward(const pl_gated_shape* m, const void* grad_out, const void* x, const void* gate_weight, const void* up_weight,
+                          const void* down_weight, const void* gate_bias, const void* up_bias, pl_gated_gradients d, void* workspace,
+                          size_t workspace_bytes, void* stream) {
     size_t need = 0;
     PL_TRY(pl_gated_mix_workspace_bytes(m, 1, &need));
     const cudaStream_t st = (cudaStream_t)stream;
@@ -95,10 +99,10 @@ int pl_gated_mix_backward(const pl_gated_shape* m, const void* grad_out, const v
             if (a.to) PL_CUDA(cudaMemsetAsync(a.to, 0, size * a.count, st));
         return PL_OK;
     }
-    if (!grad_out || !x || !w || !w->gate_weight || !w->up_weight || !w->down_weight) return PL_INVALID_ARGUMENT;
+    if (!grad_out || !x || !gate_weight || !up_weight || !down_weight) return PL_INVALID_ARGUMENT;
     if (!workspace || workspace_bytes < need) return PL_WORKSPACE_TOO_SMALL;
     if (!gated_aligned(workspace)) return PL_INVALID_ARGUMENT;
-    GatedArgs p = gated_args(m, x, w);
+    GatedArgs p = gated_args(m, x, gate_weight, up_weight, down_weight, gate_bias, up_bias);
     p.grad = grad_out;
     p.wide_grad = p.n % 8 == 0 && gated_aligned(grad_out);
     p.biased = p.biased || d.gate_bias || d.up_bias;   // (the ones' column sums dg and du)
@@ -111,7 +115,7 @@ int pl_gated_mix_backward(const pl_gated_shape* m, const void* grad_out, const v
         PL_TRY(run_gated(p, m->dtype, GATED_DX, true, st));
     } else if (d.residual) {
         const pl_dropout none = {};
-        PL_TRY(pl_channel_dropout(nullptr, d.residual, grad_out, nullptr, m->rows * m->n, m->dtype, m->residual_scale, &none, stream));
+        PL_TRY(pl_channel_dropout(nullptr, d.residual, grad_out, nullptr, m->rows * m->n, m->dtype, m->residual_scale, &none, nullptr, stream));
     }
     if (!sums) return PL_OK;
     p.down_bias_wanted = d.down_bias != nullptr;

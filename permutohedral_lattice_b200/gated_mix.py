@@ -7,7 +7,6 @@ again from x.  The reference ships no such operator; the networks that give CRF-
 """
 import ctypes
 import functools
-from typing import NamedTuple
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -24,30 +23,16 @@ _WEIGHTS = ("gate_weight", "up_weight", "down_weight", "gate_bias", "up_bias", "
 _NAMES = ("x", "residual") + _WEIGHTS
 
 
-class _Shape(NamedTuple):
-    rows: int
-    k: int
-    h: int
-    n: int
-    activation: str
-    dtype: torch.dtype
-    residual_scale: float
-
-
 @functools.lru_cache(maxsize=1024)
-def _structure(s):
-    return ctypes.byref(capi.PlGated(s.rows, s.k, s.h, s.n, _ACTIVATIONS[s.activation], _DTYPES[s.dtype], s.residual_scale))
-
-
-@functools.lru_cache(maxsize=1024)
-def _workspace_bytes(s, backward):
+def _structure(rows, k, h, n, activation, dtype, residual_scale):
+    """The C structure of a call, which the library only reads, and the bytes of workspace that it takes, forward and backward."""
+    m = ctypes.byref(capi.PlGated(rows, k, h, n, _ACTIVATIONS[activation], _DTYPES[dtype], residual_scale))
     nbytes = ctypes.c_size_t(0)
-    capi.check(capi.lib().pl_gated_mix_workspace_bytes(_structure(s), backward, ctypes.byref(nbytes)), "pl_gated_mix_workspace_bytes")
-    return nbytes.value
-
-
-def _workspace(s, backward, device):
-    return torch.empty(_workspace_bytes(s, backward), dtype=torch.uint8, device=device)
+    sizes = []
+    for backward in (0, 1):
+        capi.check(capi.lib().pl_gated_mix_workspace_bytes(m, backward, ctypes.byref(nbytes)), "pl_gated_mix_workspace_bytes")
+        sizes.append(nbytes.value)
+    return m, sizes[0], sizes[1]
 
 
 def _check(x, residual, weights, activation):
@@ -79,25 +64,29 @@ def _check(x, residual, weights, activation):
         _check_values(residual, "residual", x.dtype)
         if tuple(residual.shape) != tuple(x.shape[:-1]) + (n,):
             raise ValueError("residual must have the output's shape")
-    device = _check_device((("x", x), ("residual", residual)) + tuple(zip(_WEIGHTS, weights)))
-    return device, h, n
+    index = x.get_device()
+    if index < 0 or (residual is not None and residual.get_device() != index) or any(w is not None and w.get_device() != index for w in weights):
+        _check_device((("x", x), ("residual", residual)) + tuple(zip(_WEIGHTS, weights)))
+    return h, n
 
 
-def _forward(device, s, x, residual, weights):
-    out = x.new_empty(x.shape[:-1] + (s.n,))
+def _forward(device, s, n, x, residual, gate, up, down, gate_bias, up_bias, down_bias):
+    out = x.new_empty(x.shape[:-1] + (n,))
     with _OnDevice(device):
-        workspace = _workspace(s, False, device)
-        capi.check(capi.lib().pl_gated_mix(_structure(s), out.data_ptr(), x.data_ptr(), ctypes.byref(capi.PlGatedWeights(*map(_ptr, weights))),
-                                           _ptr(residual), workspace.data_ptr(), workspace.numel(), _stream_handle(device)), "pl_gated_mix")
+        workspace = torch.empty(s[1], dtype=torch.uint8, device=device)
+        rc = capi.lib().pl_gated_mix(s[0], out.data_ptr(), x.data_ptr(), gate.data_ptr(), up.data_ptr(), down.data_ptr(), _ptr(gate_bias), _ptr(up_bias),
+                                     _ptr(down_bias), _ptr(residual), workspace.data_ptr(), s[1], _stream_handle(device))
+        if rc != capi.PL_OK:
+            capi.check(rc, "pl_gated_mix")
     return out
 
 
 class _GatedMix(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, device, s, x, residual, *weights):
+    def forward(ctx, device, s, n, x, residual, *weights):
         ctx.args = device, s
         ctx.save_for_backward(x, *weights)
-        return _forward(device, s, x, residual, weights)
+        return _forward(device, s, n, x, residual, *weights)
 
     @staticmethod
     @once_differentiable
@@ -107,14 +96,14 @@ class _GatedMix(torch.autograd.Function):
         grad = grad.contiguous()
         like = dict(zip(_NAMES, (x, grad, *weights)))
         made = {name: torch.empty(like[name].shape, dtype=x.dtype, device=device)
-                for name, wanted in zip(_NAMES, ctx.needs_input_grad[2:]) if wanted}
+                for name, wanted in zip(_NAMES, ctx.needs_input_grad[3:]) if wanted}
         with _OnDevice(device):
-            workspace = _workspace(s, True, device)
+            workspace = torch.empty(s[2], dtype=torch.uint8, device=device)
             capi.check(capi.lib().pl_gated_mix_backward(
-                _structure(s), grad.data_ptr(), x.data_ptr(), ctypes.byref(capi.PlGatedWeights(*map(_ptr, weights))),
-                capi.PlGatedGradients(**{name: t.data_ptr() for name, t in made.items()}), workspace.data_ptr(),
-                workspace.numel(), _stream_handle(device)), "pl_gated_mix_backward")
-        return (None, None) + tuple(made.get(name) for name in _NAMES)
+                s[0], grad.data_ptr(), x.data_ptr(), *map(_ptr, weights[:5]),
+                capi.PlGatedGradients(**{name: t.data_ptr() for name, t in made.items()}), workspace.data_ptr(), s[2], _stream_handle(device)),
+                "pl_gated_mix_backward")
+        return (None, None, None) + tuple(made.get(name) for name in _NAMES)
 
 
 def gated_mix(x, gate_weight, up_weight, down_weight, gate_bias=None, up_bias=None, down_bias=None, residual=None, activation="silu",
@@ -131,10 +120,11 @@ def gated_mix(x, gate_weight, up_weight, down_weight, gate_bias=None, up_bias=No
     they would be; the weights' gradients are then not finite.  In a CUDA graph: one ordinary call of the same sizes before the
     capture, forward and backward, which sets the kernels up; forward and backward together, on leaves made inside it."""
     weights = (gate_weight, up_weight, down_weight, gate_bias, up_bias, down_bias)
-    device, h, n = _check(x, residual, weights, activation)
+    h, n = _check(x, residual, weights, activation)
     k = x.shape[-1]
-    s = _Shape(x.numel() // k, k, h, n, activation, x.dtype, float(residual_scale))
-    tensors = tuple(_contiguous(t) for t in (x, residual) + weights)
+    s = _structure(x.numel() // k, k, h, n, activation, x.dtype, float(residual_scale))
+    tensors = (x.contiguous(), _contiguous(residual), gate_weight.contiguous(), up_weight.contiguous(), down_weight.contiguous(), _contiguous(gate_bias),
+               _contiguous(up_bias), _contiguous(down_bias))
     if not _follows(tensors):
-        return _forward(device, s, tensors[0], tensors[1], tensors[2:])
-    return _GatedMix.apply(device, s, *tensors)
+        return _forward(x.device, s, n, *tensors)
+    return _GatedMix.apply(x.device, s, n, *tensors)

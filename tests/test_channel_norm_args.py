@@ -55,21 +55,21 @@ def test_channel_dropout_refuses():
 
 def test_c_entries_refuse_before_any_launch():
     L = capi.lib()
-    none = capi.PlNorm(0, 0.0, 0, 0)
-    rms = capi.PlNorm(2, 1e-5, 0, 0)
+    none = capi.PlNorm(0, 0.0)
+    rms = capi.PlNorm(2, 1e-5)
 
     def shape(**kw):
         fields = dict(rows=4, channels=3, dtype=0, vector_dtype=0, gate_of_values=0, residual_scale=1.0, after=none, before=rms,
-                      dropout=capi.PlDropout(0.0, 0, 0, 0))
+                      dropout=capi.PlDropout(0.0, 0, 0))
         return ctypes.byref(capi.PlChannelNorm(**{**fields, **kw}))
 
     def forward(m, h=0, y=16, x=16):
-        return L.pl_channel_norm(m, h, y, x, 0, 0, 0)
+        return L.pl_channel_norm(m, h, y, x, 0, 0, 0, 0, 0, 0, 0, 0)
 
     assert forward(None) == capi.PL_INVALID_ARGUMENT
-    for bad in ({"rows": -1}, {"rows": (1 << 40) + 1}, {"channels": 0}, {"dtype": 3}, {"vector_dtype": 1}, {"after": capi.PlNorm(3, 1.0, 0, 0)},
-                {"before": capi.PlNorm(1, 0.0, 0, 0)}, {"before": capi.PlNorm(1, float("nan"), 0, 0)}, {"dropout": capi.PlDropout(1.0, 0, 0, 0)},
-                {"dropout": capi.PlDropout(float("nan"), 0, 0, 0)}):
+    for bad in ({"rows": -1}, {"rows": (1 << 40) + 1}, {"channels": 0}, {"dtype": 3}, {"vector_dtype": 1}, {"after": capi.PlNorm(3, 1.0)},
+                {"before": capi.PlNorm(1, 0.0)}, {"before": capi.PlNorm(1, float("nan"))}, {"dropout": capi.PlDropout(1.0, 0, 0)},
+                {"dropout": capi.PlDropout(float("nan"), 0, 0)}):
         assert forward(shape(**bad)) == capi.PL_INVALID_ARGUMENT, bad
     assert forward(shape(channels=513)) == capi.PL_UNSUPPORTED_DIMS
     assert forward(shape(), x=0) == capi.PL_INVALID_ARGUMENT
@@ -78,7 +78,7 @@ def test_c_entries_refuse_before_any_launch():
     assert forward(shape(rows=0), 0, 0, 0) == capi.PL_OK
 
     def back(m, dh=0, dy=16, x=16, d=None, ws=16, nbytes=1 << 30):
-        return L.pl_channel_norm_backward(m, dh, dy, x, 0, 0, capi.PlNormGradients(**(d or {"x": 16})), ws, nbytes, 0)
+        return L.pl_channel_norm_backward(m, dh, dy, x, 0, 0, 0, 0, 0, 0, capi.PlNormGradients(**(d or {"x": 16})), ws, nbytes, 0)
 
     assert back(shape(), dy=0) == capi.PL_INVALID_ARGUMENT
     assert back(shape(), dh=16, dy=0) == capi.PL_INVALID_ARGUMENT
@@ -88,12 +88,12 @@ def test_c_entries_refuse_before_any_launch():
     assert back(shape(), nbytes=0) == capi.PL_WORKSPACE_TOO_SMALL
     assert back(shape(), ws=0) == capi.PL_WORKSPACE_TOO_SMALL
     assert back(shape(), ws=20) == capi.PL_INVALID_ARGUMENT
-    p = ctypes.byref(capi.PlDropout(0.5, 0, 0, 0))
-    assert L.pl_channel_dropout(16, 0, 16, 0, -1, 0, 1.0, p, 0) == capi.PL_INVALID_ARGUMENT
-    assert L.pl_channel_dropout(16, 0, 16, 0, 4, 3, 1.0, p, 0) == capi.PL_INVALID_ARGUMENT
-    assert L.pl_channel_dropout(0, 0, 16, 0, 4, 0, 1.0, p, 0) == capi.PL_INVALID_ARGUMENT
-    assert L.pl_channel_dropout(16, 0, 16, 0, 4, 0, 1.0, None, 0) == capi.PL_INVALID_ARGUMENT
-    assert L.pl_channel_dropout(0, 0, 0, 0, 0, 0, 1.0, p, 0) == capi.PL_OK
+    p = ctypes.byref(capi.PlDropout(0.5, 0, 0))
+    assert L.pl_channel_dropout(16, 0, 16, 0, -1, 0, 1.0, p, 0, 0) == capi.PL_INVALID_ARGUMENT
+    assert L.pl_channel_dropout(16, 0, 16, 0, 4, 3, 1.0, p, 0, 0) == capi.PL_INVALID_ARGUMENT
+    assert L.pl_channel_dropout(0, 0, 16, 0, 4, 0, 1.0, p, 0, 0) == capi.PL_INVALID_ARGUMENT
+    assert L.pl_channel_dropout(16, 0, 16, 0, 4, 0, 1.0, None, 0, 0) == capi.PL_INVALID_ARGUMENT
+    assert L.pl_channel_dropout(0, 0, 0, 0, 0, 0, 1.0, p, 0, 0) == capi.PL_OK
 
 
 def test_the_reference_generator():

@@ -49,26 +49,24 @@ def test_c_entries_refuse_before_any_launch():
         fields = dict(rows=4, k=3, h=5, n=2, activation=0, dtype=0, residual_scale=1.0)
         return ctypes.byref(capi.PlGated(**{**fields, **kw}))
 
-    whole = capi.PlGatedWeights(16, 16, 16, 0, 0, 0)
-
-    def forward(m, out=16, x=16, w=whole, ws=16, nbytes=1 << 40):
-        return L.pl_gated_mix(m, out, x, None if w is None else ctypes.byref(w), 0, ws, nbytes, 0)
+    def forward(m, out=16, x=16, w=(16, 16, 16), ws=16, nbytes=1 << 40):
+        return L.pl_gated_mix(m, out, x, *w, 0, 0, 0, 0, ws, nbytes, 0)
 
     assert forward(None) == capi.PL_INVALID_ARGUMENT
     for bad in ({"rows": -1}, {"rows": (1 << 40) + 1}, {"k": 0}, {"h": 0}, {"n": 0}, {"activation": 4}, {"activation": -1}, {"dtype": 3}):
         assert forward(shape(**bad)) == capi.PL_INVALID_ARGUMENT, bad
     for bad in ({"k": 129}, {"h": 513}, {"n": 129}):
         assert forward(shape(**bad)) == capi.PL_UNSUPPORTED_DIMS, bad
-    for bad in ({"out": 0}, {"x": 0}, {"w": None}, {"w": capi.PlGatedWeights(16, 16, 0, 0, 0, 0)}):
+    for bad in ({"out": 0}, {"x": 0}, {"w": (0, 16, 16)}, {"w": (16, 16, 0)}):
         assert forward(shape(), **bad) == capi.PL_INVALID_ARGUMENT, bad
-    assert forward(shape(rows=0), 0, 0, None, 0, 0) == capi.PL_OK
+    assert forward(shape(rows=0), 0, 0, (0, 0, 0), 0, 0) == capi.PL_OK
     assert forward(shape(), ws=0) == capi.PL_WORKSPACE_TOO_SMALL
     assert forward(shape(), nbytes=100) == capi.PL_WORKSPACE_TOO_SMALL
     assert forward(shape(), ws=24) == capi.PL_INVALID_ARGUMENT
 
-    def back(m, grad=16, x=16, w=whole, d=None, ws=16, nbytes=1 << 40):
+    def back(m, grad=16, x=16, d=None, ws=16, nbytes=1 << 40):
         d = capi.PlGatedGradients(**({"gate_weight": 16} if d is None else d))
-        return L.pl_gated_mix_backward(m, grad, x, ctypes.byref(w), d, ws, nbytes, 0)
+        return L.pl_gated_mix_backward(m, grad, x, 16, 16, 16, 0, 0, d, ws, nbytes, 0)
 
     assert back(shape(), grad=0) == capi.PL_INVALID_ARGUMENT
     assert back(shape(), x=0) == capi.PL_INVALID_ARGUMENT
