@@ -170,16 +170,24 @@ __device__ __forceinline__ void gated_act(const float2 (&g)[4], float2 (&act)[4]
             }
         }
     } else if constexpr (ACT == PL_GATE_GELU) {
-        const float2 half = make_float2(0.5f, 0.5f);
+        // g Phi(g), Phi by Abramowitz and Stegun 7.1.26: with t = 1 / (1 + p |g|) and e = exp(-g^2 / 2), which the slope takes anyway, the smaller of Phi
+        // and 1 - Phi is e (a1 t + ... + a5 t^5) / 2, 7.5e-8 off at most.  (erff took as long as all the rest.)
+        auto both = [](float v) { return make_float2(v, v); };
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float2 z = mul2(g[i], make_float2(0.70710678118654752f, 0.70710678118654752f));
-            const float2 cdf = fma2(half, make_float2(erff(z.x), erff(z.y)), half);
+            const float2 q = mul2(mul2(g[i], g[i]), both(-0.72134752044448170f));
+            const float2 e = make_float2(exp2_approx(q.x), exp2_approx(q.y));
+            const float2 d = fma2(make_float2(fabsf(g[i].x), fabsf(g[i].y)), both(0.23164189f), one);
+            const float2 t = make_float2(__fdividef(1.f, d.x), __fdividef(1.f, d.y));
+            float2 p = fma2(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+            p = fma2(t, p, both(0.5f * 1.421413741f));
+            p = fma2(t, p, both(0.5f * -0.284496736f));
+            p = fma2(t, p, both(0.5f * 0.254829592f));
+            p = mul2(mul2(p, t), e);
+            const float2 rest = fma2(p, minus, one);
+            const float2 cdf = make_float2(g[i].x < 0.f ? p.x : rest.x, g[i].y < 0.f ? p.y : rest.y);
             act[i] = mul2(g[i], cdf);
-            if constexpr (SLOPE) {
-                const float2 q = mul2(mul2(g[i], g[i]), make_float2(-0.72134752044448170f, -0.72134752044448170f));
-                slope[i] = fma2(mul2(g[i], make_float2(0.3989422804014327f, 0.3989422804014327f)), make_float2(exp2_approx(q.x), exp2_approx(q.y)), cdf);
-            }
+            if constexpr (SLOPE) slope[i] = fma2(mul2(g[i], both(0.3989422804014327f)), e, cdf);
         }
     } else {
         auto relu = [](float v) { return v < 0.f ? 0.f : v; };
@@ -492,9 +500,9 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
     float* bias_s = reinterpret_cast<float*>(smem + 1024);   // of out
     const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     // The last of the loaders brings the residual and takes the output away, and takes dout to the residual's gradient.
-    const bool beside = p.io_buffers || (PASS == GATED_DX && p.dresidual);
+    const bool scales = PASS == GATED_DX && p.dresidual && p.boxes && p.wide_dresidual;   // by the first of them, from the tile of dout: another that reads it
+    const bool beside = p.io_buffers || (PASS == GATED_DX && p.dresidual && !scales);
     const int row_loaders = LOADERS - (beside ? 1 : 0);
-    const bool scales = PASS == GATED_DX && p.dresidual && p.boxes && p.wide_dresidual;   // from the tile of dout: another that reads it
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.x_buffers; i++) mbar_init(&b.x_full[i], p.boxes ? 1 : 32 * row_loaders), mbar_init(&b.x_free[i], scales ? 2 : 1);
         for (int i = 0; i < 2; i++) {
@@ -551,7 +559,7 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
             const int width = PASS == GATED_OUT ? p.n : p.k;
             const bool one = one_of_warp(), loads = PASS == GATED_OUT && p.residual;
             long long arrived = 0;      // tiles whose buffer has been given to the workers
-            Turn xt, out, given;
+            Turn out, given;
             auto give = [&]() {         // the next tile's, with its residual
                 u64* bar = &b.io_full[given.at];
                 unsigned char* io = smem + at.at_io + given.at * at.io;
@@ -568,19 +576,9 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                 while (arrived < min(mine, (long long)p.io_buffers)) give();
             for (long long t = 0; t < mine && wait.alive; t++) {
                 const long long row0 = (split + t * step) * ROWS;
-                if constexpr (PASS == GATED_DX) {
-                    const int valid = (int)min((long long)ROWS, p.rows - row0);
-                    T* to = static_cast<T*>(p.dresidual) + row0 * p.n;
-                    if (scales) {
-                        if (!wait.full(b.x_full, xt)) break;
-                        if constexpr (sizeof(T) == 2) scale_tile<T, ROWS>(to, smem + at.at_x + xt.at * at.x, valid, p.n / 8, p.scale);
-                        __syncwarp();
-                        if (one) mbar_arrive(&b.x_free[xt.at]);
-                        xt.next(p.x_buffers);
-                    } else if (p.dresidual) {
-                        scale_rows<T>(to, static_cast<const T*>(p.grad) + row0 * p.n, valid * p.n, p.scale, p.wide_dresidual);
-                    }
-                }
+                if (PASS == GATED_DX && p.dresidual && !scales)
+                    scale_rows<T>(static_cast<T*>(p.dresidual) + row0 * p.n, static_cast<const T*>(p.grad) + row0 * p.n,
+                                  (int)min((long long)ROWS, p.rows - row0) * p.n, p.scale, p.wide_dresidual);
                 if (p.io_buffers) {
                     if (!wait.full(b.io_done, out)) break;
                     if (one) {
@@ -601,20 +599,38 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                         Waits{&b.dead}.on(&b.io_full[i % p.io_buffers], (int)(i / p.io_buffers), true);
             }
         } else if (p.boxes) {
-            if (loader == 0 && one_of_warp()) {
-                Turn xt;
+            if (loader == 0) {
+                const bool one = one_of_warp();
+                Turn xt, st;
+                auto scale = [&](long long t) {
+                    if constexpr (sizeof(T) == 2) {
+                        if (!wait.full(b.x_full, st)) return;
+                        const long long row0 = (split + t * step) * ROWS;
+                        scale_tile<T, ROWS>(static_cast<T*>(p.dresidual) + row0 * p.n, smem + at.at_x + st.at * at.x, (int)min((long long)ROWS, p.rows - row0),
+                                            p.n / 8, p.scale);
+                        __syncwarp();
+                        if (one) mbar_arrive(&b.x_free[st.at]);
+                        st.next(p.x_buffers);
+                    }
+                };
+                const int behind = p.x_buffers >= 2 ? 1 : 0;      // a tile is scaled when the next one has been asked for
                 for (long long t = 0; t < mine; t++) {
                     const int row0 = (int)((split + t * step) * ROWS);
                     if (!wait.free(b.x_free, xt)) break;
-                    unsigned char* x = smem + at.at_x + xt.at * at.x;
-                    mbar_expect_tx(&b.x_full[xt.at], at.x);
-                    if (PASS != GATED_OUT)
-                        for (int c = 0; c < p.n; c += 64) box_load(x + c * ROWS * 2, &maps.grad, c, row0, &b.x_full[xt.at]);
-                    for (int c = 0; c < p.k; c += 64) box_load(x + at.grad + c * ROWS * 2, &maps.x, c, row0, &b.x_full[xt.at]);
+                    if (one) {
+                        unsigned char* x = smem + at.at_x + xt.at * at.x;
+                        mbar_expect_tx(&b.x_full[xt.at], at.x);
+                        if (PASS != GATED_OUT)
+                            for (int c = 0; c < p.n; c += 64) box_load(x + c * ROWS * 2, &maps.grad, c, row0, &b.x_full[xt.at]);
+                        for (int c = 0; c < p.k; c += 64) box_load(x + at.grad + c * ROWS * 2, &maps.x, c, row0, &b.x_full[xt.at]);
+                    }
+                    __syncwarp();
                     xt.next(p.x_buffers);
+                    if (scales && t >= behind) scale(t - behind);
                 }
+                if (scales && behind && mine > 0 && wait.alive) scale(mine - 1);
                 // nothing on its way when others have given up
-                if (b_dead(b))
+                if (one && b_dead(b))
                     for (int i = 0; i < p.x_buffers; i++) {
                         const int turns = xt.turns - (i >= xt.at ? 1 : 0);
                         if (turns >= 0) Waits{&b.dead}.on(&b.x_full[i], turns, true);

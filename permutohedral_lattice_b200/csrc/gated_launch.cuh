@@ -26,12 +26,12 @@ static bool gated_plan(GatedArgs& p) {
         // that leave together; more of all where there is room.  (154 401 rows of 128 to 512 to 128 float16 channels: 109 us with two buffers of weights
         // and rows that leave together, 119 with three and none.)
         const int io = PASS != GATED_DW && p.wide_out, two = std::min(2, chunks), three = std::min(3, chunks);
-        const int tries[][4] = {{2, chunks, 2 * io, 2}, {2, chunks, io, 2}, {2, chunks, 2 * io, 1}, {2, chunks, io, 1}, {1, chunks, io, 1}, {2, three, io, 2},
+        const int before = PASS == GATED_DX ? 0 : io;      // (its operands are twice as large: two of them are worth more)
+        const int tries[][4] = {{2, chunks, 2 * io, 2}, {2, chunks, io, 2}, {2, chunks, before, 2}, {2, chunks, 2 * io, 1}, {2, chunks, io, 1}, {1, chunks, io, 1}, {2, three, io, 2},
                                 {2, three, io, 1}, {2, three, 0, 1}, {2, two, io, 2}, {2, two, io, 1}, {1, three, io, 2}, {1, three, io, 1}, {2, two, 0, 1},
                                 {1, two, io, 2}, {1, two, io, 1}, {1, two, 0, 1}, {1, 1, io, 1}, {1, 1, 0, 1}};
         for (const auto& one : tries) {
             p.x_buffers = one[0], p.w_buffers[0] = p.w_buffers[1] = one[1], p.io_buffers = one[2], p.a_buffers = one[3];
-            if (PASS == GATED_DW && p.a_buffers == 2) continue;   // (its second products take as long as its first: nothing waits for them)
             if (GatedSmem<T, PASS, ROWS>(p).total > (int)GATED_SMEM) continue;
             while (p.x_buffers >= 2 && p.x_buffers < 4) {
                 p.x_buffers++;
