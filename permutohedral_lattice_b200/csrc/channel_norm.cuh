@@ -90,12 +90,24 @@ struct Piece {
 };
 
 // Rows in registers: E values a lane at most, piece i of lane l of a row the (l + i LANES)-th.
-template <typename T, bool WIDE, int E, int LANES>
+// PACKED: two elements an instruction (the gradients of 3.4 million rows of 21 floats 450 us without, 392 with; but 16 million rows' worth of 16-bit pieces
+// forward 178 without, 212 with, for what it takes to pair registers).
+template <typename T, bool WIDE, int E, int LANES, bool PACKED>
 struct RowLanes {
     using P = Piece<T, WIDE>;
     using Raw = typename P::Raw;
     static constexpr int V = P::V, N = E / V;
-    static_assert(E % V == 0);
+    static_assert(E % V == 0 && E % 2 == 0);
+    __device__ __forceinline__ static float2 mul(float2 a, float2 b) { return PACKED ? mul2(a, b) : make_float2(a.x * b.x, a.y * b.y); }
+    __device__ __forceinline__ static float2 add(float2 a, float2 b) { return PACKED ? add2(a, b) : make_float2(a.x + b.x, a.y + b.y); }
+    __device__ __forceinline__ static float2 fma(float2 a, float2 b, float2 c) { return PACKED ? fma2(a, b, c) : make_float2(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)); }
+    __device__ __forceinline__ static float2 two(const float (&v)[E], int e) { return make_float2(v[e], v[e + 1]); }
+    __device__ __forceinline__ static void set(float (&v)[E], int e, float2 q) { v[e] = q.x, v[e + 1] = q.y; }
+    template <typename F>
+    __device__ __forceinline__ static void each(F f) {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) f(e);
+    }
     int l, c, whole;                   // pieces that all lanes of a row have
     float per;                         // 1 / c
     bool tail, there;                  // whether this lane has the piece behind the whole ones; whether its row is
@@ -129,24 +141,20 @@ struct RowLanes {
             if (there && has(i)) P::store(p + i * LANES * V, v + i * V);
         }
     }
-    template <typename F>
-    __device__ __forceinline__ void each(F f) const {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-#pragma unroll
-            for (int j = 0; j < V; j++) f(i * V + j);
-        }
-    }
-    // f(element, the vector's value for it); a lane without a channel gets another channel's
+    // f(element, the vector's value for it) of pairs; a lane without a channel gets another channel's
     template <typename F>
     __device__ __forceinline__ void with(const float* vector, F f) const {
+        float w[E];
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            float w[V];
-            P::shared(w, vector + min(channel(i), c - V));
+        for (int i = 0; i < N; i++) P::shared(w + i * V, vector + min(channel(i), c - V));
 #pragma unroll
-            for (int j = 0; j < V; j++) f(i * V + j, w[j]);
-        }
+        for (int e = 0; e < E; e += 2) f(e, make_float2(w[e], w[e + 1]));
+    }
+    __device__ __forceinline__ void times(float (&v)[E], const float* vector) const {
+        with(vector, [&](int e, float2 w) { set(v, e, mul(two(v, e), w)); });
+    }
+    __device__ __forceinline__ void plus(float (&v)[E], const float* vector) const {
+        with(vector, [&](int e, float2 w) { set(v, e, add(two(v, e), w)); });
     }
     __device__ __forceinline__ float sum(float v) const {   // of the row's lanes, the same in all of them
 #pragma unroll
@@ -154,34 +162,41 @@ struct RowLanes {
             if (o < LANES) v += __shfl_xor_sync(~0u, v, o);
         return v;
     }
-    // f(element) summed over the row's channels
-    template <typename F>
-    __device__ __forceinline__ float sum_of(F f) const {
+    // a[e] b[e] (or a[e]) summed over the row's channels.  (What lanes without a channel hold is never summed nor stored.)
+    template <bool PRODUCT>
+    __device__ __forceinline__ float sum_of(const float (&a)[E], const float (&b)[E]) const {
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            float p = 0.f;
+            if constexpr (V == 1) {
+                s = has(i) ? (PRODUCT ? fmaf(a[i], b[i], s) : s + a[i]) : s;
+            } else {
+                float2 p = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int j = 0; j < V; j++) p += f(i * V + j);
-            s += has(i) ? p : 0.f;
+                for (int e = i * V; e < i * V + V; e += 2) p = PRODUCT ? fma(two(a, e), two(b, e), p) : add(p, two(a, e));
+                s += has(i) ? p.x + p.y : 0.f;
+            }
         }
         return sum(s);
     }
-    // v to its normed form without weight and bias; returns the reciprocal deviation.  (What lanes without a channel hold is never summed nor stored.)
+    // v to its normed form without weight and bias; returns the reciprocal deviation.
     __device__ __forceinline__ float normalise(float (&v)[E], int kind, float eps) const {
         if (kind == PL_NORM_LAYER) {
-            const float mean = sum_of([&](int e) { return v[e]; }) * per;
-            each([&](int e) { v[e] -= mean; });
+            const float mean = sum_of<false>(v, v) * per;
+            each([&](int e) { set(v, e, add(two(v, e), make_float2(-mean, -mean))); });
         }
-        const float rstd = rsqrtf(fmaf(sum_of([&](int e) { return v[e] * v[e]; }), per, eps));
-        each([&](int e) { v[e] *= rstd; });
+        const float rstd = rsqrtf(fmaf(sum_of<true>(v, v), per, eps));
+        each([&](int e) { set(v, e, mul(two(v, e), make_float2(rstd, rstd))); });
         return rstd;
     }
-    // d, the gradient of the normed form, to that of what went in
+    // d, the gradient of the normed form, to that of what went in: rstd (d - mean(d) - hat mean(d hat))
     __device__ __forceinline__ void back(float (&d)[E], const float (&hat)[E], float rstd, int kind) const {
-        const float q = sum_of([&](int e) { return d[e] * hat[e]; }) * per;
-        const float s = kind == PL_NORM_LAYER ? sum_of([&](int e) { return d[e]; }) * per : 0.f;
-        each([&](int e) { d[e] = rstd * (d[e] - s - hat[e] * q); });
+        const float q = -sum_of<true>(d, hat) * per;
+        if (kind == PL_NORM_LAYER) {
+            const float s = -sum_of<false>(d, d) * per;
+            each([&](int e) { set(d, e, add(two(d, e), make_float2(s, s))); });
+        }
+        each([&](int e) { set(d, e, mul(fma(two(hat, e), make_float2(q, q), two(d, e)), make_float2(rstd, rstd))); });
     }
     // mask[e]: all ones where element e stays, else zero.  Values are counted through the whole tensor.  Single values: the words of the warp's
     // rows, which follow one another, by way of shared memory (a word for every value by its own lane would make each four times).
@@ -209,7 +224,10 @@ struct RowLanes {
         }
     }
     __device__ __forceinline__ void drop(float (&v)[E], const u32 (&mask)[E], float scale) const {   // what is dropped is zero, whatever it was
-        each([&](int e) { v[e] = __uint_as_float(__float_as_uint(v[e] * scale) & mask[e]); });
+        each([&](int e) {
+            const float2 q = mul(two(v, e), make_float2(scale, scale));
+            v[e] = __uint_as_float(__float_as_uint(q.x) & mask[e]), v[e + 1] = __uint_as_float(__float_as_uint(q.y) & mask[e + 1]);
+        });
     }
 };
 // Quads of words that the rows of a warp may need: 32 E values at most, not begun at a quad's first one.
@@ -222,14 +240,14 @@ __device__ __forceinline__ void norm_vectors_to(float* vectors_s, const NormArgs
     __syncthreads();
 }
 
-template <typename T, bool WIDE, int E, int LANES>
-__global__ void __launch_bounds__(NORM_THREADS) norm_forward(const __grid_constant__ NormArgs a) {
+// CTAs of an SM: where nothing is dropped four of 16-bit rows (2 470 000 x 256: 227 us with three, 202), with the generator's keys three.
+template <typename T, bool WIDE, int E, int LANES, bool DROPS>
+__global__ void __launch_bounds__(NORM_THREADS, E > 8 ? 2 : WIDE && sizeof(T) == 2 && !DROPS ? 4 : 1) norm_forward(const __grid_constant__ NormArgs a) {
     __shared__ __align__(16) float vectors_s[NORM_VECTORS * NORM_MOST];
-    __shared__ uint4 words_s[WIDE ? 1 : NORM_WARPS * norm_words(E)];
+    __shared__ uint4 words_s[WIDE || !DROPS ? 1 : NORM_WARPS * norm_words(E)];
     norm_vectors_to(vectors_s, a);
-    using Row = RowLanes<T, WIDE, E, LANES>;
+    using Row = RowLanes<T, WIDE, E, LANES, !(WIDE && sizeof(T) == 2)>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool drops = a.drop.threshold != 0;
     const Philox random(a.drop);
     Row r(a);
     const int per_warp = 32 / LANES, own = lane / LANES;
@@ -253,22 +271,22 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_forward(const __grid_consta
         r.at(r0 + own, a.rows);
         if (a.after) {
             r.normalise(v, a.after, a.eps_after);
-            if (a.vectors[NORM_WA]) r.with(vectors_s + NORM_WA * NORM_MOST, [&](int e, float w) { v[e] *= w; });
-            if (a.vectors[NORM_BA]) r.with(vectors_s + NORM_BA * NORM_MOST, [&](int e, float w) { v[e] += w; });
+            if (a.vectors[NORM_WA]) r.times(v, vectors_s + NORM_WA * NORM_MOST);
+            if (a.vectors[NORM_BA]) r.plus(v, vectors_s + NORM_BA * NORM_MOST);
         }
-        if (drops) {
+        if constexpr (DROPS) {
             u32 mask[E];
             r.kept(mask, random, a.drop.threshold, r0 * a.c, words_s + (WIDE ? 0 : warp * norm_words(E)));
             r.drop(v, mask, a.drop.scale);
         }
-        if (a.gate) r.each([&](int e) { v[e] *= gate[e]; });
-        else if (a.vectors[NORM_GATE]) r.with(vectors_s + NORM_GATE * NORM_MOST, [&](int e, float w) { v[e] *= w; });
-        if (a.residual) r.each([&](int e) { v[e] = fmaf(a.scale, residual[e], v[e]); });
+        if (a.gate) r.each([&](int e) { r.set(v, e, r.mul(r.two(v, e), r.two(gate, e))); });
+        else if (a.vectors[NORM_GATE]) r.times(v, vectors_s + NORM_GATE * NORM_MOST);
+        if (a.residual) r.each([&](int e) { r.set(v, e, r.fma(make_float2(a.scale, a.scale), r.two(residual, e), r.two(v, e))); });
         if (a.h) r.store(a.h, v);
         if (a.before) {
             r.normalise(v, a.before, a.eps_before);
-            if (a.vectors[NORM_WB]) r.with(vectors_s + NORM_WB * NORM_MOST, [&](int e, float w) { v[e] *= w; });
-            if (a.vectors[NORM_BB]) r.with(vectors_s + NORM_BB * NORM_MOST, [&](int e, float w) { v[e] += w; });
+            if (a.vectors[NORM_WB]) r.times(v, vectors_s + NORM_WB * NORM_MOST);
+            if (a.vectors[NORM_BB]) r.plus(v, vectors_s + NORM_BB * NORM_MOST);
             r.store(a.y, v);
         }
     }
@@ -279,7 +297,7 @@ __global__ void __launch_bounds__(NORM_THREADS, E <= 8 ? 2 : 1) norm_backward(co
     __shared__ __align__(16) float vectors_s[NORM_VECTORS * NORM_MOST];
     __shared__ uint4 words_s[WIDE ? 1 : NORM_WARPS * norm_words(E)];
     norm_vectors_to(vectors_s, a);
-    using Row = RowLanes<T, WIDE, E, LANES>;
+    using Row = RowLanes<T, WIDE, E, LANES, true>;
     constexpr bool AHEAD = WIDE && sizeof(T) == 2 && E <= 8;   // room for the next rows as they come
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool drops = a.drop.threshold != 0;
@@ -307,17 +325,17 @@ __global__ void __launch_bounds__(NORM_THREADS, E <= 8 ? 2 : 1) norm_backward(co
         if (!AHEAD) fetch(r0);
         float x[E], h[E], gate[E], d[E], dy[E], rstd = 0.f;
         if (a.x) r.values(x, raw_x);
-        else r.each([&](int e) { x[e] = 0.f; });
+        else r.each([&](int e) { x[e] = x[e + 1] = 0.f; });
         if (a.dh) r.values(d, raw_dh);
-        else r.each([&](int e) { d[e] = 0.f; });
+        else r.each([&](int e) { d[e] = d[e + 1] = 0.f; });
         if constexpr (BEFORE) {
             if (a.residual) r.values(h, raw_residual);
-            else r.each([&](int e) { h[e] = 0.f; });
+            else r.each([&](int e) { h[e] = h[e + 1] = 0.f; });
             r.values(dy, raw_dy);
         }
         if (a.gate) r.values(gate, raw_gate);
-        else if (a.vectors[NORM_GATE]) r.with(vectors_s + NORM_GATE * NORM_MOST, [&](int e, float w) { gate[e] = w; });
-        else r.each([&](int e) { gate[e] = 1.f; });
+        else if (a.vectors[NORM_GATE]) r.with(vectors_s + NORM_GATE * NORM_MOST, [&](int e, float2 w) { r.set(gate, e, w); });
+        else r.each([&](int e) { gate[e] = gate[e + 1] = 1.f; });
         if (AHEAD) {
             fetch(r0 + step);
             r.at(r0 + own, a.rows);
@@ -326,47 +344,39 @@ __global__ void __launch_bounds__(NORM_THREADS, E <= 8 ? 2 : 1) norm_backward(co
         if (drops) r.kept(mask, random, a.drop.threshold, r0 * a.c, words_s + (WIDE ? 0 : warp * norm_words(E)));
         if constexpr (AFTER) rstd = r.normalise(x, a.after, a.eps_after);   // x is x^ from here on
         float v[E];
-        r.each([&](int e) { v[e] = x[e]; });
+        r.each([&](int e) { r.set(v, e, r.two(x, e)); });
         if constexpr (AFTER) {
-            if (a.vectors[NORM_WA]) r.with(vectors_s + NORM_WA * NORM_MOST, [&](int e, float w) { v[e] *= w; });
-            if (a.vectors[NORM_BA]) r.with(vectors_s + NORM_BA * NORM_MOST, [&](int e, float w) { v[e] += w; });
+            if (a.vectors[NORM_WA]) r.times(v, vectors_s + NORM_WA * NORM_MOST);
+            if (a.vectors[NORM_BA]) r.plus(v, vectors_s + NORM_BA * NORM_MOST);
         }
         if (drops) r.drop(v, mask, a.drop.scale);
         if constexpr (BEFORE) {
-            r.each([&](int e) { h[e] = fmaf(a.scale, h[e], v[e] * gate[e]); });
+            r.each([&](int e) { r.set(h, e, r.fma(make_float2(a.scale, a.scale), r.two(h, e), r.mul(r.two(v, e), r.two(gate, e)))); });
             const float rstd_h = r.normalise(h, a.before, a.eps_before);
-            if (a.shares) {
-                r.each([&](int e) {
-                    sum_wb[e] = fmaf(dy[e], h[e], sum_wb[e]);
-                    sum_bb[e] += dy[e];
-                });
-            }
-            if (a.vectors[NORM_WB]) r.with(vectors_s + NORM_WB * NORM_MOST, [&](int e, float w) { dy[e] *= w; });
+            if (a.wanted >> NORM_WB & 1) r.each([&](int e) { r.set(sum_wb, e, r.fma(r.two(dy, e), r.two(h, e), r.two(sum_wb, e))); });
+            if (a.wanted >> NORM_BB & 1) r.each([&](int e) { r.set(sum_bb, e, r.add(r.two(sum_bb, e), r.two(dy, e))); });
+            if (a.vectors[NORM_WB]) r.times(dy, vectors_s + NORM_WB * NORM_MOST);
             r.back(dy, h, rstd_h, a.before);
-            r.each([&](int e) { d[e] += dy[e]; });
+            r.each([&](int e) { r.set(d, e, r.add(r.two(d, e), r.two(dy, e))); });
         }
         if (a.dresidual) {
             float t[E];
-            r.each([&](int e) { t[e] = a.scale * d[e]; });
+            r.each([&](int e) { r.set(t, e, r.mul(make_float2(a.scale, a.scale), r.two(d, e))); });
             r.store(a.dresidual, t);
         }
         if (a.dgate) {
             float t[E];
-            r.each([&](int e) { t[e] = d[e] * v[e]; });
+            r.each([&](int e) { r.set(t, e, r.mul(r.two(d, e), r.two(v, e))); });
             r.store(a.dgate, t);
-        } else if (a.shares) {
-            r.each([&](int e) { sum_gate[e] = fmaf(d[e], v[e], sum_gate[e]); });
+        } else if (a.wanted >> NORM_GATE & 1) {
+            r.each([&](int e) { r.set(sum_gate, e, r.fma(r.two(d, e), r.two(v, e), r.two(sum_gate, e))); });
         }
-        r.each([&](int e) { d[e] *= gate[e]; });
+        if (a.gate || a.vectors[NORM_GATE]) r.each([&](int e) { r.set(d, e, r.mul(r.two(d, e), r.two(gate, e))); });
         if (drops) r.drop(d, mask, a.drop.scale);
         if constexpr (AFTER) {
-            if (a.shares) {
-                r.each([&](int e) {
-                    sum_wa[e] = fmaf(d[e], x[e], sum_wa[e]);
-                    sum_ba[e] += d[e];
-                });
-            }
-            if (a.vectors[NORM_WA]) r.with(vectors_s + NORM_WA * NORM_MOST, [&](int e, float w) { d[e] *= w; });
+            if (a.wanted >> NORM_WA & 1) r.each([&](int e) { r.set(sum_wa, e, r.fma(r.two(d, e), r.two(x, e), r.two(sum_wa, e))); });
+            if (a.wanted >> NORM_BA & 1) r.each([&](int e) { r.set(sum_ba, e, r.add(r.two(sum_ba, e), r.two(d, e))); });
+            if (a.vectors[NORM_WA]) r.times(d, vectors_s + NORM_WA * NORM_MOST);
             r.back(d, x, rstd, a.after);
         }
         if (a.dx) r.store(a.dx, d);

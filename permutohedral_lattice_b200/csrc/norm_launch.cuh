@@ -17,7 +17,8 @@ template <typename T, bool WIDE, int E, int LANES>
 static int launch_norm(NormArgs& a, bool backward, int ctas, cudaStream_t st) {
     const long long per_cta = (long long)NORM_WARPS * (32 / LANES), all = (a.rows + per_cta - 1) / per_cta;
     const unsigned grid = (unsigned)std::max(1ll, std::min(all, (long long)ctas));
-    if (!backward) norm_forward<T, WIDE, E, LANES><<<grid, NORM_THREADS, 0, st>>>(a);
+    if (!backward && a.drop.threshold) norm_forward<T, WIDE, E, LANES, true><<<grid, NORM_THREADS, 0, st>>>(a);
+    else if (!backward) norm_forward<T, WIDE, E, LANES, false><<<grid, NORM_THREADS, 0, st>>>(a);
     else if (a.after && a.before) norm_backward<T, WIDE, E, LANES, true, true><<<grid, NORM_THREADS, 0, st>>>(a);
     else if (a.after) norm_backward<T, WIDE, E, LANES, true, false><<<grid, NORM_THREADS, 0, st>>>(a);
     else if (a.before) norm_backward<T, WIDE, E, LANES, false, true><<<grid, NORM_THREADS, 0, st>>>(a);
