@@ -44,7 +44,8 @@ static int run_norm(NormArgs& a, int dtype, bool backward, cudaStream_t st) {
 template <typename T>
 static int launch_drop(const DropArgs& a, cudaStream_t st) {
     constexpr int V = Piece<T, true>::V;
-    const unsigned grid = (unsigned)std::max(1ll, std::min((a.n + 256 * V - 1) / (256 * V), (long long)num_sms() * 8));
+    const long long per = 256 * V * DROP_PIECES;
+    const unsigned grid = (unsigned)std::max(1ll, std::min((a.n + per - 1) / per, (long long)num_sms() * 8));
     if (norm_aligned(a.x) && norm_aligned(a.residual) && norm_aligned(a.out) && norm_aligned(a.scaled)) drop_values<T, true><<<grid, 256, 0, st>>>(a);
     else drop_values<T, false><<<grid, 256, 0, st>>>(a);
     PL_COUNT_LAUNCHES(1);

@@ -443,54 +443,70 @@ struct DropArgs {
     float scale;
     Dropout drop;
 };
+// Two pieces a thread at a time, both on their way before the first is worked on (88 million floats and a residual: 164 us, one 186, four 170; bfloat16 values take 112, bound by the generator, some 40 products and exclusive ors for four).
+constexpr int DROP_PIECES = 2;
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) drop_values(const __grid_constant__ DropArgs a) {
     using P = Piece<T, true>;
-    constexpr int V = P::V;
+    constexpr int V = P::V, U = DROP_PIECES;
     const Philox random(a.drop);
     const T *x = static_cast<const T*>(a.x), *residual = static_cast<const T*>(a.residual);
     T *out = static_cast<T*>(a.out), *scaled = static_cast<T*>(a.scaled);
-    const long long step = (long long)gridDim.x * 256 * V;
-    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * V; i < a.n; i += step) {
-        const int count = (int)min((long long)V, a.n - i);
-        const bool whole = WIDE && count == V;
-        float v[V], q[V];
-        if (whole) {
-            P::load(v, x + i);
-            if (residual) P::load(q, residual + i);
-        } else {
+    const long long step = (long long)gridDim.x * 256 * V * U;
+    for (long long i0 = (long long)blockIdx.x * 256 * V * U + threadIdx.x * V; i0 < a.n; i0 += step) {
+        uint4 raw[U], raw_residual[U];
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                v[j] = j < count ? to_float(x[i + j]) : 0.f;
-                if (residual) q[j] = j < count ? to_float(residual[i + j]) : 0.f;
+        for (int u = 0; u < U; u++) {
+            const long long i = i0 + u * 256 * V;
+            if (WIDE && i + V <= a.n) {
+                raw[u] = *reinterpret_cast<const uint4*>(x + i);
+                if (residual) raw_residual[u] = *reinterpret_cast<const uint4*>(residual + i);
             }
         }
-        if (scaled) {
-            float t[V];
 #pragma unroll
-            for (int j = 0; j < V; j++) t[j] = a.scale * v[j];
-            if (whole) P::store(scaled + i, t);
+        for (int u = 0; u < U; u++) {
+            const long long i = i0 + u * 256 * V;
+            if (i >= a.n) break;
+            const int count = (int)min((long long)V, a.n - i);
+            const bool whole = WIDE && count == V;
+            float v[V], q[V];
+            if (whole) {
+                P::values(v, raw[u]);
+                if (residual) P::values(q, raw_residual[u]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    v[j] = j < count ? to_float(x[i + j]) : 0.f;
+                    if (residual) q[j] = j < count ? to_float(residual[i + j]) : 0.f;
+                }
+            }
+            if (scaled) {
+                float t[V];
+#pragma unroll
+                for (int j = 0; j < V; j++) t[j] = a.scale * v[j];
+                if (whole) P::store(scaled + i, t);
+                else
+                    for (int j = 0; j < V; j++)
+                        if (j < count) scaled[i + j] = from_float<T>(t[j]);
+            }
+            if (!out) continue;
+#pragma unroll
+            for (int j = 0; j < V; j += 4) {
+                const uint4 w = random.words((u64)(i + j) >> 2);
+                v[j] = w.x >= a.drop.threshold ? v[j] * a.drop.scale : 0.f;
+                v[j + 1] = w.y >= a.drop.threshold ? v[j + 1] * a.drop.scale : 0.f;
+                v[j + 2] = w.z >= a.drop.threshold ? v[j + 2] * a.drop.scale : 0.f;
+                v[j + 3] = w.w >= a.drop.threshold ? v[j + 3] * a.drop.scale : 0.f;
+            }
+            if (residual) {
+#pragma unroll
+                for (int j = 0; j < V; j++) v[j] = fmaf(a.scale, q[j], v[j]);
+            }
+            if (whole) P::store(out + i, v);
             else
                 for (int j = 0; j < V; j++)
-                    if (j < count) scaled[i + j] = from_float<T>(t[j]);
+                    if (j < count) out[i + j] = from_float<T>(v[j]);
         }
-        if (!out) continue;
-#pragma unroll
-        for (int j = 0; j < V; j += 4) {
-            const uint4 w = random.words((u64)(i + j) >> 2);
-            v[j] = w.x >= a.drop.threshold ? v[j] * a.drop.scale : 0.f;
-            v[j + 1] = w.y >= a.drop.threshold ? v[j + 1] * a.drop.scale : 0.f;
-            v[j + 2] = w.z >= a.drop.threshold ? v[j + 2] * a.drop.scale : 0.f;
-            v[j + 3] = w.w >= a.drop.threshold ? v[j + 3] * a.drop.scale : 0.f;
-        }
-        if (residual) {
-#pragma unroll
-            for (int j = 0; j < V; j++) v[j] = fmaf(a.scale, q[j], v[j]);
-        }
-        if (whole) P::store(out + i, v);
-        else
-            for (int j = 0; j < V; j++)
-                if (j < count) out[i + j] = from_float<T>(v[j]);
     }
 }
 
