@@ -37,8 +37,9 @@ struct GatedArgs {
     int x_buffers, w_buffers[2], a_buffers, s_buffers, d_buffers, io_buffers, drain;
     float scale;
     const void *x, *gate_weight, *up_weight, *down_weight, *gate_bias, *up_bias, *down_bias, *residual, *grad;
-    int biased, boxes, wide_x, wide_grad, wide_out;   // wide: rows of whole 16 bytes on 16-byte boundaries; boxes: of 16-bit values, what is read
-    int wide_dresidual, down_bias_wanted;             // (DX, DW)
+    int biased, wide_x, wide_grad, wide_out;          // wide: rows of whole 16 bytes on 16-byte boundaries
+    int box_x, box_grad;                              // rows that the TMA brings: wide ones of 16-bit values
+    int wide_dresidual, down_bias_wanted;             // (DX: dout and dresidual begin on 16-byte boundaries; DW)
     int split;                       // (OUT, DX, floats) the sums of every other chunk apart: over more than 256 hidden channels too much would be cut
     int stacked;                     // (DW, floats) the terms of a product's second operand side by side: a sum for every order of magnitude
     unsigned char* packed;           // the weights, a chunk after another: Wd, Wg and Wu as tiles
@@ -200,8 +201,26 @@ __device__ __forceinline__ void gated_act(const float2 (&g)[4], float2 (&act)[4]
     }
 }
 
-// Rows of `width` values to a tile of `blocks` blocks of columns by some warps: `valid` rows, zeros behind and beside.  wide: read by 16 bytes.
-// Eight rows of four blocks a warp at a time: whole sectors of memory, all banks of shared memory.
+template <typename T>
+struct Piece16 {   // 16 bytes of values
+    static constexpr int V = 16 / sizeof(T);
+    __device__ __forceinline__ static void store(void* to, const float* v) {
+        uint4 q;
+        T* e = reinterpret_cast<T*>(&q);
+#pragma unroll
+        for (int i = 0; i < V; i++) e[i] = from_float<T>(v[i]);
+        *static_cast<uint4*>(to) = q;
+    }
+    __device__ __forceinline__ static void load(float* v, const void* from) {
+        const uint4 q = *static_cast<const uint4*>(from);
+        const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = to_float(e[i]);
+    }
+};
+// Rows of `width` values to a tile of `blocks` blocks of columns by some warps: `valid` rows, zeros behind and beside.  wide: read by 16 bytes (floats;
+// wide 16-bit rows come by the TMA).  Eight rows of four blocks a warp at a time: whole sectors of memory, all banks of shared memory.  (16-bit values
+// by words of 4 bytes, shifted where rows begin between them, took half as long again as one by one.)
 template <typename T, int ROWS>
 __device__ __forceinline__ void stage(unsigned char* to, int blocks, const T* src, int width, int valid, bool wide, int warp, int warps) {
     const int lane = threadIdx.x & 31, r8 = lane & 7, b0 = lane >> 3, plane = tile_bytes(ROWS, 8 * blocks);
@@ -299,23 +318,6 @@ struct Waits {
 };
 
 template <typename T>
-struct Piece16 {   // 16 bytes of values
-    static constexpr int V = 16 / sizeof(T);
-    __device__ __forceinline__ static void store(void* to, const float* v) {
-        uint4 q;
-        T* e = reinterpret_cast<T*>(&q);
-#pragma unroll
-        for (int i = 0; i < V; i++) e[i] = from_float<T>(v[i]);
-        *static_cast<uint4*>(to) = q;
-    }
-    __device__ __forceinline__ static void load(float* v, const void* from) {
-        const uint4 q = *static_cast<const uint4*>(from);
-        const T* e = reinterpret_cast<const T*>(&q);
-#pragma unroll
-        for (int i = 0; i < V; i++) v[i] = to_float(e[i]);
-    }
-};
-template <typename T>
 __device__ __forceinline__ void store16(T* to, const float (&v)[16], int left, bool wide) {
     constexpr int V = 16 / sizeof(T);
     if (wide) {
@@ -390,29 +392,27 @@ __device__ __forceinline__ void scale_tile(T* to, const unsigned char* tile, int
         Piece16<T>::store(to + 8 * i, v);
     }
 }
-// to = s from, `count` values, by a warp.
+// to = s from, `count` values, by a warp.  aligned: both begin on 16-byte boundaries, which tiles of contiguous rows do wherever the first one does.
 template <typename T>
-__device__ __forceinline__ void scale_rows(T* to, const T* from, int count, float s, bool wide) {
+__device__ __forceinline__ void scale_rows(T* to, const T* from, int count, float s, bool aligned) {
     constexpr int V = 16 / sizeof(T), U = 8;
-    const int lane = threadIdx.x & 31;
-    if (!wide) {
-        for (int i = lane; i < count; i += 32) to[i] = from_float<T>(s * to_float(from[i]));
-        return;
-    }
-    for (int i0 = V * lane; i0 < count; i0 += 32 * V * U) {
+    const int lane = threadIdx.x & 31, whole = aligned ? count / V * V : 0;
+    for (int i0 = V * lane; i0 < whole; i0 += 32 * V * U) {
         uint4 q[U];
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (i0 + 32 * V * u < count) q[u] = *reinterpret_cast<const uint4*>(from + i0 + 32 * V * u);
+            if (i0 + 32 * V * u < whole) q[u] = *reinterpret_cast<const uint4*>(from + i0 + 32 * V * u);
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (i0 + 32 * V * u < count) {
+            if (i0 + 32 * V * u < whole) {
                 T* e = reinterpret_cast<T*>(&q[u]);
 #pragma unroll
                 for (int i = 0; i < V; i++) e[i] = from_float<T>(s * to_float(e[i]));
                 *reinterpret_cast<uint4*>(to + i0 + 32 * V * u) = q[u];
             }
     }
+#pragma unroll 8
+    for (int i = whole + lane; i < count; i += 32) to[i] = from_float<T>(s * to_float(from[i]));
 }
 
 // Some hidden channels of a row: from g, u (and da) to what the second products take.
@@ -500,11 +500,12 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
     float* bias_s = reinterpret_cast<float*>(smem + 1024);   // of out
     const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     // The last of the loaders brings the residual and takes the output away, and takes dout to the residual's gradient.
-    const bool scales = PASS == GATED_DX && p.dresidual && p.boxes && p.wide_dresidual;   // by the first of them, from the tile of dout: another that reads it
+    const bool scales = PASS == GATED_DX && p.dresidual && p.box_x && p.box_grad && p.wide_dresidual;   // by the first of them, from the tile of dout: another that reads it
     const bool beside = p.io_buffers || (PASS == GATED_DX && p.dresidual && !scales);
     const int row_loaders = LOADERS - (beside ? 1 : 0);
+    const bool boxes = p.box_x || p.box_grad, staged_rows = !p.box_x || (PASS != GATED_OUT && !p.box_grad);
     if (threadIdx.x == 0) {
-        for (int i = 0; i < p.x_buffers; i++) mbar_init(&b.x_full[i], p.boxes ? 1 : 32 * row_loaders), mbar_init(&b.x_free[i], scales ? 2 : 1);
+        for (int i = 0; i < p.x_buffers; i++) mbar_init(&b.x_full[i], (boxes ? 1 : 0) + (staged_rows ? 32 * row_loaders : 0)), mbar_init(&b.x_free[i], scales ? 2 : 1);
         for (int i = 0; i < 2; i++) {
             mbar_init(&b.s_full[i], 1), mbar_init(&b.s_free[i], WORKERS / 2);
             mbar_init(&b.a_full[i], WORKERS / 2), mbar_init(&b.a_free[i], 1);
@@ -598,45 +599,8 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                     for (long long i = max(0ll, arrived - p.io_buffers); i < arrived; i++)
                         Waits{&b.dead}.on(&b.io_full[i % p.io_buffers], (int)(i / p.io_buffers), true);
             }
-        } else if (p.boxes) {
-            if (loader == 0) {
-                const bool one = one_of_warp();
-                Turn xt, st;
-                auto scale = [&](long long t) {
-                    if constexpr (sizeof(T) == 2) {
-                        if (!wait.full(b.x_full, st)) return;
-                        const long long row0 = (split + t * step) * ROWS;
-                        scale_tile<T, ROWS>(static_cast<T*>(p.dresidual) + row0 * p.n, smem + at.at_x + st.at * at.x, (int)min((long long)ROWS, p.rows - row0),
-                                            p.n / 8, p.scale);
-                        __syncwarp();
-                        if (one) mbar_arrive(&b.x_free[st.at]);
-                        st.next(p.x_buffers);
-                    }
-                };
-                const int behind = p.x_buffers >= 2 ? 1 : 0;      // a tile is scaled when the next one has been asked for
-                for (long long t = 0; t < mine; t++) {
-                    const int row0 = (int)((split + t * step) * ROWS);
-                    if (!wait.free(b.x_free, xt)) break;
-                    if (one) {
-                        unsigned char* x = smem + at.at_x + xt.at * at.x;
-                        mbar_expect_tx(&b.x_full[xt.at], at.x);
-                        if (PASS != GATED_OUT)
-                            for (int c = 0; c < p.n; c += 64) box_load(x + c * ROWS * 2, &maps.grad, c, row0, &b.x_full[xt.at]);
-                        for (int c = 0; c < p.k; c += 64) box_load(x + at.grad + c * ROWS * 2, &maps.x, c, row0, &b.x_full[xt.at]);
-                    }
-                    __syncwarp();
-                    xt.next(p.x_buffers);
-                    if (scales && t >= behind) scale(t - behind);
-                }
-                if (scales && behind && mine > 0 && wait.alive) scale(mine - 1);
-                // nothing on its way when others have given up
-                if (one && b_dead(b))
-                    for (int i = 0; i < p.x_buffers; i++) {
-                        const int turns = xt.turns - (i >= xt.at ? 1 : 0);
-                        if (turns >= 0) Waits{&b.dead}.on(&b.x_full[i], turns, true);
-                    }
-            }
-        } else {
+        } else if (!boxes) {
+            // (by themselves: beside the boxes' code in one loop these took half as long again)
             Turn xt;
             for (long long t = 0; t < mine && wait.alive; t++) {
                 const long long row0 = (split + t * step) * ROWS;
@@ -650,6 +614,54 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                 mbar_arrive(&b.x_full[xt.at]);
                 xt.next(p.x_buffers);
             }
+        } else if (staged_rows || loader == 0) {
+            const bool one = loader == 0 && one_of_warp();
+            const int box_bytes = (p.box_x ? at.x - at.grad : 0) + (p.box_grad ? at.grad : 0);
+            Turn xt, st;
+            auto scale = [&](long long t) {
+                if constexpr (sizeof(T) == 2) {
+                    if (!wait.full(b.x_full, st)) return;
+                    const long long row0 = (split + t * step) * ROWS;
+                    scale_tile<T, ROWS>(static_cast<T*>(p.dresidual) + row0 * p.n, smem + at.at_x + st.at * at.x, (int)min((long long)ROWS, p.rows - row0),
+                                        p.n / 8, p.scale);
+                    __syncwarp();
+                    if (one) mbar_arrive(&b.x_free[st.at]);
+                    st.next(p.x_buffers);
+                }
+            };
+            const int behind = p.x_buffers >= 2 ? 1 : 0;      // a tile is scaled when the next one has been asked for
+            for (long long t = 0; t < mine; t++) {
+                const long long row0 = (split + t * step) * ROWS;
+                const int valid = (int)min((long long)ROWS, p.rows - row0);
+                if (!wait.free(b.x_free, xt)) break;
+                unsigned char* x = smem + at.at_x + xt.at * at.x;
+                u64* full = &b.x_full[xt.at];
+                if (one) {
+                    mbar_expect_tx(full, box_bytes);
+                    if (p.box_grad)
+                        for (int c = 0; c < p.n; c += 64) box_load(x + c * ROWS * 2, &maps.grad, c, (int)row0, full);
+                    if (p.box_x)
+                        for (int c = 0; c < p.k; c += 64) box_load(x + at.grad + c * ROWS * 2, &maps.x, c, (int)row0, full);
+                }
+                __syncwarp();
+                if (staged_rows) {
+                    if (PASS != GATED_OUT && !p.box_grad)
+                        stage<T, ROWS>(x, p.np / 8, static_cast<const T*>(p.grad) + row0 * p.n, p.n, valid, p.wide_grad, loader, row_loaders);
+                    if (!p.box_x)
+                        stage<T, ROWS>(x + at.grad, p.kx / 8, static_cast<const T*>(p.x) + row0 * p.k, p.k, valid, p.wide_x, loader, row_loaders);
+                    fence_async_proxy();
+                    mbar_arrive(full);
+                }
+                xt.next(p.x_buffers);
+                if (scales && t >= behind) scale(t - behind);
+            }
+            if (scales && behind && mine > 0 && wait.alive) scale(mine - 1);
+            // nothing on its way when others have given up (of tiles that are not whole there may be something: half a second each)
+            if (one && b_dead(b))
+                for (int i = 0; i < p.x_buffers; i++) {
+                    const int turns = xt.turns - (i >= xt.at ? 1 : 0);
+                    if (turns >= 0) Waits{&b.dead}.on(&b.x_full[i], turns, true);
+                }
         }
     } else if (warp == WORKERS) {   // the first products: g, u (, da) of a step
         if (one_of_warp()) {

@@ -20,7 +20,7 @@ inline int gated_splits(int chunks, long long rows, int sms) { return (int)std::
 template <typename T, GatedPass PASS, int ROWS>
 static bool gated_plan(GatedArgs& p) {
     const int chunks = PASS == GATED_DW ? 1 : p.chunks;
-    p.boxes = sizeof(T) == 2 && p.wide_x && (PASS == GATED_OUT || p.wide_grad);
+    p.box_x = sizeof(T) == 2 && p.wide_x, p.box_grad = sizeof(T) == 2 && PASS != GATED_OUT && p.wide_grad;
     auto fits = [&]() {
         // The weights of all chunks first, or of three: of a step's first products, of its second ones, and on their way; two tiles of rows, and rows
         // that leave together; more of all where there is room.  (154 401 rows of 128 to 512 to 128 float16 channels: 109 us with two buffers of weights
@@ -73,10 +73,8 @@ template <typename T, GatedPass PASS, int ROWS>
 static int launch_gated_rows(GatedArgs& p, cudaStream_t st) {
     const int smem = GatedSmem<T, PASS, ROWS>(p).total;
     GatedMaps maps = {};
-    if (p.boxes) {
-        PL_TRY(matrix_map<T>(maps.x, p.x, p.rows, p.k, ROWS));
-        if (PASS != GATED_OUT) PL_TRY(matrix_map<T>(maps.grad, p.grad, p.rows, p.n, ROWS));
-    }
+    if (p.box_x) PL_TRY(matrix_map<T>(maps.x, p.x, p.rows, p.k, ROWS));
+    if (p.box_grad) PL_TRY(matrix_map<T>(maps.grad, p.grad, p.rows, p.n, ROWS));
     if (p.io_buffers) {
         PL_TRY(matrix_map<T>(maps.out, p.out, p.rows, PASS == GATED_OUT ? p.n : p.k, ROWS));
         if (PASS == GATED_OUT && p.residual) PL_TRY(matrix_map<T>(maps.residual, p.residual, p.rows, p.n, ROWS));

@@ -104,18 +104,21 @@ int pl_gated_mix_backward(const pl_gated_shape* m, const void* grad_out, const v
     if (!gated_aligned(workspace)) return PL_INVALID_ARGUMENT;
     GatedArgs p = gated_args(m, x, gate_weight, up_weight, down_weight, gate_bias, up_bias);
     p.grad = grad_out;
-    p.wide_grad = p.n % 8 == 0 && gated_aligned(grad_out);
+    p.wide_grad = p.n % 8 == 0 && gated_aligned(grad_out) && p.rows < (1ll << 31) - 128;
     p.biased = p.biased || d.gate_bias || d.up_bias;   // (the ones' column sums dg and du)
     set_columns(p);
     p.packed = static_cast<unsigned char*>(workspace);
-    if (d.x) {
-        p.out = d.x, p.dresidual = d.residual;
-        p.wide_out = p.k % (m->dtype == PL_F32 ? 4 : 8) == 0 && gated_aligned(d.x) && p.rows < (1ll << 31) - 128;
-        p.wide_dresidual = p.n % (m->dtype == PL_F32 ? 4 : 8) == 0 && gated_aligned(grad_out) && gated_aligned(d.residual);
-        PL_TRY(run_gated(p, m->dtype, GATED_DX, true, st));
-    } else if (d.residual) {
+    // s dout by the kernel of dx where it has the rows at hand (16-bit rows by the TMA) or a loader to spare (floats), else by itself.
+    const bool beside = d.x && (m->dtype == PL_F32 || (p.wide_x && p.wide_grad && gated_aligned(d.residual)));
+    if (d.residual && !beside) {
         const pl_dropout none = {};
         PL_TRY(pl_channel_dropout(nullptr, d.residual, grad_out, nullptr, m->rows * m->n, m->dtype, m->residual_scale, &none, nullptr, stream));
+    }
+    if (d.x) {
+        p.out = d.x, p.dresidual = beside ? d.residual : nullptr;
+        p.wide_out = p.k % (m->dtype == PL_F32 ? 4 : 8) == 0 && gated_aligned(d.x) && p.rows < (1ll << 31) - 128;
+        p.wide_dresidual = gated_aligned(grad_out) && gated_aligned(d.residual);
+        PL_TRY(run_gated(p, m->dtype, GATED_DX, true, st));
     }
     if (!sums) return PL_OK;
     p.down_bias_wanted = d.down_bias != nullptr;
