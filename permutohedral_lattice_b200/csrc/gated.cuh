@@ -300,12 +300,12 @@ struct Turn {
 struct Waits {
     volatile u32* dead;
     bool alive = true;
-    // Gives up half a second after it began, or (unless it is `last`) when others have.
+    // Gives up two seconds after it began, or (unless it is `last`) when others have.
     __device__ __forceinline__ bool on(u64* bar, int parity, bool last = false) {
         if (!alive || mbar_done(bar, parity & 1)) return alive;
         const u64 began = global_timer();
         for (int i = 1; !mbar_done(bar, parity & 1); i++)
-            if ((*dead && !last) || i >= 1 << 26 || ((i & 63) == 0 && global_timer() - began > 500000000ull)) {
+            if ((*dead && !last) || i >= 1 << 26 || ((i & 63) == 0 && global_timer() - began > 2000000000ull)) {
                 *dead = 1;
                 return alive = false;
             }
@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                 if (scales && t >= behind) scale(t - behind);
             }
             if (scales && behind && mine > 0 && wait.alive) scale(mine - 1);
-            // nothing on its way when others have given up (of tiles that are not whole there may be something: half a second each)
+            // nothing on its way when others have given up
             if (one && b_dead(b))
                 for (int i = 0; i < p.x_buffers; i++) {
                     const int turns = xt.turns - (i >= xt.at ? 1 : 0);
