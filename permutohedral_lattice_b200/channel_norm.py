@@ -163,7 +163,6 @@ class _ChannelNorm(torch.autograd.Function):
     def backward(ctx, *grads):
         x, residual, gate, seed, *weights = ctx.saved_tensors
         m, device = ctx.m, ctx.device
-        needs = [name for name, wanted in zip(_NAMES, ctx.needs_input_grad[6:]) if wanted]
         with_h, with_y = ctx.outputs
         dh, dy = grads if with_h and with_y else (grads[0], None) if with_h else (None, grads[0])
         if dh is None and dy is None:
@@ -172,9 +171,7 @@ class _ChannelNorm(torch.autograd.Function):
             dy = torch.zeros_like(dh)
         dh, dy = _contiguous(dh), _contiguous(dy)
         like = dh if dy is None else dy
-        shapes = {"x": like, "residual": like, "gate": gate, "after_weight": weights[0], "after_bias": weights[1],
-                  "before_weight": weights[2], "before_bias": weights[3]}
-        made = {name: torch.empty(shapes[name].shape, dtype=shapes[name].dtype, device=device) for name in needs}
+        made = {name: torch.empty_like(t) for name, t, wanted in zip(_NAMES, (like, like, gate, *weights), ctx.needs_input_grad[6:]) if wanted}
         with _OnDevice(device):
             workspace = torch.empty(_workspace_bytes(like.shape[-1]), dtype=torch.uint8, device=device)
             d = capi.PlNormGradients(**{name: t.data_ptr() for name, t in made.items()})

@@ -94,9 +94,7 @@ class _GatedMix(torch.autograd.Function):
         x, *weights = ctx.saved_tensors
         device, s = ctx.args
         grad = grad.contiguous()
-        like = dict(zip(_NAMES, (x, grad, *weights)))
-        made = {name: torch.empty(like[name].shape, dtype=x.dtype, device=device)
-                for name, wanted in zip(_NAMES, ctx.needs_input_grad[3:]) if wanted}
+        made = {name: torch.empty_like(t) for name, t, wanted in zip(_NAMES, (x, grad, *weights), ctx.needs_input_grad[3:]) if wanted}
         with _OnDevice(device):
             workspace = torch.empty(s[2], dtype=torch.uint8, device=device)
             capi.check(capi.lib().pl_gated_mix_backward(
