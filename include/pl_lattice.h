@@ -224,7 +224,7 @@ int pl_crf_step_f32(float* q_out, const float* q, const float* unaries, float bi
                     void* bilateral_workspace, size_t bilateral_bytes, int64_t bilateral_entries,
                     void* spatial_workspace, size_t spatial_bytes, int64_t spatial_entries, void* stream);
 
-/* Number of kernels the library has launched in this process so far (filter stages, pl_crf_update_f32, the products and packs below;
+/* Number of kernels the library has launched in this process so far (filter stages, pl_crf_update_f32, and all below;
  * memsets, copies and event records are not counted).  The difference across a region is the number
  * of kernels that region launched.  No counterpart in the reference. */
 unsigned long long pl_launch_count(void);
