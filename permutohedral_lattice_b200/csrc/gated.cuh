@@ -64,11 +64,16 @@ __host__ __device__ inline int gated_down_bytes(int np) { return Tensor<T>::TERM
 template <typename T>
 __host__ __device__ inline int gated_up_bytes(int kp) { return Tensor<T>::TERMS * tile_bytes(kp, 2 * gated_chunk<T>()); }
 
+// Terms of a hidden value on its way to the second products.  16-bit types round it once more, which makes results 1.4 times as far off as a single
+// rounding does; FINE: they take two terms, 15 % of a large call's time, nothing where there is a tile a CTA.
+template <typename T, bool FINE>
+__host__ __device__ constexpr int hidden_terms() { return sizeof(T) == 4 ? 3 : FINE ? 2 : 1; }
+
 // Where things lie in shared memory: offsets, bytes of a buffer, in all.
-template <typename T, GatedPass PASS, int ROWS>
+template <typename T, GatedPass PASS, int ROWS, bool FINE>
 struct GatedSmem {
-    static constexpr int C = gated_chunk<T>(), TERMS = Tensor<T>::TERMS;
-    static constexpr int A = TERMS * tile_bytes(ROWS, PASS == GATED_OUT ? C : 2 * C), ACT = PASS == GATED_DW ? TERMS * tile_bytes(ROWS, C) : 0;
+    static constexpr int C = gated_chunk<T>(), TERMS = Tensor<T>::TERMS, HIDDEN = hidden_terms<T, FINE>();
+    static constexpr int A = HIDDEN * tile_bytes(ROWS, PASS == GATED_OUT ? C : 2 * C), ACT = PASS == GATED_DW ? HIDDEN * tile_bytes(ROWS, C) : 0;
     static constexpr int BARRIERS = 2048;
     __host__ __device__ static int rows_bytes(int columns) { return TERMS == 1 ? swizzled_bytes(ROWS, 2 * columns) : TERMS * tile_bytes(ROWS, columns); }
     int grad, x, io;                 // bytes: a tile of dout, of x with it, of rows on their way out
@@ -421,7 +426,7 @@ __device__ __forceinline__ void scale_rows(T* to, const T* from, int count, floa
 }
 
 // Some hidden channels of a row: from g, u (and da) to what the second products take.
-template <typename T, GatedPass PASS, int ACT, int ROWS, int W>
+template <typename T, GatedPass PASS, int ACT, int ROWS, int HIDDEN, int W>
 __device__ __forceinline__ void gated_work(const float (&g)[W], const float (&u)[W], const float (&da)[W], unsigned char* a, int row, int column) {
     constexpr int C = gated_chunk<T>(), CB = column_blocks(ROWS), PLANE = tile_bytes(ROWS, PASS == GATED_OUT ? C : 2 * C);
 #pragma unroll
@@ -442,14 +447,14 @@ __device__ __forceinline__ void gated_work(const float (&g)[W], const float (&u)
                 const float2 q = value(i);
                 v[2 * i] = q.x, v[2 * i + 1] = q.y;
             }
-            store_terms8<T>(where, plane, v);
+            store_terms8<T, HIDDEN>(where, plane, v);
         };
         if constexpr (PASS == GATED_OUT) {
             put(to, PLANE, [&](int i) { return mul2(act[i], u2[i]); });
         } else {
             put(to, PLANE, [&](int i) { return mul2(mul2(d2[i], u2[i]), slope[i]); });
             put(to + C / 8 * CB, PLANE, [&](int i) { return mul2(d2[i], act[i]); });
-            if constexpr (PASS == GATED_DW) put(to + Tensor<T>::TERMS * PLANE, tile_bytes(ROWS, C), [&](int i) { return mul2(act[i], u2[i]); });
+            if constexpr (PASS == GATED_DW) put(to + HIDDEN * PLANE, tile_bytes(ROWS, C), [&](int i) { return mul2(act[i], u2[i]); });
         }
     }
 }
@@ -492,12 +497,12 @@ struct WeightRing {
     }
 };
 
-template <typename T, GatedPass PASS, int ROWS>
+template <typename T, GatedPass PASS, int ROWS, bool FINE>
 __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const __grid_constant__ GatedArgs p, const __grid_constant__ GatedMaps maps) {
     extern __shared__ __align__(1024) unsigned char smem[];
-    using Smem = GatedSmem<T, PASS, ROWS>;
+    using Smem = GatedSmem<T, PASS, ROWS, FINE>;
     using Columns = GatedColumns<T, PASS>;
-    constexpr int C = gated_chunk<T>(), TERMS = Tensor<T>::TERMS;
+    constexpr int C = gated_chunk<T>(), TERMS = Tensor<T>::TERMS, HIDDEN = Smem::HIDDEN;
     constexpr int WORKERS = GatedWarps<T>::WORKERS, LOADERS = GatedWarps<T>::LOADERS, THREADS = GatedWarps<T>::THREADS;
     const Smem at(p);
     const Columns col(p);
@@ -719,14 +724,21 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                 const u32 d = tensor + col.d + dt.at * col.d_all;
                 const bool add = in_group > 0, add_main = p.split ? in_group > 1 : add;
                 const u32 main = d + (p.split ? (in_group & 1) * col.up_part : 0), small = d + (p.split ? 2 : 1) * col.up_part;
-                if constexpr (PASS == GATED_OUT) {
+                if constexpr (PASS == GATED_OUT && TERMS == 1) {
+                    few_products<T, HIDDEN, 1>(d, over_columns(a, ROWS, C), over_rows(w1, C, p.np), p.np, C / 16, add);
+                } else if constexpr (PASS == GATED_DX && TERMS == 1) {
+                    few_products<T, HIDDEN, 1>(d, over_columns(a, ROWS, 2 * C), over_columns(w1, p.kp, 2 * C), p.kx, 2 * C / 16, add);
+                } else if constexpr (PASS == GATED_OUT) {
                     products<T>(main, small, over_columns(a, ROWS, C), over_rows(w1, C, p.np), p.np, C / 16, add_main, add);
                 } else if constexpr (PASS == GATED_DX) {
                     products<T>(main, small, over_columns(a, ROWS, 2 * C), over_columns(w1, p.kp, 2 * C), p.kx, 2 * C / 16, add_main, add);
                 } else {
                     const Operand hidden = over_rows(a, ROWS, 2 * C), grad = rows_over_rows(x, p.np);
                     const Operand rows = rows_over_rows(x + at.grad, p.kx), act = over_rows(a + Smem::A, ROWS, C);
-                    if (TERMS == 3 && p.stacked) {
+                    if constexpr (TERMS == 1) {
+                        few_products<T, HIDDEN, 1>(d, hidden, rows, p.kx, ROWS / 16, add);
+                        few_products<T, 1, HIDDEN>(d + col.down, grad, act, C, ROWS / 16, add);
+                    } else if (p.stacked) {
                         stacked_products<T>(d, hidden, rows, p.kx, ROWS / 16, add);
                         stacked_products<T>(d + col.down, grad, act, C, ROWS / 16, add);
                     } else {
@@ -735,14 +747,15 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                     }
                     // the biases': times ones (which have one term)
                     const Operand one = over_rows(shared_address(smem + at.at_ones), ROWS, 16);
-                    auto column_sums = [&](const Operand& of, u32 to) {
+                    auto column_sums = [&](const Operand& of, u32 to, int terms) {   // (16-bit: small terms in the same place, before)
                         const u32 shape = product_shape<T>(of, one, 16);
-                        for (int t = TERMS - 1; t >= 0; t--)
+                        for (int t = terms - 1; t >= 0; t--)
                             for (int s = 0; s < ROWS / 16; s++)
-                                tensor_product(to + (t ? col.bias_part : 0), of.at(s, t), one.at(s, 0), shape, add || s > 0 || (TERMS == 3 && t == 1));
+                                tensor_product(to + (t ? col.bias_part : 0), of.at(s, t), one.at(s, 0), shape,
+                                               add || s > 0 || (TERMS == 3 ? t == 1 : t < terms - 1));
                     };
-                    if (p.biased) column_sums(hidden, d + col.up_bias);
-                    if (p.down_bias_wanted) column_sums(grad, d + col.down_bias);
+                    if (p.biased) column_sums(hidden, d + col.up_bias, HIDDEN);
+                    if (p.down_bias_wanted) column_sums(grad, d + col.down_bias, TERMS);
                     tensor_commit(&b.x_free[xt.at]);
                     xt.next(p.x_buffers);
                 }
@@ -865,10 +878,10 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                 }
                 if (j == 0 && q >= p.a_buffers && !wait.step(b.a_free, q - p.a_buffers)) break;
                 if (works) {
-                    if (p.activation == PL_GATE_SILU) gated_work<T, PASS, PL_GATE_SILU, ROWS>(g, u, da, a, row, W * part + j);
-                    else if (p.activation == PL_GATE_GELU) gated_work<T, PASS, PL_GATE_GELU, ROWS>(g, u, da, a, row, W * part + j);
-                    else if (p.activation == PL_GATE_SIGMOID) gated_work<T, PASS, PL_GATE_SIGMOID, ROWS>(g, u, da, a, row, W * part + j);
-                    else gated_work<T, PASS, PL_GATE_RELU, ROWS>(g, u, da, a, row, W * part + j);
+                    if (p.activation == PL_GATE_SILU) gated_work<T, PASS, PL_GATE_SILU, ROWS, HIDDEN>(g, u, da, a, row, W * part + j);
+                    else if (p.activation == PL_GATE_GELU) gated_work<T, PASS, PL_GATE_GELU, ROWS, HIDDEN>(g, u, da, a, row, W * part + j);
+                    else if (p.activation == PL_GATE_SIGMOID) gated_work<T, PASS, PL_GATE_SIGMOID, ROWS, HIDDEN>(g, u, da, a, row, W * part + j);
+                    else gated_work<T, PASS, PL_GATE_RELU, ROWS, HIDDEN>(g, u, da, a, row, W * part + j);
                 }
                 __syncwarp();
             }

@@ -17,7 +17,7 @@ inline int gated_splits(int chunks, long long rows, int sms) { return (int)std::
 
 // Buffers, as far as there is room: rows that leave together (or a thread stores its own), the weights of all chunks (else they come anew for every
 // tile), of everything else two, so that what comes next is fetched while products run.
-template <typename T, GatedPass PASS, int ROWS>
+template <typename T, GatedPass PASS, int ROWS, bool FINE>
 static bool gated_plan(GatedArgs& p) {
     const int chunks = PASS == GATED_DW ? 1 : p.chunks;
     p.box_x = sizeof(T) == 2 && p.wide_x, p.box_grad = sizeof(T) == 2 && PASS != GATED_OUT && p.wide_grad;
@@ -32,10 +32,10 @@ static bool gated_plan(GatedArgs& p) {
                                 {1, two, io, 2}, {1, two, io, 1}, {1, two, 0, 1}, {1, 1, io, 1}, {1, 1, 0, 1}};
         for (const auto& one : tries) {
             p.x_buffers = one[0], p.w_buffers[0] = p.w_buffers[1] = one[1], p.io_buffers = one[2], p.a_buffers = one[3];
-            if (GatedSmem<T, PASS, ROWS>(p).total > (int)GATED_SMEM) continue;
+            if (GatedSmem<T, PASS, ROWS, FINE>(p).total > (int)GATED_SMEM) continue;
             while (p.x_buffers >= 2 && p.x_buffers < 4) {
                 p.x_buffers++;
-                if (GatedSmem<T, PASS, ROWS>(p).total <= (int)GATED_SMEM) continue;
+                if (GatedSmem<T, PASS, ROWS, FINE>(p).total <= (int)GATED_SMEM) continue;
                 p.x_buffers--;
                 break;
             }
@@ -69,9 +69,9 @@ static int matrix_map(CUtensorMap& map, const void* p, long long rows, int colum
     return encode_matrix(map, p, dtype, rows, columns, 128 / sizeof(T), box);
 }
 
-template <typename T, GatedPass PASS, int ROWS>
+template <typename T, GatedPass PASS, int ROWS, bool FINE>
 static int launch_gated_rows(GatedArgs& p, cudaStream_t st) {
-    const int smem = GatedSmem<T, PASS, ROWS>(p).total;
+    const int smem = GatedSmem<T, PASS, ROWS, FINE>(p).total;
     GatedMaps maps = {};
     if (p.box_x) PL_TRY(matrix_map<T>(maps.x, p.x, p.rows, p.k, ROWS));
     if (p.box_grad) PL_TRY(matrix_map<T>(maps.grad, p.grad, p.rows, p.n, ROWS));
@@ -81,26 +81,26 @@ static int launch_gated_rows(GatedArgs& p, cudaStream_t st) {
     }
     const long long tiles = (p.rows + ROWS - 1) / ROWS;
     const unsigned grid = PASS == GATED_DW ? p.chunks * p.splits : (unsigned)std::min<long long>(tiles, num_sms());
-    PL_TRY((ensure_dynamic_smem<gated_kernel<T, PASS, ROWS>>(smem)));
+    PL_TRY((ensure_dynamic_smem<gated_kernel<T, PASS, ROWS, FINE>>(smem)));
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(grid), config.blockDim = dim3(GatedWarps<T>::THREADS), config.dynamicSmemBytes = smem, config.stream = st;
     cudaLaunchAttribute early[1];   // on the SMs, with its barriers set up, when the kernel before it (gated_pack, usually) ends
     early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early[0].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = early, config.numAttrs = 1;
-    PL_CUDA(cudaLaunchKernelEx(&config, gated_kernel<T, PASS, ROWS>, (const GatedArgs)p, (const GatedMaps)maps));
+    PL_CUDA(cudaLaunchKernelEx(&config, gated_kernel<T, PASS, ROWS, FINE>, (const GatedArgs)p, (const GatedMaps)maps));
     PL_COUNT_LAUNCHES(1);
     return PL_OK;
 }
-template <typename T, GatedPass PASS>
+template <typename T, GatedPass PASS, bool FINE>
 static int launch_gated(GatedArgs& p, cudaStream_t st) {
     // Tiles of 64 rows, the other half of a product idle, where 128 leave no room: three terms of everything, from some 90 channels on; and the sums
     // over rows of 16-bit values where two tiles of 128 do not fit.
-    const bool fits = gated_plan<T, PASS, 128>(p);
-    if (fits && (PASS != GATED_DW || p.x_buffers >= 2)) return launch_gated_rows<T, PASS, 128>(p, st);
-    if constexpr (sizeof(T) == 4 || PASS == GATED_DW)
-        if (gated_plan<T, PASS, 64>(p)) return launch_gated_rows<T, PASS, 64>(p, st);
-    return fits && gated_plan<T, PASS, 128>(p) ? launch_gated_rows<T, PASS, 128>(p, st) : PL_INTERNAL_ERROR;
+    const bool fits = gated_plan<T, PASS, 128, FINE>(p);
+    if (fits && (PASS != GATED_DW || p.x_buffers >= 2)) return launch_gated_rows<T, PASS, 128, FINE>(p, st);
+    if constexpr (sizeof(T) == 4 || PASS == GATED_DW || FINE)
+        if (gated_plan<T, PASS, 64, FINE>(p)) return launch_gated_rows<T, PASS, 64, FINE>(p, st);
+    return fits && gated_plan<T, PASS, 128, FINE>(p) ? launch_gated_rows<T, PASS, 128, FINE>(p, st) : PL_INTERNAL_ERROR;
 }
 template <typename T>
 static int pack_gated(const GatedArgs& p, cudaStream_t st) {
@@ -110,6 +110,13 @@ static int pack_gated(const GatedArgs& p, cudaStream_t st) {
     PL_CUDA(cudaGetLastError());
     return PL_OK;
 }
+template <typename T, bool FINE>
+static int launch_pass(GatedArgs& p, GatedPass pass, cudaStream_t st) {
+    return pass == GATED_OUT  ? launch_gated<T, GATED_OUT, FINE>(p, st)
+           : pass == GATED_DX ? launch_gated<T, GATED_DX, FINE>(p, st)
+                              : launch_gated<T, GATED_DW, FINE>(p, st);
+}
+constexpr long long GATED_FINE_ROWS = 16384;
 // pack: the weights first (a backward pass packs them once for both of its kernels).
 template <typename T>
 static int gated_of(GatedArgs& p, GatedPass pass, bool pack, cudaStream_t st) {
@@ -117,7 +124,10 @@ static int gated_of(GatedArgs& p, GatedPass pass, bool pack, cudaStream_t st) {
     p.splits = gated_splits(p.chunks, p.rows, num_sms());
     p.drain = sizeof(T) == 4 ? 4 : 64;   // tiles: float32 sums of 512 rows are 7e-7 off, of 1024 1.3e-6, of 2048 2.5e-6 (and 1377, 1307, 1272 us a million of 32 to 128 to 32)
     if (pack) PL_TRY(pack_gated<T>(p, st));
-    return pass == GATED_OUT ? launch_gated<T, GATED_OUT>(p, st) : pass == GATED_DX ? launch_gated<T, GATED_DX>(p, st) : launch_gated<T, GATED_DW>(p, st);
+    // hidden values of 16-bit types in two terms as long as that costs nothing (2, and 21.3 us a point either way; 16 384 rows: a tile on most SMs)
+    if constexpr (sizeof(T) == 2)
+        if (p.rows <= GATED_FINE_ROWS) return launch_pass<T, true>(p, pass, st);
+    return launch_pass<T, false>(p, pass, st);
 }
 
 }  // namespace pl

@@ -61,6 +61,20 @@ template <typename T>
 __device__ __forceinline__ u32 product_shape(const Operand& a, const Operand& b, int n) {   // 128 x n
     return 1u << 4 | Tensor<T>::FORMAT << 7 | Tensor<T>::FORMAT << 10 | a.transposed << 15 | b.transposed << 16 | (u32)(n / 8) << 17 | 8u << 24;
 }
+// The same of 16-bit operands, one of which may be of two terms: the small one's products first.
+template <typename T, int A_TERMS, int B_TERMS>
+__device__ __forceinline__ void few_products(u32 d, const Operand& a, const Operand& b, int n, int steps, bool add) {
+    static_assert(A_TERMS * B_TERMS <= 2);
+    const u32 shape = product_shape<T>(a, b, n);
+#pragma unroll
+    for (int i = A_TERMS * B_TERMS - 1; i >= 0; i--) {
+#pragma unroll 4
+        for (int s = 0; s < steps; s++) {
+            tensor_product(d, a.at(s, A_TERMS == 2 ? i : 0), b.at(s, B_TERMS == 2 ? i : 0), shape, add);
+            add = true;
+        }
+    }
+}
 // d (+)= a b^T over 16 `steps` terms, 128 x n; small: where products with a term but the first go (may be d).  add, add_small: to what is there.
 template <typename T>
 __device__ __forceinline__ void products(u32 d, u32 small, const Operand& a, const Operand& b, int n, int steps, bool add, bool add_small) {
@@ -150,21 +164,21 @@ __device__ __forceinline__ void box_store(const void* map, int x, int y, const v
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // Eight values as terms to a row of a block, 16 bytes each.
-template <typename T>
+template <typename T, int TERMS = Tensor<T>::TERMS>
 __device__ __forceinline__ void store_terms8(unsigned char* to, int plane, const float (&v)[8]) {
     using Term = typename Tensor<T>::Term;
     float left[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) left[i] = v[i];
 #pragma unroll
-    for (int t = 0; t < Tensor<T>::TERMS; t++) {
+    for (int t = 0; t < TERMS; t++) {
         uint4 q;
         Term* e = reinterpret_cast<Term*>(&q);
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
             if constexpr (std::is_same<Term, __half>::value) reinterpret_cast<__half2*>(&q)[i / 2] = __floats2half2_rn(left[i], left[i + 1]);
             else reinterpret_cast<__nv_bfloat162*>(&q)[i / 2] = __floats2bfloat162_rn(left[i], left[i + 1]);
-            if (t + 1 < Tensor<T>::TERMS) left[i] -= to_float(e[i]), left[i + 1] -= to_float(e[i + 1]);
+            if (t + 1 < TERMS) left[i] -= to_float(e[i]), left[i + 1] -= to_float(e[i + 1]);
         }
         *reinterpret_cast<uint4*>(to + t * plane) = q;
     }
