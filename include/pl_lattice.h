@@ -425,7 +425,7 @@ typedef enum pl_gate { PL_GATE_SILU = 0, PL_GATE_GELU = 1, PL_GATE_SIGMOID = 2, 
 /* out[rows, n] = (act(x @ gate_weight + gate_bias) * (x @ up_weight + up_bias)) @ down_weight + down_bias + residual_scale * residual,
  * x [rows, k], gate_weight and up_weight [k, h], down_weight [h, n]; biases and residual may be NULL.  Up to 128 channels in and out, 512
  * in between; everything of one type.  Products and sums are float or better; of 16-bit types the values in between are
- * rounded once on their way to the next product.  Values and weights have to be finite, and below 3.38e38. */
+ * rounded once on their way to the next product, in calls of more than 65 536 rows.  Values and weights have to be finite, and below 3.38e38. */
 typedef struct pl_gated_shape {
     int64_t rows;
     int k, h, n;

@@ -65,7 +65,7 @@ template <typename T>
 __host__ __device__ inline int gated_up_bytes(int kp) { return Tensor<T>::TERMS * tile_bytes(kp, 2 * gated_chunk<T>()); }
 
 // Terms of a hidden value on its way to the second products.  16-bit types round it once more, which makes results 1.4 times as far off as a single
-// rounding does; FINE: they take two terms, 15 % of a large call's time, nothing where there is a tile a CTA.
+// rounding does (sums of a few values up to 1.7); FINE: they take two terms, and are off by that single rounding.
 template <typename T, bool FINE>
 __host__ __device__ constexpr int hidden_terms() { return sizeof(T) == 4 ? 3 : FINE ? 2 : 1; }
 

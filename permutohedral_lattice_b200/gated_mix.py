@@ -112,7 +112,8 @@ def gated_mix(x, gate_weight, up_weight, down_weight, gate_bias=None, up_bias=No
     x [*, K], gate_weight and up_weight [K, H], down_weight [H, N], biases [H], [H], [N], residual and the output [*, N]: all of one type,
     float32, float16 or bfloat16; up to 128 channels in and out and 512 in between.  activation: "silu", "gelu" (by erf),
     "sigmoid" or "relu".  Products of floats are off by some 2^-24, sums are float32; of 16-bit types the hidden values (and, in the
-    backward pass, their gradients) are rounded once to that type on their way to the next product.  Gradients' sums over rows have
+    backward pass, their gradients) are rounded once to that type on their way to the next product, in calls of more than 65 536 rows; in smaller ones they go on
+    as two terms of it.  Gradients' sums over rows have
     a fixed order.  x, the weights and hidden values have to be finite, and below 3.38e38 (of float16
     all of them below 65504): of a row that is not, values come out infinite or NaN, other rows are as
     they would be; the weights' gradients are then not finite.  In a CUDA graph: one ordinary call of the same sizes before the
