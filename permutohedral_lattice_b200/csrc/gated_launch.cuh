@@ -94,11 +94,11 @@ static int launch_gated_rows(GatedArgs& p, cudaStream_t st) {
 }
 template <typename T, GatedPass PASS, bool FINE>
 static int launch_gated(GatedArgs& p, cudaStream_t st) {
-    // Tiles of 64 rows, the other half of a product idle, where 128 leave no room: three terms of everything, from some 90 channels on; and the sums
-    // over rows of 16-bit values where two tiles of 128 do not fit.
+    // Tiles of 64 rows, the other half of a product idle, where 128 leave no room: the gradients of floats, three terms of everything, from some 90
+    // channels on; and the sums over rows of 16-bit values where two tiles of 128 do not fit.
     const bool fits = gated_plan<T, PASS, 128, FINE>(p);
     if (fits && (PASS != GATED_DW || p.x_buffers >= 2)) return launch_gated_rows<T, PASS, 128, FINE>(p, st);
-    if constexpr (sizeof(T) == 4 || PASS == GATED_DW || FINE)
+    if constexpr (PASS == GATED_DW || (PASS == GATED_DX && sizeof(T) == 4))
         if (gated_plan<T, PASS, 64, FINE>(p)) return launch_gated_rows<T, PASS, 64, FINE>(p, st);
     return fits && gated_plan<T, PASS, 128, FINE>(p) ? launch_gated_rows<T, PASS, 128, FINE>(p, st) : PL_INTERNAL_ERROR;
 }
