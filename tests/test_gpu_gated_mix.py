@@ -201,3 +201,17 @@ def test_empty_tensors(plb):
     a, _ = make(0, 21, 42, 5)
     out, d = train(plb, a, torch.zeros(1, 0, 5, device="cuda"))
     assert out.shape == (1, 0, 5) and d["x"].shape == (1, 0, 21) and all(bool((d[m] == 0).all()) for m in d)
+
+
+@pytest.mark.parametrize("k", [1, 16, 75, 128])
+def test_biases_far_above_the_products_cost_the_sums_nothing(plb, k):
+    """out = relu(x Wg + 1000) times one: the bias is added once, with a part in 2^23 cut at most, and not to every one of up to 48 products."""
+    g = torch.Generator().manual_seed(k)
+    x = torch.randn(300, k, generator=g).cuda()
+    gate = torch.randn(k, 1, generator=g).cuda()
+    up, down = torch.zeros(k, 1, device="cuda"), torch.ones(1, 1, device="cuda")
+    out = plb.gated_mix(x, gate, up, down, torch.full((1,), 1000.0, device="cuda"), torch.ones(1, device="cuda"), activation="relu")
+    want = x.double() @ gate.double() + 1000.0
+    # cut: the bias's step, and the two steps of 16 hidden channels of the second product; rounded: on the way out.  u is 1, a its three terms to 2^-27;
+    # the eight steps of the products' first terms, whose sums are some 30 here, cut a quarter of such a part.
+    assert ((out.double() - want).abs() / want).max().item() <= 4 * 2.0 ** -23
