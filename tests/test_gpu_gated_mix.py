@@ -215,3 +215,21 @@ def test_biases_far_above_the_products_cost_the_sums_nothing(plb, k):
     # cut: the bias's step, and the two steps of 16 hidden channels of the second product; rounded: on the way out.  u is 1, a its three terms to 2^-27;
     # the eight steps of the products' first terms, whose sums are some 30 here, cut a quarter of such a part.
     assert ((out.double() - want).abs() / want).max().item() <= 4 * 2.0 ** -23
+
+
+@pytest.mark.parametrize("k", [16, 15])     # by boxes, value by value
+def test_values_beyond_2_31(plb, k):
+    """Rows whose values lie beyond 2^31 of their tensors, forward and backward, against those rows by themselves."""
+    rows, last = (1 << 31) // k + 300, 500
+    a, grad = make(last, k, 32, k, BF16, "gud", True)
+    far = {m: torch.zeros(1, rows, k, dtype=BF16, device="cuda") for m in ("x", "residual")}
+    for m, t in far.items():
+        t[:, -last:] = a[m]
+    far_grad = torch.zeros_like(far["x"])
+    far_grad[:, -last:] = grad
+    want = ref.gated(a, "silu", 0.75, grad)
+    out, d = train(plb, {**a, **far}, far_grad, wanted=("x", "residual"))
+    assert_within(out[:, -last:], *want["out"], "out")
+    assert_within(d["x"][:, -last:], *want["x"], "dx")
+    assert_within(d["residual"][:, -last:], *want["residual"], "dresidual")
+    assert not d["x"][:, :-last].any() and not d["residual"][:, :-last].any()
