@@ -92,7 +92,7 @@ PL_GATE_SILU, PL_GATE_GELU, PL_GATE_SIGMOID, PL_GATE_RELU = 0, 1, 2, 3
 
 class PlGated(ctypes.Structure):
     _fields_ = [("rows", ctypes.c_int64), ("k", ctypes.c_int), ("h", ctypes.c_int), ("n", ctypes.c_int), ("activation", ctypes.c_int),
-                ("dtype", ctypes.c_int), ("residual_scale", ctypes.c_float)]
+                ("dtype", ctypes.c_int), ("residual_scale", ctypes.c_float), ("round_hidden", ctypes.c_int)]
 
 
 class PlGatedGradients(ctypes.Structure):

@@ -116,9 +116,6 @@ static int launch_pass(GatedArgs& p, GatedPass pass, cudaStream_t st) {
            : pass == GATED_DX ? launch_gated<T, GATED_DX, FINE>(p, st)
                               : launch_gated<T, GATED_DW, FINE>(p, st);
 }
-// Hidden values of 16-bit types in two terms up to so many rows: there the host takes as long (20 us a call, 170 a training step of any size).  Two million
-// rows of 64 to 256 to 64 channels take 498, 945, 1268 us with two terms, 426, 582, 665 with one.
-constexpr long long GATED_FINE_ROWS = 65536;
 // pack: the weights first (a backward pass packs them once for both of its kernels).
 template <typename T>
 static int gated_of(GatedArgs& p, GatedPass pass, bool pack, cudaStream_t st) {
@@ -127,7 +124,7 @@ static int gated_of(GatedArgs& p, GatedPass pass, bool pack, cudaStream_t st) {
     p.drain = sizeof(T) == 4 ? 4 : 64;   // tiles: float32 sums of 512 rows are 7e-7 off, of 1024 1.3e-6, of 2048 2.5e-6 (and 1377, 1307, 1272 us a million of 32 to 128 to 32)
     if (pack) PL_TRY(pack_gated<T>(p, st));
     if constexpr (sizeof(T) == 2)
-        if (p.rows <= GATED_FINE_ROWS) return launch_pass<T, true>(p, pass, st);
+        if (!p.round_hidden) return launch_pass<T, true>(p, pass, st);
     return launch_pass<T, false>(p, pass, st);
 }
 

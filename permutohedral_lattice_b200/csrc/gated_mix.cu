@@ -32,6 +32,7 @@ static GatedArgs gated_args(const pl_gated_shape* m, const void* x, const void* 
                             const void* gate_bias, const void* up_bias) {
     GatedArgs p = {};
     p.rows = m->rows, p.k = m->k, p.h = m->h, p.n = m->n, p.activation = m->activation, p.scale = m->residual_scale;
+    p.round_hidden = m->round_hidden != 0;
     p.x = x;
     p.gate_weight = gate_weight, p.up_weight = up_weight, p.down_weight = down_weight;
     p.gate_bias = gate_bias, p.up_bias = up_bias;
