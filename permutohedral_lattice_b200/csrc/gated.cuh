@@ -132,36 +132,41 @@ struct GatedColumns {
     }
 };
 
-// Eight sigmoids, e: eight values of g, then of the sigmoid.  A quarter of the reciprocals, the other three by products: with 16-bit types the
-// exponentials and reciprocals of all, two an element, took longer than their other instructions.  2^31 in place of larger exponentials (of -g above
-// 21.5) keeps the product of four in range; 2^-31 is then off by no more than itself.  Floats, whose products take longer, do without.
-template <typename T>
-__device__ __forceinline__ void gated_sigmoids(float2 (&e)[4]) {
-    const float2 minus = make_float2(-1.4426950408889634f, -1.4426950408889634f), one = make_float2(1.f, 1.f);
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        e[i] = mul2(e[i], minus);
-        if constexpr (sizeof(T) == 2) {
-            asm("min.NaN.f32 %0, %0, 0f41F80000;" : "+f"(e[i].x));
-            asm("min.NaN.f32 %0, %0, 0f41F80000;" : "+f"(e[i].y));
-        }
-        e[i].x = exp2_approx(e[i].x), e[i].y = exp2_approx(e[i].y);
-        e[i] = add2(e[i], one);
-    }
+// Eight sigmoids of g and (REST) what is left to one.  16-bit types: by e = exp(-|g|), at most one, of which 1 / (1 + e) and e / (1 + e) are the two, whichever way
+// round, so that neither loses its bits where a gate is shut or open.  A quarter of the reciprocals, the other three by products, which stay below 16: the
+// exponentials and reciprocals of all, two an element, took longer than their other instructions.  Floats, whose products take longer, do without.
+template <typename T, bool REST>
+__device__ __forceinline__ void gated_sigmoids(const float2 (&g)[4], float2 (&s)[4], float2 (&rest)[4]) {
+    const float2 one = make_float2(1.f, 1.f);
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-            const float2 pairs = mul2(e[i], e[i + 1]);                     // x, y: of two each
+            float2 e[2], d[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                e[j] = make_float2(exp2_approx(-1.4426950408889634f * fabsf(g[i + j].x)), exp2_approx(-1.4426950408889634f * fabsf(g[i + j].y)));
+                d[j] = add2(e[j], one);
+            }
+            const float2 pairs = mul2(d[0], d[1]);                     // x, y: of two each
             float all;
             asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(all) : "f"(pairs.x * pairs.y));
             const float2 of_pairs = mul2(make_float2(all, all), make_float2(pairs.y, pairs.x));
-            const float2 first = mul2(of_pairs, e[i + 1]);
-            e[i + 1] = mul2(of_pairs, e[i]);
-            e[i] = first;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float2 large = mul2(of_pairs, d[1 - j]), small = mul2(large, e[j]);
+                const bool x = g[i + j].x < 0.f, y = g[i + j].y < 0.f;
+                s[i + j] = make_float2(x ? small.x : large.x, y ? small.y : large.y);
+                if constexpr (REST) rest[i + j] = make_float2(x ? large.x : small.x, y ? large.y : small.y);
+            }
         }
     } else {
+        const float2 minus = make_float2(-1.4426950408889634f, -1.4426950408889634f);
 #pragma unroll
-        for (int i = 0; i < 4; i++) e[i].x = __fdividef(1.f, e[i].x), e[i].y = __fdividef(1.f, e[i].y);
+        for (int i = 0; i < 4; i++) {
+            const float2 q = mul2(g[i], minus), d = add2(make_float2(exp2_approx(q.x), exp2_approx(q.y)), one);
+            s[i] = make_float2(__fdividef(1.f, d.x), __fdividef(1.f, d.y));
+            if constexpr (REST) rest[i] = fma2(s[i], make_float2(-1.f, -1.f), one);
+        }
     }
 }
 // act(g) of eight values; SLOPE: act'(g) too
@@ -169,17 +174,12 @@ template <typename T, int ACT, bool SLOPE>
 __device__ __forceinline__ void gated_act(const float2 (&g)[4], float2 (&act)[4], float2 (&slope)[4]) {
     const float2 one = make_float2(1.f, 1.f), minus = make_float2(-1.f, -1.f);
     if constexpr (ACT == PL_GATE_SILU || ACT == PL_GATE_SIGMOID) {
-        float2 s[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) s[i] = g[i];
-        gated_sigmoids<T>(s);
+        float2 s[4], rest[4];
+        gated_sigmoids<T, SLOPE>(g, s, rest);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             act[i] = ACT == PL_GATE_SILU ? mul2(g[i], s[i]) : s[i];
-            if constexpr (SLOPE) {   // s (1 + g (1 - s)) or s (1 - s)
-                const float2 rest = fma2(s[i], minus, one);
-                slope[i] = ACT == PL_GATE_SILU ? fma2(act[i], rest, s[i]) : mul2(s[i], rest);
-            }
+            if constexpr (SLOPE) slope[i] = ACT == PL_GATE_SILU ? fma2(act[i], rest[i], s[i]) : mul2(s[i], rest[i]);   // s (1 + g (1 - s)) or s (1 - s)
         }
     } else if constexpr (ACT == PL_GATE_GELU) {
         // g Phi(g), Phi by Abramowitz and Stegun 7.1.26: with t = 1 / (1 + p |g|) and e = exp(-g^2 / 2), which the slope takes anyway, the smaller of Phi
