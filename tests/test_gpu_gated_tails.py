@@ -69,3 +69,22 @@ def test_gates_shut_far_out(plb, dtype):
         assert not out.any() and not dx.any(), (g, out[0], dx[0])
         out, dx = alone(plb, torch.full((130,), -g, dtype=dtype, device="cuda"), 1.0, "silu")
         assert bool((out == torch.tensor(-g, dtype=dtype)).all()) and bool((dx == 1).all())
+
+
+def gelu_forms(g, own):
+    """act, act' and what either may be off.  own: of the smaller of Phi and 1 - Phi, its polynomial of t = 1 / (1 + p |g|), whose relative slope in t is at
+    most 1, beside t's own 3 u; it is times exp(-g^2 / 2), (1.5 g^2 + 8) u off, from three roundings of its exponent and an instruction of 2^-22."""
+    small = 0.5 * torch.erfc(g.abs() / math.sqrt(2))
+    cdf = torch.where(g < 0, small, 1 - small)
+    density = g * torch.exp(-g * g / 2) / math.sqrt(2 * math.pi)
+    ecdf = ((1.5 * g * g + 12) * U + own) * small + U * cdf
+    return g * cdf, g.abs() * ecdf + U * (g * cdf).abs(), cdf + density, ecdf + (1.5 * g * g + 10) * U * density.abs() + U * (cdf + density).abs()
+
+
+def test_gelu_of_floats(plb):
+    """To some u of the value, in the tails too."""
+    g = points(F32, 1.0, 10.0)
+    out, dx = alone(plb, g, 1.0, "gelu")
+    act, eact, slope, eslope = gelu_forms(g.double(), 6 * U)
+    assert_within(out, act, eact + REST[F32] * act.abs(), "act")
+    assert_within(dx, slope, eslope + REST[F32] * slope.abs(), "slope")
