@@ -182,15 +182,15 @@ __device__ __forceinline__ void gated_act(const float2 (&g)[4], float2 (&act)[4]
             if constexpr (SLOPE) slope[i] = ACT == PL_GATE_SILU ? fma2(act[i], rest[i], s[i]) : mul2(s[i], rest[i]);   // s (1 + g (1 - s)) or s (1 - s)
         }
     } else if constexpr (ACT == PL_GATE_GELU) {
-        // g Phi(g).  With t = 1 / (1 + p |g|) and e = exp(-g^2 / 2), which the slope takes anyway, the smaller of Phi and 1 - Phi is e times a polynomial of t.
-        // Floats: nine terms, fitted to erfcx(|g| / sqrt 2) / 2 for the least relative error, 0.6 2^-24 and evaluated 6 2^-24, however small Phi is.  (erfcf's
-        // registers took 5 % of every activation's time.)  16-bit types: five, by Abramowitz and Stegun 7.1.26, 7.5e-8 off at most.  (erff took as long as all the rest.)
+        // g Phi(g).  With t = 1 / (1 + p |g|) and e = exp(-g^2 / 2), which the slope takes anyway, the smaller of Phi and 1 - Phi is e times a polynomial of t,
+        // fitted to erfcx(|g| / sqrt 2) / 2 for the least relative error, which holds however small Phi is.  Floats: nine terms, 0.6 2^-24 off and evaluated
+        // 6 2^-24 (erfcf's registers took 5 % of every activation's time).  16-bit types: six, 2^-18 (erff took as long as all the rest).
         auto both = [](float v) { return make_float2(v, v); };
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const float2 q = mul2(mul2(g[i], g[i]), both(-0.72134752044448170f));
             const float2 e = make_float2(exp2_approx(q.x), exp2_approx(q.y));
-            const float2 d = fma2(make_float2(fabsf(g[i].x), fabsf(g[i].y)), both(sizeof(T) == 4 ? 0.35f : 0.23164189f), one);
+            const float2 d = fma2(make_float2(fabsf(g[i].x), fabsf(g[i].y)), both(sizeof(T) == 4 ? 0.35f : 0.30816703f), one);
             const float2 t = make_float2(__fdividef(1.f, d.x), __fdividef(1.f, d.y));
             float2 p;
             if constexpr (sizeof(T) == 4) {
@@ -203,10 +203,11 @@ __device__ __forceinline__ void gated_act(const float2 (&g)[4], float2 (&act)[4]
                 p = fma2(t, p, both(0.13986186683177948f));
                 p = fma2(t, p, both(0.13962140679359436f));
             } else {
-                p = fma2(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
-                p = fma2(t, p, both(0.5f * 1.421413741f));
-                p = fma2(t, p, both(0.5f * -0.284496736f));
-                p = fma2(t, p, both(0.5f * 0.254829592f));
+                p = fma2(t, both(-0.07539591193199158f), both(0.1891007274389267f));
+                p = fma2(t, p, both(0.00772145064547658f));
+                p = fma2(t, p, both(0.1364033967256546f));
+                p = fma2(t, p, both(0.11898145079612732f));
+                p = fma2(t, p, both(0.12318693846464157f));
             }
             p = mul2(mul2(p, t), e);
             const float2 rest = fma2(p, minus, one);

@@ -88,3 +88,18 @@ def test_gelu_of_floats(plb):
     act, eact, slope, eslope = gelu_forms(g.double(), 6 * U)
     assert_within(out, act, eact + REST[F32] * act.abs(), "act")
     assert_within(dx, slope, eslope + REST[F32] * slope.abs(), "slope")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gelu_of_16_bit_types(plb, dtype):
+    """To 2^-18 of the smaller of Phi and 1 - Phi, in the tails too, where either type holds more of it than an absolute 1e-7."""
+    for up in (1.0, 30000.0):
+        g = points(dtype, 3.0, 6.5 if dtype == F16 else 12.0)
+        out, dx = alone(plb, g, up, "gelu")
+        held = float(torch.tensor(up, dtype=dtype))      # (29 952 in bfloat16, whose numbers are 128 apart there)
+        act, eact, slope, eslope = (held * v for v in gelu_forms(g.double(), 2.0 ** -18 + 6 * U))
+        if dtype == F16 and up > 1.0:      # (what it holds)
+            keep = (act.abs() < 60000.0) & (slope.abs() < 60000.0)
+            out, dx, act, eact, slope, eslope = (v[keep] for v in (out, dx, act, eact, slope, eslope))
+        assert_within(out, act, eact + (REST[dtype] + U) * act.abs() + TINY[dtype], "act")
+        assert_within(dx, slope, eslope + (REST[dtype] + U) * slope.abs() + TINY[dtype], "slope")
