@@ -881,6 +881,7 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
             tensor_after_sync();
             const u32 s = lanes + ((int)q & (p.s_buffers - 1)) * Columns::WIDE + W * part;
             unsigned char* a = smem + at.at_a + ((int)q & (p.a_buffers - 1)) * (Smem::A + Smem::ACT);
+            const bool behind = PASS == GATED_DW && (split + q * step) * ROWS + row >= p.rows;
 #pragma unroll 1
             for (int j = 0; j < W; j += 16) {
                 float g[16], u[16], da[16];
@@ -894,6 +895,12 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
                     if (lane == 0) mbar_arrive(&b.s_free[half]);
                 }
                 if (j == 0 && q >= p.a_buffers && !wait.step(b.a_free, q - p.a_buffers)) break;
+                // Rows behind the last one have zeros for x and dout, but g and u are the biases: a must be zero too, since infinity (float16: biases of some 300)
+                // times a zero of dout is not.
+                if (PASS == GATED_DW && behind) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) u[i] = 0.f;
+                }
                 if (works) {
                     if (p.activation == PL_GATE_SILU) gated_work<T, PASS, PL_GATE_SILU, ROWS, HIDDEN>(g, u, da, a, row, W * part + j);
                     else if (p.activation == PL_GATE_GELU) gated_work<T, PASS, PL_GATE_GELU, ROWS, HIDDEN>(g, u, da, a, row, W * part + j);
