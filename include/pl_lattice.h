@@ -425,7 +425,8 @@ typedef enum pl_gate { PL_GATE_SILU = 0, PL_GATE_GELU = 1, PL_GATE_SIGMOID = 2, 
 /* out[rows, n] = (act(x @ gate_weight + gate_bias) * (x @ up_weight + up_bias)) @ down_weight + down_bias + residual_scale * residual,
  * x [rows, k], gate_weight and up_weight [k, h], down_weight [h, n]; biases and residual may be NULL.  Up to 128 channels in and out, 512
  * in between; everything of one type.  Products and sums are float or better; of 16-bit types the values in between go on to
- * the next product as two terms of the type, or (round_hidden) rounded once to it, 1.4 times as far off and faster.  Values and weights have to be finite, and below 3.38e38. */
+ * the next product as two terms of the type, or (round_hidden) rounded once to it, 1.4 times as far off and faster.  Values and weights have to be finite, and below 3.38e38.
+ * A wait inside a kernel that lasts two seconds (a GPU that was taken away meanwhile) is given up: NaN in the rows and sums concerned, in every output. */
 typedef struct pl_gated_shape {
     int64_t rows;
     int k, h, n;

@@ -24,7 +24,7 @@ HEADERS = [os.path.join(CSRC, h) for h in ("simplex.cuh", "common.cuh", "lattice
                                              "mix_forward.cuh", "mix_backward.cuh", "mix_tensor.cuh", "mix_tiny.cuh",
                                              "mix_host.h", "mix_launch.cuh", "mix_back_launch.cuh",
                                              "philox.cuh", "channel_norm.cuh", "norm_launch.cuh", "gated_tensor.cuh", "gated.cuh",
-                                             "gated_launch.cuh")] + [
+                                             "gated_launch.cuh", "gated_give_up.h")] + [
     os.path.join(ROOT, "include", "pl_lattice.h")]
 
 

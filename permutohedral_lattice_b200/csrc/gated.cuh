@@ -14,7 +14,7 @@
 // Warps: workers turn the first products into the second's operand, and take out the sums, one half of them every other step, so that one half
 // computes while the other waits, loads or stores; two warps ask for the first and the second
 // products, and for the weights that only theirs read; loaders fetch rows.  They meet at barriers in shared memory; every wait is bounded.
-// If one runs out, all give up and the results are NaN.
+// If one runs out (two seconds: it should not happen), all give up and what the CTA was to write is NaN, which nothing else reports.
 //
 // Tiles of 128 rows, the rows of a product; chunks of 64 hidden channels (floats: 32), so that g and u of two chunks and the sums fit into tensor memory and
 // the weights of all chunks, mostly, into shared memory.  2 097 152 rows of 64 to 256 to 64 bfloat16 channels: 421 us (245 TFLOP/s, 1.9 TB/s), gradients of
@@ -22,6 +22,7 @@
 // pipe is busy 19 to 32 % of it, memory less: what bounds them are the workers' instructions (half of the issue slots), half of these at barriers.
 #pragma once
 #include <cuda.h>
+#include "gated_give_up.h"
 #include "gated_tensor.cuh"
 
 namespace pl {
@@ -927,11 +928,8 @@ __global__ void __launch_bounds__(GatedWarps<T>::THREADS, 1) gated_kernel(const 
             float* share = p.shares + ((long long)chunk0 * p.splits + split) * col.d_one * 128;
             for (int i = threadIdx.x; i < col.d_one * 128; i += THREADS) share[i] = NAN;
         } else {
-            const int width = PASS == GATED_OUT ? p.n : p.k;
-            for (long long t = 0; t < mine; t++) {
-                const long long row0 = (split + t * step) * ROWS, count = min((long long)ROWS, p.rows - row0) * width;
-                for (long long i = threadIdx.x; i < count; i += THREADS) static_cast<T*>(p.out)[row0 * width + i] = from_float<T>(NAN);
-            }
+            const GatedRows<T> outputs[2] = {{static_cast<T*>(p.out), PASS == GATED_OUT ? p.n : p.k}, {PASS == GATED_DX ? static_cast<T*>(p.dresidual) : nullptr, p.n}};
+            give_up(outputs, GatedTiles{p.rows, split, step, ROWS}, from_float<T>(NAN), (int)threadIdx.x, THREADS);
         }
     }
     tensor_before_sync();
