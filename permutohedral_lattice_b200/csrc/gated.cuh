@@ -969,10 +969,10 @@ __global__ void __launch_bounds__(256) gated_sums(const __grid_constant__ GatedS
         chunk = r == p.h ? 0 : r / p.chunk, column = r == p.h ? p.bias : p.down + r % p.chunk, line = i;
     }
     const float* from = p.shares + ((long long)chunk * p.splits * p.columns + column) * 128 + line;
-    float sum = 0.f;
+    double sum = 0.0;   // (its place in the time is not seen; a float was 1e-7 off)
 #pragma unroll 8
-    for (int s = 0; s < p.splits; s++) sum += from[(long long)s * p.columns * 128];
-    *to = from_float<T>(sum);
+    for (int s = 0; s < p.splits; s++) sum += (double)from[(long long)s * p.columns * 128];
+    *to = from_float<T>((float)sum);
 }
 
 }  // namespace pl
