@@ -45,6 +45,7 @@ static void set_columns(GatedArgs& p) { p.kx = (p.k + 15) / 16 * 16, p.kp = p.kx
 static int run_gated(const GatedArgs& p, int dtype, GatedPass pass, bool pack, cudaStream_t st) {
     return dtype == PL_F32 ? gated_floats(p, pass, pack, st) : gated_halves(p, dtype, pass, pack, st);
 }
+static int most_peaks() { return 2 * num_sms(); }   // CTAs of gated_peak
 static size_t packed_bytes(const pl_gated_shape* m) {   // with all biases
     const int chunk = chunk_of(m), chunks = (m->h + chunk - 1) / chunk, kp = (m->k + 15) / 16 * 16 + 16, np = (m->n + 15) / 16 * 16;
     const size_t one = m->dtype == PL_F32 ? gated_down_bytes<float>(np) + gated_up_bytes<float>(kp) : gated_down_bytes<__half>(np) + gated_up_bytes<__half>(kp);
@@ -65,6 +66,7 @@ int pl_gated_mix_workspace_bytes(const pl_gated_shape* m, int backward, size_t* 
     const int chunk = chunk_of(m), chunks = (m->h + chunk - 1) / chunk;
     const size_t columns = (m->k + 15) / 16 * 16 + 16 + chunk + 16;   // with all biases
     *bytes += sizeof(float) * 128 * columns * chunks * gated_splits(chunks, m->rows, num_sms());
+    if (m->dtype == PL_F16) *bytes += sizeof(u32) * most_peaks();
     return PL_OK;
 }
 
@@ -114,6 +116,14 @@ int pl_gated_mix_backward(const pl_gated_shape* m, const void* grad_out, const v
     if (d.residual && !beside) {
         const pl_dropout none = {};
         PL_TRY(pl_channel_dropout(nullptr, d.residual, grad_out, nullptr, m->rows * m->n, m->dtype, m->residual_scale, &none, nullptr, stream));
+    }
+    if (m->dtype == PL_F16 && (d.x || sums)) {
+        const long long count = m->rows * m->n, per = 256 * 8 * 4;
+        u32* peaks = reinterpret_cast<u32*>(p.packed + need) - most_peaks();
+        p.peaks = peaks, p.peak_count = (int)std::min<long long>((count + per - 1) / per, most_peaks());
+        gated_peak<<<p.peak_count, 256, 0, st>>>(static_cast<const __half*>(grad_out), count, peaks);
+        PL_COUNT_LAUNCHES(1);
+        PL_CUDA(cudaGetLastError());
     }
     if (d.x) {
         p.out = d.x, p.dresidual = beside ? d.residual : nullptr;
