@@ -223,11 +223,11 @@ def channel_norm(x, residual=None, gate=None, after=None, before=None, residual_
     return _ChannelNorm.apply(device, m, after is not None, wants_h, before is not None, seed, *tensors)
 
 
-def _drop(device, x, residual, share, seed, residual_scale, wants_scaled):
-    out = torch.empty_like(x)
+def _drop(device, x, residual, share, seed, residual_scale, wants_out, wants_scaled):
+    out = torch.empty_like(x) if wants_out else None
     scaled = torch.empty_like(x) if wants_scaled else None
     with _OnDevice(device):
-        rc = capi.lib().pl_channel_dropout(out.data_ptr(), _ptr(scaled), x.data_ptr(), _ptr(residual), x.numel(), _DTYPES[x.dtype],
+        rc = capi.lib().pl_channel_dropout(_ptr(out), _ptr(scaled), x.data_ptr(), _ptr(residual), x.numel(), _DTYPES[x.dtype],
                                            residual_scale, share, _ptr(seed), _stream_handle(device))
         if rc != capi.PL_OK:
             capi.check(rc, "pl_channel_dropout")
@@ -239,15 +239,14 @@ class _ChannelDropout(torch.autograd.Function):
     def forward(ctx, device, share, residual_scale, seed, x, residual):
         ctx.args = device, share, residual_scale
         ctx.save_for_backward(seed)
-        return _drop(device, x, residual, share, seed, residual_scale, False)[0]
+        return _drop(device, x, residual, share, seed, residual_scale, True, False)[0]
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         (seed,) = ctx.saved_tensors
         device, share, residual_scale = ctx.args
-        dx, dresidual = _drop(device, grad.contiguous(), None, share, seed, residual_scale, ctx.needs_input_grad[5])
-        return None, None, None, None, dx if ctx.needs_input_grad[4] else None, dresidual
+        return (None, None, None, None) + _drop(device, grad.contiguous(), None, share, seed, residual_scale, *ctx.needs_input_grad[4:])
 
 
 def channel_dropout(x, p, seed, residual=None, residual_scale=1.0):
@@ -267,5 +266,5 @@ def channel_dropout(x, p, seed, residual=None, residual_scale=1.0):
     share = _dropout_of(p, 0, 0) if on_gpu else _dropout_of(p, *seed)
     x, residual, tensor = x.contiguous(), _contiguous(residual), _contiguous(tensor)
     if not _follows((x, residual)):
-        return _drop(x.device, x, residual, share, tensor, float(residual_scale), False)[0]
+        return _drop(x.device, x, residual, share, tensor, float(residual_scale), True, False)[0]
     return _ChannelDropout.apply(x.device, share, float(residual_scale), tensor, x, residual)
