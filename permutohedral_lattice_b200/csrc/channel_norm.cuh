@@ -413,7 +413,8 @@ __global__ void __launch_bounds__(NORM_THREADS, E <= 8 ? 2 : 1) norm_backward(co
     gather(sum_gate, NORM_GATE);
 }
 
-// The vectors' gradients from the CTAs' shares: 32 values a CTA, 8 warps with an eighth of the shares each.
+// The vectors' gradients from the CTAs' shares: 32 values a CTA, 8 warps with an eighth of the shares each.  In doubles: floats' chain of 74 was as much off
+// as all that went before (a million rows of 32 channels: 2e-7, 1.3e-7 in doubles).
 struct NormSums {
     const float* shares;
     int ctas, c, dtype;
@@ -425,18 +426,18 @@ __device__ __forceinline__ void store_weight(void* w, int i, int dtype, float v)
     else static_cast<__nv_bfloat16*>(w)[i] = __float2bfloat16_rn(v);
 }
 static __global__ void __launch_bounds__(NORM_THREADS) norm_sums(const __grid_constant__ NormSums a) {
-    __shared__ float part_s[NORM_WARPS][33];
+    __shared__ double part_s[NORM_WARPS][33];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, which = blockIdx.y, i = blockIdx.x * 32 + lane;
     if (!a.to[which]) return;
-    float t = 0.f;
+    double t = 0.0;
     if (i < a.c)
-        for (int s = warp; s < a.ctas; s += NORM_WARPS) t += a.shares[((long long)s * NORM_VECTORS + which) * a.c + i];
+        for (int s = warp; s < a.ctas; s += NORM_WARPS) t += (double)a.shares[((long long)s * NORM_VECTORS + which) * a.c + i];
     part_s[warp][lane] = t;
     __syncthreads();
     if (warp || i >= a.c) return;
 #pragma unroll
     for (int w = 1; w < NORM_WARPS; w++) t += part_s[w][lane];
-    store_weight(a.to[which], i, a.dtype, t);
+    store_weight(a.to[which], i, a.dtype, (float)t);
 }
 
 // out = s residual + x keep / (1 - p), value by value; scaled: s x besides (the residual's gradient, where x is that of out).  Either may be NULL.
