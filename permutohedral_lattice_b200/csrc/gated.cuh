@@ -215,11 +215,12 @@ __device__ __forceinline__ void gated_act(const float2 (&g)[4], float2 (&act)[4]
     const float2 one = make_float2(1.f, 1.f), minus = make_float2(-1.f, -1.f);
     if constexpr (ACT == PL_GATE_SILU || ACT == PL_GATE_SIGMOID) {
         float2 s[4], rest[4];
-        gated_sigmoids<T, SLOPE>(g, s, rest);
+        gated_sigmoids<T, SLOPE && ACT == PL_GATE_SIGMOID>(g, s, rest);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             act[i] = ACT == PL_GATE_SILU ? mul2(g[i], s[i]) : s[i];
-            if constexpr (SLOPE) slope[i] = ACT == PL_GATE_SILU ? fma2(act[i], rest[i], s[i]) : mul2(s[i], rest[i]);   // s (1 + g (1 - s)) or s (1 - s)
+            if constexpr (SLOPE && ACT == PL_GATE_SILU) slope[i] = fma2(act[i], fma2(s[i], minus, one), s[i]);   // s (1 + g (1 - s)): of 1 - s nothing small is wanted
+            if constexpr (SLOPE && ACT == PL_GATE_SIGMOID) slope[i] = mul2(s[i], rest[i]);
         }
     } else if constexpr (ACT == PL_GATE_GELU) {
         // g Phi(g).  With t = 1 / (1 + p |g|) and e = exp(-g^2 / 2), which the slope takes anyway, the smaller of Phi and 1 - Phi is e times a polynomial of t,
