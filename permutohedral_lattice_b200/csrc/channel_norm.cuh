@@ -244,9 +244,10 @@ __device__ __forceinline__ void norm_vectors_to(float* vectors_s, const NormArgs
     __syncthreads();
 }
 
-// CTAs of an SM: where nothing is dropped four of 16-bit rows (2 470 000 x 256: 227 us with three, 202), with the generator's keys three.
+// CTAs of an SM: where nothing is dropped four of 16-bit rows (2 470 000 x 256: 227 us with three, 202), with the generator's keys three.  Single values of more than 256
+// channels: one, whose threads have registers for a row (150 000 x 511 floats, residual and two norms: 241 us; with two, which spilled some 300 bytes a thread, 837).
 template <typename T, bool WIDE, int E, int LANES, bool DROPS>
-__global__ void __launch_bounds__(NORM_THREADS, E > 8 ? 2 : WIDE && sizeof(T) == 2 && !DROPS ? 4 : 1) norm_forward(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(NORM_THREADS, E > 8 ? (WIDE ? 2 : 1) : WIDE && sizeof(T) == 2 && !DROPS ? 4 : 1) norm_forward(const __grid_constant__ NormArgs a) {
     __shared__ __align__(16) float vectors_s[NORM_VECTORS * NORM_MOST];
     __shared__ uint4 words_s[WIDE || !DROPS ? 1 : NORM_WARPS * norm_words(E)];
     norm_vectors_to(vectors_s, a);
