@@ -420,12 +420,15 @@ int pl_channel_norm_backward(const pl_channel_norm_shape* m, const void* dh, con
 int pl_channel_dropout(void* out, void* scaled, const void* x, const void* residual, int64_t n, int dtype, float residual_scale,
                        const pl_dropout* dropout, const int64_t* seed, void* stream);
 
-typedef enum pl_gate { PL_GATE_SILU = 0, PL_GATE_GELU = 1, PL_GATE_SIGMOID = 2, PL_GATE_RELU = 3 } pl_gate;   /* GELU: by erf */
+typedef enum pl_gate { PL_GATE_SILU = 0, PL_GATE_GELU = 1, PL_GATE_SIGMOID = 2, PL_GATE_RELU = 3 } pl_gate;   /* GELU: of the normal distribution itself; to 2^-18 of it in 16-bit types */
 
 /* out[rows, n] = (act(x @ gate_weight + gate_bias) * (x @ up_weight + up_bias)) @ down_weight + down_bias + residual_scale * residual,
  * x [rows, k], gate_weight and up_weight [k, h], down_weight [h, n]; biases and residual may be NULL.  Up to 128 channels in and out, 512
- * in between; everything of one type.  Products and sums are float or better; of 16-bit types the values in between go on to
- * the next product as two terms of the type, or (round_hidden) rounded once to it, 1.4 times as far off and faster.  Values and weights have to be finite, and below 3.38e38.
+ * in between; everything of one type.  Products of floats are 2^-25 off at most and sums of all types are floats that the tensor cores cut,
+ * some 2^-24 at each of 16 terms: results of floats are 3e-7 to 6e-7 off in the norm.  Of 16-bit types the values in between, and in the backward pass
+ * their gradients, go on to the next product as two terms of the type, or (round_hidden) rounded once to it, 1.4 times as far off and faster.  Values, weights and values in
+ * between have to be finite, and below 3.38e38 (PL_F16: 65504; below 2^-25 they are zero.  Their gradients, too, where the largest of grad_out is 2^-6
+ * or more; where it is less, they are held as if it were 2^-6.)
  * A wait inside a kernel that lasts two seconds (a GPU that was taken away meanwhile) is given up: NaN in the rows and sums concerned, in every output. */
 typedef struct pl_gated_shape {
     int64_t rows;

@@ -6,7 +6,7 @@
 
 over channels-last tensors [*, C] of points, in one pass, and their gradients in one more, from what came in: neither the
 normed values nor the dropout's mask are kept (`channel_norm`).  `channel_dropout` is dropout by itself, with the residual.
-The reference ships no such operators; the networks that give CRF-as-RNN (its README.md:15-16) its unaries do.
+The reference ships no such operators; networks that make a CRF's features or unaries of points have them.
 """
 import ctypes
 import functools

@@ -15,6 +15,8 @@
 // 617 604 rows of 256 float16 channels, residual and norm: 199 us, 6.35 TB/s of what has to be moved.  4 194 304 of 32 bfloat16 between two blocks, with
 // dropout: 242 us, 4.4 TB/s, and the gradients 535, 3.0 TB/s; 174 and 388 without the generator.  3 409 920 of 21 floats with a gate of every value: 205 and 393,
 // 5.6 and 4.4 TB/s.  Issue slots bound the narrow ones (60 % busy): shuffles, conversions, and of the generator a product for each of ten rounds and value pair.
+// The gradients through two norms of 8 values a lane take more than the 128 registers of a thread: 36 to 204 bytes of them go by way of local memory.  Rows that are not whole pieces,
+// of more than 256 channels: 150 000 x 511 floats, residual and two norms 241 us forward, 1480 backward, where 512 channels take 200 and 380.
 #pragma once
 #include "mix_common.cuh"
 #include "philox.cuh"
@@ -310,7 +312,7 @@ __global__ void __launch_bounds__(NORM_THREADS, E <= 8 ? 2 : 1) norm_backward(co
     Row r(a);
     const int per_warp = 32 / LANES, own = lane / LANES;
     const long long step = (long long)gridDim.x * NORM_WARPS * per_warp;
-    float sum_wa[E], sum_ba[E], sum_wb[E], sum_bb[E], sum_gate[E];   // (those without a use take no registers)
+    float sum_wa[E], sum_ba[E], sum_wb[E], sum_bb[E], sum_gate[E];   // (of a norm that is there both, a bias or not; with two norms a part of all this spills, see above)
 #pragma unroll
     for (int e = 0; e < E; e++) sum_wa[e] = sum_ba[e] = sum_wb[e] = sum_bb[e] = sum_gate[e] = 0.f;
     typename Row::Raw raw_x[Row::N], raw_residual[Row::N], raw_gate[Row::N], raw_dh[Row::N], raw_dy[Row::N];
@@ -449,7 +451,7 @@ struct DropArgs {
     float scale;
     Dropout drop;
 };
-// Two pieces a thread at a time, both on their way before the first is worked on (88 million floats and a residual: 164 us, one 186, four 170; bfloat16 values take 112, bound by the generator, some 40 products and exclusive ors for four).
+// Two pieces a thread at a time, both on their way before the first is worked on (88 million floats and a residual: 164 us, one 186, four 170; bfloat16 values take 118, issue slots 62 % busy: the generator's some 40 products and exclusive ors for four).
 constexpr int DROP_PIECES = 2;
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) drop_values(const __grid_constant__ DropArgs a) {

@@ -17,9 +17,9 @@
 // If one runs out (two seconds: it should not happen), all give up and what the CTA was to write is NaN, which nothing else reports.
 //
 // Tiles of 128 rows, the rows of a product; chunks of 64 hidden channels (floats: 32), so that g and u of two chunks and the sums fit into tensor memory and
-// the weights of all chunks, mostly, into shared memory.  2 097 152 rows of 64 to 256 to 64 bfloat16 channels: 421 us (245 TFLOP/s, 1.9 TB/s), gradients of
-// rows 583, of weights 660; 154 401 of 128 to 512 to 128 float16 108, 233, 253 (281 TFLOP/s forward); a million of 32 to 128 to 32 floats 282, 652, 1386.  The tensor
-// pipe is busy 19 to 32 % of it, memory less: what bounds them are the workers' instructions (half of the issue slots), half of these at barriers.
+// the weights of all chunks, mostly, into shared memory.  2 097 152 rows of 64 to 256 to 64 bfloat16 channels: 528 us (390 TFLOP/s, 1.5 TB/s), gradients of
+// rows 1001, of weights 1349; 154 401 of 128 to 512 to 128 float16 152, 330, 395 (400 TFLOP/s forward); a million of 32 to 128 to 32 floats 277, 650, 1521.  The tensor
+// pipe is busy 17 to 24 % of it, memory less: what bounds them are the workers' instructions (40 to 58 % of the issue slots), half of these at barriers.
 #pragma once
 #include <cuda.h>
 #include "gated_give_up.h"
@@ -106,7 +106,7 @@ __host__ __device__ inline int gated_up_bytes(int kp) { return Tensor<T>::TERMS 
 
 // Terms of a hidden value on its way to the second products.  FINE: 16-bit types take two, and results are off by their own rounding alone.  Else (who
 // calls says so) it is rounded once more, which makes results 1.4 times as far off (sums of a few values up to 1.7).  Two million rows of 64 to 256 to
-// 64 bfloat16 channels, forward, gradients of rows, of weights: 498, 945, 1268 us with two terms, 426, 582, 665 with one.
+// 64 bfloat16 channels, forward, gradients of rows, of weights: 528, 1001, 1349 us with two terms, 461, 708, 715 with one.
 template <typename T, bool FINE>
 __host__ __device__ constexpr int hidden_terms() { return sizeof(T) == 4 ? 3 : FINE ? 2 : 1; }
 

@@ -39,8 +39,9 @@ static int launch_norm_lanes(NormArgs& a, int lanes, bool backward, int ctas, cu
     return launch_norm<T, WIDE, E, 32>(a, backward, ctas, st);
 }
 
-// a.ctas: how many ran, and left a share of the sums each.  Up to 8 values a lane with as few lanes a row as that takes (6 where they do, 16 where
-// it is all lanes).
+// a.ctas: how many ran, and left a share of the sums each.  Up to 8 values a lane with as few lanes a row as that takes (16 where
+// it is all lanes).  Single values: 6 where those do, as much again backward otherwise (3 380 000 rows of 21 floats, gate of every value, two norms: 247 us forward and 568 backward, 275 and
+// 1162 with 8; bfloat16 217 and 590, 270 and 1302).
 template <typename T>
 static int norm_of(NormArgs& a, bool backward, int ctas, cudaStream_t st) {
     constexpr int V = 16 / sizeof(T);

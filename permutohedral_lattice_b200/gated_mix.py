@@ -2,8 +2,8 @@
 
     out = (act(x @ gate_weight + gate_bias) * (x @ up_weight + up_bias)) @ down_weight + down_bias + residual_scale * residual
 
-over channels-last tensors [*, K], in one kernel: the hidden channels' values are neither written nor kept, the backward pass makes them
-again from x.  The reference ships no such operator; the networks that give CRF-as-RNN (its README.md:15-16) its unaries do.
+over channels-last tensors [*, K], in one kernel after one that lays out the weights: the hidden channels' values are neither written nor kept, the
+backward pass makes them again from x.  The reference ships no such operator; networks that make a CRF's features or unaries of points have it.
 """
 import ctypes
 import functools
@@ -110,14 +110,21 @@ def gated_mix(x, gate_weight, up_weight, down_weight, gate_bias=None, up_bias=No
     gradients for all tensors.
 
     x [*, K], gate_weight and up_weight [K, H], down_weight [H, N], biases [H], [H], [N], residual and the output [*, N]: all of one type,
-    float32, float16 or bfloat16; up to 128 channels in and out and 512 in between.  activation: "silu", "gelu" (by erf),
-    "sigmoid" or "relu".  Products of floats are off by some 2^-24, sums are float32; of 16-bit types the hidden values (and, in the
-    backward pass, their gradients) go on to the next product as two terms of that type.  round_hidden: rounded once to it, as between
-    layers of their own; results are then 1.4 times as far off, and large calls faster (forward by a sixth, a training step by 40 %).
-    Gradients' sums over rows have a fixed order.  x, the weights and hidden values have to be finite, and below 3.38e38 (of float16
-    all of them below 65504): of a row that is not, values come out infinite or NaN, other rows are as
-    they would be; the weights' gradients are then not finite.  In a CUDA graph: one ordinary call of the same sizes before the
-    capture, forward and backward, which sets the kernels up; forward and backward together, on leaves made inside it."""
+    float32, float16 or bfloat16; up to 128 channels in and out and 512 in between.  activation: "silu", "gelu" (of the normal distribution
+    itself, to 2^-18 of it in 16-bit types), "sigmoid" or "relu".
+
+    Products of floats are off by 2^-25, sums are float32, cut on the tensor cores: results of floats are 3e-7 to 6e-7 off in the norm.  Of
+    16-bit types the hidden values (and, in the backward pass, their gradients) go on to the next product as two terms of that type, so that
+    results are off by their own rounding.  round_hidden: rounded once to it, as between layers of their own; results are then 1.4 times as
+    far off, and large calls faster (forward by an eighth, a training step by 40 %).  Gradients' sums over rows have a fixed order.
+
+    x, the weights and hidden values have to be finite, and below 3.38e38 (of float16 all of them below 65504): of a row that is not, values
+    come out infinite or NaN, other rows are as they would be; the weights' gradients are then not finite.  Hidden values of float16 below
+    2^-25 are zeros.  So are their gradients, but where all of the upstream gradient is below 2^-6 they are scaled: zeros below 2^-19 of its
+    largest value, and to stay below 2^22 of it.
+
+    In a CUDA graph: one ordinary call of the same sizes before the capture, forward and backward, which sets the kernels up; forward and
+    backward together, on leaves made inside it."""
     weights = (gate_weight, up_weight, down_weight, gate_bias, up_bias, down_bias)
     h, n = _check(x, residual, weights, activation)
     k = x.shape[-1]
