@@ -112,3 +112,34 @@ def test_a_captured_step_scales_by_what_it_finds(plb):
         torch.cuda.synchronize()
         want = gradients(plb, a, grad)
         assert all(torch.equal(found[m], want[m]) for m in NAMES)
+
+
+def test_two_steps_at_once_have_scales_of_their_own(plb):
+    calls = [make(5000, 64, 128, 64, size) for size in (2.0 ** -20, 1.0)]
+    want = [gradients(plb, *c) for c in calls]
+    sides = [torch.cuda.Stream() for _ in calls]
+    for _ in range(4):
+        got = []
+        for side, c in zip(sides, calls):
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                got.append(gradients(plb, *c))
+        for side in sides:
+            torch.cuda.current_stream().wait_stream(side)
+        for g, w in zip(got, want):
+            assert all(torch.equal(g[m], w[m]) for m in NAMES)
+
+
+def test_the_largest_one_beyond_2_31(plb):
+    """Only the last rows, whose values lie beyond 2^31 of dout, are not zeros: their scale is found there."""
+    rows, last, k = (1 << 31) // 16 + 300, 200, 16
+    a, few = make(last, k, 32, 16, 2.0 ** -20)
+    want = exact(a, few)
+    x = torch.zeros(rows, k, dtype=F16, device="cuda")
+    grad = torch.zeros(rows, 16, dtype=F16, device="cuda")
+    x[-last:], grad[-last:] = a["x"], few
+    leaves = {m: a[m].clone().requires_grad_(True) for m in ("gate_weight", "up_weight", "gate_bias", "up_bias")}
+    out = plb.gated_mix(x, leaves["gate_weight"], leaves["up_weight"], a["down_weight"], leaves["gate_bias"], leaves["up_bias"], a["down_bias"])
+    for (m, leaf), d in zip(leaves.items(), torch.autograd.grad(out, list(leaves.values()), grad)):
+        floor = 2.0 ** -25 * math.sqrt(d.numel())
+        assert float((d.double() - want[m]).norm()) <= floor + (2.0 ** -11 + 2.0 ** -14) * float(want[m].norm()), m
