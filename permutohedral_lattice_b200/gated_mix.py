@@ -116,7 +116,7 @@ def gated_mix(x, gate_weight, up_weight, down_weight, gate_bias=None, up_bias=No
     Products of floats are off by 2^-25, sums are float32, cut on the tensor cores: results of floats are 3e-7 to 6e-7 off in the norm.  Of
     16-bit types the hidden values (and, in the backward pass, their gradients) go on to the next product as two terms of that type, so that
     results are off by their own rounding.  round_hidden: rounded once to it, as between layers of their own; results are then 1.4 times as
-    far off, and large calls faster (forward by an eighth, a training step by 40 %).  Gradients' sums over rows have a fixed order.
+    far off, and large calls faster (forward by an eighth, a training step by up to a third).  Gradients' sums over rows have a fixed order.
 
     x, the weights and hidden values have to be finite, and below 3.38e38 (of float16 all of them below 65504): of a row that is not, values
     come out infinite or NaN, other rows are as they would be; the weights' gradients are then not finite.  Hidden values of float16 below
